@@ -422,6 +422,94 @@ int rq_short_attention(const void *q, int32_t dtype, int64_t total_q, int32_t nu
                        void *workspace, int64_t workspace_bytes,
                        void *stream);
 
+/*
+ * ---- 8-bit KV cache -----------------------------------------------------------
+ *
+ * A second cache, beside the packed codebook cache above: K and V as 8-bit codes with a
+ * power-of-two scale for each group of 16 consecutive slots, kv head and side.  Twice the bytes of
+ * 4-bit indices, no rotation, and an error of a 16-bit model's size rather than a
+ * codebook's.  No counterpart in the reference, whose codecs stop at 4 bits.
+ *
+ * A value is c * 2^e.  e is the smallest integer of [-40, 60] with amax <= Q * 2^e, where amax
+ * is the largest finite magnitude written to the group and Q = 127.5 (int8) or 448 (e4m3);
+ * c = x * 2^-e rounded to even, clamped to the largest code (infinities take it), NaN as 0.
+ * Writing slot 16 n of the cache begins its group anew: rows not written by the same call become 0.
+ * Other writes keep the group's rows; where their amax needs a larger e, the codes
+ * that stay are rounded again at the new scale.  So tokens are written forward within a group, as a
+ * server does; a slot may be written again (a rejected draft's), which never lowers the scale.
+ *
+ * Page of block_size slots (a multiple of 16), H kv heads, D = head_dim:
+ *   [block_size / 16 groups][H][K codes 16 D | V codes 16 D], then the scales
+ *   [block_size / 16 groups][H]{float 2^e_k, float 2^e_v, 8 unused bytes};
+ * rq_q8_slot_bytes() is a page's bytes per slot, H (2 D + 1) rounded up to 8 (the cache
+ * tensor is num_blocks x block_size x that).  Token t of the group, dim d:
+ *   K code: byte 1024 (d / 64) + 256 ((d / 16) % 4) + 16 t + d % 16
+ *   V code: byte 1024 (d / 64) + 256 (t / 4) + 16 (d % 16) + 4 ((d / 16) % 4) + t % 4
+ * int8 codes are stored as c + 128.  A zeroed page (scale 0) reads as zeros.
+ *
+ * head_dim 64 or 128.  Pages: `stride_block` bytes apart, 16-byte aligned.
+ */
+enum rq_q8_format {
+    RQ_Q8_INT8 = 0,
+    RQ_Q8_E4M3 = 1
+};
+
+/* Bytes of a cache slot (block_size of them make a page); 0 for sizes below 1. */
+int rq_q8_slot_bytes(int32_t num_kv_heads, int32_t head_dim);
+
+/*
+ * Quantise n_tokens tokens' K and V (dtype F16, BF16 or F32; strides in elements, rows 16-byte
+ * aligned) into the slots of slot_mapping (block * block_size + offset).  Slots outside the cache
+ * (vLLM's padding id -1) are skipped; of tokens with the same slot the last one counts.
+ * workspace: rq_q8_store_workspace_bytes() bytes, 16-byte aligned, no initialisation needed;
+ * 0 (none) for calls of up to 512 tokens, which take one launch, longer ones three.
+ */
+int64_t rq_q8_store_workspace_bytes(int64_t n_tokens, int64_t num_blocks, int32_t block_size);
+int rq_q8_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
+                int64_t k_stride_token, int64_t k_stride_head,
+                int64_t v_stride_token, int64_t v_stride_head,
+                int32_t num_kv_heads, int32_t head_dim, int32_t format,
+                const int64_t *slot_mapping,
+                uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+                void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * K and V of each sequence's first seq_lens[b] tokens as plain rows: token i of sequence b to row
+ * starts[b] + i of out_k and out_v (total rows x num_kv_heads x head_dim of out_dtype, contiguous,
+ * 16-byte aligned), the layout of a variable-length attention over unpacked K and V.  starts rises by at
+ * least the sequence's length; rows that belong to no sequence are left as they are.
+ */
+int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+               int32_t num_kv_heads, int32_t head_dim, int32_t format,
+               const int32_t *block_table, int64_t max_blocks, int64_t bt_stride_seq,
+               const int32_t *seq_lens, const int32_t *starts, int64_t num_seqs, int64_t total,
+               void *out_k, void *out_v, int32_t out_dtype, void *stream);
+
+/*
+ * Attention of new query tokens over the 8-bit cache: single tokens (decodes), drafts of a few,
+ * prompts and chunks behind a prefix.  Query i of sequence b sits at position seq_lens[b] - q_len_b + i; causal != 0: it
+ * sees cache positions up to its own, causal == 0: all seq_lens[b].  A row that sees no key gives zeros.
+ *
+ * q / out: total_q x num_q_heads x head_dim of F16 or BF16 (element strides; q rows 16-byte, out rows
+ * 8-byte aligned), num_q_heads a multiple of num_kv_heads.  cu_seqlens_q: num_seqs + 1 int32, or NULL
+ * for one token per sequence.  max_q_len bounds every q_len_b and max_seq_len every seq_lens[b]: tokens
+ * and keys past them, or past the block table's capacity, are not read.  Products are exact, sums and
+ * the softmax's statistics fp32, its weights rounded to fp16 for P V.
+ * workspace: rq_q8_attention_workspace_bytes() bytes, 16-byte aligned, no initialisation needed.
+ * Launches depend on host arguments only, so a captured call may be replayed with other lengths up to max_seq_len.
+ */
+int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int64_t max_q_len, int64_t max_seq_len);
+int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads,
+                    int64_t q_stride_tok, int64_t q_stride_head,
+                    const int32_t *cu_seqlens_q, int64_t num_seqs, int64_t max_q_len, int32_t causal,
+                    const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t format,
+                    const int32_t *block_table, int64_t max_blocks, int64_t bt_stride_seq,
+                    const int32_t *seq_lens, int64_t max_seq_len, float sm_scale,
+                    void *out, int64_t out_stride_tok, int64_t out_stride_head,
+                    void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,16 @@ _SIGNATURES = {
                                     _c_i64, _c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64,
                                     _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_i32, _c_f32, _c_p, _c_i64, _c_i64,
                                     _c_p, _c_i64, _c_p]),
+    "rq_q8_slot_bytes": (_c_i32, [_c_i32, _c_i32]),
+    "rq_q8_store_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i32]),
+    "rq_q8_store": (_c_i32, [_c_p, _c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p,
+                             _c_p, _c_i64, _c_i32, _c_i64, _c_p, _c_i64, _c_p]),
+    "rq_q8_read": (_c_i32, [_c_p, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64,
+                            _c_i64, _c_p, _c_p, _c_i32, _c_p]),
+    "rq_q8_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64]),
+    "rq_q8_attention": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_i64,
+                                 _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f32, _c_p,
+                                 _c_i64, _c_i64, _c_p, _c_i64, _c_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

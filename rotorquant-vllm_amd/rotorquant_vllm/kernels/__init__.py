@@ -29,6 +29,7 @@ import weakref
 import torch
 
 from .. import _lib
+from .q8 import q8_attention, q8_read, q8_slot_bytes, q8_store
 
 __all__ = [
     "iso_compress",
@@ -43,6 +44,10 @@ __all__ = [
     "paged_prefill",
     "rotation_block",
     "shared_workspace",
+    "q8_slot_bytes",
+    "q8_store",
+    "q8_read",
+    "q8_attention",
 ]
 
 

@@ -1,0 +1,206 @@
+"""Op-level API of the 8-bit KV cache: write (q8_store), read back (q8_read), attention (q8_attention).
+
+The cache is a (num_blocks, block_size, q8_slot_bytes(num_kv_heads, head_dim)) uint8 tensor whose
+pages hold K and V as int8 or e4m3 codes (fmt "int8" or "fp8") with a power-of-two scale for each
+group of 16 consecutive slots, kv head and side; include/rq_abi.h defines the bytes.  head_dim 64 or 128,
+block_size a multiple of 16.  No counterpart in the reference, whose codecs stop at 4 bits.
+
+As everywhere in this package, tensors are on one ROCm device and there is no CPU path; calls run on the
+current stream of that device, whichever device is current, and are safe on several
+streams at once (scratch comes from torch's allocator unless passed).
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+
+from .. import _lib
+
+__all__ = ["q8_slot_bytes", "q8_store", "q8_read", "q8_attention"]
+
+_FORMATS = {"int8": 0, "fp8": 1}
+_NULL = contextlib.nullcontext()
+
+
+def _format(fmt: str) -> int:
+    try:
+        return _FORMATS[fmt]
+    except (KeyError, TypeError):
+        raise ValueError(f"fmt must be 'int8' or 'fp8', got {fmt!r}") from None
+
+
+def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The device that all tensors are on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("rotorquant_vllm.kernels runs only on ROCm device tensors (got a "
+                               f"{t.device.type} tensor); there is no CPU path")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _on(dev: torch.device):
+    """A launch goes to the current device's context: make it the tensors' own."""
+    return _NULL if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def q8_slot_bytes(num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of a cache slot: the last dimension of the cache tensor (2056 for 8 heads of 128)."""
+    return -(-num_kv_heads * (2 * head_dim + 1) // 8) * 8
+
+
+def _check_cache(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> tuple[int, int, int]:
+    """(pages, block_size, bytes between pages) of an 8-bit cache."""
+    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 3:
+        raise ValueError("kv_cache must be a (num_blocks, block_size, q8_slot_bytes) uint8 tensor")
+    NB, BS, SB = kv_cache.shape
+    if SB < q8_slot_bytes(num_kv_heads, head_dim):
+        raise ValueError(f"cache slots of {SB} bytes; {num_kv_heads} heads of {head_dim} take {q8_slot_bytes(num_kv_heads, head_dim)}")
+    if kv_cache.stride(2) != 1 or kv_cache.stride(1) != SB:
+        raise ValueError("the slots of a page must be contiguous")
+    return NB, BS, kv_cache.stride(0)
+
+
+def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != dim:
+        raise ValueError(f"{name} must be a {dim}-dimensional {dtype} tensor, got {t.dim()} dimensions of {t.dtype}")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _scratch(workspace: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor | None:
+    """The caller's buffer, or one of this call from the stream's allocator (none for 0 bytes)."""
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor")
+    return workspace
+
+
+def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor, fmt: str = "int8",
+             workspace: torch.Tensor | None = None) -> None:
+    """Quantise key / value (N, H, D) fp16, bf16 or fp32 into the slots slot_mapping[:N] of an 8-bit cache.
+
+    Slots outside the cache (vLLM's padding id -1) are skipped; of tokens with the same slot the last one counts.
+    A write of a group's first slot begins the group anew (its rows that this call does not write
+    become 0); other writes keep its rows and never lower its scale.
+    workspace: scratch of calls of more than 512 tokens (rq_q8_store_workspace_bytes bytes),
+    by default from torch's allocator; a graph captured without torch's graph classes needs it.
+    """
+    dev = _one_device(key, value, kv_cache, slot_mapping, workspace)
+    if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError("key and value must have the same (tokens, heads, head_dim) shape and dtype")
+    N, H, D = key.shape
+    if D > 1 and (key.stride(-1) != 1 or value.stride(-1) != 1):
+        raise ValueError("key/value must be contiguous over head_dim")
+    NB, BS, stride = _check_cache(kv_cache, H, D)
+    sm = _index(slot_mapping, "slot_mapping", torch.int64, 1)
+    if sm.numel() < N:
+        raise ValueError("slot_mapping shorter than the number of tokens")
+    code = _format(fmt)
+    L = _lib.load()
+    with _on(dev):
+        ws = _scratch(workspace, L.rq_q8_store_workspace_bytes(N, NB, BS), dev)
+        rc = L.rq_q8_store(key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), N, key.stride(0), key.stride(1),
+                           value.stride(0), value.stride(1), H, D, code, sm.data_ptr(), kv_cache.data_ptr(), NB, BS, stride,
+                           _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr(dev))
+    _lib.check(rc, "rq_q8_store")
+
+
+def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor, num_kv_heads: int,
+            head_dim: int, dtype: torch.dtype, fmt: str = "int8", out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None,
+            total: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V of a batch's contexts as plain rows, (total, H, D) each: token i of sequence b in row starts[b] + i.
+
+    block_table (num_seqs, max_blocks), seq_lens (num_seqs,) and starts (num_seqs or num_seqs + 1, rising by
+    at least each length) are int32.  out_k / out_v: buffers to fill, whose rows of no sequence stay as they are;
+    without them `total` rows are allocated (rows of no sequence are then not initialised).
+    The layout is that of variable-length attention over plain K and V.
+    """
+    dev = _one_device(kv_cache, block_table, seq_lens, starts, out_k, out_v)
+    NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
+    bt = _index(block_table, "block_table", torch.int32, 2)
+    sl, st = _index(seq_lens, "seq_lens", torch.int32, 1), _index(starts, "starts", torch.int32, 1)
+    B = bt.shape[0]
+    if sl.numel() < B or st.numel() < B:
+        raise ValueError("block_table, seq_lens and starts differ in the number of sequences")
+    given = [t for t in (out_k, out_v) if t is not None]
+    if total is None:
+        if not given:
+            raise ValueError("total (the number of rows) is needed without out_k and out_v")
+        total = given[0].shape[0]
+    shape = (total, num_kv_heads, head_dim)
+    for t in given:
+        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"outputs must be contiguous {shape} tensors of {dtype}")
+    code = _format(fmt)
+    L = _lib.load()
+    with _on(dev):
+        out_k = torch.empty(shape, dtype=dtype, device=dev) if out_k is None else out_k
+        out_v = torch.empty(shape, dtype=dtype, device=dev) if out_v is None else out_v
+        rc = L.rq_q8_read(kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, head_dim, code, bt.data_ptr(), bt.shape[1], bt.stride(0),
+                          sl.data_ptr(), st.data_ptr(), B, total, out_k.data_ptr(), out_v.data_ptr(), _lib.dtype_code(dtype),
+                          _lib.stream_ptr(dev))
+    _lib.check(rc, "rq_q8_read")
+    return out_k, out_v
+
+
+def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, num_kv_heads: int,
+                 head_dim: int, fmt: str = "int8", sm_scale: float | None = None, causal: bool = True,
+                 cu_seqlens_q: torch.Tensor | None = None, max_q_len: int | None = None, max_seq_len: int | None = None,
+                 out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new query tokens q (num_tokens, H_Q, D) fp16 or bf16 over an 8-bit cache.
+
+    block_table (num_seqs, max_blocks) and seq_lens (num_seqs,), the contexts with the new tokens
+    included, are int32.  cu_seqlens_q (num_seqs + 1,) int32 splits q among the sequences; without it each has one token
+    (a decode step).  Query i of sequence b sits at position seq_lens[b] - q_len_b + i; a row that sees no key is zeros.
+    max_q_len and max_seq_len: host ints that bound the query and context lengths (default: all of q, and the
+    block table's capacity); what lies past them is not read.
+    workspace: scratch (rq_q8_attention_workspace_bytes bytes), by default of this call from torch's allocator; a graph
+    captured without torch's graph classes needs it, since nothing else keeps the scratch for its replays.
+    """
+    if q.dim() != 3 or q.shape[2] != head_dim or num_kv_heads < 1 or q.shape[1] % num_kv_heads:
+        raise ValueError(f"q must be (tokens, a multiple of {num_kv_heads} heads, {head_dim}), got {tuple(q.shape)}")
+    dev = _one_device(q, kv_cache, block_table, seq_lens, cu_seqlens_q, out, workspace)
+    NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
+    bt = _index(block_table, "block_table", torch.int32, 2)
+    sl = _index(seq_lens, "seq_lens", torch.int32, 1)
+    T, HQ, D = q.shape
+    B = sl.numel()
+    if bt.shape[0] != B:
+        raise ValueError("block_table and seq_lens differ in the number of sequences")
+    cu = None
+    if cu_seqlens_q is None:
+        if T != B:
+            raise ValueError(f"{T} query tokens and {B} sequences: cu_seqlens_q is needed")
+        max_q_len = 1
+    else:
+        cu = _index(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+        if cu.numel() != B + 1:
+            raise ValueError(f"cu_seqlens_q must have {B + 1} entries, got {cu.numel()}")
+        max_q_len = T if max_q_len is None else min(int(max_q_len), T)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1):
+        raise ValueError("out must have q's shape and dtype and be contiguous over head_dim")
+    capacity = bt.shape[1] * BS
+    max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
+    code = _format(fmt)
+    L = _lib.load()
+    with _on(dev):
+        out = torch.empty_like(q) if out is None else out
+        ws = _scratch(workspace, L.rq_q8_attention_workspace_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), dev)
+        rc = L.rq_q8_attention(q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, q.stride(0), q.stride(1), _lib.ptr(cu), B, max_q_len,
+                               1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(),
+                               bt.shape[1], bt.stride(0), sl.data_ptr(), max_seq_len,
+                               float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale), out.data_ptr(), out.stride(0), out.stride(1),
+                               _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr(dev))
+    _lib.check(rc, "rq_q8_attention")
+    return out
