@@ -18,87 +18,25 @@
 // the weights come out of S^T in the order that P V takes.
 #include <algorithm>
 
-#include "rq_q8.h"
+#include "rq_q8_attn.h"
 
 namespace rq {
 
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-
-constexpr int kQ8Tile = 32;     // keys of a tile: two groups
 constexpr int kQ8Waves = 4;     // of a workgroup; tile t of a segment goes to wave t % 4
 constexpr int kQ8Cols = 16;     // columns of a workgroup
 constexpr int kQ8MinChunk = 8;  // tiles of a workgroup, at least
-constexpr float kQ8Log2e = 1.4426950408889634f;
 
-struct Q8AttnArgs {
-    const void *q;
-    int64_t q_st, q_sh;
-    const int32_t *cu_q;  // NULL: one token per sequence
-    int64_t total_q, num_seqs;
-    int causal;
-    const uint8_t *cache;
-    int64_t num_blocks, stride_block;
-    int H, G, groups, block_size;
-    const int32_t *bt;
-    int64_t max_blocks, bt_ss;
-    const int32_t *seq_lens;
-    int64_t cap;  // keys of a sequence that may be read: its table's capacity, max_seq_len
-    int max_q;    // tokens of a query that count
-    float score_scale;  // |sm_scale| log2(e)
-    float q_sign;       // sign of sm_scale (0 for 0)
-    void *out;
-    int64_t o_st, o_sh;
-    float *part;
-    int split;  // 1: equal shares of the tiles of all items; 0: one workgroup per item
-};
-
-__device__ __forceinline__ f32x4 q8_mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t q8_pack(float lo, float hi) {
-    const f16x2 v = {(_Float16)lo, (_Float16)hi};
-    return __builtin_bit_cast(uint32_t, v);
-}
-
-// The codes of a dword in fp16: two dwords.  int8: bytes under 0x64 are 1024 + (c + 128).
-template <int FMT>
-__device__ __forceinline__ void q8_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (FMT == RQ_Q8_INT8) {
-        const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
-        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, perm(0x64646464u, w, 0x04010400u)) - off);
-        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, perm(0x64646464u, w, 0x04030402u)) - off);
-    } else {
-        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
-        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
-    }
-}
-
-// A sequence's query tokens (q0 .. q0 + T), keys L, and tiles.
-struct Q8Seq {
-    int q0, T, L, vis;
-    __device__ __forceinline__ int tiles() const { return max(1, (vis + kQ8Tile - 1) / kQ8Tile); }
-};
-__device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
-    Q8Seq s;
-    s.q0 = a.cu_q ? a.cu_q[b] : (int)b;
-    const int end = a.cu_q ? a.cu_q[b + 1] : (int)b + 1;
-    s.T = min(max(min((int64_t)end, a.total_q) - max(s.q0, 0), (int64_t)0), (int64_t)a.max_q);
-    if (s.q0 < 0) s.T = 0;
-    s.L = a.seq_lens[b];
-    s.vis = (int)max((int64_t)0, min((int64_t)s.L, a.cap));
-    return s;
-}
 __device__ __forceinline__ int q8_col_blocks(const Q8AttnArgs &a, int T) { return (T * a.G + kQ8Cols - 1) / kQ8Cols; }
+
+constexpr int kQ8Tile = 32;     // keys of a tile: two groups
+__device__ __forceinline__ int q8_tiles(const Q8Seq &s) { return max(1, (s.vis + kQ8Tile - 1) / kQ8Tile); }
 
 // Items are (sequence, block of 16 columns, kv head), in that order; the tiles of all items in a row are cut into
 // equal shares.  Tiles of all items, in 64-bit; each workgroup sums over the sequences itself (64 at a time).
 __device__ __forceinline__ int64_t q8_seq_tiles(const Q8AttnArgs &a, int64_t b) {
     if (b >= a.num_seqs) return 0;
     const Q8Seq s = q8_seq(a, b);
-    return (int64_t)s.tiles() * q8_col_blocks(a, s.T) * a.H;
+    return (int64_t)q8_tiles(s) * q8_col_blocks(a, s.T) * a.H;
 }
 __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 #pragma unroll
@@ -138,20 +76,14 @@ __device__ __forceinline__ float q8_query(const Q8AttnArgs &a, const Q8Seq &s, i
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
         raw[k] = valid ? *reinterpret_cast<const u32x4 *>(row + 64 * (k >> 1) + 16 * g + 8 * (k & 1)) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) big = max(big, max(raw[k][e] & 0x7fffu, (raw[k][e] >> 16) & 0x7fffu));
+        big = q8_max_bits(raw[k], big);
     }
     big = max(big, (uint32_t)__shfl_xor((int)big, 16));
     big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-    // the row's largest magnitude to 2^14 (small rows by at most 2^60)
-    const int e = (int)((__float_as_uint(Elem<DT>::to_f32(big)) >> 23) & 0xffu) - 127;
-    const int up = min(60, 14 - e);
+    const int up = q8_query_exp<DT>(big);
     const float f = exp2i(up) * a.q_sign;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4)
-            qop[k][e4] = q8_pack(Elem<DT>::to_f32(raw[k][e4] & 0xffffu) * f, Elem<DT>::to_f32(raw[k][e4] >> 16) * f);
+    for (int k = 0; k < D / 32; ++k) qop[k] = q8_query_f16<DT>(raw[k], f);
     return a.score_scale * exp2i(-up);
 }
 
@@ -196,7 +128,7 @@ __global__ __launch_bounds__(64 * kQ8Waves) void q8_stream_kernel(Q8AttnArgs a) 
             }
         }
         const Q8Seq s = q8_seq(a, seq);
-        const int n = s.tiles();
+        const int n = q8_tiles(s);
         const int64_t in_seq = pos - seq_base;
         const int64_t item = in_seq / n;
         const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
@@ -269,7 +201,7 @@ __global__ __launch_bounds__(64 * kQ8Waves) void q8_stream_kernel(Q8AttnArgs a) 
                     q8_to_f16<FMT>(w[2 * (k & 1)], x[0], x[1]);
                     q8_to_f16<FMT>(w[2 * (k & 1) + 1], x[2], x[3]);
                     op = u32x4{x[0], x[1], x[2], x[3]};
-                    S[gr] = q8_mfma(op, qop[k], S[gr]);
+                    S[gr] = mfma_f16(op, qop[k], S[gr]);
                 }
             }
             if (k0 + kQ8Tile > lim_first) {
@@ -313,8 +245,8 @@ __global__ __launch_bounds__(64 * kQ8Waves) void q8_stream_kernel(Q8AttnArgs a) 
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[gr][i], f[gr], add));
-                pw[2 * gr] = q8_pack(w[0], w[1]);
-                pw[2 * gr + 1] = q8_pack(w[2], w[3]);
+                pw[2 * gr] = pack_f16(w[0], w[1]);
+                pw[2 * gr + 1] = pack_f16(w[2], w[3]);
                 // the sum of the weights before their rounding to fp16 (which has no bias)
                 l_run = __builtin_fmaf((w[0] + w[1]) + (w[2] + w[3]), exp2i(-ev[gr]), l_run);
             }
@@ -325,7 +257,7 @@ __global__ __launch_bounds__(64 * kQ8Waves) void q8_stream_kernel(Q8AttnArgs a) 
                     uint32_t x[4];
                     q8_to_f16<FMT>(cur.v[0][j][i], x[0], x[1]);
                     q8_to_f16<FMT>(cur.v[1][j][i], x[2], x[3]);
-                    acc[4 * j + i] = q8_mfma(u32x4{x[0], x[1], x[2], x[3]}, pw, acc[4 * j + i]);
+                    acc[4 * j + i] = mfma_f16(u32x4{x[0], x[1], x[2], x[3]}, pw, acc[4 * j + i]);
                 }
         }
 
@@ -379,7 +311,7 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgro
     const int64_t b = blockIdx.y;
     const Q8Seq s = q8_seq(a, b);
     if ((int64_t)blockIdx.x >= (int64_t)q8_col_blocks(a, s.T) * a.H) return;
-    const int n = s.tiles();
+    const int n = q8_tiles(s);
     int64_t total = 0, before = 0;
     for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
         const int64_t mine = q8_seq_tiles(a, b0 + lane);
@@ -441,6 +373,10 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
     fmt == RQ_Q8_INT8 ? launch_stream_d<DT, RQ_Q8_INT8>(a, D, wgs, st) : launch_stream_d<DT, RQ_Q8_E4M3>(a, D, wgs, st);
 }
 
+// Calls of so many columns per kv head or more go to the prefill kernels.
+constexpr int64_t kQ8PromptCols = 128;
+static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= kQ8PromptCols; }
+
 }  // namespace rq
 
 using namespace rq;
@@ -448,7 +384,9 @@ using namespace rq;
 extern "C" int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
                                                    int32_t head_dim, int64_t max_q_len, int64_t max_seq_len) {
     if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_q_len <= 0 || max_seq_len < 0) return 0;
-    const int64_t wgs = q8_workgroups(num_seqs, num_q_heads / num_kv_heads, num_kv_heads, max_q_len, max_seq_len);
+    const int G = num_q_heads / num_kv_heads;
+    if (q8_is_prompt(max_q_len, G)) return q8_prefill_workspace(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
+    const int64_t wgs = q8_workgroups(num_seqs, G, num_kv_heads, max_q_len, max_seq_len);
     return 2 * wgs * kQ8Cols * (head_dim + 2) * 4;
 }
 
@@ -487,15 +425,16 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     a.seq_lens = seq_lens;
     a.cap = std::min<int64_t>(std::min<int64_t>(max_blocks * block_size, max_seq_len), INT32_MAX - 64);
     a.max_q = (int)(cu_seqlens_q ? max_q_len : 1);
-    a.score_scale = sm_scale == 0.f ? 1.f : __builtin_fabsf(sm_scale) * kQ8Log2e;
+    a.score_scale = sm_scale == 0.f ? 1.f : __builtin_fabsf(sm_scale) * kAttnLog2e;
     a.q_sign = sm_scale > 0.f ? 1.f : sm_scale < 0.f ? -1.f : 0.f;
     a.out = out, a.o_st = out_stride_tok, a.o_sh = out_stride_head;
-    const int64_t need = rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, a.cap);
+    const int64_t need = rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, a.max_q, a.cap);
     RQ_CHECK_SPACE(workspace_bytes >= need, "workspace too small: the call needs %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
     RQ_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
     a.part = static_cast<float *>(workspace);
-    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, a.max_q, a.cap);
     hipStream_t st = (hipStream_t)stream;
+    if (q8_is_prompt(a.max_q, a.G)) return q8_prefill(a, dtype, format, head_dim, workspace, st);
+    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, a.max_q, a.cap);
     if (dtype == RQ_DTYPE_BF16) launch_stream_f<RQ_DTYPE_BF16>(a, format, head_dim, wgs, st);
     else launch_stream_f<RQ_DTYPE_F16>(a, format, head_dim, wgs, st);
     return check_launch("q8_stream_kernel");

@@ -320,3 +320,13 @@ def test_long_context_splits_agree():
     short = K.q8_attention(q.to(DEV), cache, i32(table), i32(lens), H, D, max_seq_len=500)  # keys past the bound are not read
     out, tol = Q.attention(q, ref.values(), table, [500, 3, 500], [0, 1, 2, 3], block)
     assert (np.abs(short.double().cpu().numpy() - out) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H,G,D,lens,queries,causal", [
+    (2, 4, 128, [200, 64, 1, 0, 450], [200, 33, 1, 0, 130], True), (1, 8, 64, [300, 129], [65, 129], True), (3, 3, 128, [97], [97], False),
+    (1, 1, 128, [2500], [160], True), (2, 5, 64, [1100, 40], [40, 40], True), (1, 4, 128, [30, 70], [90, 70], True)])
+def test_prompts(fmt, H, G, D, lens, queries, causal):
+    """Query lengths that take the prefill kernels: odd ones, none, more queries than keys, few queries over long contexts."""
+    attend(lens, queries, 16, H, G, D, fmt, torch.float16, 31, causal=causal)
+    attend(lens, queries, 32, H, G, D, fmt, torch.bfloat16, 32, causal=causal)
