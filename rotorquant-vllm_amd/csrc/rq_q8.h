@@ -113,7 +113,7 @@ inline int check_q8_cache(int head_dim, int num_kv_heads, int block_size, int64_
     RQ_CHECK_ARG(num_kv_heads >= 1 && num_kv_heads <= 4096, "num_kv_heads %d unsupported", num_kv_heads);
     RQ_CHECK_ARG(block_size >= kQ8Group && block_size % kQ8Group == 0 && block_size <= 65536,
                  "block_size %d must be a multiple of %d", block_size, kQ8Group);
-    RQ_CHECK_ARG(num_blocks >= 0 && num_blocks <= INT32_MAX, "num_blocks %lld out of range", (long long)num_blocks);
+    RQ_CHECK_ARG(num_blocks >= 0 && num_blocks <= INT32_MAX / (block_size / kQ8Group), "num_blocks %lld out of range", (long long)num_blocks);
     const int64_t page = Q8Layout(num_kv_heads, head_dim, block_size).scale_at(block_size / kQ8Group, 0);
     RQ_CHECK_ARG(stride_block >= page && stride_block % 16 == 0,
                  "pages must be %lld bytes or more, a multiple of 16 (got %lld)", (long long)page, (long long)stride_block);

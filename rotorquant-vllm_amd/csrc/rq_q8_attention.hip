@@ -22,351 +22,447 @@
 
 namespace rq {
 
-constexpr int kQ8Waves = 4;     // of a workgroup; tile t of a segment goes to wave t % 4
-constexpr int kQ8Cols = 16;     // columns of a workgroup
+constexpr int kQ8Cols = 16;     // columns of an MFMA; a workgroup takes NB blocks of them
 constexpr int kQ8MinChunk = 8;  // tiles of a workgroup, at least
-
-__device__ __forceinline__ int q8_col_blocks(const Q8AttnArgs &a, int T) { return (T * a.G + kQ8Cols - 1) / kQ8Cols; }
 
 constexpr int kQ8Tile = 32;     // keys of a tile: two groups
 __device__ __forceinline__ int q8_tiles(const Q8Seq &s) { return max(1, (s.vis + kQ8Tile - 1) / kQ8Tile); }
+template <int NB>
+__device__ __forceinline__ int q8_col_blocks(const Q8AttnArgs &a, int T) { return (T * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols); }
 
-// Items are (sequence, block of 16 columns, kv head), in that order; the tiles of all items in a row are cut into
-// equal shares.  Tiles of all items, in 64-bit; each workgroup sums over the sequences itself (64 at a time).
+// ---- shares -------------------------------------------------------------------
+// Items are (sequence, block of 16 NB columns, kv head), in that order; the tiles of all items in a row are cut into
+// equal shares, one per workgroup.  Each workgroup sums over the sequences itself, 64 at a time.
+template <int NB>
 __device__ __forceinline__ int64_t q8_seq_tiles(const Q8AttnArgs &a, int64_t b) {
     if (b >= a.num_seqs) return 0;
     const Q8Seq s = q8_seq(a, b);
-    return (int64_t)q8_tiles(s) * q8_col_blocks(a, s.T) * a.H;
+    return (int64_t)q8_tiles(s) * q8_col_blocks<NB>(a, s.T) * a.H;
 }
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
     return x;
 }
-__device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    return x;
+// Of values under 2^41: the low 16 bits and the rest are summed apart.
+__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
+    return (int64_t)wave_scan((uint32_t)x & 0xffffu) + ((int64_t)wave_scan((uint32_t)((uint64_t)x >> 16)) << 16);
 }
-__device__ __forceinline__ int64_t q8_share(int64_t tiles, int64_t workgroups) {
-    return max((int64_t)kQ8MinChunk, (tiles + workgroups - 1) / workgroups);
-}
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+__device__ __forceinline__ int64_t lane64(int64_t x, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), lane);
     return (int64_t)((uint64_t)hi << 32 | lo);
+}
+// a / b; in 32 bits (a tenth of the instructions) where both fit.
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int64_t q8_share(int64_t tiles, int workgroups) {
+    return max((int64_t)kQ8MinChunk, div64(tiles + workgroups - 1, workgroups));
 }
 
 template <int D>
 struct Q8Partial {
-    static constexpr int kFloats = kQ8Cols * (D + 2);  // accumulators by column, then (M, l) by column
+    static constexpr int kFloats = kQ8Cols * (D + 2);  // of a block: accumulators by column, then (M, l) by column
 };
 
+// ---- one segment ----------------------------------------------------------------
+__device__ __forceinline__ uint32_t rows_umax(uint32_t x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(r[0], r[1]);
+    auto t = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max(t[0], t[1]);
+}
 // One column's operands: q 2^s in fp16 in K's dim order, and f without the group's 2^e_k.
 template <int DT, int D>
-__device__ __forceinline__ float q8_query(const Q8AttnArgs &a, const Q8Seq &s, int c0, int h, int lane, u32x4 (&qop)[D / 32]) {
-    const int col = c0 + (lane & 15), g = lane >> 4;
-    const int i = col / a.G, hq = h * a.G + col % a.G;
-    u32x4 raw[D / 32];
-    const bool valid = i < s.T;
-    const uint16_t *row = static_cast<const uint16_t *>(a.q) + (int64_t)(s.q0 + (valid ? i : 0)) * a.q_st + (int64_t)(valid ? hq : h * a.G) * a.q_sh;
+__device__ __forceinline__ float q8_query(const Q8AttnArgs &a, u32x4 (&qop)[D / 32]) {
     uint32_t big = 0;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-        raw[k] = valid ? *reinterpret_cast<const u32x4 *>(row + 64 * (k >> 1) + 16 * g + 8 * (k & 1)) : u32x4{0u, 0u, 0u, 0u};
-        big = q8_max_bits(raw[k], big);
-    }
-    big = max(big, (uint32_t)__shfl_xor((int)big, 16));
-    big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-    const int up = q8_query_exp<DT>(big);
+    for (int k = 0; k < D / 32; ++k) big = q8_max_bits(qop[k], big);
+    const int up = q8_query_exp<DT>(rows_umax(big));
     const float f = exp2i(up) * a.q_sign;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) qop[k] = q8_query_f16<DT>(raw[k], f);
+    for (int k = 0; k < D / 32; ++k) qop[k] = q8_query_f16<DT>(qop[k], f);
     return a.score_scale * exp2i(-up);
 }
 
-// Codes and scales of one tile: two groups.
+// Codes of one tile: two groups.
 template <int D>
 struct Q8Tile {
     u32x4 k[2][D / 64], v[2][D / 64];
-    float ks[2], vs[2];
+};
+template <int D, int W>
+struct Q8Sums {  // of a workgroup's W waves
+    float acc[W][kQ8Cols][D + 4];
+    float2 ml[W][kQ8Cols];
 };
 
-template <int DT, int FMT, int D>
-__global__ __launch_bounds__(64 * kQ8Waves) void q8_stream_kernel(Q8AttnArgs a) {
+// Stores N values of a row (N = 2 or a multiple of 4).
+template <int DT, int N>
+__device__ __forceinline__ void q8_put(uint16_t *row, const float (&o)[N], float f) {
+    if constexpr (N == 2) {
+        *reinterpret_cast<uint32_t *>(row) = pack_pair<DT>(o[0] * f, o[1] * f);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 4)
+            *reinterpret_cast<uint2 *>(row + k) = make_uint2(pack_pair<DT>(o[k] * f, o[k + 1] * f), pack_pair<DT>(o[k + 2] * f, o[k + 3] * f));
+    }
+}
+
+// Tiles [t0, t1) of the item (sequence, kv head h, columns from c0) by the workgroup's W waves, tile t0 + i by wave i % W.  The result is
+// the output rows (part == NULL) or partials.
+template <int DT, int FMT, int D, int NB, int W>
+__device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, const Q8Seq &s, int h, int c0, int t0, int t1, float *part,
+                                           Q8Sums<D, W> &lds) {
     constexpr int kSteps = D / 32, kChunks = D / 64, kBlocks = D / 16;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, g = lane >> 4;
-    __shared__ float lds_acc[kQ8Waves][kQ8Cols][D + 4];
-    __shared__ float2 lds_ml[kQ8Waves][kQ8Cols];
-
-    // this workgroup's share [pos, end) of the row of tiles
-    int64_t total = 0;
-    for (int64_t b = 0; b < a.num_seqs; b += 64) total += wave_sum64(q8_seq_tiles(a, b + lane));
-    total = uniform64(total);
-    const int64_t share = q8_share(total, gridDim.x);
-    int64_t pos = blockIdx.x * share;
-    const int64_t end = min(total, pos + share);
-
-    int64_t seq = -1, seq_base = 0, seq_tiles = 0;  // the sequence of pos: its first tile in the row, its tiles
-    int64_t scan_b = 0, scan_base = 0;
-    while (pos < end) {
-        if (seq < 0 || pos >= seq_base + seq_tiles) {
-            for (;; scan_b += 64) {
-                const int64_t mine = q8_seq_tiles(a, scan_b + lane), upto = wave_scan64(mine, lane);
-                const uint64_t hit = __ballot(scan_base + upto > pos);
-                if (hit) {
-                    const int l = __builtin_ctzll(hit);
-                    seq = scan_b + l;
-                    seq_tiles = uniform64(__shfl(mine, l));
-                    seq_base = uniform64(scan_base + __shfl(upto, l)) - seq_tiles;
-                    break;
-                }
-                scan_base = uniform64(scan_base + __shfl(upto, 63));
+    const Q8Layout lay(a.H, D, a.block_size);
+    // Lane l looks up group l % 2 of the (l / 2)-th of this wave's next 32 tiles.
+    const int last_group = max(0, (s.vis + kQ8Group - 1) / kQ8Group - 1);
+    int64_t at = 0;
+    float2 sc = make_float2(0.f, 0.f);
+    auto look_up = [&](int first) {
+        const uint32_t gi = (uint32_t)min(2 * (first + W * (lane >> 1)) + (lane & 1), last_group);
+        const uint32_t p = gi / (uint32_t)a.groups;
+        int64_t page = s.vis > 0 ? a.bt[seq * a.bt_ss + p] : 0;
+        page = page < 0 || page >= a.num_blocks ? 0 : page;
+        at = page * a.stride_block + lay.codes_at(gi - p * a.groups, h);
+        sc = *reinterpret_cast<const float2 *>(a.cache + page * a.stride_block + lay.scale_at(gi - p * a.groups, h));
+    };
+    auto slot = [&](int t) { return (t - t0) / W & 31; };
+    // The codes are read once: non-temporal loads (64 sequences of 4600 keys on average, 8 kv heads: 126 us -> 114).
+    Q8Tile<D> next;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+            const uint8_t *p = a.cache + lane64(at, 2 * slot(t) + gr);
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                next.k[gr][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 1024 * j + 16 * lane));
+                next.v[gr][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + kQ8Group * D + 1024 * j + 16 * lane));
             }
         }
-        const Q8Seq s = q8_seq(a, seq);
-        const int n = q8_tiles(s);
-        const int64_t in_seq = pos - seq_base;
-        const int64_t item = in_seq / n;
-        const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
-        const int h = (int)(item % a.H), c0 = (int)(item / a.H) * kQ8Cols;
-
-        u32x4 qop[kSteps];
-        const float colf = q8_query<DT, D>(a, s, c0, h, lane, qop);
-        // keys that this lane's column sees, and the fewest that any column of the block sees
-        const int i_mine = (c0 + col) / a.G, i_first = c0 / a.G;
-        const int lim = a.causal ? min(s.vis, s.L - s.T + i_mine + 1) : s.vis;
-        const int lim_first = a.causal ? min(s.vis, s.L - s.T + i_first + 1) : s.vis;
-
-        f32x4 acc[kBlocks];
+    };
+    int t = t0 + wave;
+    // (the look-up's loads depend on one another; the query's are issued between them)
+    if (t < t1) look_up(t);
+    u32x4 qop[NB][kSteps];
 #pragma unroll
-        for (int m = 0; m < kBlocks; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float M = -INFINITY, l_run = 0.f;
+    for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t c = c0 + kQ8Cols * nb + col, i = c / (uint32_t)a.G;
+        const bool valid = (int)i < s.T;
+        const uint16_t *row = static_cast<const uint16_t *>(a.q) + (int64_t)(s.q0 + (valid ? (int)i : 0)) * a.q_st +
+                              (int64_t)(h * a.G + (valid ? (int)(c - i * a.G) : 0)) * a.q_sh + 16 * g;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+            qop[nb][k] = valid ? *reinterpret_cast<const u32x4 *>(row + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0u, 0u, 0u, 0u};
+    }
+    if (t < t1) fetch(t);
+    float colf[NB], M[NB], l_run[NB];
+    int lim[NB];  // keys that this lane's column sees
+    f32x4 acc[NB][kBlocks];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        colf[nb] = q8_query<DT, D>(a, qop[nb]);
+        lim[nb] = a.causal ? min(s.vis, s.L - s.T + (c0 + kQ8Cols * nb + col) / a.G + 1) : s.vis;
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) acc[nb][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        M[nb] = -INFINITY, l_run[nb] = 0.f;
+    }
+    const int lim_first = a.causal ? min(s.vis, s.L - s.T + c0 / a.G + 1) : s.vis;  // the fewest that any column sees
 
-        const Q8Layout lay(a.H, D, a.block_size);
-        // tiles of this wave: t0 + wave, + 4, ...; lane l looks up group l % 2 of the (l / 2)-th of the next 32
-        const int last_group = max(0, (s.vis + kQ8Group - 1) / kQ8Group - 1);
-        int64_t at = 0;
-        float2 sc = make_float2(0.f, 0.f);
-        auto look_up = [&](int first) {
-            const int gi = min(2 * (first + kQ8Waves * (lane >> 1)) + (lane & 1), last_group);
-            const int p = gi / a.groups;
-            int64_t page = s.vis > 0 ? a.bt[seq * a.bt_ss + p] : 0;
-            page = page < 0 || page >= a.num_blocks ? 0 : page;
-            at = page * a.stride_block + lay.codes_at(gi - p * a.groups, h);
-            sc = *reinterpret_cast<const float2 *>(a.cache + page * a.stride_block + lay.scale_at(gi - p * a.groups, h));
-        };
-        Q8Tile<D> next;
-        auto fetch = [&](int t) {  // tile t of the segment, slot (t - t0) / 4 % 32 of the looked-up ones
+    for (; t < t1; t += W) {
+        int ev[2];
+        float ks[2];
 #pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                const int from = 2 * (((t - t0) / kQ8Waves) & 31) + gr;
-                const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, from), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)at >> 32), from);
-                const uint8_t *p = a.cache + ((uint64_t)hi << 32 | lo);
-                next.ks[gr] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.x), from));
-                next.vs[gr] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), from));
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j) {
-                    next.k[gr][j] = *reinterpret_cast<const u32x4 *>(p + 1024 * j + 16 * lane);
-                    next.v[gr][j] = *reinterpret_cast<const u32x4 *>(p + kQ8Group * D + 1024 * j + 16 * lane);
-                }
-            }
-        };
-        int t = t0 + wave;
-        if (t < t1) {
-            look_up(t);
-            fetch(t);
+        for (int gr = 0; gr < 2; ++gr) {
+            ks[gr] = exp2i(q8_scale_exp(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.x), 2 * slot(t) + gr))));
+            ev[gr] = q8_scale_exp(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), 2 * slot(t) + gr)));
         }
-        for (; t < t1; t += kQ8Waves) {
-            Q8Tile<D> cur = next;
-            const int tn = t + kQ8Waves;
-            if (tn < t1) {
-                if ((((tn - t0) / kQ8Waves) & 31) == 0) look_up(tn);
-                fetch(tn);
-            }
-            const int k0 = t * kQ8Tile;
-            // scores
-            f32x4 S[2];
+        Q8Tile<D> cur = next;
+        const int tn = t + W;
+        if (tn < t1) {
+            if (slot(tn) == 0) look_up(tn);
+            fetch(tn);
+        }
+        const int k0 = t * kQ8Tile;
+        f32x4 S[NB][2];
 #pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                S[gr] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int gr = 0; gr < 2; ++gr) {
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    u32x4 op;
-                    const u32x4 w = cur.k[gr][k >> 1];
-                    uint32_t x[4];
-                    q8_to_f16<FMT>(w[2 * (k & 1)], x[0], x[1]);
-                    q8_to_f16<FMT>(w[2 * (k & 1) + 1], x[2], x[3]);
-                    op = u32x4{x[0], x[1], x[2], x[3]};
-                    S[gr] = mfma_f16(op, qop[k], S[gr]);
-                }
+            for (int nb = 0; nb < NB; ++nb) S[nb][gr] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const u32x4 w = cur.k[gr][k >> 1];
+                uint32_t x[4];
+                q8_to_f16<FMT>(w[2 * (k & 1)], x[0], x[1]);
+                q8_to_f16<FMT>(w[2 * (k & 1) + 1], x[2], x[3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) S[nb][gr] = mfma_f16(u32x4{x[0], x[1], x[2], x[3]}, qop[nb][k], S[nb][gr]);
             }
-            if (k0 + kQ8Tile > lim_first) {
+        }
+        if (k0 + kQ8Tile > lim_first) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) S[gr][i] = k0 + 16 * gr + 4 * g + i < lim ? S[gr][i] : -INFINITY;
-                if (FMT == RQ_Q8_E4M3 && k0 + kQ8Tile > s.vis) {
-                    // what lies behind the context may be a NaN's code, and 0 * NaN is one
+                    for (int i = 0; i < 4; ++i) S[nb][gr][i] = k0 + 16 * gr + 4 * g + i < lim[nb] ? S[nb][gr][i] : -INFINITY;
+            if (FMT == RQ_Q8_E4M3 && k0 + kQ8Tile > s.vis) {
+                // what lies behind the context may be a NaN's code, and 0 * NaN is one
 #pragma unroll
-                    for (int gr = 0; gr < 2; ++gr) {
-                        const int left = min(4, max(0, s.vis - (k0 + 16 * gr + 4 * g)));
-                        const uint32_t keep = left == 4 ? ~0u : (1u << (8 * left)) - 1u;
+                for (int gr = 0; gr < 2; ++gr) {
+                    const int left = min(4, max(0, s.vis - (k0 + 16 * gr + 4 * g)));
+                    const uint32_t keep = left == 4 ? ~0u : (1u << (8 * left)) - 1u;
 #pragma unroll
-                        for (int j = 0; j < kChunks; ++j) cur.v[gr][j] &= u32x4{keep, keep, keep, keep};
-                    }
+                    for (int j = 0; j < kChunks; ++j) cur.v[gr][j] &= u32x4{keep, keep, keep, keep};
                 }
             }
-            int ev[2];
-            float f[2], tmax = -INFINITY;
+        }
+        u32x4 pw[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float f[2] = {colf[nb] * ks[0], colf[nb] * ks[1]};
+            float tmax = -INFINITY;
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
-                ev[gr] = q8_scale_exp(cur.vs[gr]);
-                f[gr] = colf * exp2i(q8_scale_exp(cur.ks[gr]));
-                const float m = fmaxf(fmaxf(S[gr][0], S[gr][1]), fmaxf(S[gr][2], S[gr][3]));
-                tmax = fmaxf(tmax, __builtin_fmaf(m, f[gr], (float)ev[gr]));
+                const f32x4 x = S[nb][gr];
+                tmax = fmaxf(tmax, __builtin_fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), f[gr], (float)ev[gr]));
             }
-            if (__any(tmax - M > 8.f)) {
-                const float m_new = fmaxf(M, rows_max(tmax));
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - m_new);
+            if (__any(tmax - M[nb] > 8.f)) {
+                const float m_new = fmaxf(M[nb], rows_max(tmax));
+                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M[nb] - m_new);
 #pragma unroll
-                for (int m = 0; m < kBlocks; ++m) acc[m] *= alpha;
-                l_run *= alpha;
-                M = m_new;
+                for (int m = 0; m < kBlocks; ++m) acc[nb][m] *= alpha;
+                l_run[nb] *= alpha;
+                M[nb] = m_new;
             }
-            const float bias = M == -INFINITY ? 0.f : -M;
-            u32x4 pw;
+            const float bias = M[nb] == -INFINITY ? 0.f : -M[nb];
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
                 const float add = bias + (float)ev[gr];
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[gr][i], f[gr], add));
-                pw[2 * gr] = pack_f16(w[0], w[1]);
-                pw[2 * gr + 1] = pack_f16(w[2], w[3]);
+                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[nb][gr][i], f[gr], add));
+                pw[nb][2 * gr] = pack_f16(w[0], w[1]);
+                pw[nb][2 * gr + 1] = pack_f16(w[2], w[3]);
                 // the sum of the weights before their rounding to fp16 (which has no bias)
-                l_run = __builtin_fmaf((w[0] + w[1]) + (w[2] + w[3]), exp2i(-ev[gr]), l_run);
+                l_run[nb] = __builtin_fmaf((w[0] + w[1]) + (w[2] + w[3]), exp2i(-ev[gr]), l_run[nb]);
             }
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t x[4];
-                    q8_to_f16<FMT>(cur.v[0][j][i], x[0], x[1]);
-                    q8_to_f16<FMT>(cur.v[1][j][i], x[2], x[3]);
-                    acc[4 * j + i] = mfma_f16(u32x4{x[0], x[1], x[2], x[3]}, pw, acc[4 * j + i]);
-                }
         }
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t x[4];
+                q8_to_f16<FMT>(cur.v[0][j][i], x[0], x[1]);
+                q8_to_f16<FMT>(cur.v[1][j][i], x[2], x[3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) acc[nb][4 * j + i] = mfma_f16(u32x4{x[0], x[1], x[2], x[3]}, pw[nb], acc[nb][4 * j + i]);
+            }
+    }
 
-        // the four waves' sums of this segment
-        l_run = rows_sum(l_run);
-        __syncthreads();  // (the previous segment's are read)
+    // the waves' sums
 #pragma unroll
-        for (int m = 0; m < kBlocks; ++m) *reinterpret_cast<f32x4 *>(&lds_acc[wave][col][16 * m + 4 * g]) = acc[m];
-        if (g == 0) lds_ml[wave][col] = make_float2(M, l_run);
+    for (int nb = 0; nb < NB; ++nb) {
+        const float l_col = rows_sum(l_run[nb]);
+        __syncthreads();  // (the sums before these are read)
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) *reinterpret_cast<f32x4 *>(&lds.acc[wave][col][16 * m + 4 * g]) = acc[nb][m];
+        if (g == 0) lds.ml[wave][col] = make_float2(M[nb], l_col);
         __syncthreads();
-        {
-            constexpr int kDims = D / 16;  // dims of a thread
-            const int c = tid >> 4, d0 = (tid & 15) * kDims;
-            float Mt = -INFINITY, l = 0.f, o[kDims] = {};
+        constexpr int kPer = 4 * W, kDims = D / kPer;  // threads of a column, dims of a thread
+        const int c = tid / kPer, d0 = tid % kPer * kDims;
+        const uint32_t cc = c0 + kQ8Cols * nb + c, i = cc / (uint32_t)a.G;
+        if ((int)i >= s.T) continue;
+        float Mt = -INFINITY, l = 0.f, o[kDims] = {};
 #pragma unroll
-            for (int w = 0; w < kQ8Waves; ++w) Mt = fmaxf(Mt, lds_ml[w][c].x);
+        for (int w = 0; w < W; ++w) Mt = fmaxf(Mt, lds.ml[w][c].x);
 #pragma unroll
-            for (int w = 0; w < kQ8Waves; ++w) {
-                const float2 ml = lds_ml[w][c];
-                const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
-                l += r * ml.y;
+        for (int w = 0; w < W; ++w) {
+            const float2 ml = lds.ml[w][c];
+            const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
+            l += r * ml.y;
 #pragma unroll
-                for (int k = 0; k < kDims; ++k) o[k] += r * lds_acc[w][c][d0 + k];
-            }
-            const int i = (c0 + c) / a.G;
-            if (t0 == 0 && t1 == n) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key: zeros
-                if (i < s.T) {
-                    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + (c0 + c) % a.G) * a.o_sh + d0;
-#pragma unroll
-                    for (int k = 0; k < kDims; k += 4)
-                        *reinterpret_cast<uint2 *>(row + k) = make_uint2(Elem<DT>::from_f32(o[k] * inv) | Elem<DT>::from_f32(o[k + 1] * inv) << 16,
-                                                                         Elem<DT>::from_f32(o[k + 2] * inv) | Elem<DT>::from_f32(o[k + 3] * inv) << 16);
-                }
-            } else {
-                // an item cut in two or more: the share that begins it ends with it, the others begin with it
-                float *pt = a.part + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * Q8Partial<D>::kFloats;
-#pragma unroll
-                for (int k = 0; k < kDims; k += 4) *reinterpret_cast<float4 *>(pt + c * D + d0 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                if ((tid & 15) == 0) *reinterpret_cast<float2 *>(pt + kQ8Cols * D + 2 * c) = make_float2(Mt, l);
-            }
+            for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][d0 + k];
         }
+        if (part == nullptr) {
+            uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + (int)i) * a.o_st + (int64_t)(h * a.G + (int)(cc - i * a.G)) * a.o_sh + d0;
+            q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);  // a row that sees no key: zeros
+        } else {
+            float *pt = part + nb * Q8Partial<D>::kFloats;
+#pragma unroll
+            for (int k = 0; k < kDims; k += 2) *reinterpret_cast<float2 *>(pt + c * D + d0 + k) = make_float2(o[k], o[k + 1]);
+            if (tid % kPer == 0) *reinterpret_cast<float2 *>(pt + kQ8Cols * D + 2 * c) = make_float2(Mt, l);
+        }
+    }
+}
+
+// Workgroups of a CU at once (by registers, 4 waves each).
+template <int D, int NB>
+constexpr int kQ8Resident = D == 64 ? (NB == 1 ? 4 : 3) : 2;
+
+// Equal shares of all items' tiles.
+template <int DT, int FMT, int D, int NB>
+__global__ __launch_bounds__(256, (kQ8Resident<D, NB>)) void q8_stream_kernel(Q8AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    __shared__ Q8Sums<D, 4> lds;
+    int64_t block = 0, block_base = 0;  // 64 sequences: their tiles, and the row's up to each
+    int64_t mine = q8_seq_tiles<NB>(a, lane), upto = wave_scan64(mine);
+    int64_t total = lane64(upto, 63);
+    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(q8_seq_tiles<NB>(a, b + lane)), 63);
+    const int64_t share = q8_share(total, gridDim.x);
+    int64_t pos = blockIdx.x * share;
+    const int64_t end = min(total, pos + share);
+    while (pos < end) {
+        uint64_t hit = __ballot(block_base + upto > pos);
+        while (hit == 0) {
+            block_base += lane64(upto, 63);
+            block += 64;
+            mine = q8_seq_tiles<NB>(a, block + lane);
+            upto = wave_scan64(mine);
+            hit = __ballot(block_base + upto > pos);
+        }
+        const int of = __builtin_ctzll(hit);
+        const int64_t seq = block + of, in_seq = pos - (block_base + lane64(upto, of) - lane64(mine, of));
+        const Q8Seq s = q8_seq(a, seq);
+        const int n = q8_tiles(s);
+        const int64_t item = div64(in_seq, n), block_of = div64(item, a.H);
+        const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
+        // an item cut in two or more: the share that begins it ends with it, the others begin with it
+        float *part = t0 == 0 && t1 == n ? nullptr : a.part + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * NB * Q8Partial<D>::kFloats;
+        q8_segment<DT, FMT, D, NB, 4>(a, seq, s, (int)(item - block_of * a.H), (int)block_of * (NB * kQ8Cols), t0, t1, part, lds);
         pos += t1 - t0;
     }
 }
 
-// Adds up the partials of the items that were cut: one workgroup per item, thread (column, part).
-template <int DT, int D>
+// Adds up the partials of the items that were cut: one workgroup per item and block of 16 columns.  A wave takes four
+// columns (lane: column % 4, part of D / 16 dims); with few columns, as decodes have, several waves share them
+// and take every second or fourth partial.  Two partials are in flight per wave.
+template <int DT, int D, int NB>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgroups) {
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int64_t b = blockIdx.y;
+    const int item = blockIdx.x / NB, nb = blockIdx.x % NB;
     const Q8Seq s = q8_seq(a, b);
-    if ((int64_t)blockIdx.x >= (int64_t)q8_col_blocks(a, s.T) * a.H) return;
+    const int h = item % a.H, c0 = (item / a.H) * (NB * kQ8Cols) + nb * kQ8Cols;
+    const int cols = min(kQ8Cols, s.T * a.G - c0);
+    if (cols <= 0) return;
     const int n = q8_tiles(s);
     int64_t total = 0, before = 0;
     for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
-        const int64_t mine = q8_seq_tiles(a, b0 + lane);
-        total += wave_sum64(mine);
-        before += wave_sum64(b0 + lane < b ? mine : 0);
+        const int64_t mine = q8_seq_tiles<NB>(a, b0 + lane), upto = wave_scan64(mine);
+        if (b >= b0 && b < b0 + 64) before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
+        total += lane64(upto, 63);
     }
     const int64_t share = q8_share(total, workgroups);
-    const int64_t first = before + (int64_t)blockIdx.x * n;
-    const int64_t w0 = first / share, w1 = (first + n - 1) / share;
+    const int64_t first = before + (int64_t)item * n;
+    const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
     if (w0 == w1) return;
     constexpr int kDims = D / 16;
-    const int h = blockIdx.x % a.H, c0 = (blockIdx.x / a.H) * kQ8Cols;
-    const int c = tid >> 4, d0 = (tid & 15) * kDims;
-    float M = -INFINITY, l = 0.f, o[kDims] = {};
-    for (int64_t w = w0; w <= w1; ++w) {
-        const float *pt = a.part + (2 * w + (w == w0 ? 1 : 0)) * Q8Partial<D>::kFloats;
-        const float2 ml = *reinterpret_cast<const float2 *>(pt + kQ8Cols * D + 2 * c);
-        const float Mn = fmaxf(M, ml.x);
-        const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
-        const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mn);
-        M = Mn;
-        l = l * keep + r * ml.y;
+    __shared__ Q8Sums<D, 4> lds;
+    const int quads = cols > 8 ? 4 : cols > 4 ? 2 : 1, ways = 4 / quads;  // column quads, waves of each
+    const int way = wave / quads, d0 = (lane & 15) * kDims;
+    {
+        const int c = 4 * (wave % quads) + (lane >> 4), cv = min(c, cols - 1);
+        float M = -INFINITY, l = 0.f, o[kDims] = {};
+        for (int w = w0 + way; w <= w1; w += 2 * ways) {
+            float2 ml[2];
+            float4 x[2][kDims / 4];
 #pragma unroll
-        for (int k = 0; k < kDims; k += 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(pt + c * D + d0 + k);
-            o[k] = o[k] * keep + r * x.x, o[k + 1] = o[k + 1] * keep + r * x.y;
-            o[k + 2] = o[k + 2] * keep + r * x.z, o[k + 3] = o[k + 3] * keep + r * x.w;
+            for (int u = 0; u < 2; ++u) {
+                const int wu = min(w + ways * u, w1);
+                const float *pt = a.part + ((2 * (int64_t)wu + (wu == w0 ? 1 : 0)) * NB + nb) * Q8Partial<D>::kFloats;
+                ml[u] = *reinterpret_cast<const float2 *>(pt + kQ8Cols * D + 2 * cv);
+#pragma unroll
+                for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + cv * D + d0 + 4 * k);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (w + ways * u > w1) continue;
+                const float Mn = fmaxf(M, ml[u].x);
+                const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+                const float r = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - Mn);
+                M = Mn;
+                l = l * keep + r * ml[u].y;
+#pragma unroll
+                for (int k = 0; k < kDims / 4; ++k) {
+                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
+                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+                }
+            }
         }
+#pragma unroll
+        for (int k = 0; k < kDims; k += 4) *reinterpret_cast<float4 *>(&lds.acc[way][c][d0 + k]) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        if ((lane & 15) == 0) lds.ml[way][c] = make_float2(M, l);
+    }
+    __syncthreads();
+    const int c = tid >> 4;
+    if (c >= cols) return;
+    float Mt = -INFINITY, l = 0.f, o[kDims] = {};
+    for (int w = 0; w < ways; ++w) Mt = fmaxf(Mt, lds.ml[w][c].x);
+    for (int w = 0; w < ways; ++w) {
+        const float2 ml = lds.ml[w][c];
+        const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
+        l += r * ml.y;
+#pragma unroll
+        for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][(tid & 15) * kDims + k];
     }
     const int i = (c0 + c) / a.G;
-    if (i >= s.T) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + (c0 + c) % a.G) * a.o_sh + d0;
-#pragma unroll
-    for (int k = 0; k < kDims; k += 4)
-        *reinterpret_cast<uint2 *>(row + k) = make_uint2(Elem<DT>::from_f32(o[k] * inv) | Elem<DT>::from_f32(o[k + 1] * inv) << 16,
-                                                         Elem<DT>::from_f32(o[k + 2] * inv) | Elem<DT>::from_f32(o[k + 3] * inv) << 16);
+    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + (c0 + c) % a.G) * a.o_sh + (tid & 15) * kDims;
+    q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);
 }
 
-// Workgroups of the stream kernel: what the GPU holds at once, or fewer where the bound on the lengths gives less work.
-static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int64_t max_q_len, int64_t max_keys) {
-    const int64_t tiles = std::max<int64_t>(1, (max_keys + kQ8Tile - 1) / kQ8Tile), cols = (max_q_len * G + kQ8Cols - 1) / kQ8Cols;
-    const int64_t work = num_seqs * cols * H * tiles;
-    return std::max<int64_t>(1, std::min<int64_t>(3 * (int64_t)device_cus(), (work + kQ8MinChunk - 1) / kQ8MinChunk));
+// One workgroup of 8 waves per item: one launch, no partials.
+template <int DT, int FMT, int D, int NB>
+__global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
+    __shared__ Q8Sums<D, 8> lds;
+    const int64_t seq = blockIdx.y;
+    const Q8Seq s = q8_seq(a, seq);
+    const int block = blockIdx.x / (uint32_t)a.H, h = blockIdx.x - block * a.H;
+    if (block >= q8_col_blocks<NB>(a, s.T)) return;
+    q8_segment<DT, FMT, D, NB, 8>(a, seq, s, h, block * (NB * kQ8Cols), 0, q8_tiles(s), nullptr, lds);
 }
 
-template <int DT, int FMT, int D>
+// Blocks of 16 columns that a workgroup takes, and the workgroups: what the GPU holds at once, or fewer where the bound on the lengths
+// gives less work.
+static int q8_blocks(int G, int64_t max_q_len) { return max_q_len * G > kQ8Cols ? 2 : 1; }
+static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
+    const int nb = q8_blocks(G, max_q_len), cols = nb * kQ8Cols;
+    const int resident = D == 128 ? (nb == 1 ? kQ8Resident<128, 1> : kQ8Resident<128, 2>) : (nb == 1 ? kQ8Resident<64, 1> : kQ8Resident<64, 2>);
+    const int64_t tiles = std::max<int64_t>(1, (max_keys + kQ8Tile - 1) / kQ8Tile);
+    const int64_t work = num_seqs * ((max_q_len * G + cols - 1) / cols) * H * tiles;
+    return std::max<int64_t>(1, std::min<int64_t>(resident * (int64_t)device_cus(), (work + kQ8MinChunk - 1) / kQ8MinChunk));
+}
+
+// Calls of short contexts, by the bound on their lengths, take a workgroup per item.
+constexpr int64_t kQ8ItemTiles = 60;
+static bool q8_is_short(int64_t max_keys) {
+    return max_keys <= kQ8ItemTiles * kQ8Tile;
+}
+
+template <int DT, int FMT, int D, int NB>
 static void launch_stream(const Q8AttnArgs &a, int64_t workgroups, hipStream_t st) {
-    hipLaunchKernelGGL((q8_stream_kernel<DT, FMT, D>), dim3((unsigned)workgroups), dim3(64 * kQ8Waves), 0, st, a);
-    const int64_t items = (int64_t)((int64_t)a.max_q * a.G + kQ8Cols - 1) / kQ8Cols * a.H;
-    hipLaunchKernelGGL((q8_merge_kernel<DT, D>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)workgroups);
+    if (q8_is_short(a.cap)) {
+        const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
+        hipLaunchKernelGGL((q8_item_kernel<DT, FMT, D, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(512), 0, st, a);
+        return;
+    }
+    hipLaunchKernelGGL((q8_stream_kernel<DT, FMT, D, NB>), dim3((unsigned)workgroups), dim3(256), 0, st, a);
+    const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
+    hipLaunchKernelGGL((q8_merge_kernel<DT, D, NB>), dim3((unsigned)(items * NB), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)workgroups);
+}
+template <int DT, int FMT, int D>
+static void launch_stream_b(const Q8AttnArgs &a, int64_t wgs, hipStream_t st) {
+    q8_blocks(a.G, a.max_q) == 1 ? launch_stream<DT, FMT, D, 1>(a, wgs, st) : launch_stream<DT, FMT, D, 2>(a, wgs, st);
 }
 template <int DT, int FMT>
 static void launch_stream_d(const Q8AttnArgs &a, int D, int64_t wgs, hipStream_t st) {
-    D == 128 ? launch_stream<DT, FMT, 128>(a, wgs, st) : launch_stream<DT, FMT, 64>(a, wgs, st);
+    D == 128 ? launch_stream_b<DT, FMT, 128>(a, wgs, st) : launch_stream_b<DT, FMT, 64>(a, wgs, st);
 }
 template <int DT>
 static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hipStream_t st) {
@@ -386,8 +482,8 @@ extern "C" int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num
     if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_q_len <= 0 || max_seq_len < 0) return 0;
     const int G = num_q_heads / num_kv_heads;
     if (q8_is_prompt(max_q_len, G)) return q8_prefill_workspace(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
-    const int64_t wgs = q8_workgroups(num_seqs, G, num_kv_heads, max_q_len, max_seq_len);
-    return 2 * wgs * kQ8Cols * (head_dim + 2) * 4;
+    const int64_t wgs = q8_workgroups(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
+    return 2 * wgs * q8_blocks(G, max_q_len) * kQ8Cols * (head_dim + 2) * 4;
 }
 
 extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads,
@@ -434,7 +530,7 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     a.part = static_cast<float *>(workspace);
     hipStream_t st = (hipStream_t)stream;
     if (q8_is_prompt(a.max_q, a.G)) return q8_prefill(a, dtype, format, head_dim, workspace, st);
-    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, a.max_q, a.cap);
+    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, head_dim, a.max_q, a.cap);
     if (dtype == RQ_DTYPE_BF16) launch_stream_f<RQ_DTYPE_BF16>(a, format, head_dim, wgs, st);
     else launch_stream_f<RQ_DTYPE_F16>(a, format, head_dim, wgs, st);
     return check_launch("q8_stream_kernel");

@@ -23,9 +23,11 @@ struct Q8StoreArgs {
     uint8_t *cache;
     int64_t num_slots, stride_block;
     int H, groups, block_size;  // groups of a page
+    int per_wave;  // units of a wave
     // calls of many tokens: per group of the cache the last run of tokens linked to it, per token the
-    // run linked before its own (-1: none), and the first run's token of each group written
-    int32_t *last, *before, *list, *count;
+    // run linked before its own (-1: none), and of each group written the token linked first and the group
+    int32_t *last, *before, *count;
+    int2 *list;
 };
 
 constexpr int kStoreWaves = 4;
@@ -38,8 +40,8 @@ __device__ __forceinline__ int64_t q8_group_of(const Q8StoreArgs &a, int64_t t) 
 
 // ---- which tokens a group gets ------------------------------------------------
 // Tokens come as runs: consecutive ones of the same group (one run per group in any call that a
-// server makes).  Few tokens: every unit looks at all of them (below).  Many: two launches first link the
-// runs of each group, and list the groups, each by the token of the run that was linked first.
+// server makes).  Few tokens: every wave looks at all of them (below).  Many: two launches first link the
+// runs of each group, and list the groups, each with the token of the run that was linked first.
 __device__ __forceinline__ int64_t q8_run_start(const Q8StoreArgs &a, int64_t t) {
     const int64_t g = q8_group_of(a, t);
     return g >= 0 && (t == 0 || q8_group_of(a, t - 1) != g) ? g : -1;
@@ -58,17 +60,26 @@ __global__ __launch_bounds__(256) void q8_link_kernel(Q8StoreArgs a) {
     if (g < 0) return;
     const int32_t p = atomicExch(a.last + g, (int32_t)t);
     a.before[t] = p;
-    if (p < 0) a.list[atomicAdd(a.count, 1)] = (int32_t)t;
+    if (p < 0) a.list[atomicAdd(a.count, 1)] = make_int2((int)t, (int)g);
 }
 
-// rows[r] = the last token that writes row r of group g, -1 for none.  LINKED: from the group's runs.
-// Otherwise from all tokens; false if a token before t0 is of the same group (its unit does the work).
+// rows[r] = the last token that writes row r of group g, -1 for none.  LINKED: t0 is the token of the group's list entry.  Otherwise
+// from all tokens; false if one before t0 is of the same group (its wave does the work).
 template <bool LINKED>
 __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, int64_t g, int *rows, int lane) {
     if (lane < kQ8Group) rows[lane] = -1;
     __builtin_amdgcn_wave_barrier();
     if constexpr (LINKED) {
-        for (int64_t r = a.last[g]; r >= 0; r = a.before[r]) {
+        const int64_t s0 = t0 + lane < a.n_tokens ? a.slots[t0 + lane] : -1;
+        int64_t r = a.last[g];
+        if (r == t0) {  // the only run (its slots are loaded beside the link); of 64 tokens or more: below
+            const uint64_t out = ~__ballot(s0 >= 0 && s0 >> 4 == g);
+            if (out) {
+                if (lane < __builtin_ctzll(out)) atomicMax(rows + (s0 & 15), (int)(t0 + lane));
+                r = -1;
+            }
+        }
+        for (; r >= 0; r = a.before[r]) {
             for (int64_t s = r;; s += 64) {  // the run: up to the first token of another group
                 const bool in = s + lane < a.n_tokens && q8_group_of(a, s + lane) == g;
                 const uint64_t out = ~__ballot(in);
@@ -96,22 +107,32 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
     return true;
 }
 
-// Eight elements (16-byte aligned) as fp32.
+// Eight elements (16-byte aligned), as loaded and as fp32.
 template <int DT>
-__device__ __forceinline__ void q8_load8(const void *p, int64_t at, float (&x)[8]) {
-    if constexpr (DT == RQ_DTYPE_F32) {
-        const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
-        const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at + 4);
-        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-    } else {
-        const q8_u32x4 u = *reinterpret_cast<const q8_u32x4 *>(static_cast<const uint16_t *>(p) + at);
+struct Q8Raw {
+    q8_u32x4 w[DT == RQ_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Q8Raw<DT> q8_load8(const void *p, int64_t at) {
+    Q8Raw<DT> r;
+    const q8_u32x4 *q = reinterpret_cast<const q8_u32x4 *>(static_cast<const uint8_t *>(p) + at * (DT == RQ_DTYPE_F32 ? 4 : 2));
+    r.w[0] = __builtin_nontemporal_load(q);
+    if constexpr (DT == RQ_DTYPE_F32) r.w[1] = __builtin_nontemporal_load(q + 1);
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void q8_floats(const Q8Raw<DT> &r, float (&x)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = Elem<DT>::to_f32((u[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (DT == RQ_DTYPE_F32) x[i] = __uint_as_float(r.w[i >> 2][i & 3]);
+        else x[i] = Elem<DT>::to_f32((r.w[0][i >> 1] >> (16 * (i & 1))) & 0xffffu);
     }
 }
 
-// One unit per wave.  Lane: token row t = lane % 16, half = (lane / 16) % 2 of the 16-dim parts; the wave's
-// upper 32 lanes are the second 64-dim chunk (D = 128) or the V side (D = 64).
+// A wave takes a.per_wave units of one group, the next one's rows on their way while one is coded.  Lane: token row
+// t = lane % 16, half = (lane / 16) % 2 of the 16-dim parts; the wave's upper 32 lanes are the second 64-dim chunk
+// (D = 128) or the V side (D = 64).
+// Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in STORE_US.
 template <int DT, int FMT, int D, bool LINKED>
 __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a) {
     constexpr int kUnits = D == 128 ? 2 : 1;  // units per head
@@ -119,102 +140,118 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int *const rows = rows_of[wave];
     const int t = lane & 15, half = (lane >> 4) & 1, q = t & 3;
-    const uint32_t per = kUnits * a.H;
+    const int units = kUnits * a.H, waves = (units + a.per_wave - 1) / a.per_wave;  // of a group
     const int64_t entries = LINKED ? *a.count : a.n_tokens;
-    for (int64_t unit = (int64_t)blockIdx.x * kStoreWaves + wave; unit < entries * per; unit += (int64_t)gridDim.x * kStoreWaves) {
-        const int64_t entry = unit / per;
-        const int of_entry = (int)(unit - entry * per), h = of_entry / kUnits;
-        const int side = D == 128 ? of_entry & 1 : lane >> 5, chunk = D == 128 ? lane >> 5 : 0;
-        const int64_t t0 = LINKED ? a.list[entry] : entry;
-        const int64_t g = q8_group_of(a, t0);
-        if (g < 0 || (!LINKED && t0 > 0 && q8_group_of(a, t0 - 1) == g)) continue;
+    const Q8Layout lay(a.H, D, a.block_size);
+    for (int64_t item = (int64_t)blockIdx.x * kStoreWaves + wave; item < entries * waves; item += (int64_t)gridDim.x * kStoreWaves) {
+        const uint32_t entry = (uint32_t)item / (uint32_t)waves;
+        const int first = (int)((uint32_t)item - entry * waves) * a.per_wave, end = min(units, first + a.per_wave);
+        int64_t t0 = entry, g;
+        if constexpr (LINKED) {
+            const int2 e = a.list[entry];
+            t0 = e.x, g = e.y;
+        } else {
+            g = q8_group_of(a, t0);
+            if (g < 0 || (t0 > 0 && q8_group_of(a, t0 - 1) == g)) continue;
+        }
         if (!q8_find_rows<LINKED>(a, t0, g, rows, lane)) continue;
         const int tok = rows[t];
         const bool anew = rows[0] >= 0;
-        const bool quad_hit = (__ballot(tok >= 0) >> (lane & 60)) & 15;  // four tokens share their V dwords
+        const uint64_t written = __ballot(tok >= 0);
+        const bool quad_hit = (written >> (lane & 60)) & 15;  // four tokens share their V dwords
         const uint32_t page = (uint32_t)g / (uint32_t)a.groups, gi = (uint32_t)g - page * a.groups;
-        const Q8Layout lay(a.H, D, a.block_size);
         uint8_t *const base = a.cache + (int64_t)page * a.stride_block;
-        uint8_t *const tile = base + lay.codes_at(gi, h) + side * (kQ8Group * D) + chunk * 1024;
-        float *const scale = reinterpret_cast<float *>(base + lay.scale_at(gi, h)) + side;
-        const float old_scale = *scale;
 
-        float x[4][8];  // dims 64 chunk + 16 i + 8 half + ...
-        uint32_t big = 0;
-        const void *src = side ? a.value : a.key;
-        const int64_t at = (int64_t)max(tok, 0) * (side ? a.v_st : a.k_st) + (int64_t)h * (side ? a.v_sh : a.k_sh) + 64 * chunk + 8 * half;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (tok >= 0) {
-                q8_load8<DT>(src, at + 16 * i, x[i]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[i][k] = 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t b = __float_as_uint(x[i][k]) & 0x7fffffffu;
-                big = max(big, b < 0x7f800000u ? b : 0u);  // infinities and NaN do not set the scale
-            }
-        }
-#pragma unroll
-        for (int o = D == 128 ? 32 : 16; o >= 1; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
-        const bool begun = !anew && old_scale != 0.f;  // the rows not written keep their tokens
-        const int e_old = q8_scale_exp(old_scale), e_new = max(q8_exponent<FMT>(big), begun ? e_old : kQ8MinExp);
-        const bool moved = !begun || e_new != e_old;   // every row is written
-        const float inv = exp2i(-e_new);
-        uint32_t c[4][2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float lo[4] = {x[i][0], x[i][1], x[i][2], x[i][3]}, hi[4] = {x[i][4], x[i][5], x[i][6], x[i][7]};
-            c[i][0] = q8_encode4<FMT>(lo, inv);
-            c[i][1] = q8_encode4<FMT>(hi, inv);
-        }
-        uint8_t *const krow = tile + 16 * t + 8 * half;              // + 256 i: dims 16 i + 8 half ..
-        uint8_t *const vrow = tile + 256 * (t >> 2) + 16 * (8 * half + q);  // + 64 k: dim 8 half + 4 k + q of four parts
-        if (begun && __any(tok < 0)) {
-            // codes of the rows that stay, in this lane's order, moved to the new scale
-            uint32_t old[4][2];
-            if (side == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const q8_u32x2 w = *reinterpret_cast<const q8_u32x2 *>(krow + 256 * i);
-                    old[i][0] = w[0], old[i][1] = w[1];
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const q8_u32x4 w = *reinterpret_cast<const q8_u32x4 *>(vrow + 64 * k);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) old[i][k] = quad_transpose(w[i], q);
-                }
-            }
-            const float shift = exp2i(e_old - e_new);
+        auto side_of = [&](int unit) { return D == 128 ? unit & 1 : lane >> 5; };
+        const int chunk = D == 128 ? lane >> 5 : 0;
+        Q8Raw<DT> raw[4];
+        float old_next;
+        auto scale_at = [&](int unit) { return reinterpret_cast<float *>(base + lay.scale_at(gi, unit / kUnits)) + side_of(unit); };
+        auto load = [&](int unit) {  // dims 64 chunk + 16 i + 8 half .. of this lane's row
+            const int h = unit / kUnits, side = side_of(unit);
+            old_next = *scale_at(unit);
+            const int64_t at = (int64_t)tok * (side ? a.v_st : a.k_st) + (int64_t)h * (side ? a.v_sh : a.k_sh) + 64 * chunk + 8 * half;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
+                if (tok >= 0) raw[i] = q8_load8<DT>(side ? a.value : a.key, at + 16 * i);
+        };
+        load(first);
+        for (int unit = first; unit < end; ++unit) {
+            const int h = unit / kUnits, side = side_of(unit);
+            uint8_t *const tile = base + lay.codes_at(gi, h) + side * (kQ8Group * D) + chunk * 1024;
+            const float old_scale = old_next;
+            float x[4][8];
+            uint32_t big = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q8_floats<DT>(raw[i], x[i]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (tok < 0) x[i][k] = 0.f;
+                    const uint32_t b = __float_as_uint(x[i][k]) & 0x7fffffffu;
+                    big = max(big, b < 0x7f800000u ? b : 0u);  // infinities and NaN do not set the scale
+                }
+            }
+            if (unit + 1 < end) load(unit + 1);
+#pragma unroll
+            for (int o = D == 128 ? 32 : 16; o >= 1; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
+            const bool begun = !anew && old_scale != 0.f;  // the rows not written keep their tokens
+            const int e_old = q8_scale_exp(old_scale), e_new = max(q8_exponent<FMT>(big), begun ? e_old : kQ8MinExp);
+            const bool moved = !begun || e_new != e_old;   // every row is written
+            const float inv = exp2i(-e_new);
+            uint32_t c[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float lo[4] = {x[i][0], x[i][1], x[i][2], x[i][3]}, hi[4] = {x[i][4], x[i][5], x[i][6], x[i][7]};
+                c[i][0] = q8_encode4<FMT>(lo, inv);
+                c[i][1] = q8_encode4<FMT>(hi, inv);
+            }
+            uint8_t *const krow = tile + 16 * t + 8 * half;                     // + 256 i: dims 16 i + 8 half ..
+            uint8_t *const vrow = tile + 256 * (t >> 2) + 16 * (8 * half + q);  // + 64 k: dim 8 half + 4 k + q of four parts
+            if ((uint32_t)(written & 0xffff) != 0xffffu && __any(begun)) {
+                // codes of the rows that stay, in this lane's order, moved to the new scale
+                uint32_t old[4][2];
+                if (side == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const q8_u32x2 w = *reinterpret_cast<const q8_u32x2 *>(krow + 256 * i);
+                        old[i][0] = w[0], old[i][1] = w[1];
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const q8_u32x4 w = *reinterpret_cast<const q8_u32x4 *>(vrow + 64 * k);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) old[i][k] = quad_transpose(w[i], q);
+                    }
+                }
+                const float shift = exp2i(e_old - e_new);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (tok >= 0 || !begun) continue;
+                        float y[4];
+                        q8_decode4<FMT>(old[i][k], y);
+                        c[i][k] = moved ? q8_encode4<FMT>(y, shift) : old[i][k];
+                    }
+            }
+            if (side == 0) {
+                if (tok >= 0 || moved) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<q8_u32x2 *>(krow + 256 * i) = q8_u32x2{c[i][0], c[i][1]};
+                }
+            } else {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    if (tok >= 0) continue;
-                    float y[4];
-                    q8_decode4<FMT>(old[i][k], y);
-                    c[i][k] = moved ? q8_encode4<FMT>(y, shift) : old[i][k];
+                    q8_u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = quad_transpose(c[i][k], q);
+                    if (moved || quad_hit) *reinterpret_cast<q8_u32x4 *>(vrow + 64 * k) = w;
                 }
-        }
-        if (side == 0) {
-            if (tok >= 0 || moved) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *reinterpret_cast<q8_u32x2 *>(krow + 256 * i) = q8_u32x2{c[i][0], c[i][1]};
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                q8_u32x4 w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = quad_transpose(c[i][k], q);
-                if (moved || quad_hit) *reinterpret_cast<q8_u32x4 *>(vrow + 64 * k) = w;
-            }
+            if (t == 0 && half == 0 && chunk == 0) *scale_at(unit) = exp2i(e_new);
         }
-        if (t == 0 && half == 0 && chunk == 0) *scale = exp2i(e_new);
     }
 }
 
@@ -227,6 +264,7 @@ struct Q8ReadArgs {
     int64_t max_blocks, bt_ss;
     const int32_t *seq_lens, *starts;
     int64_t num_seqs, total;
+    int per_wave;  // heads of a wave
     void *out_k, *out_v;
 };
 
@@ -237,26 +275,43 @@ constexpr int kReadWaves = 4;
 // the numbers need no prefix sum over the lengths; those in between stay idle.
 __device__ __forceinline__ int64_t q8_first_unit(const Q8ReadArgs &a, int64_t b) { return (int64_t)(a.starts[b] >> 4) + b; }
 
-// Stores n (2 or 4) consecutive elements.
-template <int DT>
-__device__ __forceinline__ void q8_put4(void *p, int64_t at, const float (&x)[4]) {
+// Eight codes (two dwords) times scale as eight consecutive elements.
+template <int DT, int FMT>
+__device__ __forceinline__ void q8_put8(void *p, int64_t at, uint32_t w0, uint32_t w1, float scale) {
+    float x[8], lo[4], hi[4];
+    q8_decode4<FMT>(w0, lo);
+    q8_decode4<FMT>(w1, hi);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = lo[k] * scale, x[4 + k] = hi[k] * scale;
     if constexpr (DT == RQ_DTYPE_F32) {
-        *reinterpret_cast<float4 *>(static_cast<float *>(p) + at) = make_float4(x[0], x[1], x[2], x[3]);
+        float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
+        q[0] = make_float4(x[0], x[1], x[2], x[3]);
+        q[1] = make_float4(x[4], x[5], x[6], x[7]);
     } else {
-        const uint32_t lo = Elem<DT>::from_f32(x[0]) | Elem<DT>::from_f32(x[1]) << 16;
-        const uint32_t hi = Elem<DT>::from_f32(x[2]) | Elem<DT>::from_f32(x[3]) << 16;
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = make_uint2(lo, hi);
+        q8_u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(x[2 * k]) | Elem<DT>::from_f32(x[2 * k + 1]) << 16;
+        *reinterpret_cast<q8_u32x4 *>(static_cast<uint16_t *>(p) + at) = w;
     }
 }
+// The value of lane l ^ 4.
+__device__ __forceinline__ uint32_t lane_xor4(uint32_t x) {
+    const int from_above = __builtin_amdgcn_update_dpp(0, (int)x, 0x104, 0xf, 0x5, false);             // lanes with bit 2 clear: row_shl 4
+    return (uint32_t)__builtin_amdgcn_update_dpp(from_above, (int)x, 0x114, 0xf, 0xa, false);          // the others: row_shr 4
+}
 
-// One wave per (group of a sequence, head).
+// One wave per (group of a sequence, a.per_wave heads), the next head's codes on their way while one is written.  Codes change
+// lanes (and bytes of V, quads) so that every store is 16 bytes a lane (8 elements of 16 bits) and four lanes' are 64
+// consecutive bytes of a row.
+// Bound by memory: 32768 tokens of 8 heads (67 MB in, 134 out) in READ_US.
 template <int DT, int FMT, int D>
 __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) {
     constexpr int kChunks = D / 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * kReadWaves + wave;
-    const int64_t unit = item / a.H;
-    const int h = (int)(item - unit * a.H);
+    const int64_t item = (int64_t)blockIdx.x * kReadWaves + wave;  // (fits 32 bits)
+    const int waves = (a.H + a.per_wave - 1) / a.per_wave;  // of a group
+    const uint32_t unit = (uint32_t)item / (uint32_t)waves;
+    const int h0 = (int)((uint32_t)item - unit * waves) * a.per_wave, h1 = min(a.H, h0 + a.per_wave);
     // the last sequence whose first unit is not past this one, 64 at a time
     int64_t lo = 0, n = a.num_seqs;
     while (n > 1) {
@@ -267,48 +322,76 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
         n = min(step, lo + n - next);
         lo = next;
     }
-    const int64_t first = q8_first_unit(a, lo);
-    const int64_t i = unit - first;
-    const int row0 = a.starts[lo];
+    const int64_t i = unit - q8_first_unit(a, lo);
     const int64_t len = min((int64_t)a.seq_lens[lo], a.max_blocks * a.block_size);
     if (i < 0 || i * kQ8Group >= len) return;
     const int rows = (int)min((int64_t)kQ8Group, len - i * kQ8Group);
-    const int64_t out0 = row0 + i * kQ8Group;
+    const int64_t out0 = a.starts[lo] + i * kQ8Group;
     const uint32_t slot_page = (uint32_t)i / (uint32_t)a.groups, gi = (uint32_t)i - slot_page * a.groups;
     int64_t page = a.bt[lo * a.bt_ss + slot_page];
     page = page < 0 || page >= a.num_blocks ? 0 : page;
     const Q8Layout lay(a.H, D, a.block_size);
     const uint8_t *const base = a.cache + page * a.stride_block;
-    const uint8_t *const tile = base + lay.codes_at(gi, h) + 16 * lane;
     q8_u32x4 kw[kChunks], vw[kChunks];
+    float2 s;
+    auto load = [&](int h) {
+        const uint8_t *const tile = base + lay.codes_at(gi, h) + 16 * lane;
+        s = *reinterpret_cast<const float2 *>(base + lay.scale_at(gi, h));
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-        kw[j] = *reinterpret_cast<const q8_u32x4 *>(tile + 1024 * j);
-        vw[j] = *reinterpret_cast<const q8_u32x4 *>(tile + kQ8Group * D + 1024 * j);
-    }
-    const float2 s = *reinterpret_cast<const float2 *>(base + lay.scale_at(gi, h));
-    const int g = lane >> 4, c = lane & 15, q = lane & 3;
-    auto put = [&](void *out, int row, int dim, uint32_t w, float scale) {
-        if (row >= rows || out0 + row < 0 || out0 + row >= a.total) return;
-        float x[4];
-        q8_decode4<FMT>(w, x);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] *= scale;
-        q8_put4<DT>(out, ((out0 + row) * a.H + h) * D + dim, x);
-    };
-#pragma unroll
-    for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            put(a.out_k, c, 64 * j + 16 * g + 4 * k, kw[j][k], s.x);
-            // V: part k of this lane's dim, four tokens -> token 4 g + q, four dims
-            put(a.out_v, 4 * g + q, 64 * j + 16 * k + (c & 12), quad_transpose(vw[j][k], q), s.y);
+        for (int j = 0; j < kChunks; ++j) {
+            kw[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + 1024 * j));
+            vw[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + kQ8Group * D + 1024 * j));
         }
+    };
+    const int g = lane >> 4, c = lane & 15, q = lane & 3;
+    const bool upper = lane & 4;
+    auto inside = [&](int row) { return row < rows && out0 + row >= 0 && out0 + row < a.total; };
+    const bool k_in = inside(c), v_in = inside(4 * g + q);
+    const int64_t k_row = (out0 + c) * a.H * D, v_row = (out0 + 4 * g + q) * a.H * D;
+    load(h0);
+    for (int h = h0; h < h1; ++h) {
+        q8_u32x4 kc[kChunks], vc[kChunks];
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) kc[j] = kw[j], vc[j] = vw[j];
+        const float2 sc = s;
+        if (h + 1 < h1) load(h + 1);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            // K: lane group g has dims 16 g .. + 15 of token c -> dims 8 g .. + 7 and 32 + 8 g .. + 7
+            uint32_t p[2][2];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                auto x = __builtin_amdgcn_permlane16_swap(kc[j][d], kc[j][2 + d], false, false);
+                auto y = __builtin_amdgcn_permlane32_swap(x[0], x[1], false, false);
+                p[0][d] = y[0], p[1][d] = y[1];
+            }
+            if (k_in) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) q8_put8<DT, FMT>(a.out_k, k_row + h * D + 64 * j + 32 * u + 8 * g, p[u][0], p[u][1], sc.x);
+            }
+            // V: four tokens of dim 16 k + c -> dims 16 k + (c & 12) .. + 3 of token 4 g + q -> 8 dims, of part k or k + 1
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                const uint32_t w0 = quad_transpose(vc[j][k], q), w1 = quad_transpose(vc[j][k + 1], q);
+                const uint32_t other = lane_xor4(upper ? w0 : w1);
+                if (v_in)
+                    q8_put8<DT, FMT>(a.out_v, v_row + h * D + 64 * j + 16 * (k + (upper ? 1 : 0)) + (c & 8), upper ? other : w0, upper ? w1 : other, sc.y);
+            }
+        }
+    }
+}
+
+// Units of a wave: one, for the least latency, until the calls' waves are more than the GPU holds (about 24 a CU).
+static int q8_per_wave(int64_t groups, int units) {
+    const int64_t waves = groups * units, room = 24 * (int64_t)device_cus();
+    return (int)std::min<int64_t>(4, std::max<int64_t>(1, waves / room));
 }
 
 template <int DT, int FMT, int D>
-static void launch_store(const Q8StoreArgs &a, bool linked, hipStream_t st) {
-    const int64_t per = (D == 128 ? 2 : 1) * (int64_t)a.H, blocks = (a.n_tokens * per + kStoreWaves - 1) / kStoreWaves;
+static void launch_store(Q8StoreArgs a, bool linked, hipStream_t st) {
+    const int units = (D == 128 ? 2 : 1) * a.H;
+    a.per_wave = linked ? q8_per_wave(a.n_tokens / kQ8Group, units) : 1;
+    const int64_t blocks = (a.n_tokens * ((units + a.per_wave - 1) / a.per_wave) + kStoreWaves - 1) / kStoreWaves;
     if (linked) {
         const unsigned tb = (unsigned)((a.n_tokens + 255) / 256);
         hipLaunchKernelGGL(q8_unlink_kernel, dim3(tb), dim3(256), 0, st, a);
@@ -329,8 +412,10 @@ static void launch_store_f(const Q8StoreArgs &a, int fmt, int D, bool linked, hi
 }
 
 template <int DT, int FMT>
-static void launch_read_d(const Q8ReadArgs &a, int D, hipStream_t st) {
-    const int64_t items = (a.total / kQ8Group + a.num_seqs) * a.H;
+static void launch_read_d(Q8ReadArgs a, int D, hipStream_t st) {
+    const int64_t groups = a.total / kQ8Group + a.num_seqs;
+    a.per_wave = q8_per_wave(groups, a.H);
+    const int64_t items = groups * ((a.H + a.per_wave - 1) / a.per_wave);
     const dim3 grid((unsigned)((items + kReadWaves - 1) / kReadWaves)), block(64 * kReadWaves);
     if (D == 128) hipLaunchKernelGGL((q8_read_kernel<DT, FMT, 128>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((q8_read_kernel<DT, FMT, 64>), grid, block, 0, st, a);
@@ -354,7 +439,7 @@ extern "C" int rq_q8_slot_bytes(int32_t num_kv_heads, int32_t head_dim) {
 
 extern "C" int64_t rq_q8_store_workspace_bytes(int64_t n_tokens, int64_t num_blocks, int32_t block_size) {
     if (n_tokens <= kStoreScan || num_blocks <= 0 || block_size <= 0) return 0;
-    return (num_blocks * (block_size / kQ8Group) + 2 * n_tokens + 4) * 4;
+    return (num_blocks * (block_size / kQ8Group) + 3 * n_tokens + 4) * 4;
 }
 
 extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
@@ -365,7 +450,7 @@ extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, in
     RQ_CHECK_ARG(dtype == RQ_DTYPE_F16 || dtype == RQ_DTYPE_BF16 || dtype == RQ_DTYPE_F32, "bad dtype %d", dtype);
     const int rc = check_q8_cache(head_dim, num_kv_heads, block_size, num_blocks, kv_cache, stride_block, format);
     if (rc) return rc;
-    RQ_CHECK_ARG(n_tokens >= 0 && n_tokens <= (1 << 24), "n_tokens %lld out of range", (long long)n_tokens);
+    RQ_CHECK_ARG(n_tokens >= 0 && n_tokens <= (1 << 30) / num_kv_heads, "n_tokens %lld out of range", (long long)n_tokens);
     if (n_tokens == 0 || num_blocks == 0) return RQ_OK;
     RQ_CHECK_ARG(key && value && slot_mapping, "null pointer");
     const int eb = dtype == RQ_DTYPE_F32 ? 4 : 2;
@@ -389,8 +474,8 @@ extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, in
     a.groups = block_size / kQ8Group;
     if (need) {
         a.count = static_cast<int32_t *>(workspace);
-        a.list = a.count + 4;
-        a.before = a.list + n_tokens;
+        a.list = reinterpret_cast<int2 *>(a.count + 4);
+        a.before = reinterpret_cast<int32_t *>(a.list + n_tokens);
         a.last = a.before + n_tokens;
     }
     hipStream_t st = (hipStream_t)stream;
@@ -408,6 +493,7 @@ extern "C" int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t b
     const int rc = check_q8_cache(head_dim, num_kv_heads, block_size, num_blocks, kv_cache, stride_block, format);
     if (rc) return rc;
     RQ_CHECK_ARG(num_seqs >= 0 && num_seqs <= (1 << 24) && total >= 0 && total <= INT32_MAX && max_blocks >= 0, "bad sizes");
+    RQ_CHECK_ARG((total / kQ8Group + num_seqs) * num_kv_heads <= INT32_MAX, "too many rows and heads for one call");
     if (num_seqs == 0 || total == 0 || max_blocks == 0 || num_blocks == 0) return RQ_OK;
     RQ_CHECK_ARG(block_table && seq_lens && starts && out_k && out_v, "null pointer");
     RQ_CHECK_ARG((uintptr_t)out_k % 16 == 0 && (uintptr_t)out_v % 16 == 0, "outputs must be 16-byte aligned");

@@ -73,7 +73,7 @@ def test_c_abi_refuses_bad_attention(change, status, msg):
 
 
 @pytest.mark.parametrize("change,status,msg", [
-    (dict(dtype=3), 1, b"dtype"), (dict(n=-1), 1, b"n_tokens"), (dict(n=1 << 30), 1, b"n_tokens"), (dict(k=None), 1, b"null"), (dict(slots=None), 1, b"null"),
+    (dict(dtype=3), 1, b"dtype"), (dict(n=-1), 1, b"n_tokens"), (dict(n=1 << 30), 1, b"n_tokens"), (dict(n=(1 << 27) + 1), 1, b"n_tokens"), (dict(k=None), 1, b"null"), (dict(slots=None), 1, b"null"),
     (dict(v=18), 1, b"16-byte"), (dict(kst=1028), 1, b"16-byte"), (dict(dtype=2, ksh=130), 1, b"16-byte"), (dict(n=513), 2, b"workspace too small"),
     (dict(n=513, ws=20, wsb=1 << 20), 1, b"aligned"), (dict(n=0), 0, None), (dict(nb=0), 0, None)])
 def test_c_abi_refuses_bad_stores(change, status, msg):
@@ -83,7 +83,7 @@ def test_c_abi_refuses_bad_stores(change, status, msg):
 
 
 @pytest.mark.parametrize("change,status,msg", [
-    (dict(dtype=3), 1, b"dtype"), (dict(ns=-1), 1, b"bad sizes"), (dict(total=1 << 40), 1, b"bad sizes"), (dict(starts=None), 1, b"null"),
+    (dict(dtype=3), 1, b"dtype"), (dict(ns=-1), 1, b"bad sizes"), (dict(total=1 << 40), 1, b"bad sizes"), (dict(ns=1 << 24, h=200, sb=1 << 20), 1, b"too many rows"), (dict(starts=None), 1, b"null"),
     (dict(ok=8), 1, b"16-byte"), (dict(ns=0), 0, None), (dict(total=0), 0, None), (dict(mb=0), 0, None)])
 def test_c_abi_refuses_bad_reads(change, status, msg):
     lib = _lib.load()
