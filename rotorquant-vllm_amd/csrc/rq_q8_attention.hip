@@ -439,7 +439,10 @@ static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_
     return std::max<int64_t>(1, std::min<int64_t>(resident * (int64_t)device_cus(), (work + kQ8MinChunk - 1) / kQ8MinChunk));
 }
 
-// Calls of short contexts, by the bound on their lengths, take a workgroup per item.
+// Calls of short contexts, by the bound on their lengths, take a workgroup per item.  One launch without partials saves 4 to 7 us; a long item
+// by itself is slower, as one workgroup walks it.  8 kv heads x 4, equal lengths, graph replays, items / shares:
+//   1 sequence of 800 keys 8.6 / 12.7 us, 1600: 12.7 / 14.0, 3200: 19.3 / 14.3;  8: 9.5 / 14.5, 13.6 / 17.2, 22.1 / 20.3;
+//   64: 24.6 / 25.0, 40.8 / 42.4, 73.5 / 78.0.
 constexpr int64_t kQ8ItemTiles = 60;
 static bool q8_is_short(int64_t max_keys) {
     return max_keys <= kQ8ItemTiles * kQ8Tile;
@@ -447,7 +450,7 @@ static bool q8_is_short(int64_t max_keys) {
 
 template <int DT, int FMT, int D, int NB>
 static void launch_stream(const Q8AttnArgs &a, int64_t workgroups, hipStream_t st) {
-    if (q8_is_short(a.cap)) {
+    if (q8_is_short(a.bound)) {
         const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
         hipLaunchKernelGGL((q8_item_kernel<DT, FMT, D, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(512), 0, st, a);
         return;
@@ -473,6 +476,9 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
 constexpr int64_t kQ8PromptCols = 128;
 static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= kQ8PromptCols; }
 
+// Lengths are ints in the kernels.
+static int64_t q8_bound(int64_t max_seq_len) { return std::min<int64_t>(max_seq_len, INT32_MAX - 64); }
+
 }  // namespace rq
 
 using namespace rq;
@@ -481,7 +487,9 @@ extern "C" int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num
                                                    int32_t head_dim, int64_t max_q_len, int64_t max_seq_len) {
     if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_q_len <= 0 || max_seq_len < 0) return 0;
     const int G = num_q_heads / num_kv_heads;
+    max_seq_len = q8_bound(max_seq_len);
     if (q8_is_prompt(max_q_len, G)) return q8_prefill_workspace(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
+    if (q8_is_short(max_seq_len)) return 0;
     const int64_t wgs = q8_workgroups(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
     return 2 * wgs * q8_blocks(G, max_q_len) * kQ8Cols * (head_dim + 2) * 4;
 }
@@ -501,7 +509,8 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
                  "num_q_heads %d must be a multiple of num_kv_heads %d", num_q_heads, num_kv_heads);
     RQ_CHECK_ARG(num_seqs >= 0 && num_seqs <= 65535 && total_q >= 0 && total_q <= INT32_MAX && max_q_len >= 0 && max_q_len <= (1 << 20) &&
                      max_blocks >= 0 && max_seq_len >= 0, "bad sizes");
-    RQ_CHECK_ARG(cu_seqlens_q != nullptr || total_q == num_seqs, "without cu_seqlens_q there is one query token per sequence");
+    RQ_CHECK_ARG(cu_seqlens_q != nullptr || (total_q == num_seqs && max_q_len <= 1),
+                 "without cu_seqlens_q there is one query token per sequence");
     uint32_t scale_bits;  // (by its bits: this file is compiled for arithmetic without NaN)
     __builtin_memcpy(&scale_bits, &sm_scale, 4);
     RQ_CHECK_ARG((scale_bits & 0x7f800000u) != 0x7f800000u, "sm_scale must be finite");
@@ -519,18 +528,19 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     a.H = num_kv_heads, a.G = num_q_heads / num_kv_heads, a.groups = block_size / kQ8Group, a.block_size = block_size;
     a.bt = block_table, a.max_blocks = max_blocks, a.bt_ss = bt_stride_seq;
     a.seq_lens = seq_lens;
-    a.cap = std::min<int64_t>(std::min<int64_t>(max_blocks * block_size, max_seq_len), INT32_MAX - 64);
-    a.max_q = (int)(cu_seqlens_q ? max_q_len : 1);
+    a.bound = q8_bound(max_seq_len);
+    a.cap = std::min<int64_t>(a.bound, max_blocks > a.bound / block_size ? a.bound : max_blocks * block_size);
+    a.max_q = (int)max_q_len;
     a.score_scale = sm_scale == 0.f ? 1.f : __builtin_fabsf(sm_scale) * kAttnLog2e;
     a.q_sign = sm_scale > 0.f ? 1.f : sm_scale < 0.f ? -1.f : 0.f;
     a.out = out, a.o_st = out_stride_tok, a.o_sh = out_stride_head;
-    const int64_t need = rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, a.max_q, a.cap);
+    const int64_t need = rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len);
     RQ_CHECK_SPACE(workspace_bytes >= need, "workspace too small: the call needs %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
-    RQ_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+    RQ_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace must be 16-byte aligned");
     a.part = static_cast<float *>(workspace);
     hipStream_t st = (hipStream_t)stream;
     if (q8_is_prompt(a.max_q, a.G)) return q8_prefill(a, dtype, format, head_dim, workspace, st);
-    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, head_dim, a.max_q, a.cap);
+    const int64_t wgs = q8_workgroups(num_seqs, a.G, a.H, head_dim, a.max_q, a.bound);
     if (dtype == RQ_DTYPE_BF16) launch_stream_f<RQ_DTYPE_BF16>(a, format, head_dim, wgs, st);
     else launch_stream_f<RQ_DTYPE_F16>(a, format, head_dim, wgs, st);
     return check_launch("q8_stream_kernel");

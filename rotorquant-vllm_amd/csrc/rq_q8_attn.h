@@ -21,7 +21,8 @@ struct Q8AttnArgs {
     const int32_t *bt;
     int64_t max_blocks, bt_ss;
     const int32_t *seq_lens;
-    int64_t cap;  // keys of a sequence that may be read: its table's capacity, max_seq_len
+    int64_t bound;  // max_seq_len: sizes launches and workspace
+    int64_t cap;    // keys of a sequence that may be read: bound, its table's capacity
     int max_q;    // tokens of a query that count
     float score_scale;  // |sm_scale| log2(e)
     float q_sign;       // sign of sm_scale (0 for 0)

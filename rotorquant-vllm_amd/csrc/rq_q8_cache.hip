@@ -46,21 +46,31 @@ __device__ __forceinline__ int64_t q8_run_start(const Q8StoreArgs &a, int64_t t)
     const int64_t g = q8_group_of(a, t);
     return g >= 0 && (t == 0 || q8_group_of(a, t - 1) != g) ? g : -1;
 }
-__global__ __launch_bounds__(256) void q8_unlink_kernel(Q8StoreArgs a) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+constexpr int kLinkThreads = 1024;
+__global__ __launch_bounds__(kLinkThreads) void q8_unlink_kernel(Q8StoreArgs a) {
+    const int64_t t = (int64_t)blockIdx.x * kLinkThreads + threadIdx.x;
     if (t == 0) *a.count = 0;
     if (t >= a.n_tokens) return;
     const int64_t g = q8_run_start(a, t);
     if (g >= 0) a.last[g] = -1;
 }
-__global__ __launch_bounds__(256) void q8_link_kernel(Q8StoreArgs a) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= a.n_tokens) return;
-    const int64_t g = q8_run_start(a, t);
-    if (g < 0) return;
-    const int32_t p = atomicExch(a.last + g, (int32_t)t);
-    a.before[t] = p;
-    if (p < 0) a.list[atomicAdd(a.count, 1)] = make_int2((int)t, (int)g);
+// The list's places come from one addition per workgroup: additions of every wave to the one counter took 3 us of 8 (32768 tokens).
+__global__ __launch_bounds__(kLinkThreads) void q8_link_kernel(Q8StoreArgs a) {
+    __shared__ int found, base;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    const int64_t t = (int64_t)blockIdx.x * kLinkThreads + threadIdx.x;
+    const int64_t g = t < a.n_tokens ? q8_run_start(a, t) : -1;
+    int place = -1;
+    if (g >= 0) {
+        const int32_t p = atomicExch(a.last + g, (int32_t)t);
+        a.before[t] = p;
+        if (p < 0) place = atomicAdd(&found, 1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && found > 0) base = atomicAdd(a.count, found);
+    __syncthreads();
+    if (place >= 0) a.list[base + place] = make_int2((int)t, (int)g);
 }
 
 // rows[r] = the last token that writes row r of group g, -1 for none.  LINKED: t0 is the token of the group's list entry.  Otherwise
@@ -116,8 +126,8 @@ template <int DT>
 __device__ __forceinline__ Q8Raw<DT> q8_load8(const void *p, int64_t at) {
     Q8Raw<DT> r;
     const q8_u32x4 *q = reinterpret_cast<const q8_u32x4 *>(static_cast<const uint8_t *>(p) + at * (DT == RQ_DTYPE_F32 ? 4 : 2));
-    r.w[0] = __builtin_nontemporal_load(q);
-    if constexpr (DT == RQ_DTYPE_F32) r.w[1] = __builtin_nontemporal_load(q + 1);
+    r.w[0] = *q;
+    if constexpr (DT == RQ_DTYPE_F32) r.w[1] = q[1];
     return r;
 }
 template <int DT>
@@ -132,7 +142,8 @@ __device__ __forceinline__ void q8_floats(const Q8Raw<DT> &r, float (&x)[8]) {
 // A wave takes a.per_wave units of one group, the next one's rows on their way while one is coded.  Lane: token row
 // t = lane % 16, half = (lane / 16) % 2 of the 16-dim parts; the wave's upper 32 lanes are the second 64-dim chunk
 // (D = 128) or the V side (D = 64).
-// Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in STORE_US.
+// Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in 49 us beside 9 for the two link launches.  Non-temporal loads
+// here: 56 us (a row's 128 bytes are loaded by four instructions, which then miss the L1).
 template <int DT, int FMT, int D, bool LINKED>
 __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a) {
     constexpr int kUnits = D == 128 ? 2 : 1;  // units per head
@@ -264,7 +275,6 @@ struct Q8ReadArgs {
     int64_t max_blocks, bt_ss;
     const int32_t *seq_lens, *starts;
     int64_t num_seqs, total;
-    int per_wave;  // heads of a wave
     void *out_k, *out_v;
 };
 
@@ -300,18 +310,17 @@ __device__ __forceinline__ uint32_t lane_xor4(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_update_dpp(from_above, (int)x, 0x114, 0xf, 0xa, false);          // the others: row_shr 4
 }
 
-// One wave per (group of a sequence, a.per_wave heads), the next head's codes on their way while one is written.  Codes change
-// lanes (and bytes of V, quads) so that every store is 16 bytes a lane (8 elements of 16 bits) and four lanes' are 64
-// consecutive bytes of a row.
-// Bound by memory: 32768 tokens of 8 heads (67 MB in, 134 out) in READ_US.
+// One wave per (group of a sequence, head).  Codes change lanes (and bytes of V, quads) so that every store is 16 bytes a
+// lane (8 elements of 16 bits) and four lanes' are 64 consecutive bytes of a row.
+// Bound by memory: 131072 tokens of 8 heads (270 MB in, 537 out) in 164 us, 4.9 TB/s (a copy: 5.1); 32768 in 46.  Two or
+// four heads a wave, the next one's codes loaded ahead: 167 and 183 us; non-temporal stores: 182.
 template <int DT, int FMT, int D>
 __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) {
     constexpr int kChunks = D / 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * kReadWaves + wave;  // (fits 32 bits)
-    const int waves = (a.H + a.per_wave - 1) / a.per_wave;  // of a group
-    const uint32_t unit = (uint32_t)item / (uint32_t)waves;
-    const int h0 = (int)((uint32_t)item - unit * waves) * a.per_wave, h1 = min(a.H, h0 + a.per_wave);
+    const uint32_t unit = (uint32_t)item / (uint32_t)a.H;
+    const int h = (int)((uint32_t)item - unit * a.H);
     // the last sequence whose first unit is not past this one, 64 at a time
     int64_t lo = 0, n = a.num_seqs;
     while (n > 1) {
@@ -332,60 +341,47 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
     page = page < 0 || page >= a.num_blocks ? 0 : page;
     const Q8Layout lay(a.H, D, a.block_size);
     const uint8_t *const base = a.cache + page * a.stride_block;
-    q8_u32x4 kw[kChunks], vw[kChunks];
-    float2 s;
-    auto load = [&](int h) {
-        const uint8_t *const tile = base + lay.codes_at(gi, h) + 16 * lane;
-        s = *reinterpret_cast<const float2 *>(base + lay.scale_at(gi, h));
+    const uint8_t *const tile = base + lay.codes_at(gi, h) + 16 * lane;
+    q8_u32x4 kc[kChunks], vc[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            kw[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + 1024 * j));
-            vw[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + kQ8Group * D + 1024 * j));
-        }
-    };
+    for (int j = 0; j < kChunks; ++j) {
+        kc[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + 1024 * j));
+        vc[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + kQ8Group * D + 1024 * j));
+    }
+    const float2 scale = *reinterpret_cast<const float2 *>(base + lay.scale_at(gi, h));
     const int g = lane >> 4, c = lane & 15, q = lane & 3;
     const bool upper = lane & 4;
     auto inside = [&](int row) { return row < rows && out0 + row >= 0 && out0 + row < a.total; };
     const bool k_in = inside(c), v_in = inside(4 * g + q);
-    const int64_t k_row = (out0 + c) * a.H * D, v_row = (out0 + 4 * g + q) * a.H * D;
-    load(h0);
-    for (int h = h0; h < h1; ++h) {
-        q8_u32x4 kc[kChunks], vc[kChunks];
+    const int64_t k_row = ((out0 + c) * a.H + h) * D, v_row = ((out0 + 4 * g + q) * a.H + h) * D;
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) kc[j] = kw[j], vc[j] = vw[j];
-        const float2 sc = s;
-        if (h + 1 < h1) load(h + 1);
+    for (int j = 0; j < kChunks; ++j) {
+        // K: lane group g has dims 16 g .. + 15 of token c -> dims 8 g .. + 7 and 32 + 8 g .. + 7
+        uint32_t p[2][2];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            // K: lane group g has dims 16 g .. + 15 of token c -> dims 8 g .. + 7 and 32 + 8 g .. + 7
-            uint32_t p[2][2];
+        for (int d = 0; d < 2; ++d) {
+            auto x = __builtin_amdgcn_permlane16_swap(kc[j][d], kc[j][2 + d], false, false);
+            auto y = __builtin_amdgcn_permlane32_swap(x[0], x[1], false, false);
+            p[0][d] = y[0], p[1][d] = y[1];
+        }
+        if (k_in) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                auto x = __builtin_amdgcn_permlane16_swap(kc[j][d], kc[j][2 + d], false, false);
-                auto y = __builtin_amdgcn_permlane32_swap(x[0], x[1], false, false);
-                p[0][d] = y[0], p[1][d] = y[1];
-            }
-            if (k_in) {
+            for (int u = 0; u < 2; ++u) q8_put8<DT, FMT>(a.out_k, k_row + 64 * j + 32 * u + 8 * g, p[u][0], p[u][1], scale.x);
+        }
+        // V: four tokens of dim 16 k + c -> dims 16 k + (c & 12) .. + 3 of token 4 g + q -> 8 dims, of part k or k + 1
 #pragma unroll
-                for (int u = 0; u < 2; ++u) q8_put8<DT, FMT>(a.out_k, k_row + h * D + 64 * j + 32 * u + 8 * g, p[u][0], p[u][1], sc.x);
-            }
-            // V: four tokens of dim 16 k + c -> dims 16 k + (c & 12) .. + 3 of token 4 g + q -> 8 dims, of part k or k + 1
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-                const uint32_t w0 = quad_transpose(vc[j][k], q), w1 = quad_transpose(vc[j][k + 1], q);
-                const uint32_t other = lane_xor4(upper ? w0 : w1);
-                if (v_in)
-                    q8_put8<DT, FMT>(a.out_v, v_row + h * D + 64 * j + 16 * (k + (upper ? 1 : 0)) + (c & 8), upper ? other : w0, upper ? w1 : other, sc.y);
-            }
+        for (int k = 0; k < 4; k += 2) {
+            const uint32_t w0 = quad_transpose(vc[j][k], q), w1 = quad_transpose(vc[j][k + 1], q);
+            const uint32_t other = lane_xor4(upper ? w0 : w1);
+            if (v_in)
+                q8_put8<DT, FMT>(a.out_v, v_row + 64 * j + 16 * (k + (upper ? 1 : 0)) + (c & 8), upper ? other : w0, upper ? w1 : other, scale.y);
         }
     }
 }
 
-// Units of a wave: one, for the least latency, until the calls' waves are more than the GPU holds (about 24 a CU).
-static int q8_per_wave(int64_t groups, int units) {
-    const int64_t waves = groups * units, room = 24 * (int64_t)device_cus();
-    return (int)std::min<int64_t>(4, std::max<int64_t>(1, waves / room));
-}
+// Units of a wave in a long call: two once one each would be more waves than the GPU holds (about 24 a CU).  32768 tokens of 8
+// heads, with their read-back: one 97 us, two 94, four 96.
+static int q8_per_wave(int64_t groups, int units) { return groups * units >= 48 * (int64_t)device_cus() ? 2 : 1; }
 
 template <int DT, int FMT, int D>
 static void launch_store(Q8StoreArgs a, bool linked, hipStream_t st) {
@@ -393,9 +389,9 @@ static void launch_store(Q8StoreArgs a, bool linked, hipStream_t st) {
     a.per_wave = linked ? q8_per_wave(a.n_tokens / kQ8Group, units) : 1;
     const int64_t blocks = (a.n_tokens * ((units + a.per_wave - 1) / a.per_wave) + kStoreWaves - 1) / kStoreWaves;
     if (linked) {
-        const unsigned tb = (unsigned)((a.n_tokens + 255) / 256);
-        hipLaunchKernelGGL(q8_unlink_kernel, dim3(tb), dim3(256), 0, st, a);
-        hipLaunchKernelGGL(q8_link_kernel, dim3(tb), dim3(256), 0, st, a);
+        const dim3 tb((unsigned)((a.n_tokens + kLinkThreads - 1) / kLinkThreads));
+        hipLaunchKernelGGL(q8_unlink_kernel, tb, dim3(kLinkThreads), 0, st, a);
+        hipLaunchKernelGGL(q8_link_kernel, tb, dim3(kLinkThreads), 0, st, a);
         const unsigned grid = (unsigned)std::min<int64_t>(blocks, 8 * device_cus());
         hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true>), dim3(grid), dim3(64 * kStoreWaves), 0, st, a);
     } else {
@@ -412,10 +408,8 @@ static void launch_store_f(const Q8StoreArgs &a, int fmt, int D, bool linked, hi
 }
 
 template <int DT, int FMT>
-static void launch_read_d(Q8ReadArgs a, int D, hipStream_t st) {
-    const int64_t groups = a.total / kQ8Group + a.num_seqs;
-    a.per_wave = q8_per_wave(groups, a.H);
-    const int64_t items = groups * ((a.H + a.per_wave - 1) / a.per_wave);
+static void launch_read_d(const Q8ReadArgs &a, int D, hipStream_t st) {
+    const int64_t items = (a.total / kQ8Group + a.num_seqs) * a.H;
     const dim3 grid((unsigned)((items + kReadWaves - 1) / kReadWaves)), block(64 * kReadWaves);
     if (D == 128) hipLaunchKernelGGL((q8_read_kernel<DT, FMT, 128>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((q8_read_kernel<DT, FMT, 64>), grid, block, 0, st, a);
@@ -425,7 +419,8 @@ static void launch_read_f(const Q8ReadArgs &a, int fmt, int D, hipStream_t st) {
     fmt == RQ_Q8_INT8 ? launch_read_d<DT, RQ_Q8_INT8>(a, D, st) : launch_read_d<DT, RQ_Q8_E4M3>(a, D, st);
 }
 
-// Tokens up to which every unit looks through all slots itself: one launch, no workspace.
+// Tokens up to which every wave looks through all slots itself: one launch, no workspace.  With read-back, 256 tokens of prompts
+// 11.0 us (linked: 12.5), 512 13.5 (12.9), 1024 22.8 (14.4); 512 appended tokens 26.8 (29.6).
 constexpr int64_t kStoreScan = 512;
 
 }  // namespace rq

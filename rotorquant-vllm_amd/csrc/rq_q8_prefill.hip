@@ -484,7 +484,7 @@ static void q8_prefill_pass(const Q8PrefillArgs &p, int64_t nb, hipStream_t st) 
 }
 
 int q8_prefill(const Q8AttnArgs &a, int dtype, int format, int D, void *workspace, hipStream_t st) {
-    const Q8PrefillShape s = q8_prefill_shape(a.num_seqs, a.G, a.H, D, a.max_q, a.cap);
+    const Q8PrefillShape s = q8_prefill_shape(a.num_seqs, a.G, a.H, D, a.max_q, a.bound);
     Q8PrefillArgs p{};
     p.a = a;
     p.max_tiles = s.tiles;

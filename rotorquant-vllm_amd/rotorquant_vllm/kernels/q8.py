@@ -11,7 +11,6 @@ streams at once (scratch comes from torch's allocator unless passed).
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -21,7 +20,6 @@ from .. import _lib
 __all__ = ["q8_slot_bytes", "q8_store", "q8_read", "q8_attention"]
 
 _FORMATS = {"int8": 0, "fp8": 1}
-_NULL = contextlib.nullcontext()
 
 
 def _format(fmt: str) -> int:
@@ -31,25 +29,29 @@ def _format(fmt: str) -> int:
         raise ValueError(f"fmt must be 'int8' or 'fp8', got {fmt!r}") from None
 
 
-def _one_device(*tensors: torch.Tensor | None) -> torch.device:
-    """The device that all tensors are on."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("rotorquant_vllm.kernels runs only on ROCm device tensors (got a "
-                               f"{t.device.type} tensor); there is no CPU path")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
+# (calls of a few microseconds wait for the checks below: device indices and plain comparisons, no device objects)
+
+def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """Index of the device that all tensors are on."""
+    dev = first.get_device()
+    for t in (first, *others):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            if not (first.is_cuda and t.is_cuda):
+                raise RuntimeError("rotorquant_vllm.kernels runs only on ROCm device tensors (got a "
+                                   f"{(t if first.is_cuda else first).device.type} tensor); there is no CPU path")
+            raise ValueError(f"tensors on {first.device} and {t.device}")
     return dev
 
 
-def _on(dev: torch.device):
-    """A launch goes to the current device's context: make it the tensors' own."""
-    return _NULL if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _call(fn, name: str, dev: int, args: tuple) -> None:
+    """fn(*args, stream): a launch goes to the current device's context, so the tensors' own is made current."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _lib.stream_ptr(torch.device("cuda", dev)) if _lib._raw_stream is None else _lib._raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream_ptr(torch.device("cuda", dev)))
+    if rc:
+        _lib.check(rc, name)
 
 
 def q8_slot_bytes(num_kv_heads: int, head_dim: int) -> int:
@@ -75,13 +77,15 @@ def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> torch.Te
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _scratch(workspace: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor | None:
-    """The caller's buffer, or one of this call from the stream's allocator (none for 0 bytes)."""
+def _scratch(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int, int]:
+    """(tensor to keep, address, bytes) of the caller's buffer, or of one of this call from the stream's allocator."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        if not need:
+            return None, 0, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor")
-    return workspace
+    return workspace, workspace.data_ptr(), workspace.numel()
 
 
 def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor, fmt: str = "int8",
@@ -94,11 +98,11 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
     workspace: scratch of calls of more than 512 tokens (rq_q8_store_workspace_bytes bytes),
     by default from torch's allocator; a graph captured without torch's graph classes needs it.
     """
-    dev = _one_device(key, value, kv_cache, slot_mapping, workspace)
+    dev = _device_index(key, value, kv_cache, slot_mapping, workspace)
     if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
         raise ValueError("key and value must have the same (tokens, heads, head_dim) shape and dtype")
     N, H, D = key.shape
-    if D > 1 and (key.stride(-1) != 1 or value.stride(-1) != 1):
+    if key.stride(2) != 1 or value.stride(2) != 1:
         raise ValueError("key/value must be contiguous over head_dim")
     NB, BS, stride = _check_cache(kv_cache, H, D)
     sm = _index(slot_mapping, "slot_mapping", torch.int64, 1)
@@ -106,12 +110,10 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
         raise ValueError("slot_mapping shorter than the number of tokens")
     code = _format(fmt)
     L = _lib.load()
-    with _on(dev):
-        ws = _scratch(workspace, L.rq_q8_store_workspace_bytes(N, NB, BS), dev)
-        rc = L.rq_q8_store(key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), N, key.stride(0), key.stride(1),
-                           value.stride(0), value.stride(1), H, D, code, sm.data_ptr(), kv_cache.data_ptr(), NB, BS, stride,
-                           _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr(dev))
-    _lib.check(rc, "rq_q8_store")
+    keep, ws, ws_bytes = _scratch(workspace, L.rq_q8_store_workspace_bytes(N, NB, BS), kv_cache)
+    _call(L.rq_q8_store, "rq_q8_store", dev,
+          (key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), N, key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+           H, D, code, sm.data_ptr(), kv_cache.data_ptr(), NB, BS, stride, ws, ws_bytes))
 
 
 def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor, num_kv_heads: int,
@@ -124,7 +126,7 @@ def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.T
     without them `total` rows are allocated (rows of no sequence are then not initialised).
     The layout is that of variable-length attention over plain K and V.
     """
-    dev = _one_device(kv_cache, block_table, seq_lens, starts, out_k, out_v)
+    dev = _device_index(kv_cache, block_table, seq_lens, starts, out_k, out_v)
     NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
     bt = _index(block_table, "block_table", torch.int32, 2)
     sl, st = _index(seq_lens, "seq_lens", torch.int32, 1), _index(starts, "starts", torch.int32, 1)
@@ -138,17 +140,14 @@ def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.T
         total = given[0].shape[0]
     shape = (total, num_kv_heads, head_dim)
     for t in given:
-        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
             raise ValueError(f"outputs must be contiguous {shape} tensors of {dtype}")
     code = _format(fmt)
-    L = _lib.load()
-    with _on(dev):
-        out_k = torch.empty(shape, dtype=dtype, device=dev) if out_k is None else out_k
-        out_v = torch.empty(shape, dtype=dtype, device=dev) if out_v is None else out_v
-        rc = L.rq_q8_read(kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, head_dim, code, bt.data_ptr(), bt.shape[1], bt.stride(0),
-                          sl.data_ptr(), st.data_ptr(), B, total, out_k.data_ptr(), out_v.data_ptr(), _lib.dtype_code(dtype),
-                          _lib.stream_ptr(dev))
-    _lib.check(rc, "rq_q8_read")
+    out_k = torch.empty(shape, dtype=dtype, device=kv_cache.device) if out_k is None else out_k
+    out_v = torch.empty(shape, dtype=dtype, device=kv_cache.device) if out_v is None else out_v
+    _call(_lib.load().rq_q8_read, "rq_q8_read", dev,
+          (kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, head_dim, code, bt.data_ptr(), bt.shape[1], bt.stride(0), sl.data_ptr(),
+           st.data_ptr(), B, total, out_k.data_ptr(), out_v.data_ptr(), _lib.dtype_code(dtype)))
     return out_k, out_v
 
 
@@ -168,7 +167,7 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     """
     if q.dim() != 3 or q.shape[2] != head_dim or num_kv_heads < 1 or q.shape[1] % num_kv_heads:
         raise ValueError(f"q must be (tokens, a multiple of {num_kv_heads} heads, {head_dim}), got {tuple(q.shape)}")
-    dev = _one_device(q, kv_cache, block_table, seq_lens, cu_seqlens_q, out, workspace)
+    dev = _device_index(q, kv_cache, block_table, seq_lens, cu_seqlens_q, out, workspace)
     NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
     bt = _index(block_table, "block_table", torch.int32, 2)
     sl = _index(seq_lens, "seq_lens", torch.int32, 1)
@@ -194,13 +193,11 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
     code = _format(fmt)
     L = _lib.load()
-    with _on(dev):
-        out = torch.empty_like(q) if out is None else out
-        ws = _scratch(workspace, L.rq_q8_attention_workspace_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), dev)
-        rc = L.rq_q8_attention(q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, q.stride(0), q.stride(1), _lib.ptr(cu), B, max_q_len,
-                               1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(),
-                               bt.shape[1], bt.stride(0), sl.data_ptr(), max_seq_len,
-                               float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale), out.data_ptr(), out.stride(0), out.stride(1),
-                               _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr(dev))
-    _lib.check(rc, "rq_q8_attention")
+    out = torch.empty_like(q) if out is None else out
+    keep, ws, ws_bytes = _scratch(workspace, L.rq_q8_attention_workspace_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
+    _call(L.rq_q8_attention, "rq_q8_attention", dev,
+          (q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, q.stride(0), q.stride(1), None if cu is None else cu.data_ptr(), B, max_q_len,
+           1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(), bt.shape[1], bt.stride(0),
+           sl.data_ptr(), max_seq_len, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0),
+           out.stride(1), ws, ws_bytes))
     return out

@@ -60,11 +60,12 @@ def test_c_abi_refuses_bad_caches(change, msg):
 
 
 @pytest.mark.parametrize("change,status,msg", [
-    (dict(dtype=2), 1, b"f16 or bf16"), (dict(hq=33), 1, b"multiple"), (dict(total=2), 1, b"one query token"), (dict(scale=float("nan")), 1, b"finite"),
+    (dict(dtype=2), 1, b"f16 or bf16"), (dict(hq=33), 1, b"multiple"), (dict(total=2), 1, b"one query token"), (dict(mq=2), 1, b"one query token"), (dict(scale=float("nan")), 1, b"finite"),
     (dict(scale=float("inf")), 1, b"finite"), (dict(mq=-1), 1, b"bad sizes"), (dict(ns=65536, total=65536), 1, b"bad sizes"), (dict(nb=0), 1, b"no pages"),
     (dict(), 1, b"null"), (dict(q=8, out=16), 1, b"16-byte"), (dict(q=16, out=16, qst=4100), 1, b"16-byte"), (dict(q=16, out=12), 1, b"8-byte"),
-    (dict(q=16, out=16, osh=130), 1, b"8-byte"), (dict(q=16, out=16), 2, b"workspace too small"),
-    (dict(q=16, out=16, ws=8, wsb=1 << 30), 1, b"aligned"), (dict(q=16, out=16, ws=None, wsb=1 << 30), 1, b"aligned"),
+    (dict(q=16, out=16, osh=130), 1, b"8-byte"), (dict(q=16, out=16, mb=1000, msl=16000), 2, b"workspace too small"),
+    (dict(q=16, out=16, mb=1000, msl=16000, ws=8, wsb=1 << 30), 1, b"aligned"),
+    (dict(q=16, out=16, mb=1000, msl=16000, ws=None, wsb=1 << 30), 1, b"aligned"),
     (dict(ns=0, total=0), 0, None), (dict(total=0, cu=16), 0, None), (dict(mq=0), 0, None)])
 def test_c_abi_refuses_bad_attention(change, status, msg):
     lib = _lib.load()
@@ -95,8 +96,8 @@ def test_workspaces():
     lib = _lib.load()
     assert lib.rq_q8_store_workspace_bytes(512, 1 << 20, 16) == 0
     assert lib.rq_q8_store_workspace_bytes(513, 100, 32) >= 4 * (200 + 2 * 513)
-    small = lib.rq_q8_attention_workspace_bytes(1, 32, 8, 128, 1, 1)
-    assert 0 < small <= lib.rq_q8_attention_workspace_bytes(1, 32, 8, 128, 1, 8192) <= lib.rq_q8_attention_workspace_bytes(64, 32, 8, 128, 1, 8192)
+    assert lib.rq_q8_attention_workspace_bytes(64, 32, 8, 128, 1, 1000) == 0  # a workgroup per item
+    assert 0 < lib.rq_q8_attention_workspace_bytes(1, 32, 8, 128, 1, 8192) <= lib.rq_q8_attention_workspace_bytes(64, 32, 8, 128, 1, 8192)
     assert lib.rq_q8_attention_workspace_bytes(0, 32, 8, 128, 1, 8192) == 0
 
 
@@ -120,5 +121,7 @@ def test_python_refusals():
         q8._check_cache(cache, 3, 128)
     with pytest.raises(ValueError, match="contiguous"):
         q8._check_cache(cache.transpose(0, 1), 2, 128)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        q8._device_index(cache)
     with pytest.raises(ValueError, match="block_table must be"):
         q8._index(i.long()[None], "block_table", torch.int32, 2)
