@@ -114,7 +114,8 @@ __device__ __forceinline__ void q8_put(uint16_t *row, const float (&o)[N], float
 
 // Tiles [t0, t1) of the item (sequence, kv head h, columns from c0) by the workgroup's W waves, tile t0 + i by wave i % W.  The result is
 // the output rows (part == NULL) or partials.
-template <int DT, int FMT, int D, int NB, int W>
+// ONCE: no other workgroup reads these codes.
+template <int DT, int FMT, int D, int NB, int W, bool ONCE>
 __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, const Q8Seq &s, int h, int c0, int t0, int t1, float *part,
                                            Q8Sums<D, W> &lds) {
     constexpr int kSteps = D / 32, kChunks = D / 64, kBlocks = D / 16;
@@ -134,16 +135,22 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
         sc = *reinterpret_cast<const float2 *>(a.cache + page * a.stride_block + lay.scale_at(gi - p * a.groups, h));
     };
     auto slot = [&](int t) { return (t - t0) / W & 31; };
-    // The codes are read once: non-temporal loads (64 sequences of 4600 keys on average, 8 kv heads: 126 us -> 114).
+    // Codes read once come by non-temporal loads (64 sequences of 4600 keys on average, 8 kv heads: 126 us -> 114; 32
+    // sequences of 4000, 8 tokens x 4: 65.8 -> 60.1), codes that several column blocks read by ordinary ones (the latter with 16
+    // tokens: 82.1 -> 76.0, with 48: 265 -> 245).
     Q8Tile<D> next;
+    auto code16 = [](const uint8_t *p) {
+        const u32x4 *const q = reinterpret_cast<const u32x4 *>(p);
+        return ONCE ? __builtin_nontemporal_load(q) : *q;
+    };
     auto fetch = [&](int t) {
 #pragma unroll
         for (int gr = 0; gr < 2; ++gr) {
             const uint8_t *p = a.cache + lane64(at, 2 * slot(t) + gr);
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
-                next.k[gr][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 1024 * j + 16 * lane));
-                next.v[gr][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + kQ8Group * D + 1024 * j + 16 * lane));
+                next.k[gr][j] = code16(p + 1024 * j + 16 * lane);
+                next.v[gr][j] = code16(p + kQ8Group * D + 1024 * j + 16 * lane);
             }
         }
     };
@@ -307,7 +314,7 @@ template <int D, int NB>
 constexpr int kQ8Resident = D == 64 ? (NB == 1 ? 4 : 3) : 2;
 
 // Equal shares of all items' tiles.
-template <int DT, int FMT, int D, int NB>
+template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(256, (kQ8Resident<D, NB>)) void q8_stream_kernel(Q8AttnArgs a) {
     const int lane = threadIdx.x & 63;
     __shared__ Q8Sums<D, 4> lds;
@@ -335,7 +342,7 @@ __global__ __launch_bounds__(256, (kQ8Resident<D, NB>)) void q8_stream_kernel(Q8
         const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
         // an item cut in two or more: the share that begins it ends with it, the others begin with it
         float *part = t0 == 0 && t1 == n ? nullptr : a.part + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * NB * Q8Partial<D>::kFloats;
-        q8_segment<DT, FMT, D, NB, 4>(a, seq, s, (int)(item - block_of * a.H), (int)block_of * (NB * kQ8Cols), t0, t1, part, lds);
+        q8_segment<DT, FMT, D, NB, 4, ONCE>(a, seq, s, (int)(item - block_of * a.H), (int)block_of * (NB * kQ8Cols), t0, t1, part, lds);
         pos += t1 - t0;
     }
 }
@@ -418,14 +425,14 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgro
 }
 
 // One workgroup of 8 waves per item: one launch, no partials.
-template <int DT, int FMT, int D, int NB>
+template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
     __shared__ Q8Sums<D, 8> lds;
     const int64_t seq = blockIdx.y;
     const Q8Seq s = q8_seq(a, seq);
     const int block = blockIdx.x / (uint32_t)a.H, h = blockIdx.x - block * a.H;
     if (block >= q8_col_blocks<NB>(a, s.T)) return;
-    q8_segment<DT, FMT, D, NB, 8>(a, seq, s, h, block * (NB * kQ8Cols), 0, q8_tiles(s), nullptr, lds);
+    q8_segment<DT, FMT, D, NB, 8, ONCE>(a, seq, s, h, block * (NB * kQ8Cols), 0, q8_tiles(s), nullptr, lds);
 }
 
 // Blocks of 16 columns that a workgroup takes, and the workgroups: what the GPU holds at once, or fewer where the bound on the lengths
@@ -448,20 +455,22 @@ static bool q8_is_short(int64_t max_keys) {
     return max_keys <= kQ8ItemTiles * kQ8Tile;
 }
 
-template <int DT, int FMT, int D, int NB>
+template <int DT, int FMT, int D, int NB, bool ONCE>
 static void launch_stream(const Q8AttnArgs &a, int64_t workgroups, hipStream_t st) {
     if (q8_is_short(a.bound)) {
         const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
-        hipLaunchKernelGGL((q8_item_kernel<DT, FMT, D, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(512), 0, st, a);
+        hipLaunchKernelGGL((q8_item_kernel<DT, FMT, D, NB, ONCE>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(512), 0, st, a);
         return;
     }
-    hipLaunchKernelGGL((q8_stream_kernel<DT, FMT, D, NB>), dim3((unsigned)workgroups), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((q8_stream_kernel<DT, FMT, D, NB, ONCE>), dim3((unsigned)workgroups), dim3(256), 0, st, a);
     const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
     hipLaunchKernelGGL((q8_merge_kernel<DT, D, NB>), dim3((unsigned)(items * NB), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)workgroups);
 }
 template <int DT, int FMT, int D>
 static void launch_stream_b(const Q8AttnArgs &a, int64_t wgs, hipStream_t st) {
-    q8_blocks(a.G, a.max_q) == 1 ? launch_stream<DT, FMT, D, 1>(a, wgs, st) : launch_stream<DT, FMT, D, 2>(a, wgs, st);
+    if (q8_blocks(a.G, a.max_q) == 1) launch_stream<DT, FMT, D, 1, true>(a, wgs, st);
+    else if ((int64_t)a.max_q * a.G <= 2 * kQ8Cols) launch_stream<DT, FMT, D, 2, true>(a, wgs, st);
+    else launch_stream<DT, FMT, D, 2, false>(a, wgs, st);
 }
 template <int DT, int FMT>
 static void launch_stream_d(const Q8AttnArgs &a, int D, int64_t wgs, hipStream_t st) {
@@ -472,8 +481,10 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
     fmt == RQ_Q8_INT8 ? launch_stream_d<DT, RQ_Q8_INT8>(a, D, wgs, st) : launch_stream_d<DT, RQ_Q8_E4M3>(a, D, wgs, st);
 }
 
-// Calls of so many columns per kv head or more go to the prefill kernels.
-constexpr int64_t kQ8PromptCols = 128;
+// Calls of so many columns per kv head or more go to the prefill kernels.  8 kv heads x 4, queries of 1 to n tokens, these / those:
+// 8 sequences of 8000 keys, n = 20: 57 / 156 us, 32: 99 / 160, 64: 164 / 195;  32 of 1000, 32: 58 / 77, 64: 109 / 81;  1 of
+// 8000, 64: 40 / 40;  head_dim 64, 8 of 4000, 32: 38 / 44, 64: 52 / 51.
+constexpr int64_t kQ8PromptCols = 192;
 static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= kQ8PromptCols; }
 
 // Lengths are ints in the kernels.

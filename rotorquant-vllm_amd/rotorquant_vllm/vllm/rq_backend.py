@@ -19,6 +19,8 @@ librq_hip.so (include/rq_abi.h):
                          longer queries rq_paged_prefill (the same arithmetic,
                          each tile decoded once); other head sizes
                          rq_paged_decompress + device attention in fp32
+    8-bit cache       -> rq_q8_store, rq_q8_attention (RQ_CACHE_8BIT=int8 | fp8: another cache
+                         layout, no rotation, no codebook; no counterpart in the reference)
 
 vLLM itself is imported lazily: without vLLM the module still imports (the
 classes then derive from small local stand-ins), which is how the tests run.
@@ -92,6 +94,20 @@ def _parse_dense3() -> bool:
     return on
 
 
+def _parse_cache_8bit() -> str | None:
+    """RQ_CACHE_8BIT=int8 | fp8 (opt-in, no counterpart in the reference): the cache holds 8-bit codes with a
+    power-of-two scale per 16 tokens and head (rotorquant_vllm.kernels.q8_store) instead of rotated 3- or
+    4-bit indices.  Unset: None."""
+    fmt = os.environ.get("RQ_CACHE_8BIT", "").lower()
+    if not fmt:
+        return None
+    if fmt not in ("int8", "fp8"):
+        raise ValueError(f"RQ_CACHE_8BIT must be 'int8' or 'fp8', got '{fmt}'")
+    if _parse_dense3():
+        raise ValueError("RQ_CACHE_8BIT and RQ_DENSE_3BIT are two cache layouts: set one of them")
+    return fmt
+
+
 def _parse_iso_mode() -> str:
     mode = os.environ.get("RQ_ISO_MODE", "fast").lower()
     if mode not in ("fast", "full"):
@@ -116,6 +132,8 @@ _paged_decompress_fn = None
 _paged_attention_fn = None
 _paged_prefill_fn = None
 _unfused_decode_fn = None
+_q8_store_fn = None
+_q8_attention_fn = None
 _shared_workspace = None
 PREFILL_SPLIT_BYTES = 0
 try:
@@ -130,6 +148,8 @@ try:
     from rotorquant_vllm.kernels import paged_decompress as _paged_decompress_fn
     from rotorquant_vllm.kernels import shared_workspace as _shared_workspace
     from rotorquant_vllm.kernels import PREFILL_SPLIT_BYTES
+    from rotorquant_vllm.kernels import q8_attention as _q8_attention_fn
+    from rotorquant_vllm.kernels import q8_store as _q8_store_fn
 
     _rq_lib.load()
     _fused_paged_kernel_available = True
@@ -148,6 +168,12 @@ RQ_UNFUSED_SHORT_Q = 16
 RQ_FUSED_HEAD_DIM = 128
 RQ_FUSED_MAX_GQA = 16
 RQ_FUSED_MAX_KV_HEADS = 64
+
+
+# Shapes of the 8-bit cache.
+RQ_8BIT_HEAD_DIMS = (64, 128)
+RQ_8BIT_GROUP = 16
+RQ_8BIT_PROMPT_COLUMNS = 192  # q8_attention's prefill kernels from here on: (token, query head) pairs of a kv head
 
 
 def _fused_shape_ok(num_heads: int, num_kv_heads: int, head_size: int) -> str | None:
@@ -219,6 +245,16 @@ def _rq_padded_slot_bytes(head_dim: int, dense3: bool = False) -> int:
 
 def _rq_total_bytes(head_dim: int, num_kv_heads: int, dense3: bool = False) -> int:
     return num_kv_heads * _rq_padded_slot_bytes(head_dim, dense3)
+
+
+def _rq_slot_bytes(head_dim: int, num_kv_heads: int, block_size: int) -> int:
+    """Slot bytes of the configured cache (RQ_CACHE_8BIT, RQ_DENSE_3BIT)."""
+    if _parse_cache_8bit() is None:
+        return _rq_total_bytes(head_dim, num_kv_heads, _parse_dense3())
+    from rotorquant_vllm.kernels import q8_slot_bytes
+    if block_size % RQ_8BIT_GROUP:
+        raise ValueError(f"RQ_CACHE_8BIT needs a block size that is a multiple of {RQ_8BIT_GROUP} (got {block_size})")
+    return q8_slot_bytes(num_kv_heads, head_dim)
 
 
 # ---------------------------------------------------------------------------
@@ -407,7 +443,7 @@ class RQFullAttentionSpec(FullAttentionSpec):
 
     @property
     def real_page_size_bytes(self) -> int:  # noqa: D102
-        return self.block_size * _rq_total_bytes(self.head_size, self.num_kv_heads, _parse_dense3())
+        return self.block_size * _rq_slot_bytes(self.head_size, self.num_kv_heads, self.block_size)
 
 
 # ---------------------------------------------------------------------------
@@ -437,17 +473,20 @@ class RQMetadataBuilder(_BuilderBase):
         """UNIFORM_SINGLE_TOKEN_DECODE when the layer's decodes run a HIP kernel whose
         launch does not depend on host data (the fused decode, or rq_paged_attention):
         the library loads, head_size 128, a GQA group the kernels take and an f16 /
-        bf16 model.  Otherwise NEVER: such decodes run the torch fallback, whose loop
+        bf16 model; with the 8-bit cache head_size 64 or 128 and any GQA group.  Otherwise NEVER: such decodes run the torch fallback, whose loop
         over host lengths cannot be captured."""
         if not _fused_paged_kernel_available:
             return AttentionCGSupport.NEVER
         head_size = getattr(kv_cache_spec, "head_size", RQ_FUSED_HEAD_DIM)
-        if head_size != RQ_FUSED_HEAD_DIM:
+        q8 = _parse_cache_8bit() is not None
+        if head_size not in (RQ_8BIT_HEAD_DIMS if q8 else (RQ_FUSED_HEAD_DIM,)):
             return AttentionCGSupport.NEVER
         model_config = getattr(vllm_config, "model_config", None)
         dtype = getattr(model_config, "dtype", None)
         if isinstance(dtype, torch.dtype) and dtype not in (torch.float16, torch.bfloat16):
             return AttentionCGSupport.NEVER
+        if q8:  # (any GQA group)
+            return AttentionCGSupport.UNIFORM_SINGLE_TOKEN_DECODE
         num_kv = getattr(kv_cache_spec, "num_kv_heads", None)
         num_heads = None
         try:
@@ -501,7 +540,7 @@ class RQAttentionBackend(_BackendBase):
     def get_kv_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int,
                            cache_dtype_str: str = "auto") -> tuple[int, ...]:
         """(num_blocks, block_size, total_bytes) uint8."""
-        return (num_blocks, block_size, _rq_total_bytes(head_size, num_kv_heads, _parse_dense3()))
+        return (num_blocks, block_size, _rq_slot_bytes(head_size, num_kv_heads, block_size))
 
     @staticmethod
     def get_kv_cache_stride_order(include_num_layers_dimension: bool = False) -> tuple[int, ...]:
@@ -525,6 +564,10 @@ class RQAttentionImpl(_ImplBase):
         iso_mode = _parse_iso_mode()
         k_bits, v_bits = _parse_kv_bits()
         self._k_bits, self._v_bits, self._rq_mode = k_bits, v_bits, rq_mode
+        self._q8_format = _parse_cache_8bit()
+        if self._q8_format is not None:
+            self._init_q8()
+            return
 
         vllm_config = None
         if _HAVE_VLLM:
@@ -583,6 +626,77 @@ class RQAttentionImpl(_ImplBase):
         logger.info("Fused paged RQ decode: %s; fused paged RQ int8 prefill: %s",
                     "enabled" if self._fused_paged_available else "disabled",
                     "enabled" if self._fused_prefill_available else "disabled")
+
+    # -- 8-bit cache ---------------------------------------------------------
+
+    def _init_q8(self) -> None:
+        """RQ_CACHE_8BIT: no rotation, no codebooks and no buffers; the shape and the library decide whether it runs."""
+        if self.head_size not in RQ_8BIT_HEAD_DIMS:
+            raise ValueError(f"RQ_CACHE_8BIT needs head_size {' or '.join(map(str, RQ_8BIT_HEAD_DIMS))} (got {self.head_size})")
+        if self.num_heads % self.num_kv_heads:
+            raise ValueError(f"RQ_CACHE_8BIT: {self.num_heads} query heads over {self.num_kv_heads} kv heads")
+        self._fused_paged_available = self._fused_prefill_available = False
+        self._total_bytes = _rq_slot_bytes(self.head_size, self.num_kv_heads, RQ_8BIT_GROUP)
+        logger.info("RQAttentionImpl: 8-bit cache (%s), %d KV heads, head_size=%d, %d bytes/token (%.2fx compression vs FP16)",
+                    self._q8_format, self.num_kv_heads, self.head_size, self._total_bytes,
+                    4 * self.num_kv_heads * self.head_size / self._total_bytes)
+
+    def _forward_q8(self, query, key, value, kv_cache, md, output):
+        """Store the new tokens, then attention over the 8-bit cache.  One call for a batch of decodes or short queries; a
+        batch with longer ones sends its leading decodes (vLLM orders decodes first), the next short ones and the rest to
+        a call each: their kernels differ.  A captured call is replayed over longer contexts, so only outside
+        capture do the host's lengths bound it."""
+        if _q8_store_fn is None:
+            raise RuntimeError("RotorQuant HIP kernels are not available")
+        if getattr(md, "use_cascade", False):
+            raise NotImplementedError("RQ does not yet support cascade attention")
+        n = md.num_actual_tokens
+        fmt, H, D = self._q8_format, self.num_kv_heads, self.head_size
+        if key is not None and value is not None:
+            m = md.slot_mapping.shape[0]
+            _q8_store_fn(key[:m], value[:m], kv_cache, md.slot_mapping, fmt=fmt)
+        q, out = query[:n], output[:n]
+        sl_cpu = getattr(md, "rq_seq_lens_cpu", None)
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            sl_cpu = None
+        qsl_cpu = getattr(md, "rq_query_start_loc_cpu", None)
+        max_q = getattr(md, "max_query_len", None)
+        if max_q is None:
+            qsl_cpu = qsl_cpu if qsl_cpu is not None else md.query_start_loc.cpu()
+            max_q = int((qsl_cpu[1:] - qsl_cpu[:-1]).max()) if qsl_cpu.numel() > 1 else 0
+        causal = bool(getattr(md, "causal", True))
+
+        def attend(b0, b1, cu, most, longest):
+            _q8_attention_fn(q if cu is not None else q[b0:b1], kv_cache, md.block_table[b0:b1], md.seq_lens[b0:b1], H, D, fmt=fmt,
+                             sm_scale=self.scale, causal=causal, cu_seqlens_q=cu, max_q_len=most, max_seq_len=longest,
+                             out=out if cu is not None else out[b0:b1])
+
+        columns = self.num_heads // H
+        if int(max_q) <= 1:
+            longest = int(sl_cpu[:n].max()) if sl_cpu is not None and n else None
+            attend(0, n, None, 1, longest)
+            return output
+        if int(max_q) * columns < RQ_8BIT_PROMPT_COLUMNS:
+            longest = int(sl_cpu.max()) if sl_cpu is not None and sl_cpu.numel() else None
+            B = md.seq_lens.numel()
+            attend(0, B, md.query_start_loc[:B + 1], int(max_q), longest)
+            return output
+        starts = (qsl_cpu if qsl_cpu is not None else md.query_start_loc.cpu()).tolist()
+        lens = (sl_cpu if sl_cpu is not None else md.seq_lens.cpu()).tolist()
+        q_lens = [b - a for a, b in zip(starts, starts[1:])]
+        B = len(lens)
+        nd = 0
+        while nd < B and q_lens[nd] == 1:
+            nd += 1
+        ns = nd
+        while ns < B and q_lens[ns] * columns < RQ_8BIT_PROMPT_COLUMNS:
+            ns += 1
+        if nd:
+            attend(0, nd, None, 1, max(lens[:nd]))
+        for b0, b1 in ((nd, ns), (ns, B)):
+            if b1 > b0:
+                attend(b0, b1, md.query_start_loc[b0:b1 + 1], max(q_lens[b0:b1]), max(lens[b0:b1]))
+        return output
 
     # -- scratch -----------------------------------------------------------
 
@@ -868,7 +982,7 @@ class RQAttentionImpl(_ImplBase):
         a batch with several sequences and multi-token ones -> leading decodes to
         the fused decode, the rest to the int8 prefill; without RQ_USE_FUSED_PAGED
         (or for shapes the fused kernels do not take) -> the non-fused path
-        (_forward_unfused)."""
+        (_forward_unfused).  With the 8-bit cache: _forward_q8."""
         assert output is not None, "Output tensor must be provided."
         if output_scale is not None or output_block_scale is not None:
             raise NotImplementedError("Fused output quantization is not supported with RotorQuant backend")
@@ -877,6 +991,9 @@ class RQAttentionImpl(_ImplBase):
         if self.attn_type in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
             n = attn_metadata.num_actual_tokens
             return self._forward_encoder_attention(query[:n], key[:n], value[:n], output[:n], attn_metadata, layer)
+
+        if getattr(self, "_q8_format", None) is not None:
+            return self._forward_q8(query, key, value, kv_cache, attn_metadata, output)
 
         num_actual_tokens = attn_metadata.num_actual_tokens
         max_query_len = getattr(attn_metadata, "max_query_len", None)

@@ -330,3 +330,188 @@ def test_prompts(fmt, H, G, D, lens, queries, causal):
     """Query lengths that take the prefill kernels: odd ones, none, more queries than keys, few queries over long contexts."""
     attend(lens, queries, 16, H, G, D, fmt, torch.float16, 31, causal=causal)
     attend(lens, queries, 32, H, G, D, fmt, torch.bfloat16, 32, causal=causal)
+
+
+# ---- together ------------------------------------------------------------------
+
+
+def _backend(monkeypatch, fmt, H, HQ, D):
+    import math
+    monkeypatch.setenv("RQ_CACHE_8BIT", fmt)
+    monkeypatch.delenv("RQ_DENSE_3BIT", raising=False)
+    from rotorquant_vllm.vllm import rq_backend as B
+    return B, B.RQAttentionImpl(HQ, D, 1 / math.sqrt(D), num_kv_heads=H)
+
+
+def _metadata(slots, table, lens, q_lens, host=True):
+    import types
+    md = types.SimpleNamespace(num_actual_tokens=sum(q_lens), max_query_len=max(q_lens), use_cascade=False, block_table=i32(table), seq_lens=i32(lens),
+                               slot_mapping=torch.from_numpy(np.asarray(slots, np.int64)).to(DEV), query_start_loc=i32(np.concatenate([[0], np.cumsum(q_lens)])))
+    if host:
+        md.rq_seq_lens_cpu, md.rq_query_start_loc_cpu = md.seq_lens.cpu(), md.query_start_loc.cpu()
+    return md
+
+
+@pytest.mark.parametrize("fmt,H,G,D,block,dtype", [("int8", 2, 4, 128, 16, torch.bfloat16), ("fp8", 3, 2, 64, 32, torch.float16)])
+def test_backend_steps(monkeypatch, fmt, H, G, D, block, dtype):
+    """Prompts, then a mixed batch (decodes, a draft, a prompt chunk), then decodes, through the backend: the cache and every
+    output against the plain implementation."""
+    B, impl = _backend(monkeypatch, fmt, H, H * G, D)
+    final = [75, 60, 40, 310]
+    table, pages = Q.layout(final, block, 3)
+    cache = torch.zeros(B.RQAttentionBackend.get_kv_cache_shape(pages, block, H, D), dtype=torch.uint8, device=DEV)
+    ref = Q.Cache(pages, block, H, D, fmt)
+    done = [0, 0, 0, 0]
+    for step, q_lens in enumerate(([70, 50, 33, 0], [1, 1, 5, 300], [1, 1, 1, 1], [2, 7, 0, 3])):
+        seqs = [b for b in range(4) if q_lens[b]]
+        q_step = [q_lens[b] for b in seqs]
+        slots = np.concatenate([Q.slots_of(table, b, done[b], done[b] + q_lens[b], block) for b in seqs])
+        for b in seqs:
+            done[b] += q_lens[b]
+        lens = [done[b] for b in seqs]
+        n = sum(q_step)
+        k, v = Q.rows(n, H, D, 50 + step, dtype)
+        q = torch.randn(n, H * G, D, generator=torch.Generator().manual_seed(step)).to(dtype)
+        out = torch.full((n + 1, H * G, D), 9.0, dtype=dtype, device=DEV)
+        md = _metadata(slots, table[seqs], lens, q_step, host=step != 2)
+        impl.forward(None, q.to(DEV), k.to(DEV), v.to(DEV), cache, md, output=out)
+        ref.store(k, v, slots)
+        agree(cache, ref, fmt)
+        want, tol = Q.attention(q, ref.values(), table[seqs], lens, np.concatenate([[0], np.cumsum(q_step)]), block)
+        assert (np.abs(out[:n].double().cpu().numpy() - want) <= tol).all(), step
+        assert bool((out[n] == 9.0).all())
+
+
+def test_backend_decode_graph(monkeypatch):
+    """A captured decode step (store and attention) replayed over longer contexts, with eager work in between."""
+    H, G, D, block, fmt = 2, 4, 128, 16, "int8"
+    B, impl = _backend(monkeypatch, fmt, H, H * G, D)
+    start, steps = [40, 700, 5], 20
+    table, pages = Q.layout([n + steps for n in start], block, 8)
+    cache, ref = new_cache(pages, block, H, D), Q.Cache(pages, block, H, D, fmt)
+    k0, v0 = Q.rows(sum(start), H, D, 60, torch.bfloat16)
+    store(cache, ref, k0, v0, np.concatenate([Q.slots_of(table, b, 0, n, block) for b, n in enumerate(start)]), fmt)
+    buf = {"q": torch.zeros(3, H * G, D, dtype=torch.bfloat16, device=DEV), "k": torch.zeros(3, H, D, dtype=torch.bfloat16, device=DEV),
+           "v": torch.zeros(3, H, D, dtype=torch.bfloat16, device=DEV), "out": torch.zeros(3, H * G, D, dtype=torch.bfloat16, device=DEV)}
+    md = _metadata([-1, -1, -1], table, start, [1, 1, 1], host=False)
+    step = lambda: impl.forward(None, buf["q"], buf["k"], buf["v"], cache, md, output=buf["out"])  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()  # (slots of -1: nothing is stored)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    lens = list(start)
+    for i in range(steps):
+        k, v = Q.rows(3, H, D, 70 + i, torch.bfloat16)
+        q = torch.randn(3, H * G, D, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16)
+        slots = np.concatenate([Q.slots_of(table, b, n, n + 1, block) for b, n in enumerate(lens)])
+        lens = [n + 1 for n in lens]
+        buf["q"].copy_(q), buf["k"].copy_(k), buf["v"].copy_(v)
+        md.slot_mapping.copy_(torch.from_numpy(slots)), md.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        ref.store(k, v, slots)
+        got = buf["out"].clone()
+        eager = K.q8_attention(buf["q"], cache, md.block_table, md.seq_lens, H, D, fmt=fmt)
+        assert torch.equal(got, eager)
+        if i % 6 == 0:
+            torch.cuda.synchronize()
+            agree(cache, ref, fmt)
+            want, tol = Q.attention(q, ref.values(), table, lens, [0, 1, 2, 3], block)
+            assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
+
+
+def test_captured_prompt_and_long_store():
+    """A store of more than 512 tokens, a prompt and a read-back in one graph: several replays with new inputs."""
+    H, G, D, block, fmt, n = 2, 4, 128, 16, "fp8", 600
+    table, pages = Q.layout([n], block, 4)
+    cache = new_cache(pages, block, H, D)
+    slots = torch.from_numpy(Q.slots_of(table, 0, 0, n, block)).to(DEV)
+    bt, sl, cu = i32(table), i32([n]), i32([0, n])
+    k, v = (x.to(DEV) for x in Q.rows(n, H, D, 1, torch.bfloat16))
+    q = torch.zeros(n, H * G, D, dtype=torch.bfloat16, device=DEV)
+
+    def work():
+        K.q8_store(k, v, cache, slots, fmt=fmt)
+        return K.q8_attention(q, cache, bt, sl, H, D, fmt=fmt, cu_seqlens_q=cu, max_q_len=n), K.q8_read(cache, bt, sl, cu, H, D, torch.bfloat16, fmt=fmt, total=n)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, (rk, rv) = work()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        a, b = Q.rows(n, H, D, 90 + i, torch.bfloat16)
+        k.copy_(a), v.copy_(b)
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        got = [x.clone() for x in (out, rk, rv)]
+        eager_out, (ek, ev) = work()
+        torch.cuda.synchronize()
+        for x, y in zip(got, (eager_out, ek, ev)):
+            assert torch.equal(x, y)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams have scratch of their own."""
+    H, G, D, block = 2, 4, 128, 16
+    lens = [5000, 300, 4000]
+    cache, ref, table = filled(lens, block, H, D, "int8", torch.bfloat16, 5)
+    bt, sl = i32(table), i32(lens)
+    qs = [torch.randn(3, H * G, D, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).to(DEV) for i in range(2)]
+    want = [K.q8_attention(q, cache, bt, sl, H, D) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(K.q8_attention(qs[i], cache, bt, sl, H, D))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_strided_and_expanded_inputs():
+    """q as a view of a fused projection, an output row stride, a transposed block table, a shared prefix (the same pages twice)."""
+    H, G, D, block = 2, 4, 128, 16
+    lens = [90, 90]
+    cache, ref, table = filled([90], block, H, D, "int8", torch.bfloat16, 6)
+    table = np.concatenate([table, table])
+    qkv = torch.randn(2, (H * G + 2 * H) * D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(DEV)
+    q = qkv[:, :H * G * D].view(2, H * G, D)
+    wide = torch.full((2, H * G, D + 8), 3.0, dtype=torch.bfloat16, device=DEV)
+    bt = i32(np.ascontiguousarray(table.T)).t()
+    got = K.q8_attention(q, cache, bt, i32(lens), H, D, out=wide[..., :D])
+    want, tol = Q.attention(q.cpu(), ref.values(), table, lens, [0, 1, 2], block)
+    assert got.data_ptr() == wide.data_ptr() and bool((wide[..., D:] == 3.0).all())
+    assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
+    odd = torch.zeros(2 * H * G * D + 4, dtype=torch.bfloat16, device=DEV)[4:].view(2, H * G, D)  # 8 bytes off
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        K.q8_attention(odd, cache, bt, i32(lens), H, D)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        K.q8_store(odd[:, :H], odd[:, :H], cache, torch.zeros(2, dtype=torch.int64, device=DEV))
+
+
+def test_empty_calls():
+    H, D = 2, 128
+    cache = new_cache(2, 16, H, D)
+    e = torch.zeros(0, H, D, dtype=torch.bfloat16, device=DEV)
+    K.q8_store(e, e, cache, torch.zeros(0, dtype=torch.int64, device=DEV))
+    k, v = K.q8_read(cache, i32(np.zeros((0, 1))), i32([]), i32([]), H, D, torch.bfloat16, total=0)
+    assert k.shape == v.shape == (0, H, D)
+    q = torch.zeros(0, 8, D, dtype=torch.bfloat16, device=DEV)
+    assert K.q8_attention(q, cache, i32(np.zeros((0, 1))), i32([]), H, D).shape == (0, 8, D)
+    # a zeroed page reads as zeros, and attends as zeros
+    k, v = K.q8_read(cache, i32([[0]]), i32([5]), i32([0]), H, D, torch.float32, total=5)
+    assert not k.any() and not v.any()
+    q = torch.ones(1, 8, D, dtype=torch.bfloat16, device=DEV)
+    assert K.q8_attention(q, cache, i32([[0]]), i32([5]), H, D).abs().max() < 1e-9
+    # a table without pages: nothing to see
+    out = K.q8_attention(q, cache, torch.zeros(1, 0, dtype=torch.int32, device=DEV), i32([5]), H, D)
+    assert not out.any()

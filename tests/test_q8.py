@@ -125,3 +125,92 @@ def test_python_refusals():
         q8._device_index(cache)
     with pytest.raises(ValueError, match="block_table must be"):
         q8._index(i.long()[None], "block_table", torch.int32, 2)
+
+
+# ---- backend ------------------------------------------------------------------
+
+
+def _impl(monkeypatch, fmt="int8", heads=8, head_size=128, kv_heads=2):
+    monkeypatch.setenv("RQ_CACHE_8BIT", fmt)
+    monkeypatch.delenv("RQ_DENSE_3BIT", raising=False)
+    from rotorquant_vllm.vllm import rq_backend as B
+    return B, B.RQAttentionImpl(heads, head_size, 0.1, num_kv_heads=kv_heads)
+
+
+def test_backend_environment(monkeypatch):
+    from rotorquant_vllm.vllm import rq_backend as B
+    for off in (None, ""):
+        monkeypatch.delenv("RQ_CACHE_8BIT", raising=False) if off is None else monkeypatch.setenv("RQ_CACHE_8BIT", off)
+        assert B._parse_cache_8bit() is None
+        assert B.RQAttentionBackend.get_kv_cache_shape(7, 16, 4, 128) == (7, 16, 1024)
+    monkeypatch.setenv("RQ_CACHE_8BIT", "FP8")
+    assert B._parse_cache_8bit() == "fp8"
+    assert B.RQAttentionBackend.get_kv_cache_shape(100, 32, 8, 128) == (100, 32, 2056)
+    assert B.RQFullAttentionSpec(block_size=32, num_kv_heads=8, head_size=128, dtype=torch.uint8).real_page_size_bytes == 32 * 2056
+    with pytest.raises(ValueError, match="multiple of 16"):
+        B.RQAttentionBackend.get_kv_cache_shape(100, 8, 8, 128)
+    monkeypatch.setenv("RQ_DENSE_3BIT", "1")
+    with pytest.raises(ValueError, match="two cache layouts"):
+        B._parse_cache_8bit()
+    monkeypatch.setenv("RQ_CACHE_8BIT", "int4")
+    with pytest.raises(ValueError, match="RQ_CACHE_8BIT must be"):
+        B._parse_cache_8bit()
+
+
+def test_backend_shapes(monkeypatch):
+    B, impl = _impl(monkeypatch, "int8", 34, 64, 2)  # any GQA group
+    assert impl._q8_format == "int8" and not impl._fused_paged_available
+    with pytest.raises(ValueError, match="head_size 64 or 128"):
+        _impl(monkeypatch, "int8", 8, 96, 2)
+    with pytest.raises(ValueError, match="query heads over"):
+        _impl(monkeypatch, "int8", 9, 128, 2)
+    support = B.RQMetadataBuilder.get_cudagraph_support
+    spec = lambda d: B.RQFullAttentionSpec(block_size=16, num_kv_heads=2, head_size=d, dtype=torch.uint8)  # noqa: E731
+    if B._fused_paged_kernel_available:
+        assert support(None, spec(64)) == support(None, spec(128)) == B.AttentionCGSupport.UNIFORM_SINGLE_TOKEN_DECODE
+    assert support(None, spec(96)) == B.AttentionCGSupport.NEVER
+
+
+@pytest.mark.parametrize("q_lens,max_query_len,want", [
+    ([1, 1, 1], 1, [(0, 3, None, 1)]),
+    ([1, 3, 2], 3, [(0, 3, 6, 3)]),
+    ([1, 1, 5, 300, 1], 300, [(0, 2, None, 1), (2, 3, 308, 5), (3, 5, 308, 300)]),
+    ([300, 1], None, [(0, 2, 301, 300)])])
+@pytest.mark.parametrize("host", [True, False])
+def test_backend_calls(monkeypatch, q_lens, max_query_len, want, host):
+    """Which sequences go to which call, with which bounds."""
+    from types import SimpleNamespace
+    B, impl = _impl(monkeypatch)
+    calls, stored = [], []
+
+    def attend(q, kv_cache, block_table, seq_lens, H, D, fmt, sm_scale, causal, cu_seqlens_q, max_q_len, max_seq_len, out):
+        b0 = int(block_table[0, 0])
+        calls.append((b0, b0 + seq_lens.numel(), None if cu_seqlens_q is None else q.shape[0], max_q_len))
+        assert block_table.shape[0] == seq_lens.numel() and (fmt, H, D, sm_scale, causal) == ("int8", 2, 128, 0.1, True)
+        assert out.shape == q.shape and out.data_ptr() == (output if cu_seqlens_q is not None else output[b0:]).data_ptr()
+        if cu_seqlens_q is None:
+            assert q.shape[0] == seq_lens.numel()
+        else:
+            assert cu_seqlens_q.tolist() == starts[b0:b0 + seq_lens.numel() + 1]
+        # host lengths bound the contexts; without them a batch of one call goes by the table's capacity
+        assert max_seq_len == (max(lens[b0:b0 + seq_lens.numel()]) if host or len(want) > 1 or max(q_lens) == 300 else None)
+
+    monkeypatch.setattr(B, "_q8_attention_fn", attend)
+    monkeypatch.setattr(B, "_q8_store_fn", lambda k, v, cache, slots, fmt: stored.append((k.shape[0], v.shape[0], slots.numel(), fmt)))
+    n, lens = sum(q_lens), [600 + i for i in range(len(q_lens))]
+    starts = [0] + list(np.cumsum(q_lens))
+    q, output = torch.zeros(n + 2, 8, 128), torch.zeros(n + 2, 8, 128)
+    k = torch.zeros(n + 2, 2, 128)
+    md = SimpleNamespace(num_actual_tokens=n, block_table=torch.arange(len(q_lens), dtype=torch.int32)[:, None].repeat(1, 3),
+                         seq_lens=torch.tensor(lens, dtype=torch.int32), query_start_loc=torch.tensor(starts, dtype=torch.int32),
+                         slot_mapping=torch.arange(n), max_query_len=max_query_len)
+    if host:
+        md.rq_query_start_loc_cpu, md.rq_seq_lens_cpu = md.query_start_loc, md.seq_lens
+    cache = torch.zeros(4, 16, 520, dtype=torch.uint8)
+    assert impl.forward(None, q, k, k, cache, md, output=output) is output
+    assert calls == want and stored == [(n, n, n, "int8")]
+    impl.forward(None, q, None, None, cache, md, output=output)  # nothing new to store
+    assert len(stored) == 1
+    md.use_cascade = True
+    with pytest.raises(NotImplementedError):
+        impl.forward(None, q, k, k, cache, md, output=output)
