@@ -11,6 +11,7 @@ streams at once (scratch comes from torch's allocator unless passed).
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -34,7 +35,7 @@ def _format(fmt: str) -> int:
 def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     """Index of the device that all tensors are on."""
     dev = first.get_device()
-    for t in (first, *others):
+    for t in others if dev >= 0 else (first,):
         if t is not None and (dev < 0 or t.get_device() != dev):
             if not (first.is_cuda and t.is_cuda):
                 raise RuntimeError("rotorquant_vllm.kernels runs only on ROCm device tensors (got a "
@@ -64,17 +65,29 @@ def _check_cache(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> tu
     if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 3:
         raise ValueError("kv_cache must be a (num_blocks, block_size, q8_slot_bytes) uint8 tensor")
     NB, BS, SB = kv_cache.shape
-    if SB < q8_slot_bytes(num_kv_heads, head_dim):
+    if SB < num_kv_heads * (2 * head_dim + 1):
         raise ValueError(f"cache slots of {SB} bytes; {num_kv_heads} heads of {head_dim} take {q8_slot_bytes(num_kv_heads, head_dim)}")
-    if kv_cache.stride(2) != 1 or kv_cache.stride(1) != SB:
+    page, slot, byte = kv_cache.stride()
+    if byte != 1 or slot != SB:
         raise ValueError("the slots of a page must be contiguous")
-    return NB, BS, kv_cache.stride(0)
+    return NB, BS, page
 
 
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> torch.Tensor:
     if t.dtype != dtype or t.dim() != dim:
         raise ValueError(f"{name} must be a {dim}-dimensional {dtype} tensor, got {t.dim()} dimensions of {t.dtype}")
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+# Sizes of scratch, by sizes alone (0.1 against 0.5 us a call).
+@functools.lru_cache(maxsize=4096)
+def _store_bytes(n_tokens: int, num_blocks: int, block_size: int) -> int:
+    return _lib.load().rq_q8_store_workspace_bytes(n_tokens, num_blocks, block_size)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_q_len: int, max_seq_len: int) -> int:
+    return _lib.load().rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len)
 
 
 def _scratch(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int, int]:
@@ -102,18 +115,17 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
     if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
         raise ValueError("key and value must have the same (tokens, heads, head_dim) shape and dtype")
     N, H, D = key.shape
-    if key.stride(2) != 1 or value.stride(2) != 1:
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1 or vs[2] != 1:
         raise ValueError("key/value must be contiguous over head_dim")
     NB, BS, stride = _check_cache(kv_cache, H, D)
     sm = _index(slot_mapping, "slot_mapping", torch.int64, 1)
     if sm.numel() < N:
         raise ValueError("slot_mapping shorter than the number of tokens")
     code = _format(fmt)
-    L = _lib.load()
-    keep, ws, ws_bytes = _scratch(workspace, L.rq_q8_store_workspace_bytes(N, NB, BS), kv_cache)
-    _call(L.rq_q8_store, "rq_q8_store", dev,
-          (key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), N, key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-           H, D, code, sm.data_ptr(), kv_cache.data_ptr(), NB, BS, stride, ws, ws_bytes))
+    keep, ws, ws_bytes = _scratch(workspace, _store_bytes(N, NB, BS), kv_cache)
+    _call(_lib.load().rq_q8_store, "rq_q8_store", dev,
+          (key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), N, ks[0], ks[1], vs[0], vs[1], H, D, code, sm.data_ptr(), kv_cache.data_ptr(), NB, BS, stride, ws, ws_bytes))
 
 
 def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor, num_kv_heads: int,
@@ -192,12 +204,12 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     capacity = bt.shape[1] * BS
     max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
     code = _format(fmt)
-    L = _lib.load()
     out = torch.empty_like(q) if out is None else out
-    keep, ws, ws_bytes = _scratch(workspace, L.rq_q8_attention_workspace_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
-    _call(L.rq_q8_attention, "rq_q8_attention", dev,
-          (q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, q.stride(0), q.stride(1), None if cu is None else cu.data_ptr(), B, max_q_len,
+    qs, os = q.stride(), out.stride()
+    keep, ws, ws_bytes = _scratch(workspace, _attention_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
+    _call(_lib.load().rq_q8_attention, "rq_q8_attention", dev,
+          (q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, qs[0], qs[1], None if cu is None else cu.data_ptr(), B, max_q_len,
            1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(), bt.shape[1], bt.stride(0),
-           sl.data_ptr(), max_seq_len, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0),
-           out.stride(1), ws, ws_bytes))
+           sl.data_ptr(), max_seq_len, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), os[0],
+           os[1], ws, ws_bytes))
     return out
