@@ -89,7 +89,8 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
                 r = -1;
             }
         }
-        for (; r >= 0; r = a.before[r]) {
+        // (each run is linked once, so the walk ends by itself; the bounds hold also where slots change under the call)
+        for (int64_t left = a.n_tokens; r >= 0 && r < a.n_tokens && left > 0; r = a.before[r], --left) {
             for (int64_t s = r;; s += 64) {  // the run: up to the first token of another group
                 const bool in = s + lane < a.n_tokens && q8_group_of(a, s + lane) == g;
                 const uint64_t out = ~__ballot(in);

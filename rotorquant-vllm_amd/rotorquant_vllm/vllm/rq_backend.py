@@ -660,7 +660,7 @@ class RQAttentionImpl(_ImplBase):
         if q.is_cuda and torch.cuda.is_current_stream_capturing():
             sl_cpu = None
         qsl_cpu = getattr(md, "rq_query_start_loc_cpu", None)
-        max_q = getattr(md, "max_query_len", None)
+        max_q = 1 if n == 1 else getattr(md, "max_query_len", None)
         if max_q is None:
             qsl_cpu = qsl_cpu if qsl_cpu is not None else md.query_start_loc.cpu()
             max_q = int((qsl_cpu[1:] - qsl_cpu[:-1]).max()) if qsl_cpu.numel() > 1 else 0

@@ -515,3 +515,115 @@ def test_empty_calls():
     # a table without pages: nothing to see
     out = K.q8_attention(q, cache, torch.zeros(1, 0, dtype=torch.int32, device=DEV), i32([5]), H, D)
     assert not out.any()
+
+
+# ---- sizes that change the path -------------------------------------------------
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_many_sequences(fmt):
+    """More than 64 sequences, some empty, shared out over the GPU (a long bound) and an item each (a short one)."""
+    H, G, D, block = 1, 3, 64, 16
+    rng = np.random.RandomState(3)
+    lens = [int(n) for n in rng.randint(0, 50, 150)]
+    lens[70], lens[140] = 700, 400
+    cache, ref, table = filled(lens, block, H, D, fmt, torch.bfloat16, 17)
+    q = torch.randn(150, H * G, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out, tol = Q.attention(q, ref.values(), table, lens, range(151), block)
+    wide = np.zeros((150, 200), np.int32)
+    wide[:, :table.shape[1]] = table
+    for t in (table, wide):
+        got = K.q8_attention(q.to(DEV), cache, i32(t), i32(lens), H, D, fmt=fmt)
+        assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+    queries = [int(n) for n in rng.randint(0, 6, 150)]
+    cu = np.concatenate([[0], np.cumsum(queries)])
+    q = torch.randn(int(cu[-1]), H * G, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    out, tol = Q.attention(q, ref.values(), table, lens, cu, block)
+    for t in (table, wide):
+        got = K.q8_attention(q.to(DEV), cache, i32(t), i32(lens), H, D, fmt=fmt, cu_seqlens_q=i32(cu), max_q_len=5)
+        assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompts_in_several_passes(D):
+    """A table so wide that the tile images of one kv head fill a pass: one launch pair per sequence and head."""
+    H, G, block = 2, 4, 32
+    lens, queries = [90, 0, 200], [90, 0, 70]
+    cache, ref, table = filled(lens, block, H, D, "int8", torch.bfloat16, 18)
+    cu = [0, 90, 90, 160]
+    q = torch.randn(160, H * G, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out, tol = Q.attention(q, ref.values(), table, lens, cu, block)
+    wide = np.zeros((3, 16384), np.int32)
+    wide[:, :table.shape[1]] = table
+    for t, bound in ((wide, None), (table, None), (wide, 200)):
+        got = K.q8_attention(q.to(DEV), cache, i32(t), i32(lens), H, D, cu_seqlens_q=i32(cu), max_q_len=90, max_seq_len=bound)
+        assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+
+
+def test_cache_past_32_bits():
+    """Pages more than 4 GiB into a cache: written, read back and attended to."""
+    H, G, D, block, n = 8, 2, 128, 16, 100
+    pages = (5 << 30) // (block * K.q8_slot_bytes(H, D))
+    cache = torch.empty(pages, block, K.q8_slot_bytes(H, D), dtype=torch.uint8, device=DEV)
+    table = np.arange(pages - 7, pages, dtype=np.int32)[None]
+    small, ref = np.arange(7, dtype=np.int32)[None], Q.Cache(7, block, H, D, "fp8")
+    k, v = Q.rows(n, H, D, 8, torch.bfloat16)
+    K.q8_store(k.to(DEV), v.to(DEV), cache, torch.from_numpy(Q.slots_of(table, 0, 0, n, block)).to(DEV), fmt="fp8")
+    ref.store(k, v, Q.slots_of(small, 0, 0, n, block))
+    kv = ref.values()
+    got = K.q8_read(cache, i32(table), i32([n]), i32([0]), H, D, torch.float32, fmt="fp8", total=n)
+    for side in range(2):
+        assert np.array_equal(got[side].cpu().numpy(), kv[side][Q.slots_of(small, 0, 0, n, block)].astype(np.float32))
+    for T in (1, 100):  # (the second by the prefill kernels)
+        q = torch.randn(T, H * G, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+        out, tol = Q.attention(q, kv, small, [n], [0, T], block)
+        got = K.q8_attention(q.to(DEV), cache, i32(table), i32([n]), H, D, fmt="fp8", cu_seqlens_q=i32([0, T]))
+        assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+
+
+def test_nan_and_infinite_queries_stay_in_their_rows():
+    H, G, D, block = 1, 4, 128, 16
+    cache, ref, table = filled([60], block, H, D, "int8", torch.bfloat16, 19)
+    for T in (1, 6, 60):  # item, columns of a block, prefill
+        q = torch.randn(T, H * G, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+        clean = K.q8_attention(q.to(DEV), cache, i32(table), i32([60]), H, D, cu_seqlens_q=i32([0, T]))
+        bad = q.clone()
+        bad[T // 2, 1, 5] = float("nan")
+        bad[T // 2, 2, 6] = float("inf")
+        got = K.q8_attention(bad.to(DEV), cache, i32(table), i32([60]), H, D, cu_seqlens_q=i32([0, T]))
+        keep = torch.ones(T, H * G, dtype=torch.bool)
+        keep[T // 2, 1:3] = False
+        assert torch.equal(got[keep.to(DEV)], clean[keep.to(DEV)])
+        assert not torch.isfinite(got[T // 2, 1:3]).any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_memory_behind_the_contexts_in_prompts(fmt):
+    """As above, for the prefill kernels: the rows of the last group behind a prompt hold NaN's codes."""
+    H, G, D, block, n = 1, 4, 128, 64, 69
+    k, v = Q.rows(n, H, D, 6, torch.bfloat16)
+    table, pages = Q.layout([n], block, 2)
+    clean, dirty = new_cache(pages, block, H, D), new_cache(pages, block, H, D, fill=0xff)
+    slots = torch.from_numpy(Q.slots_of(table, 0, 0, n, block)).to(DEV)
+    for c in (clean, dirty):
+        K.q8_store(k.to(DEV), v.to(DEV), c, slots, fmt=fmt)
+    idx_k, idx_v, _ = Q.code_index(block, H, D)
+    raw = dirty[table[0, 1]].view(-1)
+    for idx in (idx_k, idx_v):
+        raw[torch.from_numpy(idx[n - 64:16].reshape(-1)).to(DEV)] = 0x7f
+    q = torch.randn(n, H * G, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    for causal in (True, False):
+        a, b = (K.q8_attention(q, c, i32(table), i32([n]), H, D, fmt=fmt, causal=causal, cu_seqlens_q=i32([0, n])) for c in (clean, dirty))
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_shapes(seed):
+    rng = np.random.RandomState(1000 + seed)
+    H, G, D, block = int(rng.choice([1, 2, 3, 5])), int(rng.choice([1, 2, 4, 6, 9])), int(rng.choice([64, 128])), int(rng.choice([16, 32, 48, 128]))
+    fmt, dtype = FMTS[seed % 2], [torch.bfloat16, torch.float16][(seed // 2) % 2]
+    B = int(rng.randint(1, 7))
+    lens = [int(n) for n in rng.randint(0, int(rng.choice([40, 300])), B)]
+    queries = [int(rng.randint(0, int(rng.choice([2, 8, 90])) + 1)) for _ in range(B)]
+    queries[0] = max(1, queries[0])
+    attend(lens, queries, block, H, G, D, fmt, dtype, 40 + seed, causal=bool(rng.randint(0, 4)))
