@@ -31,7 +31,7 @@ struct Q8Image {
     static constexpr int kVAt = kKMeta + 1024;
     static constexpr int kVMeta = kVAt + kV * 1024;       // float 2^-e_v of the four groups
     static constexpr int kBytes = kVMeta + 1024;
-    static constexpr int kLdsK = kKMeta + 32, kLdsV = kV * 1024 + 16;
+    static constexpr int kLdsK = kKMeta + 1024, kLdsV = kV * 1024 + 1024;
     static constexpr int kPart = kQ8PW * D + kQ8PW * 2;   // floats of a wave's partial
 };
 
@@ -130,6 +130,16 @@ __global__ __launch_bounds__(256) void q8_pack_kernel(Q8PrefillArgs p) {
 }
 
 // ---- attention ----------------------------------------------------------------------
+// N consecutive KB: the immediate offset moves both the source and the place in LDS.
+template <int N>
+__device__ __forceinline__ void copy16n(const uint8_t *src, uint32_t voff, uint32_t dst) {
+    if constexpr (N == 4)
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %0, %1 offset:2048\n\tglobal_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(voff), "s"(src), "{m0}"(dst) : "memory");
+    else
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(voff), "s"(src), "{m0}"(dst) : "memory");
+}
+
 constexpr int kQ8MinTiles = 4;  // tiles of a key chunk, at least
 struct Q8Block {
     Q8Seq s;
@@ -190,20 +200,17 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
     uint8_t *const vbuf[2] = {lds + 2 * Im::kLdsK, lds + 2 * Im::kLdsK + Im::kLdsV};
     const uint8_t *const img0 = p.images + (((int64_t)bl * p.nh + hl) * p.max_tiles + t0) * Im::kBytes;
     const uint32_t lds0 = lds_addr(lds);
-    auto copy = [&](int t, int from, int meta, int meta_lanes, uint32_t dst_) {
-        const uint64_t src64 = reinterpret_cast<uint64_t>(img0 + (int64_t)t * Im::kBytes + from);
+    constexpr int kChunksW = kF / kQ8PWaves;  // 1 KB chunks of a wave: consecutive, one address and immediate offsets for all
+    auto copy = [&](int t, int from, uint32_t dst_) {
+        const uint64_t src64 = reinterpret_cast<uint64_t>(img0 + (int64_t)t * Im::kBytes + from + wave * (kChunksW * 1024));
         const uint32_t slo = __builtin_amdgcn_readfirstlane((uint32_t)src64), shi = __builtin_amdgcn_readfirstlane((uint32_t)(src64 >> 32));
         const uint8_t *src = reinterpret_cast<const uint8_t *>(((uint64_t)shi << 32) | slo);
         const uint32_t dst = __builtin_amdgcn_readfirstlane(dst_);
-#pragma unroll
-        for (int u = 0; u < kF / kQ8PWaves; ++u) {
-            const int c = u * kQ8PWaves + wave;
-            copy16(src + c * 1024, 16 * lane, dst + c * 1024);
-        }
-        if (wave == 0 && lane < meta_lanes) copy16(src + meta, 16 * lane, dst + kF * 1024);
+        copy16n<kChunksW>(src, 16 * lane, dst + wave * (kChunksW * 1024));
+        if (wave == 0) copy16(src + kF * 1024, 16 * lane, dst + kF * 1024);  // the groups' scales
     };
-    auto copy_k = [&](int t) { if (t < n_tiles) copy(t, 0, Im::kKMeta, 2, lds0 + (t & 1) * Im::kLdsK); };
-    auto copy_v = [&](int t) { if (t < n_tiles) copy(t, Im::kVAt, Im::kVMeta - Im::kVAt, 1, lds0 + 2 * Im::kLdsK + (t & 1) * Im::kLdsV); };
+    auto copy_k = [&](int t) { if (t < n_tiles) copy(t, 0, lds0 + (t & 1) * Im::kLdsK); };
+    auto copy_v = [&](int t) { if (t < n_tiles) copy(t, Im::kVAt, lds0 + 2 * Im::kLdsK + (t & 1) * Im::kLdsV); };
 
     // Q^T operand, loaded before the first copies go out (a wait for a load also waits for copies issued before it)
     u32x4 qop[kSteps];
