@@ -16,6 +16,14 @@
 //
 // Operands need neither LDS nor shuffles: a lane's 16 bytes of K and V are its operands' elements (rq_q8.h), and
 // the weights come out of S^T in the order that P V takes.
+//
+// What bounds it: the stream of codes.  64 sequences of 1024 to 8192 keys, 8 kv heads x 4 (609 MB): the stream kernel
+// 99 to 102 us, 6.0 TB/s, which is what a plain read reaches on this card; whole call 106, the merge 4.8.  A wave holds
+// the next tile (8 KB at head_dim 128) in registers while it computes one; two workgroups of four waves a CU (175
+// registers) keep 64 KB a CU on their way.  Three workgroups a CU (168 registers, 10 spilled, or one tile of registers
+// refilled as it is used) 127 to 130 us against 127 before the loads became non-temporal; two tiles ahead 109 against 107;
+// twice or four times the workgroups, which balance themselves, 130 and 139 (more partials, more prologues).  Small calls are bound by
+// their chain of dependent loads: lengths, block table, codes, then the sums of the waves.
 #include <algorithm>
 
 #include "rq_q8_attn.h"
@@ -435,8 +443,8 @@ __global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
     q8_segment<DT, FMT, D, NB, 8, ONCE>(a, seq, s, h, block * (NB * kQ8Cols), 0, q8_tiles(s), nullptr, lds);
 }
 
-// Blocks of 16 columns that a workgroup takes, and the workgroups: what the GPU holds at once, or fewer where the bound on the lengths
-// gives less work.
+// Blocks of 16 columns that a workgroup takes (two share a stream of codes and its conversions: 32 drafts of up to 8 tokens x 4 heads
+// 85 -> 77 us), and the workgroups: what the GPU holds at once, or fewer where the bound on the lengths gives less work.
 static int q8_blocks(int G, int64_t max_q_len) { return max_q_len * G > kQ8Cols ? 2 : 1; }
 static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
     const int nb = q8_blocks(G, max_q_len), cols = nb * kQ8Cols;

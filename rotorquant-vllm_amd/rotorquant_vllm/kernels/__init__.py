@@ -19,6 +19,8 @@ the C ABI (include/rq_abi.h).  Differences, all deliberate:
   with each 64-key tile decoded once, for long queries (two launches, or three
   where few query blocks are spread over the GPU by key chunks).  Calls of at most 16
   tokens per sequence run on the decode kernels (three launches) where that is faster.
+* q8_store, q8_read and q8_attention (kernels/q8.py) work on the 8-bit cache,
+  which the reference does not have.
 """
 from __future__ import annotations
 
