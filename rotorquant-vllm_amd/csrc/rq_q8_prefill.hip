@@ -160,9 +160,9 @@ __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int 
 __device__ __forceinline__ int q8_chunk_tiles(int n_tiles, int split) { return max(kQ8MinTiles, (n_tiles + split - 1) / split); }
 
 // What bounds it: the matrix cores and vector issue together, under the card's power limit.  8 prompts of 2222 to 4096 tokens, 32 / 8
-// heads (0.84 TFLOP): 855 to 885 us, 950 to 985 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
+// heads (0.84 TFLOP): 845 to 885 us, 950 to 995 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
 // 1800 of zeros).  The matrix cores are busy half of the cycles, at 1.8 GHz (the memory-bound kernels run at 2.1).  A wave's tile
-// is 32 MFMAs, 32 exponentials and about 77 other vector instructions; measured by itself, an MFMA with a pair of exponentials
+// is 32 MFMAs, 32 exponentials and about 93 other vector instructions; measured by itself, an MFMA with a pair of exponentials
 // and its packing takes 21.4 ns of a SIMD, without 13.8, so the first phase is bound by issue.  Without the tile copies 9 %
 // less time, without exponentials 6 %.  Tried without gain: two units a wave at one wave a SIMD (half the LDS reads; 226
 // registers spilled), eight waves on one tile (926 -> 931 us, one prompt of 700 tokens 24 -> 32), two sets of four waves on alternate
@@ -281,14 +281,14 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
     };
     auto k_op = [&](const uint8_t *kt, int fi) { return *reinterpret_cast<const u32x4 *>(kt + 16 * lane + 1024 * fi); };
     auto meta4 = [](const uint8_t *at) { return *reinterpret_cast<const float4 *>(at); };
-    // pair i of weights: its place in the operand, and its group's sum
+    // pair i of weights: its place in the operand, and its group's sum, of the weights before their rounding: fp16 loses those of
+    // groups whose V is 2^20 times smaller than others' (or zero), which the softmax's sum still has to hold
     auto exp_pair = [&](const f32x16 (&sc)[2], int i, uint32_t (&pop)[16], float (&l)[4]) {
-        const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
         const int t = i >> 2, e = 8 * (t & 1) + 2 * (i & 3);
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e], fg[t], add[t]));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e + 1], fg[t], add[t]));
         pop[i] = pack_f16(p0, p1);
-        l[t] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pop[i]), one, l[t], false);
+        l[t] += p0 + p1;
     };
     auto add_sums = [&](const float (&l)[4], const float4 iv) {
         l_run = __builtin_fmaf(l[0], iv.x, __builtin_fmaf(l[1], iv.y, __builtin_fmaf(l[2], iv.z, __builtin_fmaf(l[3], iv.w, l_run))));

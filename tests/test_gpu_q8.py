@@ -285,6 +285,25 @@ def test_groups_of_very_different_scales(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H,G,D,n,t", [(1, 4, 128, 96, 96), (2, 8, 64, 200, 30), (1, 1, 128, 193, 193)])
+def test_prompts_of_very_different_scales(fmt, H, G, D, n, t):
+    """As above, prompts: tokens whose weights fp16 does not hold (their V is 2^20 to 2^30 times smaller, or zero) keep their
+    place in the sum of the softmax."""
+    block = 16
+    k, v = Q.rows(n, H, D, 4, torch.float32, outliers=False)
+    k *= 0.25
+    for g in range(-(-n // 16)):
+        v[16 * g:16 * g + 16] *= (2.0 ** 10, 2.0 ** -20, 0.0, 1.0, 2.0 ** -10)[g % 5]
+    table, pages = Q.layout([n], block, 2)
+    ref, cache = Q.Cache(pages, block, H, D, fmt), new_cache(pages, block, H, D)
+    store(cache, ref, k, v, Q.slots_of(table, 0, 0, n, block), fmt)
+    q = torch.randn(t, H * G, D, generator=torch.Generator().manual_seed(2)).to(torch.float16)
+    out, tol = Q.attention(q, ref.values(), table, [n], [0, t], block)
+    got = K.q8_attention(q.to(DEV), cache, i32(table), i32([n]), H, D, fmt=fmt, cu_seqlens_q=i32([0, t]), max_q_len=t)
+    assert (np.abs(got.double().cpu().numpy() - out) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_memory_behind_the_contexts_is_not_read_as_numbers(fmt):
     """Pages full of bytes that no store wrote (NaN codes, infinite scales) behind a context's end, and never-begun groups."""
     H, D, block, n = 2, 128, 64, 37
