@@ -454,7 +454,7 @@ enum rq_q8_format {
     RQ_Q8_E4M3 = 1
 };
 
-/* Bytes of a cache slot (block_size of them make a page); 0 for sizes below 1. */
+/* Bytes of a cache slot (block_size of them make a page); 0 for sizes below 1 and for slots of 2^31 bytes or more. */
 int rq_q8_slot_bytes(int32_t num_kv_heads, int32_t head_dim);
 
 /*

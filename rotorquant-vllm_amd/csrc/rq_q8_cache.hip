@@ -430,7 +430,8 @@ using namespace rq;
 
 extern "C" int rq_q8_slot_bytes(int32_t num_kv_heads, int32_t head_dim) {
     if (num_kv_heads < 1 || head_dim < 1) return 0;
-    return (num_kv_heads * (2 * head_dim + 1) + 7) / 8 * 8;
+    const int64_t bytes = (num_kv_heads * (2 * (int64_t)head_dim + 1) + 7) / 8 * 8;
+    return bytes <= INT32_MAX ? (int)bytes : 0;
 }
 
 extern "C" int64_t rq_q8_store_workspace_bytes(int64_t n_tokens, int64_t num_blocks, int32_t block_size) {

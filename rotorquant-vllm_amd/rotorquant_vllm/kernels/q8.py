@@ -30,13 +30,17 @@ def _format(fmt: str) -> int:
         raise ValueError(f"fmt must be 'int8' or 'fp8', got {fmt!r}") from None
 
 
-# (calls of a few microseconds wait for the checks below: device indices and plain comparisons, no device objects)
+# Calls of a few microseconds wait for the checks below: device indices and plain comparisons, no device objects, and each
+# tensor's sizes and strides fetched once.
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (0.06 against 0.24 us)
+
 
 def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     """Index of the device that all tensors are on."""
     dev = first.get_device()
     for t in others if dev >= 0 else (first,):
-        if t is not None and (dev < 0 or t.get_device() != dev):
+        if dev < 0 or t is not None and t.get_device() != dev:
             if not (first.is_cuda and t.is_cuda):
                 raise RuntimeError("rotorquant_vllm.kernels runs only on ROCm device tensors (got a "
                                    f"{(t if first.is_cuda else first).device.type} tensor); there is no CPU path")
@@ -46,7 +50,7 @@ def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 
 def _call(fn, name: str, dev: int, args: tuple) -> None:
     """fn(*args, stream): a launch goes to the current device's context, so the tensors' own is made current."""
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         rc = fn(*args, _lib.stream_ptr(torch.device("cuda", dev)) if _lib._raw_stream is None else _lib._raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -62,9 +66,10 @@ def q8_slot_bytes(num_kv_heads: int, head_dim: int) -> int:
 
 def _check_cache(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> tuple[int, int, int]:
     """(pages, block_size, bytes between pages) of an 8-bit cache."""
-    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 3:
+    shape = kv_cache.shape
+    if kv_cache.dtype != torch.uint8 or len(shape) != 3:
         raise ValueError("kv_cache must be a (num_blocks, block_size, q8_slot_bytes) uint8 tensor")
-    NB, BS, SB = kv_cache.shape
+    NB, BS, SB = shape
     if SB < num_kv_heads * (2 * head_dim + 1):
         raise ValueError(f"cache slots of {SB} bytes; {num_kv_heads} heads of {head_dim} take {q8_slot_bytes(num_kv_heads, head_dim)}")
     page, slot, byte = kv_cache.stride()
@@ -76,7 +81,7 @@ def _check_cache(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> tu
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> torch.Tensor:
     if t.dtype != dtype or t.dim() != dim:
         raise ValueError(f"{name} must be a {dim}-dimensional {dtype} tensor, got {t.dim()} dimensions of {t.dtype}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
 
 # Sizes of scratch, by sizes alone (0.1 against 0.5 us a call).
@@ -112,9 +117,10 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
     by default from torch's allocator; a graph captured without torch's graph classes needs it.
     """
     dev = _device_index(key, value, kv_cache, slot_mapping, workspace)
-    if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
+    shape = key.shape
+    if len(shape) != 3 or value.shape != shape or value.dtype != key.dtype:
         raise ValueError("key and value must have the same (tokens, heads, head_dim) shape and dtype")
-    N, H, D = key.shape
+    N, H, D = shape
     ks, vs = key.stride(), value.stride()
     if ks[2] != 1 or vs[2] != 1:
         raise ValueError("key/value must be contiguous over head_dim")
@@ -142,23 +148,22 @@ def q8_read(kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.T
     NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
     bt = _index(block_table, "block_table", torch.int32, 2)
     sl, st = _index(seq_lens, "seq_lens", torch.int32, 1), _index(starts, "starts", torch.int32, 1)
-    B = bt.shape[0]
+    B, max_blocks = bt.shape
     if sl.numel() < B or st.numel() < B:
         raise ValueError("block_table, seq_lens and starts differ in the number of sequences")
-    given = [t for t in (out_k, out_v) if t is not None]
-    if total is None:
-        if not given:
-            raise ValueError("total (the number of rows) is needed without out_k and out_v")
-        total = given[0].shape[0]
-    shape = (total, num_kv_heads, head_dim)
-    for t in given:
-        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"outputs must be contiguous {shape} tensors of {dtype}")
     code = _format(fmt)
+    if total is None:
+        if out_k is None and out_v is None:
+            raise ValueError("total (the number of rows) is needed without out_k and out_v")
+        total = (out_v if out_k is None else out_k).shape[0]
+    shape = (total, num_kv_heads, head_dim)
+    for t in (out_k, out_v):
+        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"outputs must be contiguous {shape} tensors of {dtype}")
     out_k = torch.empty(shape, dtype=dtype, device=kv_cache.device) if out_k is None else out_k
     out_v = torch.empty(shape, dtype=dtype, device=kv_cache.device) if out_v is None else out_v
     _call(_lib.load().rq_q8_read, "rq_q8_read", dev,
-          (kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, head_dim, code, bt.data_ptr(), bt.shape[1], bt.stride(0), sl.data_ptr(),
+          (kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, head_dim, code, bt.data_ptr(), max_blocks, bt.stride(0), sl.data_ptr(),
            st.data_ptr(), B, total, out_k.data_ptr(), out_v.data_ptr(), _lib.dtype_code(dtype)))
     return out_k, out_v
 
@@ -177,15 +182,16 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     workspace: scratch (rq_q8_attention_workspace_bytes bytes), by default of this call from torch's allocator; a graph
     captured without torch's graph classes needs it, since nothing else keeps the scratch for its replays.
     """
-    if q.dim() != 3 or q.shape[2] != head_dim or num_kv_heads < 1 or q.shape[1] % num_kv_heads:
-        raise ValueError(f"q must be (tokens, a multiple of {num_kv_heads} heads, {head_dim}), got {tuple(q.shape)}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != head_dim or num_kv_heads < 1 or shape[1] % num_kv_heads:
+        raise ValueError(f"q must be (tokens, a multiple of {num_kv_heads} heads, {head_dim}), got {tuple(shape)}")
     dev = _device_index(q, kv_cache, block_table, seq_lens, cu_seqlens_q, out, workspace)
     NB, BS, stride = _check_cache(kv_cache, num_kv_heads, head_dim)
     bt = _index(block_table, "block_table", torch.int32, 2)
     sl = _index(seq_lens, "seq_lens", torch.int32, 1)
-    T, HQ, D = q.shape
-    B = sl.numel()
-    if bt.shape[0] != B:
+    T, HQ, D = shape
+    B, (tables, max_blocks) = sl.numel(), bt.shape
+    if tables != B:
         raise ValueError("block_table and seq_lens differ in the number of sequences")
     cu = None
     if cu_seqlens_q is None:
@@ -197,19 +203,21 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
         if cu.numel() != B + 1:
             raise ValueError(f"cu_seqlens_q must have {B + 1} entries, got {cu.numel()}")
         max_q_len = T if max_q_len is None else min(int(max_q_len), T)
-    if q.stride(-1) != 1:
+    qs = q.stride()
+    if qs[2] != 1:
         q = q.contiguous()
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1):
+        qs = q.stride()
+    out = torch.empty_like(q) if out is None else out
+    os = out.stride()
+    if out.shape != shape or out.dtype != q.dtype or os[2] != 1:
         raise ValueError("out must have q's shape and dtype and be contiguous over head_dim")
-    capacity = bt.shape[1] * BS
+    capacity = max_blocks * BS
     max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
     code = _format(fmt)
-    out = torch.empty_like(q) if out is None else out
-    qs, os = q.stride(), out.stride()
     keep, ws, ws_bytes = _scratch(workspace, _attention_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
     _call(_lib.load().rq_q8_attention, "rq_q8_attention", dev,
           (q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, qs[0], qs[1], None if cu is None else cu.data_ptr(), B, max_q_len,
-           1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(), bt.shape[1], bt.stride(0),
+           1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(), max_blocks, bt.stride(0),
            sl.data_ptr(), max_seq_len, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), os[0],
            os[1], ws, ws_bytes))
     return out

@@ -285,7 +285,7 @@ def test_groups_of_very_different_scales(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("H,G,D,n,t", [(1, 4, 128, 96, 96), (2, 8, 64, 200, 30), (1, 1, 128, 193, 193)])
+@pytest.mark.parametrize("H,G,D,n,t", [(1, 4, 128, 96, 96), (2, 8, 64, 200, 30), (1, 1, 128, 193, 193), (1, 4, 128, 2100, 50)])
 def test_prompts_of_very_different_scales(fmt, H, G, D, n, t):
     """As above, prompts: tokens whose weights fp16 does not hold (their V is 2^20 to 2^30 times smaller, or zero) keep their
     place in the sum of the softmax."""

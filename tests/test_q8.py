@@ -19,6 +19,11 @@ def test_slot_bytes():
     assert K.q8_slot_bytes(8, 128) == 2056 and lib.rq_q8_slot_bytes(0, 128) == 0
 
 
+def test_slot_bytes_past_32_bits():
+    assert _lib.load().rq_q8_slot_bytes(1 << 20, 1 << 20) == 0
+    assert _lib.load().rq_q8_slot_bytes(1 << 20, 1 << 9) == (1 << 20) * 1025
+
+
 @pytest.mark.parametrize("D,H,block", [(64, 1, 16), (128, 3, 32)])
 def test_page_bytes_are_used_once(D, H, block):
     k, v, s = Q.code_index(block, H, D)
