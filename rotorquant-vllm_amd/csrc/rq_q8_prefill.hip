@@ -160,9 +160,9 @@ __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int 
 __device__ __forceinline__ int q8_chunk_tiles(int n_tiles, int split) { return max(kQ8MinTiles, (n_tiles + split - 1) / split); }
 
 // What bounds it: the matrix cores and vector issue together, under the card's power limit.  8 prompts of 2222 to 4096 tokens, 32 / 8
-// heads (0.84 TFLOP): 845 to 885 us, 950 to 995 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
+// heads (0.84 TFLOP): 805 to 885 us, 950 to 1040 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
 // 1800 of zeros).  The matrix cores are busy half of the cycles, at 1.8 GHz (the memory-bound kernels run at 2.1).  A wave's tile
-// is 32 MFMAs, 32 exponentials and about 93 other vector instructions; measured by itself, an MFMA with a pair of exponentials
+// is 32 MFMAs, 32 exponentials and about 115 other vector instructions; measured by itself, an MFMA with a pair of exponentials
 // and its packing takes 21.4 ns of a SIMD, without 13.8, so the first phase is bound by issue.  Without the tile copies 9 %
 // less time, without exponentials 6 %.  Tried without gain: two units a wave at one wave a SIMD (half the LDS reads; 226
 // registers spilled), eight waves on one tile (926 -> 931 us, one prompt of 700 tokens 24 -> 32), two sets of four waves on alternate
