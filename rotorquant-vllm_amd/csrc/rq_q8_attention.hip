@@ -432,7 +432,8 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgro
     q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);
 }
 
-// One workgroup of 8 waves per item: one launch, no partials.
+// One workgroup of 8 waves per item: one launch, no partials.  Bound by what one CU loads (a tile a wave per 1.07 us, 61 GB/s):
+// two, three or four tiles ahead instead of one took 8.7, 9.0 and 9.0 us against 8.6 (one sequence of 777 keys).
 template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
     __shared__ Q8Sums<D, 8> lds;
