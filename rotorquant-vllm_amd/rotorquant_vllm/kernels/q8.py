@@ -113,6 +113,7 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
     Slots outside the cache (vLLM's padding id -1) are skipped; of tokens with the same slot the last one counts.
     A write of a group's first slot begins the group anew (its rows that this call does not write
     become 0); other writes keep its rows and never lower its scale.
+    Rows (and the cache) start at multiples of 16 bytes, as slices of a fused projection do; others are refused.
     workspace: scratch of calls of more than 512 tokens (rq_q8_store_workspace_bytes bytes),
     by default from torch's allocator; a graph captured without torch's graph classes needs it.
     """
@@ -179,6 +180,7 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     (a decode step).  Query i of sequence b sits at position seq_lens[b] - q_len_b + i; a row that sees no key is zeros.
     max_q_len and max_seq_len: host ints that bound the query and context lengths (default: all of q, and the
     block table's capacity); what lies past them is not read.
+    Rows of q start at multiples of 16 bytes and those of out of 8; others are refused.
     workspace: scratch (rq_q8_attention_workspace_bytes bytes), by default of this call from torch's allocator; a graph
     captured without torch's graph classes needs it, since nothing else keeps the scratch for its replays.
     """
