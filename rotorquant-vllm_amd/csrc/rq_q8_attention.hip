@@ -7,11 +7,11 @@
 //   S^T = K Q^T   on v_mfma_f32_16x16x32_f16: codes c_k (exact in fp16) times q 2^s (s per column, the row's
 //                 largest magnitude near 2^14: fp16 holds what bf16 does), fp32 sums;
 //   u = S f + e_v, f = |sm_scale| log2(e) 2^(e_k - s): the score in base 2 plus the V exponent;
-//   w = 2^(u - M) in fp16, M a column's running maximum of u (rescaled lazily: w stays under 2^8);
+//   w = 2^(u + B) in fp16, B 7 to 15 less a column's running maximum of u (rq_q8_attn.h);
 //   O^T += C_v^T w  (codes again exact), l += 2^-e_v sum w.
 // So a group's two scales cost one multiplication per column and an addend that the exponent takes anyway, the
 // weights are relative to the largest p 2^e_v whatever the groups' scales are, and out = O / l.
-// l stays in fp32 whatever the scales: a token whose w underflows has under 2^-26 of the sum of p of the
+// l stays in fp32 whatever the scales: a token whose w underflows has under 2^-33 of the sum of p of the
 // one that sets M (e_v is in -40 .. 60).
 //
 // Operands need neither LDS nor shuffles: a lane's 16 bytes of K and V are its operands' elements (rq_q8.h), and
@@ -177,7 +177,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
             qop[nb][k] = valid ? *reinterpret_cast<const u32x4 *>(row + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0u, 0u, 0u, 0u};
     }
     if (t < t1) fetch(t);
-    float colf[NB], M[NB], l_run[NB];
+    float colf[NB], B[NB], l_run[NB];
     int lim[NB];  // keys that this lane's column sees
     f32x4 acc[NB][kBlocks];
 #pragma unroll
@@ -186,7 +186,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
         lim[nb] = a.causal ? min(s.vis, s.L - s.T + (c0 + kQ8Cols * nb + col) / a.G + 1) : s.vis;
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) acc[nb][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-        M[nb] = -INFINITY, l_run[nb] = 0.f;
+        B[nb] = kQ8NoBias, l_run[nb] = 0.f;
     }
     const int lim_first = a.causal ? min(s.vis, s.L - s.T + c0 / a.G + 1) : s.vis;  // the fewest that any column sees
 
@@ -248,18 +248,17 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
                 const f32x4 x = S[nb][gr];
                 tmax = fmaxf(tmax, __builtin_fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), f[gr], (float)ev[gr]));
             }
-            if (__any(tmax - M[nb] > 8.f)) {
-                const float m_new = fmaxf(M[nb], rows_max(tmax));
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M[nb] - m_new);
+            if (__any(q8_passes(tmax, B[nb]))) {
+                const float b_new = fminf(B[nb], kQ8Peak - rows_max(tmax));
+                const float alpha = __builtin_amdgcn_exp2f(b_new - B[nb]);
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) acc[nb][m] *= alpha;
                 l_run[nb] *= alpha;
-                M[nb] = m_new;
+                B[nb] = b_new;
             }
-            const float bias = M[nb] == -INFINITY ? 0.f : -M[nb];
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
-                const float add = bias + (float)ev[gr];
+                const float add = B[nb] + (float)ev[gr];
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[nb][gr][i], f[gr], add));
@@ -288,7 +287,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
         __syncthreads();  // (the sums before these are read)
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) *reinterpret_cast<f32x4 *>(&lds.acc[wave][col][16 * m + 4 * g]) = acc[nb][m];
-        if (g == 0) lds.ml[wave][col] = make_float2(M[nb], l_col);
+        if (g == 0) lds.ml[wave][col] = make_float2(q8_max_of(B[nb]), l_col);
         __syncthreads();
         constexpr int kPer = 4 * W, kDims = D / kPer;  // threads of a column, dims of a thread
         const int c = tid / kPer, d0 = tid % kPer * kDims;

@@ -251,9 +251,9 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
     f32x16 acc[kM];
 #pragma unroll
     for (int m = 0; m < kM; ++m) acc[m] = f32x16{};
-    float l_run = 0.f, M = -INFINITY;
+    float l_run = 0.f, B = kQ8NoBias;
     f32x16 sa[2], sb[2];  // scores of an even and of an odd tile
-    float fg[4], add[4];  // of the tile whose exponentials come next: u - M = S fg + add
+    float fg[4], add[4];  // of the tile whose exponentials come next: a weight is 2^(S fg + add)
     auto mask = [&](int t, f32x16 (&sc)[2]) {
         const int k0 = (t0 + t) * kQ8KT, nk = min(kQ8KT, kv_end - k0);
         if (!(nk == kQ8KT && (!a.causal || k0 + kQ8KT - 1 <= pos_base + i0)))
@@ -266,23 +266,22 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
         float tm = -INFINITY;
 #pragma unroll
         for (int g = 0; g < 4; ++g) tm = fmaxf(tm, __builtin_fmaf(gm[g], fg[g], e[g]));
-        if (__any(tm - M > 8.f)) {
+        if (__any(q8_passes(tm, B))) {
             auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
-            const float m_new = fmaxf(M, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-            const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - m_new);
+            const float b_new = fminf(B, kQ8Peak - fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+            const float alpha = __builtin_amdgcn_exp2f(b_new - B);
 #pragma unroll
             for (int m = 0; m < kM; ++m) acc[m] *= alpha;
             l_run *= alpha;
-            M = m_new;
+            B = b_new;
         }
-        const float bias = M == -INFINITY ? 0.f : -M;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) add[g] = e[g] + bias;
+        for (int g = 0; g < 4; ++g) add[g] = e[g] + B;
     };
     auto k_op = [&](const uint8_t *kt, int fi) { return *reinterpret_cast<const u32x4 *>(kt + 16 * lane + 1024 * fi); };
     auto meta4 = [](const uint8_t *at) { return *reinterpret_cast<const float4 *>(at); };
     // pair i of weights: its place in the operand, and its group's sum, of the weights before their rounding: fp16 loses those of
-    // groups whose V is 2^20 times smaller than others' (or zero), which the softmax's sum still has to hold
+    // groups whose V is 2^31 times smaller than others' (or zero), which the softmax's sum still has to hold
     auto exp_pair = [&](const f32x16 (&sc)[2], int i, uint32_t (&pop)[16], float (&l)[4]) {
         const int t = i >> 2, e = 8 * (t & 1) + 2 * (i & 3);
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t >> 1][e], fg[t], add[t]));
@@ -399,7 +398,7 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
     const float l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if (p.split > 1) {
         float *pt = a.part + ((((bl * p.nh + hl) * p.nx + qblk) * p.split + chunk) * kQ8PWaves + wave) * (int64_t)Im::kPart;
-        if (hh == 0) *reinterpret_cast<float2 *>(pt + kQ8PW * D + 2 * col) = make_float2(M, l);
+        if (hh == 0) *reinterpret_cast<float2 *>(pt + kQ8PW * D + 2 * col) = make_float2(q8_max_of(B), l);
 #pragma unroll
         for (int m = 0; m < kM; ++m)
 #pragma unroll
