@@ -493,7 +493,8 @@ int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, 
  * q / out: total_q x num_q_heads x head_dim of F16 or BF16 (element strides; q rows 16-byte, out rows
  * 8-byte aligned), num_q_heads a multiple of num_kv_heads.  cu_seqlens_q: num_seqs + 1 int32, or NULL
  * for one token per sequence.  max_q_len bounds every q_len_b and max_seq_len every seq_lens[b]: tokens
- * and keys past them, or past the block table's capacity, are not read.  Products are exact, sums and
+ * and keys past them, or past the block table's capacity, are not read (positions go by the whole q_len_b and seq_lens[b]
+ * all the same), and out's rows of such tokens, as those of no sequence, are left as they are.  Products are exact, sums and
  * the softmax's statistics fp32, its weights rounded to fp16 for P V.
  * workspace: rq_q8_attention_workspace_bytes() bytes, 16-byte aligned, no initialisation needed.
  * Launches depend on host arguments only, so a captured call may be replayed with other lengths up to max_seq_len.

@@ -183,12 +183,12 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         colf[nb] = q8_query<DT, D>(a, qop[nb]);
-        lim[nb] = a.causal ? min(s.vis, s.L - s.T + (c0 + kQ8Cols * nb + col) / a.G + 1) : s.vis;
+        lim[nb] = a.causal ? min(s.vis, s.pos + (c0 + kQ8Cols * nb + col) / a.G + 1) : s.vis;
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) acc[nb][m] = f32x4{0.f, 0.f, 0.f, 0.f};
         B[nb] = kQ8NoBias, l_run[nb] = 0.f;
     }
-    const int lim_first = a.causal ? min(s.vis, s.L - s.T + c0 / a.G + 1) : s.vis;  // the fewest that any column sees
+    const int lim_first = a.causal ? min(s.vis, s.pos + c0 / a.G + 1) : s.vis;  // the fewest that any column sees
 
     for (; t < t1; t += W) {
         int ev[2];

@@ -44,9 +44,9 @@ __device__ __forceinline__ void q8_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi
     }
 }
 
-// A sequence's query tokens (q0 .. q0 + T), keys L, and tiles.
+// A sequence's query tokens that count (q0 .. q0 + T), the position of the first, and the keys that may be seen.
 struct Q8Seq {
-    int q0, T, L, vis;
+    int q0, T, pos, vis;
 };
 __device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
     Q8Seq s;
@@ -54,8 +54,10 @@ __device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
     const int end = a.cu_q ? a.cu_q[b + 1] : (int)b + 1;
     s.T = min(max(min((int64_t)end, a.total_q) - max(s.q0, 0), (int64_t)0), (int64_t)a.max_q);
     if (s.q0 < 0) s.T = 0;
-    s.L = a.seq_lens[b];
-    s.vis = (int)max((int64_t)0, min((int64_t)s.L, a.cap));
+    const int L = a.seq_lens[b];
+    s.vis = (int)max((int64_t)0, min((int64_t)L, a.cap));
+    // (by the query's whole length, also where max_q cuts it; far below 0, where no key is seen, the exact place is of no account)
+    s.pos = (int)max((int64_t)L - ((int64_t)end - s.q0), (int64_t)-(1 << 30));
     return s;
 }
 

@@ -153,7 +153,7 @@ __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int 
     q.units = (q.s.T + kQ8PW - 1) / kQ8PW * a.G;
     q.f0 = qblk * kQ8PWaves;
     const int last_i = min(q.s.T, (min(q.f0 + kQ8PWaves, q.units) - 1) / a.G * kQ8PW + kQ8PW) - 1;
-    q.kv_end = a.causal ? min(q.s.vis, q.s.L - q.s.T + last_i + 1) : q.s.vis;
+    q.kv_end = a.causal ? min(q.s.vis, q.s.pos + last_i + 1) : q.s.vis;
     q.n_tiles = q.kv_end > 0 ? (q.kv_end + kQ8KT - 1) / kQ8KT : 0;
     return q;
 }
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
     const int i0 = f < qb.units ? f / a.G * kQ8PW : s.T;  // first position of this wave's unit (past the end: inactive)
     const int hq = h * a.G + f % a.G;
     const bool wave_active = i0 < s.T;
-    const int my_i = i0 + col, pos_base = s.L - s.T, my_pos = pos_base + my_i;
+    const int my_i = i0 + col, pos_base = s.pos, my_pos = pos_base + my_i;
     const int kv_end = qb.kv_end;
     int t0 = 0, n_tiles = qb.n_tiles;
     if (p.split > 1) {

@@ -179,7 +179,8 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     included, are int32.  cu_seqlens_q (num_seqs + 1,) int32 splits q among the sequences; without it each has one token
     (a decode step).  Query i of sequence b sits at position seq_lens[b] - q_len_b + i; a row that sees no key is zeros.
     max_q_len and max_seq_len: host ints that bound the query and context lengths (default: all of q, and the
-    block table's capacity); what lies past them is not read.
+    block table's capacity); what lies past them is not read, and positions stay as above.  out: a buffer to fill, whose
+    rows of such tokens and of no sequence stay as they are (without it they are not initialised).
     Rows of q start at multiples of 16 bytes and those of out of 8; others are refused.
     workspace: scratch (rq_q8_attention_workspace_bytes bytes), by default of this call from torch's allocator; a graph
     captured without torch's graph classes needs it, since nothing else keeps the scratch for its replays.
