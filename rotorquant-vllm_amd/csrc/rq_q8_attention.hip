@@ -25,6 +25,7 @@
 // twice or four times the workgroups, which balance themselves, 130 and 139 (more partials, more prologues).  Small calls are bound by
 // their chain of dependent loads: lengths, block table, codes, then the sums of the waves.
 #include <algorithm>
+#include <cmath>
 
 #include "rq_q8_attn.h"
 
@@ -90,7 +91,7 @@ __device__ __forceinline__ float q8_query(const Q8AttnArgs &a, u32x4 (&qop)[D / 
     uint32_t big = 0;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) big = q8_max_bits(qop[k], big);
-    const int up = q8_query_exp<DT>(rows_umax(big));
+    const int up = q8_query_exp<DT>(a, rows_umax(big));
     const float f = exp2i(up) * a.q_sign;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) qop[k] = q8_query_f16<DT>(qop[k], f);
@@ -552,6 +553,7 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     a.max_q = (int)max_q_len;
     a.score_scale = sm_scale == 0.f ? 1.f : __builtin_fabsf(sm_scale) * kAttnLog2e;
     a.q_sign = sm_scale > 0.f ? 1.f : sm_scale < 0.f ? -1.f : 0.f;
+    a.max_up = std::min(60, 86 + std::ilogb(a.score_scale));  // (of numbers under 2^-126, too)
     a.out = out, a.o_st = out_stride_tok, a.o_sh = out_stride_head;
     const int64_t need = rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len);
     RQ_CHECK_SPACE(workspace_bytes >= need, "workspace too small: the call needs %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);

@@ -26,6 +26,7 @@ struct Q8AttnArgs {
     int max_q;    // tokens of a query that count
     float score_scale;  // |sm_scale| log2(e)
     float q_sign;       // sign of sm_scale (0 for 0)
+    int max_up;         // largest s of q 2^s (below)
     void *out;
     int64_t o_st, o_sh;
     float *part;  // partial sums of items that several workgroups share
@@ -62,10 +63,12 @@ __device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
 }
 
 // Exponent s with which a query row, its largest magnitude given by its bits, goes into fp16: q 2^s has
-// its largest magnitude in [2^14, 2^15) (rows under 2^-46: what 2^60 gives).
+// its largest magnitude in [2^14, 2^15); smaller rows take max_up.  That is 60, or less where f = score_scale 2^(e_k - s) would fall
+// under 2^-126 and to 0 at the smallest e_k (a masked score times 0 is NaN): score_scale 2^-max_up is 2^-86 or more.  A row
+// that max_up cuts short loses parts under 2^-25 of 2^max_up, which move no score by more than 2^(-25 - 86 + 67) D.
 template <int DT>
-__device__ __forceinline__ int q8_query_exp(uint32_t big) {
-    return min(60, 14 - ((int)((__float_as_uint(Elem<DT>::to_f32(big)) >> 23) & 0xffu) - 127));
+__device__ __forceinline__ int q8_query_exp(const Q8AttnArgs &a, uint32_t big) {
+    return min(a.max_up, 14 - ((int)((__float_as_uint(Elem<DT>::to_f32(big)) >> 23) & 0xffu) - 127));
 }
 __device__ __forceinline__ uint32_t q8_max_bits(u32x4 raw, uint32_t big) {
 #pragma unroll

@@ -241,7 +241,7 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) big = q8_max_bits(qop[k], big);
         big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-        const int up = q8_query_exp<DT>(big);
+        const int up = q8_query_exp<DT>(a, big);
         const float fq = exp2i(up) * a.q_sign;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) qop[k] = q8_query_f16<DT>(qop[k], fq);

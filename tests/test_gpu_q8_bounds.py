@@ -27,3 +27,38 @@ def test_queries_longer_than_their_bound(H, G, D, lens, queries, most, causal):
     keep = np.concatenate([np.arange(n) < most for n in queries])
     X.check(got[torch.from_numpy(keep).to(X.DEV)], out[keep], tol[keep])
     assert bool((got[torch.from_numpy(~keep).to(X.DEV)] == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("T,n", [(1, 5), (1, 2100), (3, 21), (40, 70), (40, 2100)])
+@pytest.mark.parametrize("sm_scale", [1e-8, 1e-17, -1e-25, 1e-38, 1.5e-45])
+def test_tiny_scales(fmt, T, n, sm_scale):
+    """Zero queries and zero keys under a scale near fp32's end: the mean of the values that a row sees."""
+    H, G, D = 1, 8, 128
+    k, v = Q.rows(n, H, D, 2, torch.bfloat16)
+    k[:16] = 0
+    k[n // 2:] = 0
+    table, pages = Q.layout([n], 16, 5)
+    ref, cache = Q.Cache(pages, 16, H, D, fmt), X.new_cache(pages, 16, H, D)
+    X.store(cache, ref, k, v, Q.slots_of(table, 0, 0, n, 16), fmt)
+    q = torch.randn(T, H * G, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    q[:, ::2] = 0
+    q[:, 1] *= 1e-30
+    out, tol = X.attention(q, ref, table, [n], [0, T], sm_scale=sm_scale)
+    got = K.q8_attention(q.to(X.DEV), cache, X.i32(table), X.i32([n]), H, D, fmt=fmt, cu_seqlens_q=X.i32([0, T]), max_q_len=T, sm_scale=sm_scale)
+    X.check(got, out, tol)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_a_tiny_scale_times_large_numbers(fmt):
+    """The scale alone says nothing about the scores: 2^-60 times queries of 2^30 and keys of 2^30."""
+    H, G, D, n = 1, 8, 64, 50
+    k, v = Q.rows(n, H, D, 4, torch.bfloat16)
+    table, pages = Q.layout([n], 16, 5)
+    ref, cache = Q.Cache(pages, 16, H, D, fmt), X.new_cache(pages, 16, H, D)
+    X.store(cache, ref, k * 2.0 ** 30, v, Q.slots_of(table, 0, 0, n, 16), fmt)
+    for T in (1, 30):
+        q = torch.randn(T, H * G, D, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16) * 2.0 ** 30
+        out, tol = X.attention(q, ref, table, [n], [0, T], sm_scale=2.0 ** -62)
+        got = K.q8_attention(q.to(X.DEV), cache, X.i32(table), X.i32([n]), H, D, fmt=fmt, cu_seqlens_q=X.i32([0, T]), max_q_len=T, sm_scale=2.0 ** -62)
+        X.check(got, out, tol)
