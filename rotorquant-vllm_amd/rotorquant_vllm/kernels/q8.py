@@ -90,9 +90,11 @@ def _store_bytes(n_tokens: int, num_blocks: int, block_size: int) -> int:
     return _lib.load().rq_q8_store_workspace_bytes(n_tokens, num_blocks, block_size)
 
 
+# (The attention's also by the GPU, whose number of CUs sizes the partial sums: asked for with that one current.)
 @functools.lru_cache(maxsize=4096)
-def _attention_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_q_len: int, max_seq_len: int) -> int:
-    return _lib.load().rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len)
+def _attention_bytes(dev: int, num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_q_len: int, max_seq_len: int) -> int:
+    with torch.cuda.device(dev):
+        return _lib.load().rq_q8_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len)
 
 
 def _scratch(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int, int]:
@@ -217,7 +219,7 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     capacity = max_blocks * BS
     max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
     code = _format(fmt)
-    keep, ws, ws_bytes = _scratch(workspace, _attention_bytes(B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
+    keep, ws, ws_bytes = _scratch(workspace, _attention_bytes(dev, B, HQ, num_kv_heads, D, max_q_len, max_seq_len), q)
     _call(_lib.load().rq_q8_attention, "rq_q8_attention", dev,
           (q.data_ptr(), _lib.dtype_code(q.dtype), T, HQ, qs[0], qs[1], None if cu is None else cu.data_ptr(), B, max_q_len,
            1 if causal else 0, kv_cache.data_ptr(), NB, BS, stride, num_kv_heads, D, code, bt.data_ptr(), max_blocks, bt.stride(0),
