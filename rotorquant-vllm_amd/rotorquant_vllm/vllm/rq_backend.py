@@ -635,11 +635,25 @@ class RQAttentionImpl(_ImplBase):
             raise ValueError(f"RQ_CACHE_8BIT needs head_size {' or '.join(map(str, RQ_8BIT_HEAD_DIMS))} (got {self.head_size})")
         if self.num_heads % self.num_kv_heads:
             raise ValueError(f"RQ_CACHE_8BIT: {self.num_heads} query heads over {self.num_kv_heads} kv heads")
+        if self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
+            self._refuse_q8_features()
         self._fused_paged_available = self._fused_prefill_available = False
         self._total_bytes = _rq_slot_bytes(self.head_size, self.num_kv_heads, RQ_8BIT_GROUP)
         logger.info("RQAttentionImpl: 8-bit cache (%s), %d KV heads, head_size=%d, %d bytes/token (%.2fx compression vs FP16)",
                     self._q8_format, self.num_kv_heads, self.head_size, self._total_bytes,
                     4 * self.num_kv_heads * self.head_size / self._total_bytes)
+
+    def _refuse_q8_features(self) -> None:
+        """q8_attention is plain causal or full softmax attention: a layer that asks for more would get wrong outputs.
+        (vLLM's base classes turn "no window" into (-1, -1) and "no cap" into 0.)"""
+        window = getattr(self, "sliding_window", None)
+        sizes = window if isinstance(window, (tuple, list)) else (-1 if window is None else window,)
+        for name, on in (("sliding_window", any(w is not None and w >= 0 for w in sizes)),
+                         ("logits_soft_cap", bool(getattr(self, "logits_soft_cap", None))),
+                         ("alibi_slopes", getattr(self, "alibi_slopes", None) is not None),
+                         ("sinks", getattr(self, "sinks", None) is not None)):
+            if on:
+                raise ValueError(f"RQ_CACHE_8BIT does not support {name} (got {getattr(self, name)})")
 
     def _forward_q8(self, query, key, value, kv_cache, md, output):
         """Store the new tokens, then attention over the 8-bit cache.  One call for a batch of decodes or short queries; a

@@ -2,6 +2,7 @@
 import contextlib
 from types import SimpleNamespace
 
+import pytest
 import torch
 
 from rotorquant_vllm.kernels import q8
@@ -27,3 +28,41 @@ def test_scratch_is_sized_for_the_tensors_device(monkeypatch):
         assert current == [0]
     finally:
         q8._attention_bytes.cache_clear()
+
+
+# ---- backend ------------------------------------------------------------------
+
+
+def _impl(monkeypatch, **kw):
+    monkeypatch.setenv("RQ_CACHE_8BIT", "int8")
+    monkeypatch.delenv("RQ_DENSE_3BIT", raising=False)
+    from rotorquant_vllm.vllm import rq_backend as B
+    return B.RQAttentionImpl(8, 128, 0.1, num_kv_heads=2, **kw)
+
+
+@pytest.mark.parametrize("kw,name", [
+    (dict(sliding_window=256), "sliding_window"), (dict(sliding_window=(255, 0)), "sliding_window"), (dict(sliding_window=(0, 0)), "sliding_window"),
+    (dict(logits_soft_cap=30.0), "logits_soft_cap"), (dict(alibi_slopes=[0.5] * 8), "alibi_slopes"), (dict(alibi_slopes=torch.ones(8)), "alibi_slopes")])
+def test_backend_refuses_what_the_kernels_do_not_do(monkeypatch, kw, name):
+    with pytest.raises(ValueError, match=f"does not support {name}"):
+        _impl(monkeypatch, **kw)
+
+
+def test_backend_refuses_sinks(monkeypatch):
+    from rotorquant_vllm.vllm import rq_backend as B
+    monkeypatch.setattr(B.RQAttentionImpl, "sinks", torch.zeros(8), raising=False)
+    with pytest.raises(ValueError, match="does not support sinks"):
+        _impl(monkeypatch)
+
+
+@pytest.mark.parametrize("kw", [
+    {}, dict(sliding_window=None), dict(sliding_window=(-1, -1)), dict(sliding_window=-1), dict(logits_soft_cap=0), dict(logits_soft_cap=0.0),
+    dict(alibi_slopes=None)])
+def test_backend_takes_what_is_off(monkeypatch, kw):
+    assert _impl(monkeypatch, **kw)._q8_format == "int8"
+
+
+def test_backend_leaves_encoders_to_their_own_attention(monkeypatch):
+    """Layers without a cache do not reach these kernels."""
+    from rotorquant_vllm.vllm import rq_backend as B
+    assert _impl(monkeypatch, sliding_window=(128, 128), attn_type=B.AttentionType.ENCODER_ONLY)._q8_format == "int8"
