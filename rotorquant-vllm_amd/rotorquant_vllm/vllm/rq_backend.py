@@ -637,11 +637,22 @@ class RQAttentionImpl(_ImplBase):
             raise ValueError(f"RQ_CACHE_8BIT: {self.num_heads} query heads over {self.num_kv_heads} kv heads")
         if self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
             self._refuse_q8_features()
+            if _HAVE_VLLM:
+                try:
+                    from vllm.config import get_current_vllm_config_or_none
+                    self._check_q8_dtype(get_current_vllm_config_or_none().model_config.dtype)
+                except (ImportError, AttributeError):  # no configuration here: forward checks the queries
+                    pass
         self._fused_paged_available = self._fused_prefill_available = False
         self._total_bytes = _rq_slot_bytes(self.head_size, self.num_kv_heads, RQ_8BIT_GROUP)
         logger.info("RQAttentionImpl: 8-bit cache (%s), %d KV heads, head_size=%d, %d bytes/token (%.2fx compression vs FP16)",
                     self._q8_format, self.num_kv_heads, self.head_size, self._total_bytes,
                     4 * self.num_kv_heads * self.head_size / self._total_bytes)
+
+    @staticmethod
+    def _check_q8_dtype(dtype) -> None:
+        if isinstance(dtype, torch.dtype) and dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"RQ_CACHE_8BIT needs a float16 or bfloat16 model (got {dtype})")
 
     def _refuse_q8_features(self) -> None:
         """q8_attention is plain causal or full softmax attention: a layer that asks for more would get wrong outputs.
@@ -664,6 +675,8 @@ class RQAttentionImpl(_ImplBase):
             raise RuntimeError("RotorQuant HIP kernels are not available")
         if getattr(md, "use_cascade", False):
             raise NotImplementedError("RQ does not yet support cascade attention")
+        if query.is_cuda:
+            self._check_q8_dtype(query.dtype)  # (before anything is stored)
         n = md.num_actual_tokens
         fmt, H, D = self._q8_format, self.num_kv_heads, self.head_size
         if key is not None and value is not None:
@@ -1001,6 +1014,8 @@ class RQAttentionImpl(_ImplBase):
         if output_scale is not None or output_block_scale is not None:
             raise NotImplementedError("Fused output quantization is not supported with RotorQuant backend")
         if attn_metadata is None or kv_cache is None:
+            if getattr(self, "_q8_format", None) is not None and self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
+                self._check_q8_dtype(query.dtype)
             return output.zero_()
         if self.attn_type in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
             n = attn_metadata.num_actual_tokens

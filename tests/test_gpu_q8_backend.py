@@ -1,0 +1,38 @@
+"""RQ_CACHE_8BIT in the backend on the GPU: refusals before a store, scratch, batches with idle sequences."""
+import math
+import types
+
+import numpy as np
+import pytest
+import torch
+
+import q8_bounds as X
+import q8_testlib as Q
+
+pytestmark = pytest.mark.gpu
+
+
+def backend(monkeypatch, fmt, H, HQ, D):
+    monkeypatch.setenv("RQ_CACHE_8BIT", fmt)
+    monkeypatch.delenv("RQ_DENSE_3BIT", raising=False)
+    from rotorquant_vllm.vllm import rq_backend as B
+    return B, B.RQAttentionImpl(HQ, D, 1 / math.sqrt(D), num_kv_heads=H)
+
+
+def metadata(slots, table, lens, q_lens, host=True):
+    md = types.SimpleNamespace(num_actual_tokens=sum(q_lens), max_query_len=max(q_lens), use_cascade=False, block_table=X.i32(table), seq_lens=X.i32(lens),
+                               slot_mapping=torch.from_numpy(np.asarray(slots, np.int64)).to(X.DEV), query_start_loc=X.i32(np.concatenate([[0], np.cumsum(q_lens)])))
+    if host:
+        md.rq_seq_lens_cpu, md.rq_query_start_loc_cpu = md.seq_lens.cpu(), md.query_start_loc.cpu()
+    return md
+
+
+def test_queries_of_32_bits_are_refused_before_the_store(monkeypatch):
+    H, HQ, D, block = 2, 8, 128, 16
+    _, impl = backend(monkeypatch, "int8", H, HQ, D)
+    cache = X.new_cache(2, block, H, D)
+    k, v = (x.to(X.DEV) for x in Q.rows(1, H, D, 1, torch.float32))
+    q = torch.zeros(1, HQ, D, device=X.DEV)
+    with pytest.raises(ValueError, match="float16 or bfloat16 model"):
+        impl.forward(None, q, k, v, cache, metadata([16], [[1]], [1], [1]), output=torch.empty_like(q))
+    assert not cache.any()

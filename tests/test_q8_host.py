@@ -1,5 +1,6 @@
 """Host side of the 8-bit cache without a GPU: sizes of scratch, refusals of the backend, strides."""
 import contextlib
+import sys
 from types import SimpleNamespace
 
 import pytest
@@ -66,3 +67,29 @@ def test_backend_leaves_encoders_to_their_own_attention(monkeypatch):
     """Layers without a cache do not reach these kernels."""
     from rotorquant_vllm.vllm import rq_backend as B
     assert _impl(monkeypatch, sliding_window=(128, 128), attn_type=B.AttentionType.ENCODER_ONLY)._q8_format == "int8"
+
+
+@pytest.mark.parametrize("dtype,ok", [(torch.float16, True), (torch.bfloat16, True), (torch.float32, False), ("auto", True)])
+def test_backend_refuses_models_of_32_bits_when_built(monkeypatch, dtype, ok):
+    from rotorquant_vllm.vllm import rq_backend as B
+    config = SimpleNamespace(model_config=SimpleNamespace(dtype=dtype))
+    monkeypatch.setattr(B, "_HAVE_VLLM", True)
+    monkeypatch.setitem(sys.modules, "vllm", SimpleNamespace())
+    monkeypatch.setitem(sys.modules, "vllm.config", SimpleNamespace(get_current_vllm_config_or_none=lambda: config))
+    if ok:
+        assert _impl(monkeypatch)._q8_format == "int8"
+    else:
+        with pytest.raises(ValueError, match="float16 or bfloat16 model"):
+            _impl(monkeypatch)
+    config = None  # outside a configuration
+    assert _impl(monkeypatch)._q8_format == "int8"
+
+
+def test_backend_refuses_queries_of_32_bits_while_profiling(monkeypatch):
+    """The run without metadata that sizes the cache, not the first request."""
+    impl = _impl(monkeypatch)
+    q, k = torch.zeros(3, 8, 128, dtype=torch.bfloat16), torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    out = torch.ones_like(q)
+    assert impl.forward(None, q, k, k, None, None, output=out) is out and not out.any()
+    with pytest.raises(ValueError, match="float16 or bfloat16 model"):
+        impl.forward(None, q.float(), k.float(), k.float(), None, None, output=out.float())
