@@ -698,14 +698,13 @@ class RQAttentionImpl(_ImplBase):
                              sm_scale=self.scale, causal=causal, cu_seqlens_q=cu, max_q_len=most, max_seq_len=longest,
                              out=out if cu is not None else out[b0:b1])
 
-        columns = self.num_heads // H
-        if int(max_q) <= 1:
+        columns, B = self.num_heads // H, md.seq_lens.numel()
+        if int(max_q) <= 1 and n == B:  # (a token each)
             longest = int(sl_cpu[:n].max()) if sl_cpu is not None and n else None
             attend(0, n, None, 1, longest)
             return output
-        if int(max_q) * columns < RQ_8BIT_PROMPT_COLUMNS:
+        if int(max_q) * columns < RQ_8BIT_PROMPT_COLUMNS or int(max_q) <= 1:
             longest = int(sl_cpu.max()) if sl_cpu is not None and sl_cpu.numel() else None
-            B = md.seq_lens.numel()
             attend(0, B, md.query_start_loc[:B + 1], int(max_q), longest)
             return output
         starts = (qsl_cpu if qsl_cpu is not None else md.query_start_loc.cpu()).tolist()

@@ -36,3 +36,18 @@ def test_queries_of_32_bits_are_refused_before_the_store(monkeypatch):
     with pytest.raises(ValueError, match="float16 or bfloat16 model"):
         impl.forward(None, q, k, v, cache, metadata([16], [[1]], [1], [1]), output=torch.empty_like(q))
     assert not cache.any()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("host", [True, False])
+def test_decodes_beside_idle_sequences(monkeypatch, fmt, host):
+    H, HQ, D, block = 2, 8, 128, 16
+    _, impl = backend(monkeypatch, fmt, H, HQ, D)
+    lens, q_lens = [40, 25, 33, 60], [1, 0, 1, 0]
+    cache, ref, table = X.filled(lens, block, H, D, fmt, torch.bfloat16, 9)
+    q = torch.randn(2, HQ, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    cu = np.concatenate([[0], np.cumsum(q_lens)])
+    want, tol = X.attention(q, ref, table, lens, cu)
+    out = torch.zeros_like(q, device=X.DEV)
+    impl.forward(None, q.to(X.DEV), None, None, cache, metadata([-1, -1], table, lens, q_lens, host), output=out)
+    X.check(out, want, tol)

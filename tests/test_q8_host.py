@@ -93,3 +93,31 @@ def test_backend_refuses_queries_of_32_bits_while_profiling(monkeypatch):
     assert impl.forward(None, q, k, k, None, None, output=out) is out and not out.any()
     with pytest.raises(ValueError, match="float16 or bfloat16 model"):
         impl.forward(None, q.float(), k.float(), k.float(), None, None, output=out.float())
+
+
+@pytest.mark.parametrize("q_lens", [[1, 0, 1], [0, 1], [0, 0, 1, 1, 0]])
+@pytest.mark.parametrize("host", [True, False])
+def test_backend_batches_of_decodes_with_idle_sequences(monkeypatch, q_lens, host):
+    """A sequence without a token in a batch of decodes: the others' tokens still go to their own contexts."""
+    from rotorquant_vllm.vllm import rq_backend as B
+    impl, calls = _impl(monkeypatch), []
+    monkeypatch.setattr(B, "_q8_store_fn", lambda *a, **k: None)
+    monkeypatch.setattr(B, "_q8_attention_fn", lambda q, cache, table, lens, H, D, **kw: calls.append((q, table, lens, kw)))
+    n, lens = sum(q_lens), [70 + b for b in range(len(q_lens))]
+    starts = [sum(q_lens[:b]) for b in range(len(q_lens) + 1)]
+    q = torch.zeros(n, 8, 128, dtype=torch.bfloat16)
+    k = torch.zeros(n, 2, 128, dtype=torch.bfloat16)
+    md = SimpleNamespace(num_actual_tokens=n, max_query_len=1, block_table=torch.arange(len(q_lens), dtype=torch.int32)[:, None],
+                         seq_lens=torch.tensor(lens, dtype=torch.int32), query_start_loc=torch.tensor(starts, dtype=torch.int32),
+                         slot_mapping=torch.arange(n))
+    if host:
+        md.rq_query_start_loc_cpu, md.rq_seq_lens_cpu = md.query_start_loc, md.seq_lens
+    impl.forward(None, q, k, k, torch.zeros(4, 16, 520, dtype=torch.uint8), md, output=torch.empty_like(q))
+    seen = {}  # query row -> sequence
+    for q_, table, lens_, kw in calls:
+        cu = kw["cu_seqlens_q"]
+        for b in range(lens_.numel()):
+            for row in range(*(cu[b:b + 2].tolist() if cu is not None else (b, b + 1))):
+                seen[row] = int(table[b, 0])
+                assert kw["max_seq_len"] is None or kw["max_seq_len"] >= int(lens_[b])
+    assert seen == {starts[b]: b for b, m in enumerate(q_lens) if m}
