@@ -501,6 +501,9 @@ int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, 
  */
 int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
                                         int32_t head_dim, int64_t max_q_len, int64_t max_seq_len);
+/* Bytes that no call over contexts of up to max_seq_len keys needs more than, whatever its sequences and queries, on the current
+ * GPU: for callers that set memory aside up front.  0 for sizes below 1. */
+int64_t rq_q8_attention_workspace_bound(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t max_seq_len);
 int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads,
                     int64_t q_stride_tok, int64_t q_stride_head,
                     const int32_t *cu_seqlens_q, int64_t num_seqs, int64_t max_q_len, int32_t causal,

@@ -514,6 +514,12 @@ extern "C" int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num
     return 2 * wgs * q8_blocks(G, max_q_len) * kQ8Cols * (head_dim + 2) * 4;
 }
 
+// (The stream's partials, two of up to 2 x 16 columns for each of up to four workgroups a CU, are smaller than the prefill's.)
+extern "C" int64_t rq_q8_attention_workspace_bound(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t max_seq_len) {
+    if (num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_seq_len < 0) return 0;
+    return q8_prefill_workspace_bound(head_dim, q8_bound(max_seq_len));
+}
+
 extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads,
                                int64_t q_stride_tok, int64_t q_stride_head, const int32_t *cu_seqlens_q, int64_t num_seqs,
                                int64_t max_q_len, int32_t causal, const uint8_t *kv_cache, int64_t num_blocks,

@@ -94,6 +94,7 @@ __device__ __forceinline__ bool q8_passes(float u, float B) { return __builtin_f
 __device__ __forceinline__ float q8_max_of(float B) { return B == kQ8NoBias ? -INFINITY : -B; }
 
 // Prompts and chunks (rq_q8_prefill.hip).  Bytes of the workspace, and the launches.
+int64_t q8_prefill_workspace_bound(int D, int64_t max_keys);
 int64_t q8_prefill_workspace(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys);
 int q8_prefill(const Q8AttnArgs &a, int dtype, int format, int D, void *workspace, hipStream_t st);
 

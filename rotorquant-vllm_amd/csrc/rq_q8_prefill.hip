@@ -490,6 +490,13 @@ int64_t q8_prefill_workspace(int64_t num_seqs, int G, int H, int D, int64_t max_
     return s.images + s.part;
 }
 
+// The images of a pass fit kQ8ImageBytes unless one pair's do not; split calls have a workgroup for each place at most.
+int64_t q8_prefill_workspace_bound(int D, int64_t max_keys) {
+    const int64_t tiles = std::max<int64_t>(1, (max_keys + kQ8KT - 1) / kQ8KT);
+    const int64_t image = D == 128 ? Q8Image<128>::kBytes : Q8Image<64>::kBytes, part = D == 128 ? Q8Image<128>::kPart : Q8Image<64>::kPart;
+    return std::max(kQ8ImageBytes, tiles * image) + 2 * (int64_t)device_cus() * kQ8PWaves * part * 4;
+}
+
 template <int DT, int FMT, int D>
 static void q8_prefill_pass(const Q8PrefillArgs &p, int64_t nb, hipStream_t st) {
     using Im = Q8Image<D>;

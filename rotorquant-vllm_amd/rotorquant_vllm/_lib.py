@@ -69,6 +69,7 @@ _SIGNATURES = {
     "rq_q8_read": (_c_i32, [_c_p, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64,
                             _c_i64, _c_p, _c_p, _c_i32, _c_p]),
     "rq_q8_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64]),
+    "rq_q8_attention_workspace_bound": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i64]),
     "rq_q8_attention": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_i64,
                                  _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f32, _c_p,
                                  _c_i64, _c_i64, _c_p, _c_i64, _c_p]),

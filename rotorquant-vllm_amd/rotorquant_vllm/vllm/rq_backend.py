@@ -637,17 +637,31 @@ class RQAttentionImpl(_ImplBase):
             raise ValueError(f"RQ_CACHE_8BIT: {self.num_heads} query heads over {self.num_kv_heads} kv heads")
         if self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
             self._refuse_q8_features()
-            if _HAVE_VLLM:
-                try:
-                    from vllm.config import get_current_vllm_config_or_none
-                    self._check_q8_dtype(get_current_vllm_config_or_none().model_config.dtype)
-                except (ImportError, AttributeError):  # no configuration here: forward checks the queries
-                    pass
+        self._max_model_len = 8192
+        if _HAVE_VLLM:
+            try:
+                from vllm.config import get_current_vllm_config_or_none
+                model_config = get_current_vllm_config_or_none().model_config
+            except (ImportError, AttributeError):  # no configuration here: forward checks the queries
+                model_config = None
+            if model_config is not None:
+                self._max_model_len = getattr(model_config, "max_model_len", self._max_model_len)
+                if self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
+                    self._check_q8_dtype(getattr(model_config, "dtype", None))
         self._fused_paged_available = self._fused_prefill_available = False
         self._total_bytes = _rq_slot_bytes(self.head_size, self.num_kv_heads, RQ_8BIT_GROUP)
         logger.info("RQAttentionImpl: 8-bit cache (%s), %d KV heads, head_size=%d, %d bytes/token (%.2fx compression vs FP16)",
                     self._q8_format, self.num_kv_heads, self.head_size, self._total_bytes,
                     4 * self.num_kv_heads * self.head_size / self._total_bytes)
+
+    def _reserve_q8_scratch(self, device) -> None:
+        """Runs without metadata are vLLM's profiling, whose peak of allocated memory decides how much the cache may take.  So
+        what the largest call asks torch's allocator for is taken and freed here; calls then find it outside the cache."""
+        if device.type != "cuda" or _q8_attention_fn is None or torch.cuda.is_current_stream_capturing():
+            return
+        with torch.cuda.device(device):
+            need = _rq_lib.load().rq_q8_attention_workspace_bound(self.num_heads, self.num_kv_heads, self.head_size, self._max_model_len)
+        torch.empty(need, dtype=torch.uint8, device=device)
 
     @staticmethod
     def _check_q8_dtype(dtype) -> None:
@@ -1015,6 +1029,7 @@ class RQAttentionImpl(_ImplBase):
         if attn_metadata is None or kv_cache is None:
             if getattr(self, "_q8_format", None) is not None and self.attn_type not in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
                 self._check_q8_dtype(query.dtype)
+                self._reserve_q8_scratch(query.device)
             return output.zero_()
         if self.attn_type in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
             n = attn_metadata.num_actual_tokens

@@ -51,3 +51,22 @@ def test_decodes_beside_idle_sequences(monkeypatch, fmt, host):
     out = torch.zeros_like(q, device=X.DEV)
     impl.forward(None, q.to(X.DEV), None, None, cache, metadata([-1, -1], table, lens, q_lens, host), output=out)
     X.check(out, want, tol)
+
+
+def test_profiling_sets_the_scratch_of_the_largest_call_aside(monkeypatch):
+    """The run without metadata reaches the memory that a call over the longest context then needs."""
+    H, HQ, D = 8, 32, 128
+    _, impl = backend(monkeypatch, "int8", H, HQ, D)
+    q = torch.zeros(16, HQ, D, dtype=torch.bfloat16, device=X.DEV)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    impl.forward(None, q, q[:, :H], q[:, :H], None, None, output=out)
+    assert not out.any()
+    from rotorquant_vllm import _lib
+    aside = torch.cuda.max_memory_allocated() - before
+    assert torch.cuda.memory_allocated() == before
+    for seqs, queries, keys in ((1, 8192, 8192), (8, 1000, 4000), (64, 100, 8192), (256, 1, 8192), (5, 40, 8192)):
+        assert _lib.load().rq_q8_attention_workspace_bytes(seqs, HQ, H, D, queries, keys) <= aside

@@ -6,6 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from rotorquant_vllm import _lib
 from rotorquant_vllm.kernels import q8
 
 
@@ -121,3 +122,17 @@ def test_backend_batches_of_decodes_with_idle_sequences(monkeypatch, q_lens, hos
                 seen[row] = int(table[b, 0])
                 assert kw["max_seq_len"] is None or kw["max_seq_len"] >= int(lens_[b])
     assert seen == {starts[b]: b for b, m in enumerate(q_lens) if m}
+
+
+def test_no_call_needs_more_than_the_bound():
+    import random
+    lib, rng = _lib.load(), random.Random(3)
+    for _ in range(3000):
+        D, H, G = rng.choice([64, 128]), rng.choice([1, 2, 4, 8, 32, 128]), rng.choice([1, 4, 7, 8, 17, 200])
+        longest = int(2 ** rng.uniform(0, 22))
+        bound = lib.rq_q8_attention_workspace_bound(H * G, H, D, longest)
+        sizes = (int(2 ** rng.uniform(0, 16)) - 1, H * G, H, D, int(2 ** rng.uniform(0, 15)), rng.choice([longest, rng.randint(0, longest)]))
+        need = lib.rq_q8_attention_workspace_bytes(*sizes)
+        assert need <= bound, (sizes, need, bound)
+        assert bound < max(256 << 20, longest * 800) + (40 << 20)
+    assert lib.rq_q8_attention_workspace_bound(0, 0, 128, 100) == lib.rq_q8_attention_workspace_bound(8, 8, 128, -1) == 0
