@@ -78,6 +78,11 @@ def _check_cache(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> tu
     return NB, BS, page
 
 
+def _row_strides(shape, strides) -> tuple:
+    """Strides of calls with one token or one head: that over a single one, which may be any number in a view, as 0."""
+    return (strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0, strides[2])
+
+
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> torch.Tensor:
     if t.dtype != dtype or t.dim() != dim:
         raise ValueError(f"{name} must be a {dim}-dimensional {dtype} tensor, got {t.dim()} dimensions of {t.dtype}")
@@ -125,6 +130,8 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
         raise ValueError("key and value must have the same (tokens, heads, head_dim) shape and dtype")
     N, H, D = shape
     ks, vs = key.stride(), value.stride()
+    if N == 1 or H == 1:
+        ks, vs = _row_strides(shape, ks), _row_strides(shape, vs)
     if ks[2] != 1 or vs[2] != 1:
         raise ValueError("key/value must be contiguous over head_dim")
     NB, BS, stride = _check_cache(kv_cache, H, D)
@@ -216,6 +223,8 @@ def q8_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     os = out.stride()
     if out.shape != shape or out.dtype != q.dtype or os[2] != 1:
         raise ValueError("out must have q's shape and dtype and be contiguous over head_dim")
+    if T == 1 or HQ == 1:
+        qs, os = _row_strides(shape, qs), _row_strides(shape, os)
     capacity = max_blocks * BS
     max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
     code = _format(fmt)

@@ -62,3 +62,21 @@ def test_a_tiny_scale_times_large_numbers(fmt):
         out, tol = X.attention(q, ref, table, [n], [0, T], sm_scale=2.0 ** -62)
         got = K.q8_attention(q.to(X.DEV), cache, X.i32(table), X.i32([n]), H, D, fmt=fmt, cu_seqlens_q=X.i32([0, T]), max_q_len=T, sm_scale=2.0 ** -62)
         X.check(got, out, tol)
+
+
+def test_one_row_of_any_stride():
+    """One token, and one head, as views whose stride over it is odd: stored, and attended to."""
+    D, block = 128, 16
+    wide = torch.randn(3, 4 * D + 3, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(X.DEV)
+    for H, HQ in ((2, 4), (1, 1)):
+        cache, ref = X.new_cache(2, block, H, D), Q.Cache(2, block, H, D, "int8")
+        k = torch.as_strided(wide, (1, H, D), (4 * D + 3, D if H > 1 else 5, 1))
+        slots = torch.tensor([16], device=X.DEV)
+        K.q8_store(k, k, cache, slots)
+        ref.store(k.cpu(), k.cpu(), [16])
+        assert Q.same_numbers(cache.cpu().numpy(), ref.to_bytes(), "int8")
+        q = torch.as_strided(wide, (1, HQ, D), (4 * D + 3, D if HQ > 1 else 7, 1))
+        out = torch.as_strided(torch.zeros(5 * D, dtype=torch.bfloat16, device=X.DEV), (1, HQ, D), (9, D if HQ > 1 else 11, 1))
+        table = np.array([[1]], np.int32)
+        want, tol = X.attention(q.cpu(), ref, table, [1], [0, 1])
+        X.check(K.q8_attention(q, cache, X.i32(table), X.i32([1]), H, D, out=out), want, tol)

@@ -136,3 +136,10 @@ def test_no_call_needs_more_than_the_bound():
         assert need <= bound, (sizes, need, bound)
         assert bound < max(256 << 20, longest * 800) + (40 << 20)
     assert lib.rq_q8_attention_workspace_bound(0, 0, 128, 100) == lib.rq_q8_attention_workspace_bound(8, 8, 128, -1) == 0
+
+
+def test_strides_over_one_element_do_not_count():
+    assert q8._row_strides((3, 2, 64), (500, 64, 1)) == (500, 64, 1)
+    assert q8._row_strides((1, 2, 64), (501, 64, 1)) == (0, 64, 1)
+    assert q8._row_strides((3, 1, 64), (64, 5, 1)) == (64, 0, 1)
+    assert q8._row_strides((1, 1, 64), (7, 5, 2)) == (0, 0, 2)
