@@ -427,8 +427,10 @@ int rq_short_attention(const void *q, int32_t dtype, int64_t total_q, int32_t nu
  *
  * A second cache, beside the packed codebook cache above: K and V as 8-bit codes with a
  * power-of-two scale for each group of 16 consecutive slots, kv head and side.  Twice the bytes of
- * 4-bit indices, no rotation, and an error of a 16-bit model's size rather than a
- * codebook's.  No counterpart in the reference, whose codecs stop at 4 bits.
+ * 4-bit indices, no rotation, and an error between a 16-bit cache's and the codebooks': relative error of the attention's output
+ * against unrounded K and V, 1024 keys of 128 dims, N(0, 1): bf16 0.0025, int8 0.016, e4m3 0.039, 4-bit codebook 0.14, 3-bit 0.27; keys
+ * with strong channels (1 + |N(0, 3)|), which set the scale of all the others: 0.0046, 0.045, 0.091, 0.39, 0.60.  No counterpart in
+ * the reference, whose codecs stop at 4 bits.
  *
  * A value is c * 2^e.  e is the smallest integer of [-40, 60] with amax <= Q * 2^e, where amax
  * is the largest finite magnitude written to the group and Q = 127.5 (int8) or 448 (e4m3);
