@@ -456,6 +456,10 @@ enum rq_q8_format {
     RQ_Q8_E4M3 = 1
 };
 
+/* (Token, query head) pairs of a kv head, max_q_len times the group, from which rq_q8_attention takes a call of several tokens a
+ * sequence to its prompt kernels. */
+#define RQ_Q8_PROMPT_COLUMNS 192
+
 /* Bytes of a cache slot (block_size of them make a page); 0 for sizes below 1 and for slots of 2^31 bytes or more. */
 int rq_q8_slot_bytes(int32_t num_kv_heads, int32_t head_dim);
 

@@ -490,11 +490,10 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
     fmt == RQ_Q8_INT8 ? launch_stream_d<DT, RQ_Q8_INT8>(a, D, wgs, st) : launch_stream_d<DT, RQ_Q8_E4M3>(a, D, wgs, st);
 }
 
-// Calls of so many columns per kv head or more go to the prefill kernels.  8 kv heads x 4, queries of 1 to n tokens, these / those:
+// Calls of RQ_Q8_PROMPT_COLUMNS per kv head or more go to the prefill kernels.  8 kv heads x 4, queries of 1 to n tokens, these / those:
 // 8 sequences of 8000 keys, n = 20: 57 / 156 us, 32: 99 / 160, 64: 164 / 195;  32 of 1000, 32: 58 / 77, 64: 109 / 81;  1 of
 // 8000, 64: 40 / 40;  head_dim 64, 8 of 4000, 32: 38 / 44, 64: 52 / 51.
-constexpr int64_t kQ8PromptCols = 192;
-static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= kQ8PromptCols; }
+static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= RQ_Q8_PROMPT_COLUMNS; }
 
 // Lengths are ints in the kernels.
 static int64_t q8_bound(int64_t max_seq_len) { return std::min<int64_t>(max_seq_len, INT32_MAX - 64); }

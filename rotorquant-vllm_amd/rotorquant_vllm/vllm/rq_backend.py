@@ -173,7 +173,7 @@ RQ_FUSED_MAX_KV_HEADS = 64
 # Shapes of the 8-bit cache.
 RQ_8BIT_HEAD_DIMS = (64, 128)
 RQ_8BIT_GROUP = 16
-RQ_8BIT_PROMPT_COLUMNS = 192  # q8_attention's prefill kernels from here on: (token, query head) pairs of a kv head
+RQ_8BIT_PROMPT_COLUMNS = 192  # q8_attention's prefill kernels from here on (RQ_Q8_PROMPT_COLUMNS of include/rq_abi.h)
 
 
 def _fused_shape_ok(num_heads: int, num_kv_heads: int, head_size: int) -> str | None:

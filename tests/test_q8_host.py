@@ -1,5 +1,7 @@
 """Host side of the 8-bit cache without a GPU: sizes of scratch, refusals of the backend, strides."""
 import contextlib
+import os
+import re
 import sys
 from types import SimpleNamespace
 
@@ -143,3 +145,12 @@ def test_strides_over_one_element_do_not_count():
     assert q8._row_strides((1, 2, 64), (501, 64, 1)) == (0, 64, 1)
     assert q8._row_strides((3, 1, 64), (64, 5, 1)) == (64, 0, 1)
     assert q8._row_strides((1, 1, 64), (7, 5, 2)) == (0, 0, 2)
+
+
+def test_the_backend_and_the_library_agree_on_prompts():
+    """One number in two languages, and the sizes of scratch change with it: images from there on."""
+    from rotorquant_vllm.vllm import rq_backend as B
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "rq_abi.h")) as f:
+        assert int(re.search(r"#define RQ_Q8_PROMPT_COLUMNS (\d+)", f.read())[1]) == B.RQ_8BIT_PROMPT_COLUMNS
+    need, cols = _lib.load().rq_q8_attention_workspace_bytes, B.RQ_8BIT_PROMPT_COLUMNS
+    assert need(1, 1, 1, 128, cols - 1, 64) == 0 < need(1, 1, 1, 128, cols, 64)
