@@ -57,8 +57,9 @@ __device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
     if (s.q0 < 0) s.T = 0;
     const int L = a.seq_lens[b];
     s.vis = (int)max((int64_t)0, min((int64_t)L, a.cap));
-    // (by the query's whole length, also where max_q cuts it; far below 0, where no key is seen, the exact place is of no account)
-    s.pos = (int)max((int64_t)L - ((int64_t)end - s.q0), (int64_t)-(1 << 30));
+    // (by the query's whole length, also where max_q cuts it; far below 0, where no key is seen, or far above, where all are, the
+    // exact place is of no account, and sums with a query's tokens stay ints)
+    s.pos = (int)min(max((int64_t)L - ((int64_t)end - s.q0), (int64_t)-(1 << 30)), (int64_t)INT32_MAX - (1 << 21));
     return s;
 }
 

@@ -80,3 +80,18 @@ def test_one_row_of_any_stride():
         table = np.array([[1]], np.int32)
         want, tol = X.attention(q.cpu(), ref, table, [1], [0, 1])
         X.check(K.q8_attention(q, cache, X.i32(table), X.i32([1]), H, D, out=out), want, tol)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T,keys", [(1, 60), (1, 2500), (5, 60), (5, 2500), (70, 150), (70, 2500)])
+def test_lengths_near_the_end_of_an_int(T, keys, causal):
+    """Contexts said to be longer than anything: what the table holds is seen, by every query."""
+    H, G, D = 1, 4, 64
+    cache, ref, table = X.filled([keys], 16, H, D, "int8", torch.bfloat16, 3)
+    table = table[:, :keys // 16]
+    q = torch.randn(3 * T, H * G, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    lens, table, cu = [2 ** 31 - 1, 2 ** 31 - 40, -2 ** 31], np.repeat(table, 3, axis=0), [0, T, 2 * T, 3 * T]
+    out, tol = X.attention(q, ref, table, lens, cu, causal)
+    got = K.q8_attention(q.to(X.DEV), cache, X.i32(table), X.i32(lens), H, D, cu_seqlens_q=X.i32(cu), max_q_len=T, causal=causal)
+    X.check(got, out, tol)
+    assert not got[2 * T:].any()
