@@ -438,7 +438,8 @@ int rq_short_attention(const void *q, int32_t dtype, int64_t total_q, int32_t nu
  * Writing slot 16 n of the cache begins its group anew: rows not written by the same call become 0.
  * Other writes keep the group's rows; where their amax needs a larger e, the codes
  * that stay are rounded again at the new scale.  So tokens are written forward within a group, as a
- * server does; a slot may be written again (a rejected draft's), which never lowers the scale.
+ * server does; a slot may be written again (a rejected draft's), which never lowers the scale.  A store reads and writes whole groups,
+ * so stores to one group, and reads of it beside a store, have to be ordered (one stream, or events).
  *
  * Page of block_size slots (a multiple of 16), H kv heads, D = head_dim:
  *   [block_size / 16 groups][H][K codes 16 D | V codes 16 D], then the scales

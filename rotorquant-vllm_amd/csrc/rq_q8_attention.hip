@@ -22,8 +22,8 @@
 // the next tile (8 KB at head_dim 128) in registers while it computes one; two workgroups of four waves a CU (175
 // registers) keep 64 KB a CU on their way.  Three workgroups a CU (168 registers, 10 spilled, or one tile of registers
 // refilled as it is used) 127 to 130 us against 127 before the loads became non-temporal; two tiles ahead 109 against 107;
-// twice or four times the workgroups, which balance themselves, 130 and 139 (more partials, more prologues).  Small calls are bound by
-// their chain of dependent loads: lengths, block table, codes, then the sums of the waves.
+// twice or four times the workgroups, which balance themselves, 130 and 139 (more partials, more prologues).  Small calls: at
+// q8_item_kernel.
 #include <algorithm>
 #include <cmath>
 
@@ -432,8 +432,11 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgro
     q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);
 }
 
-// One workgroup of 8 waves per item: one launch, no partials.  Bound by what one CU loads (a tile a wave per 1.07 us, 61 GB/s):
-// two, three or four tiles ahead instead of one took 8.7, 9.0 and 9.0 us against 8.6 (one sequence of 777 keys).
+// One workgroup of 8 waves per item: one launch, no partials.  What bounds it is two things in a row.  A chain of dependent loads and its
+// launch -- lengths, block table, codes, then the sums of the waves: 5.2 us (one sequence of 16 keys, 8 kv heads x 4).  Then
+// what one CU loads, since an item is one workgroup's: 4.7 us for each 1000 keys beyond the first 100 (a tile a wave per 1.07 us, 54 to
+// 61 GB/s; 777 to 800 keys 8.6 to 9.3 us, 1600 12.4).  Two, three or four tiles ahead instead of one: 8.7, 9.0 and 9.0 us against 8.6
+// (777 keys), so it is the rate and not the latency; more CUs to an item would need a merge between workgroups.
 template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
     __shared__ Q8Sums<D, 8> lds;
@@ -457,7 +460,7 @@ static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_
 
 // Calls of short contexts, by the bound on their lengths, take a workgroup per item.  One launch without partials saves 4 to 7 us; a long item
 // by itself is slower, as one workgroup walks it.  8 kv heads x 4, equal lengths, graph replays, items / shares:
-//   1 sequence of 800 keys 8.6 / 12.7 us, 1600: 12.7 / 14.0, 3200: 19.3 / 14.3;  8: 9.5 / 14.5, 13.6 / 17.2, 22.1 / 20.3;
+//   1 sequence of 800 keys 8.6 / 13.7 us, 1600: 12.4 / 14.3, 3200: 19.3 / 14.3;  8: 9.5 / 14.5, 13.6 / 17.2, 22.1 / 20.3;
 //   64: 24.6 / 25.0, 40.8 / 42.4, 73.5 / 78.0.
 constexpr int64_t kQ8ItemTiles = 60;
 static bool q8_is_short(int64_t max_keys) {
@@ -491,7 +494,7 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
 }
 
 // Calls of RQ_Q8_PROMPT_COLUMNS per kv head or more go to the prefill kernels.  8 kv heads x 4, queries of 1 to n tokens, these / those:
-// 8 sequences of 8000 keys, n = 20: 57 / 156 us, 32: 99 / 160, 64: 164 / 195;  32 of 1000, 32: 58 / 77, 64: 109 / 81;  1 of
+// 8 sequences of 8000 keys, n = 20: 58 / 156 us, 32: 95 / 160, 47: 128, 64: 164 / 196;  32 of 1000, 32: 58 / 77, 64: 109 / 81;  1 of
 // 8000, 64: 40 / 40;  head_dim 64, 8 of 4000, 32: 38 / 44, 64: 52 / 51.
 static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= RQ_Q8_PROMPT_COLUMNS; }
 

@@ -87,6 +87,7 @@ __device__ __forceinline__ u32x4 q8_query_f16(u32x4 raw, float f) {
 // Weights are w = 2^(u + B) in fp16.  A column's B begins at kQ8NoBias (no key seen) and becomes kQ8Peak - u at its largest u so far, but only
 // when w would pass 2^kQ8Most: the largest w is 2^7 to 2^15 (fp16 ends at 2^16), so weights keep fp16's 11 bits down
 // to 2^-21 of it, and those down to 2^-31 count.  The factor 2^B is in O and in l, and so not in O / l.
+// With a peak of 1 and the same code a full batch of prompts takes 849 us against 859: small weights then have fewer bits to multiply.
 // Where |B| is large, u + B is off by up to 1.5 of its last places (the rounding of u, and of the exponent's addend): the 2^-19 |B|
 // leaves room for them up to |B| = 2^26.
 constexpr float kQ8Peak = 7.f, kQ8Most = 15.f, kQ8NoBias = 3.402823466e38f;

@@ -143,7 +143,7 @@ __device__ __forceinline__ void q8_floats(const Q8Raw<DT> &r, float (&x)[8]) {
 // A wave takes a.per_wave units of one group, the next one's rows on their way while one is coded.  Lane: token row
 // t = lane % 16, half = (lane / 16) % 2 of the 16-dim parts; the wave's upper 32 lanes are the second 64-dim chunk
 // (D = 128) or the V side (D = 64).
-// Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in 49 us beside 9 for the two link launches.  Non-temporal loads
+// Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in 47 us beside 10 for the two link launches (graph replays of all three: 48).  Non-temporal loads
 // here: 56 us (a row's 128 bytes are loaded by four instructions, which then miss the L1).
 template <int DT, int FMT, int D, bool LINKED>
 __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a) {
@@ -380,8 +380,9 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
     }
 }
 
-// Units of a wave in a long call: two once one each would be more waves than the GPU holds (about 24 a CU).  32768 tokens of 8
-// heads, with their read-back: one 97 us, two 94, four 96.
+// Units of a wave in a long call: two once one each would be more waves than the GPU holds (about 24 a CU).  GPU time of the store
+// alone, 8 heads, one / two / four units: 1024 tokens 9.7 / 10.7 / 13.5 us, 4096: 14.4 / 14.5 / 15.8, 8192 (just under the border):
+// 20.1 / 19.3 / 19.1, 32768: 54.0 / 48.3 / 49.5.
 static int q8_per_wave(int64_t groups, int units) { return groups * units >= 48 * (int64_t)device_cus() ? 2 : 1; }
 
 template <int DT, int FMT, int D>
@@ -420,8 +421,9 @@ static void launch_read_f(const Q8ReadArgs &a, int fmt, int D, hipStream_t st) {
     fmt == RQ_Q8_INT8 ? launch_read_d<DT, RQ_Q8_INT8>(a, D, st) : launch_read_d<DT, RQ_Q8_E4M3>(a, D, st);
 }
 
-// Tokens up to which every wave looks through all slots itself: one launch, no workspace.  With read-back, 256 tokens of prompts
-// 11.0 us (linked: 12.5), 512 13.5 (12.9), 1024 22.8 (14.4); 512 appended tokens 26.8 (29.6).
+// Tokens up to which every wave looks through all slots itself: one launch, no workspace.  GPU time of the store alone, 8 heads, itself /
+// linked: appended tokens (a group each) 16: 4.9 / 8.8 us, 128: 5.8 / 10.0, 256: 7.9 / 12.0, 512: 13.5 / 17.3, 1024: 27.5 / 28.0;
+// prompts 256: 7.3 / 8.9, 512: 9.7 / 9.3, 1024: 17.7 / 9.6, 2048: 39 / 10.7.  (Its work grows with the square of the tokens.)
 constexpr int64_t kStoreScan = 512;
 
 }  // namespace rq

@@ -160,13 +160,16 @@ __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int 
 __device__ __forceinline__ int q8_chunk_tiles(int n_tiles, int split) { return max(kQ8MinTiles, (n_tiles + split - 1) / split); }
 
 // What bounds it: the matrix cores and vector issue together, under the card's power limit.  8 prompts of 2222 to 4096 tokens, 32 / 8
-// heads (0.84 TFLOP): 805 to 885 us, 950 to 1040 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
+// heads (0.84 TFLOP): 820 to 880 us, 955 to 1020 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
 // 1800 of zeros).  The matrix cores are busy half of the cycles, at 1.8 GHz (the memory-bound kernels run at 2.1).  A wave's tile
-// is 32 MFMAs, 32 exponentials and about 115 other vector instructions; measured by itself, an MFMA with a pair of exponentials
-// and its packing takes 21.4 ns of a SIMD, without 13.8, so the first phase is bound by issue.  Without the tile copies 9 %
-// less time, without exponentials 6 %.  Tried without gain: two units a wave at one wave a SIMD (half the LDS reads; 226
-// registers spilled), eight waves on one tile (926 -> 931 us, one prompt of 700 tokens 24 -> 32), two sets of four waves on alternate
-// tiles (1000 tokens 35 -> 30 us, 700 and less 1 us slower), one wait for two operand reads, other depths of reading ahead.
+// is 32 MFMAs, 32 exponentials and 117 other vector instructions (the listing: 50 in the first phase, 67 in the second), a tile on the
+// diagonal 69 more, a raised maximum 73; with those, the first and the last tile and the prologue the counters give 148 a tile.
+// Measured by itself, an MFMA with a pair of exponentials and its packing takes 21.4 ns of a SIMD, without 13.8, so the first phase is
+// bound by issue.  Without the tile copies 9 % less time, without exponentials 6 %.
+// Tried without gain: two units a wave at one wave a SIMD (half the LDS reads; 226 registers spilled), eight waves on one tile
+// (926 -> 931 us, one prompt of 700 tokens 24 -> 32), one wait for two operand reads, other depths of reading ahead.
+// A gain that is not taken: two sets of four waves on alternate tiles, one prompt of 1000 tokens 35 -> 30 us, of 700 and less 1 us slower; it
+// would be a second form of this kernel, for calls of few workgroups and many tiles.
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void q8_prefill_kernel(Q8PrefillArgs p) {
     using Im = Q8Image<D>;
@@ -465,7 +468,8 @@ __global__ __launch_bounds__(256) void q8_prefill_merge_kernel(Q8PrefillArgs p) 
 constexpr int64_t kQ8ImageBytes = 256LL << 20;
 constexpr int kQ8SplitTiles = 8;  // tiles of a key chunk by the call's bound on the lengths, at least
 // Key chunks where the workgroups fill at most half of the places (two a CU).  Chunks elsewhere, us for none / 2 / 3: one prompt of 700
-// 24 / 33 / 33, of 2500 74 / 92 / 107; 500 tokens behind 3500 keys 55 / 57 / 58; two of about 1480 behind 4100 at head_dim 64 174 / 165 / 173.
+// 24 / 33 / 33, of 2500 74 / 92 / 107; 500 tokens behind 3500 keys 55 / 57 / 58; two of about 1480 behind 4100 at head_dim 64 174 / 165 / 173 (1.47 rounds of
+// workgroups there: two chunks gain, and no rule that takes them there and not elsewhere was looked for).
 struct Q8PrefillShape {
     int64_t tiles, nb, nh, nx, split, image, images, part;
 };

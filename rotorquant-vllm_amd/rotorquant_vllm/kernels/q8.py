@@ -119,7 +119,8 @@ def q8_store(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slo
 
     Slots outside the cache (vLLM's padding id -1) are skipped; of tokens with the same slot the last one counts.
     A write of a group's first slot begins the group anew (its rows that this call does not write
-    become 0); other writes keep its rows and never lower its scale.
+    become 0); other writes keep its rows and never lower its scale.  A store reads and writes whole groups: stores to one
+    group, and reads of it, on several streams have to be ordered by the caller.
     Rows (and the cache) start at multiples of 16 bytes, as slices of a fused projection do; others are refused.
     workspace: scratch of calls of more than 512 tokens (rq_q8_store_workspace_bytes bytes),
     by default from torch's allocator; a graph captured without torch's graph classes needs it.
