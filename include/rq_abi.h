@@ -495,7 +495,7 @@ int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, 
 /*
  * Attention of new query tokens over the 8-bit cache: single tokens (decodes), drafts of a few,
  * prompts and chunks behind a prefix.  Query i of sequence b sits at position seq_lens[b] - q_len_b + i; causal != 0: it
- * sees cache positions up to its own, causal == 0: all seq_lens[b].  A row that sees no key gives zeros.
+ * sees cache positions up to its own, causal == 0: all seq_lens[b].  A row that sees no key gives zeros.  |sm_scale| is 2^127 at most.
  *
  * q / out: total_q x num_q_heads x head_dim of F16 or BF16 (element strides; q rows 16-byte, out rows
  * 8-byte aligned), num_q_heads a multiple of num_kv_heads.  cu_seqlens_q: num_seqs + 1 int32, or NULL

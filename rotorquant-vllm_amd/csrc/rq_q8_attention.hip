@@ -542,6 +542,7 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     uint32_t scale_bits;  // (by its bits: this file is compiled for arithmetic without NaN)
     __builtin_memcpy(&scale_bits, &sm_scale, 4);
     RQ_CHECK_ARG((scale_bits & 0x7f800000u) != 0x7f800000u, "sm_scale must be finite");
+    RQ_CHECK_ARG(__builtin_fabsf(sm_scale) <= 0x1p127f, "sm_scale %g is past 2^127", (double)sm_scale);  // (times log2(e) it is finite)
     if (num_seqs == 0 || total_q == 0 || max_q_len == 0) return RQ_OK;
     RQ_CHECK_ARG(num_blocks > 0, "the cache has no pages");
     RQ_CHECK_ARG(q && out && seq_lens && (block_table || max_blocks == 0), "null pointer");

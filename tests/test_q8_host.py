@@ -154,3 +154,10 @@ def test_the_backend_and_the_library_agree_on_prompts():
         assert int(re.search(r"#define RQ_Q8_PROMPT_COLUMNS (\d+)", f.read())[1]) == B.RQ_8BIT_PROMPT_COLUMNS
     need, cols = _lib.load().rq_q8_attention_workspace_bytes, B.RQ_8BIT_PROMPT_COLUMNS
     assert need(1, 1, 1, 128, cols - 1, 64) == 0 < need(1, 1, 1, 128, cols, 64)
+
+
+@pytest.mark.parametrize("scale,status", [(2.0 ** 127, 2), (-2.0 ** 127, 2), (2.0 ** 127 * 1.01, 1), (-3.4e38, 1), (1.4e-45, 2)])
+def test_scales_past_the_kernels_range_are_refused(scale, status):
+    """In base 2 a scale is 1.44 times as large; 2 (too little scratch) says that it was taken."""
+    from test_q8 import ATTN
+    assert _lib.load().rq_q8_attention(*{**ATTN, "q": 16, "out": 16, "mb": 1000, "msl": 16000, "scale": scale}.values()) == status, _lib.load().rq_last_error()
