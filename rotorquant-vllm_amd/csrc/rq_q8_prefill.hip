@@ -160,7 +160,7 @@ __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int 
 __device__ __forceinline__ int q8_chunk_tiles(int n_tiles, int split) { return max(kQ8MinTiles, (n_tiles + split - 1) / split); }
 
 // What bounds it: the matrix cores and vector issue together, under the card's power limit.  8 prompts of 2222 to 4096 tokens, 32 / 8
-// heads (0.84 TFLOP): 820 to 880 us, 955 to 1020 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
+// heads (0.84 TFLOP): 820 to 880 us by card, 955 to 1020 TFLOP/s (the library's 8192^3 product: 1240 to 1340 of random numbers,
 // 1800 of zeros).  The matrix cores are busy half of the cycles, at 1.8 GHz (the memory-bound kernels run at 2.1).  A wave's tile
 // is 32 MFMAs, 32 exponentials and 117 other vector instructions (the listing: 50 in the first phase, 67 in the second), a tile on the
 // diagonal 69 more, a raised maximum 73; with those, the first and the last tile and the prologue the counters give 148 a tile.
