@@ -521,6 +521,89 @@ int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q
                     void *out, int64_t out_stride_tok, int64_t out_stride_head,
                     void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * ---- position rotation on the way into a cache -------------------------------------
+ *
+ * A layer's rotary embedding and its store in one call: the queries' rows rotated to out_q, the keys' rotated into
+ * the cache, the values stored as they are.  One call for each of the cache's formats.  No counterpart in the reference, whose model
+ * rotates before the backend is called.
+ *
+ * cos_sin: table_rows rows (table_stride elements apart, 16-byte aligned) of rot_dim numbers, the cosines of rot_dim / 2 angles and
+ * then their sines, fp32 or of the rows' dtype (table_dtype).  Token t takes row positions[t] (int64).  Angle i turns
+ * the pair of dims (i, i + rot_dim / 2) (halves != 0) or (2 i, 2 i + 1):
+ *   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
+ * in fp32, each product and the sum rounded once; dims from rot_dim on stay.  Keys go on in fp32: norm, codes and scales are those of
+ * the unrounded result, as if a store of fp32 rows were given it, and 16-bit pages take it rounded once.  A token whose
+ * position is outside the table is rotated by NaN.  rot_dim: a multiple of 16 up to head_dim, head_dim one too (up to 512 for queries).
+ *
+ * query / out_q: n_tokens x num_q_heads x head_dim (num_q_heads 0: none; out_q may be query); rows of queries, keys, values and out_q are 16-byte
+ * aligned, strides in elements.  Queries of all tokens are rotated, also of those whose slot is outside the cache (padding), which are not stored.
+ */
+
+/* rq_compress_store of rotated keys (arguments as there); head_dim up to 256. */
+int rq_rope_compress_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                           int64_t q_stride_token, int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                           int64_t v_stride_token, int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                           const int64_t *positions, const void *cos_sin, int32_t table_dtype, int64_t table_rows, int64_t table_stride,
+                           int32_t rot_dim, int32_t halves, void *out_q, int64_t out_stride_token, int64_t out_stride_head,
+                           int32_t index_layout, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
+                           int32_t block_size, int64_t stride_block, int64_t stride_token, int32_t total_bytes,
+                           const float *rot_t_even, const float *rot_t_odd, int32_t rot_block,
+                           const float *k_boundaries, int32_t n_k_boundaries, const float *v_boundaries, int32_t n_v_boundaries,
+                           void *stream);
+
+/* rq_q8_store of rotated keys (arguments and workspace as there). */
+int rq_rope_q8_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                     int64_t q_stride_token, int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                     int64_t v_stride_token, int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                     const int64_t *positions, const void *cos_sin, int32_t table_dtype, int64_t table_rows, int64_t table_stride,
+                     int32_t rot_dim, int32_t halves, void *out_q, int64_t out_stride_token, int64_t out_stride_head, int32_t format,
+                     const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * ---- plain 16-bit pages -----------------------------------------------------------
+ *
+ * K and V (num_blocks, block_size, num_kv_heads, head_dim) of F16 or BF16 each, addressed by strides of elements between
+ * pages, slots and heads, rows 16-byte aligned: what rq_paged_decompress makes, and what a layer keeps that is not to be compressed.
+ */
+
+/* Rotated keys, and values, into the slots of slot_mapping (block * block_size + offset; those outside the cache are skipped; a
+ * slot is given once).  dtype F16 or BF16, that of the pages. */
+int rq_rope_kv16_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                       int64_t q_stride_token, int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                       int64_t v_stride_token, int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                       const int64_t *positions, const void *cos_sin, int32_t table_dtype, int64_t table_rows, int64_t table_stride,
+                       int32_t rot_dim, int32_t halves, void *out_q, int64_t out_stride_token, int64_t out_stride_head,
+                       const int64_t *slot_mapping, void *k_cache, void *v_cache, int64_t num_blocks, int32_t block_size,
+                       int64_t kc_stride_block, int64_t kc_stride_slot, int64_t kc_stride_head,
+                       int64_t vc_stride_block, int64_t vc_stride_slot, int64_t vc_stride_head, void *stream);
+
+/*
+ * Attention of new query tokens over plain 16-bit pages: single tokens (decodes) and queries of a few (drafts); longer
+ * ones are right too, but read the keys again for every 32 (token, query head) pairs of a kv head.  Query i of sequence b sits at position
+ * seq_lens[b] - q_len_b + i; causal != 0: it sees cache positions up to its own, causal == 0: all seq_lens[b].  A row that
+ * sees no key gives zeros; infinities and NaN count only where they are seen.
+ *
+ * q / out: total_q x num_q_heads x head_dim of the pages' dtype (element strides; q rows 16-byte, out rows 8-byte aligned),
+ * num_q_heads a multiple of num_kv_heads, head_dim a multiple of 8 up to 256, any block_size.  cu_seqlens_q: num_seqs + 1 int32, or NULL for one
+ * token per sequence.  max_q_len bounds every q_len_b and max_seq_len every seq_lens[b]: tokens and keys past them, or past the block table's
+ * capacity, are not read (positions go by the whole q_len_b and seq_lens[b] all the same), and out's rows of such tokens,
+ * as those of no sequence, are left as they are.  Pages outside the cache are read as page 0.  Products are exact, sums and the softmax's
+ * statistics fp32, its weights two 16-bit numbers each for P V.  |sm_scale| is 2^127 at most.
+ * workspace: rq_kv16_attention_workspace_bytes() bytes (asked for on the GPU of the call), 16-byte aligned, no initialisation needed; 0 where
+ * max_seq_len is 1024 or less.  Launches depend on host arguments only, so a captured call may be replayed with other lengths up to max_seq_len.
+ */
+int64_t rq_kv16_attention_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                          int64_t max_q_len, int64_t max_seq_len);
+int rq_kv16_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads, int64_t q_stride_tok, int64_t q_stride_head,
+                      const int32_t *cu_seqlens_q, int64_t num_seqs, int64_t max_q_len, int32_t causal, const void *k_cache,
+                      const void *v_cache, int64_t num_blocks, int32_t block_size, int64_t kc_stride_block, int64_t kc_stride_slot,
+                      int64_t kc_stride_head, int64_t vc_stride_block, int64_t vc_stride_slot, int64_t vc_stride_head,
+                      int32_t num_kv_heads, int32_t head_dim, const int32_t *block_table, int64_t max_blocks, int64_t bt_stride_seq,
+                      const int32_t *seq_lens, int64_t max_seq_len, float sm_scale, void *out, int64_t out_stride_tok,
+                      int64_t out_stride_head, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -226,6 +226,47 @@ template <> struct Elem<RQ_DTYPE_F32> {
     using storage = float;
 };
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+// Eight consecutive elements of a row (16-byte aligned) as they lie in memory.
+template <int DT>
+struct Row8 {
+    u32x4 w[DT == RQ_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Row8<DT> row8_load(const void *p, int64_t at) {
+    Row8<DT> r;
+    const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(p) + at * (DT == RQ_DTYPE_F32 ? 4 : 2));
+    r.w[0] = *q;
+    if constexpr (DT == RQ_DTYPE_F32) r.w[1] = q[1];
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void row8_floats(const Row8<DT> &r, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (DT == RQ_DTYPE_F32) x[i] = __uint_as_float(r.w[i >> 2][i & 3]);
+        else x[i] = Elem<DT>::to_f32((r.w[0][i >> 1] >> (16 * (i & 1))) & 0xffffu);
+    }
+}
+template <int DT>
+__device__ __forceinline__ Row8<DT> row8_round(const float (&x)[8]) {
+    Row8<DT> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (DT == RQ_DTYPE_F32) r.w[i >> 2][i & 3] = __float_as_uint(x[i]);
+        else if (i & 1) r.w[0][i >> 1] = Elem<DT>::from_f32(x[i - 1]) | Elem<DT>::from_f32(x[i]) << 16;
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void row8_store(void *p, int64_t at, const Row8<DT> &r) {
+    u32x4 *q = reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(p) + at * (DT == RQ_DTYPE_F32 ? 4 : 2));
+    q[0] = r.w[0];
+    if constexpr (DT == RQ_DTYPE_F32) q[1] = r.w[1];
+}
+
 // ---------------------------------------------------------------------------
 // Codebook lookup in registers with v_perm_b32.
 //

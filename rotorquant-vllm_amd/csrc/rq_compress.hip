@@ -37,7 +37,9 @@
 // are already loading into registers.  A group's rows are staged through LDS
 // with coalesced 16-byte loads; four lanes per row reduce the norm's partial
 // sums; D/8 lanes per row then produce 8 indices each (one packed dword).
-#include "rq_common.h"
+#include <type_traits>
+
+#include "rq_rope.h"
 
 namespace rq {
 
@@ -74,7 +76,8 @@ struct RowRef {
     const uint8_t *src;  // first element (nullptr: row past the end)
     uint8_t *idx_dst;    // packed indices (nullptr: row past the end or slot skipped)
     float *norm_dst;
-    int32_t is_v, pad;
+    int32_t is_v;
+    int32_t position;    // of a key that is turned by it; -1: none
 };
 
 // LDS map of one workgroup (bytes).  Row addresses and padding lists are
@@ -226,29 +229,49 @@ struct Cursor {
     int rem0;
 };
 
+// What a store with position rotation is given beside its RowMap.
+template <bool ROPE>
+struct CompressRope {};
+template <>
+struct CompressRope<true> {
+    RopeRows rows;         // the queries, by workgroups of their own behind those that compress
+    unsigned store_blocks;
+};
+
 // Four resident waves per SIMD (at most 128 VGPRs) measured fastest for rotation
 // blocks up to 4; 8x8 blocks keep their registers.
 constexpr int compress_waves_per_eu(int blk) { return blk <= 4 ? 4 : 1; }
 
 // DC: head_dim fixed at compile time (128: every loop has a constant trip count), 0 = runtime D_in.
-template <int DT, int BLK, int DC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compress_waves_per_eu(BLK)))) void compress_kernel(RowMap m, int64_t n_rows, int D_in,
+// ROPE: keys are turned by their positions between the load and LDS, whose rows are then fp32 (a rotated key is not rounded before
+// its norm and indices), and from there on everything is as for fp32 rows.
+template <int DT, int BLK, int DC, bool ROPE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE && BLK <= 4 ? 3 : compress_waves_per_eu(BLK)))) void compress_kernel(RowMap m, CompressRope<ROPE> rope, int64_t n_rows, int D_in,
                                                             const float *__restrict__ rt_even,
                                                             const float *__restrict__ rt_odd,
                                                             const float *__restrict__ kbnd, int nkb,
                                                             const float *__restrict__ vbnd, int nvb) {
-    using S = Src<DT>;
-    constexpr int EB = S::bytes;
+    unsigned blocks = gridDim.x;
+    if constexpr (ROPE) {
+        blocks = rope.store_blocks;
+        if (blockIdx.x >= blocks) {
+            rope_rows<DT>(rope.rows, (int64_t)(blockIdx.x - blocks) * kRopeThreads + threadIdx.x);
+            return;
+        }
+    }
+    constexpr int LT = ROPE ? RQ_DTYPE_F32 : DT;  // type of the rows in LDS
+    using S = Src<LT>;
+    constexpr int EB = Src<DT>::bytes;
     const int D = DC > 0 ? DC : D_in;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = tid >> 6;
     const int row_bytes = D * EB;
-    const int pitch = row_bytes + 16;  // +16 B keeps the per-row reads bank-conflict free
+    const int pitch = D * S::bytes + 16;  // +16 B keeps the per-row reads bank-conflict free
     const int half = D / 2;
     const int two_h = 2 * m.H;
     const int64_t n_groups = (n_rows + kRows - 1) / kRows;
-    const int64_t gstride = gridDim.x;
+    const int64_t gstride = blocks;
 
     extern __shared__ __align__(16) uint8_t lds[];
     RowRef *refs_all = reinterpret_cast<RowRef *>(lds + kOffRefs);
@@ -317,7 +340,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
     // Resolve the group's row addresses into buffer b (wave 0).
     auto build_refs = [&](const Cursor &c, int64_t g, int b, int64_t sid) {
         const int64_t r = g * kRows + lane;
-        RowRef ref{nullptr, nullptr, nullptr, 0, 0};
+        RowRef ref{nullptr, nullptr, nullptr, 0, -1};
         bool first = false;
         int pad_j = 0;
         uint8_t *base = nullptr;
@@ -343,6 +366,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
                     ref.norm_dst = reinterpret_cast<float *>(base + (is_v ? L.v_norm : L.k_norm) + 4 * h);
                 }
                 ref.is_v = is_v;
+                if constexpr (ROPE) {  // (those outside the table as its end, which is outside, too)
+                    if (!is_v) {
+                        const int64_t p = rope.rows.t.positions[t];
+                        ref.position = (int32_t)(p >= 0 && p < rope.rows.t.rows ? p : rope.rows.t.rows);
+                    }
+                }
                 first = rem == 0;
                 pad_j = j - (c.rem0 != 0);
             }
@@ -365,6 +394,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
                 const uint8_t *src = refs[rr].src;
                 if (src != nullptr) v[u] = *gbl(reinterpret_cast<const uint4 *>(src + my_part * 16));
             }
+        }
+    };
+
+    // A piece as loaded, to its place in the group's rows.
+    auto stage = [&](int rr, const RowRef &ref, const uint4 &w) {
+        if constexpr (ROPE) {
+            constexpr int kElems = 16 / EB;  // of a piece: 8, or 4 of fp32
+            float x[kElems];
+            if constexpr (EB == 2) row8_floats<DT>(Row8<DT>{{u32x4{w.x, w.y, w.z, w.w}}}, x);
+            else x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+            if (ref.position >= 0 && kElems * my_part < rope.rows.t.rot) rope_elems<DT, kElems>(rope.rows.t, ref.src, ref.position, kElems * my_part, x);
+            float4 *to = reinterpret_cast<float4 *>(rows + rr * pitch + my_part * (4 * kElems));
+#pragma unroll
+            for (int i = 0; i < kElems / 4; ++i) to[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        } else {
+            *reinterpret_cast<uint4 *>(rows + rr * pitch + my_part * 16) = w;
         }
     };
 
@@ -418,7 +463,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
         for (int u = 0; u < 4; ++u) {
             const int rr = my_row + u * rpi;
             if (my_row < rpi && u < n_it && rr < kRows)
-                *reinterpret_cast<uint4 *>(rows + rr * pitch + my_part * 16) = v[u];
+                stage(rr, refs[rr], v[u]);
         }
         for (int u = 4; u < n_it; ++u) {
             const int rr = my_row + u * rpi;
@@ -426,7 +471,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
                 const uint8_t *src = refs[rr].src;
                 uint4 w = make_uint4(0, 0, 0, 0);
                 if (src != nullptr) w = *gbl(reinterpret_cast<const uint4 *>(src + my_part * 16));
-                *reinterpret_cast<uint4 *>(rows + rr * pitch + my_part * 16) = w;
+                stage(rr, refs[rr], w);
             }
         }
         if (m.store) {
@@ -466,16 +511,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
         // and prepares the row's divisor d = n + 1e-10 and its split reciprocal.
         {
             const int rr = tid >> 2, q = tid & 3;
-            const uint8_t *rowq = rows + rr * pitch + 2 * q * EB;
+            const uint8_t *rowq = rows + rr * pitch + 2 * q * S::bytes;
             float s0 = 0.f, s1 = 0.f;
             for (int k = 0; k < D / 8; ++k) {
-                if constexpr (DT == RQ_DTYPE_F16) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t *>(rowq + k * 8 * EB);
+                if constexpr (LT == RQ_DTYPE_F16) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t *>(rowq + k * 8 * S::bytes);
                     s0 = mix_sq<0>(w, s0);
                     s1 = mix_sq<1>(w, s1);
                 } else {
                     float a, b;
-                    load2<S>(rowq + k * 8 * EB, a, b);
+                    load2<S>(rowq + k * 8 * S::bytes, a, b);
                     s0 = __builtin_fmaf(a, a, s0);
                     s1 = __builtin_fmaf(b, b, s1);
                 }
@@ -512,7 +557,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
             const float d = rp.x, yh = rp.y, yl = rp.z;
             bool fast = rp.w != 0.f;
             float xn[8];
-            if constexpr (DT == RQ_DTYPE_F16) {
+            if constexpr (LT == RQ_DTYPE_F16) {
                 // fp16 inputs are 0 or at least 2^-24 in magnitude: inside the guarded range
                 const uint4 w4 = *reinterpret_cast<const uint4 *>(rows + rr * pitch + part * 16);
                 const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -531,7 +576,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
                 }
             } else {
                 float x[8];
-                load8<S>(rows + rr * pitch + part * 8 * EB, x);
+                load8<S>(rows + rr * pitch + part * 8 * S::bytes, x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) fast = fast && (x[e] == 0.f || fabsf(x[e]) >= 0x1p-60f);
                 if (fast) {
@@ -595,7 +640,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(compre
 }
 
 // Resident workgroups of a compress kernel on the current device (cached).
-template <int DT, int BLK, int DC>
+template <int DT, int BLK, int DC, bool ROPE>
 static int compress_grid(size_t lds, int64_t n_groups) {
     static int per_cu[64] = {0};
     static size_t for_lds[64] = {0};
@@ -603,7 +648,7 @@ static int compress_grid(size_t lds, int64_t n_groups) {
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
     if (per_cu[dev] == 0 || for_lds[dev] != lds) {
         int nb = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, reinterpret_cast<const void *>(&compress_kernel<DT, BLK, DC>),
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, reinterpret_cast<const void *>(&compress_kernel<DT, BLK, DC, ROPE>),
                                                          kThreads, lds) != hipSuccess || nb <= 0)
             nb = 4;
         per_cu[dev] = nb;
@@ -613,43 +658,55 @@ static int compress_grid(size_t lds, int64_t n_groups) {
     return (int)(g < n_groups ? g : n_groups);
 }
 
-template <int DT, int BLK, int DC>
-static int launch_compress_dc(const RowMap &m, int64_t n_rows, int D, const float *rte, const float *rto,
-                              const float *kb, int nkb, const float *vb, int nvb, hipStream_t st) {
-    int eb = DT == RQ_DTYPE_F32 ? 4 : 2;
+// Codebooks and rotation of a call.
+struct CompressBook {
+    const float *rte, *rto;
+    int blk;
+    const float *kb;
+    int nkb;
+    const float *vb;
+    int nvb;
+};
+
+template <int DT, int BLK, int DC, bool ROPE>
+static int launch_compress_dc(const RowMap &m, CompressRope<ROPE> rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
+    int eb = ROPE || DT == RQ_DTYPE_F32 ? 4 : 2;
     size_t lds = (size_t)kOffRows + (size_t)kRows * (D * eb + 16);
-    const int grid = compress_grid<DT, BLK, DC>(lds, (n_rows + kRows - 1) / kRows);
-    hipLaunchKernelGGL((compress_kernel<DT, BLK, DC>), dim3((unsigned)grid), dim3(kThreads), lds, st, m, n_rows, D, rte,
-                       rto, kb, nkb, vb, nvb);
+    int64_t grid = compress_grid<DT, BLK, DC, ROPE>(lds, (n_rows + kRows - 1) / kRows);
+    if constexpr (ROPE) {
+        rope.store_blocks = (unsigned)grid;
+        grid += rope_blocks(rope.rows);
+    }
+    hipLaunchKernelGGL((compress_kernel<DT, BLK, DC, ROPE>), dim3((unsigned)grid), dim3(kThreads), lds, st, m, rope, n_rows, D, b.rte, b.rto,
+                       b.kb, b.nkb, b.vb, b.nvb);
     return check_launch("compress_kernel");
 }
+static_assert(kThreads == kRopeThreads, "workgroups of the queries");
 
-template <int DT, int BLK>
-static int launch_compress_blk(const RowMap &m, int64_t n_rows, int D, const float *rte, const float *rto,
-                               const float *kb, int nkb, const float *vb, int nvb, hipStream_t st) {
-    if (D == 128) return launch_compress_dc<DT, BLK, 128>(m, n_rows, D, rte, rto, kb, nkb, vb, nvb, st);
-    return launch_compress_dc<DT, BLK, 0>(m, n_rows, D, rte, rto, kb, nkb, vb, nvb, st);
+template <int DT, int BLK, bool ROPE>
+static int launch_compress_blk(const RowMap &m, const CompressRope<ROPE> &rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
+    if (D == 128) return launch_compress_dc<DT, BLK, 128, ROPE>(m, rope, n_rows, D, b, st);
+    return launch_compress_dc<DT, BLK, 0, ROPE>(m, rope, n_rows, D, b, st);
 }
 
-template <int DT>
-static int launch_compress(const RowMap &m, int64_t n_rows, int D, const float *rte, const float *rto, int blk,
-                           const float *kb, int nkb, const float *vb, int nvb, hipStream_t st) {
+template <int DT, bool ROPE>
+static int launch_compress(const RowMap &m, const CompressRope<ROPE> &rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
     if (n_rows == 0) return RQ_OK;
-    switch (blk) {
-        case 2: return launch_compress_blk<DT, 2>(m, n_rows, D, rte, rto, kb, nkb, vb, nvb, st);
-        case 4: return launch_compress_blk<DT, 4>(m, n_rows, D, rte, rto, kb, nkb, vb, nvb, st);
-        case 8: return launch_compress_blk<DT, 8>(m, n_rows, D, rte, rto, kb, nkb, vb, nvb, st);
+    switch (b.blk) {
+        case 2: return launch_compress_blk<DT, 2, ROPE>(m, rope, n_rows, D, b, st);
+        case 4: return launch_compress_blk<DT, 4, ROPE>(m, rope, n_rows, D, b, st);
+        case 8: return launch_compress_blk<DT, 8, ROPE>(m, rope, n_rows, D, b, st);
     }
-    set_error("rot_block %d unsupported", blk);
+    set_error("rot_block %d unsupported", b.blk);
     return RQ_EINVAL;
 }
 
-static int dispatch_compress(int dtype, const RowMap &m, int64_t n_rows, int D, const float *rte, const float *rto,
-                             int blk, const float *kb, int nkb, const float *vb, int nvb, hipStream_t st) {
+template <bool ROPE>
+static int dispatch_compress(int dtype, const RowMap &m, const CompressRope<ROPE> &rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
     switch (dtype) {
-        case RQ_DTYPE_F16: return launch_compress<RQ_DTYPE_F16>(m, n_rows, D, rte, rto, blk, kb, nkb, vb, nvb, st);
-        case RQ_DTYPE_BF16: return launch_compress<RQ_DTYPE_BF16>(m, n_rows, D, rte, rto, blk, kb, nkb, vb, nvb, st);
-        case RQ_DTYPE_F32: return launch_compress<RQ_DTYPE_F32>(m, n_rows, D, rte, rto, blk, kb, nkb, vb, nvb, st);
+        case RQ_DTYPE_F16: return launch_compress<RQ_DTYPE_F16, ROPE>(m, rope, n_rows, D, b, st);
+        case RQ_DTYPE_BF16: return launch_compress<RQ_DTYPE_BF16, ROPE>(m, rope, n_rows, D, b, st);
+        case RQ_DTYPE_F32: return launch_compress<RQ_DTYPE_F32, ROPE>(m, rope, n_rows, D, b, st);
     }
     set_error("unsupported dtype %d", dtype);
     return RQ_EINVAL;
@@ -683,26 +740,26 @@ extern "C" int rq_compress(const void *x, int32_t x_dtype, int64_t n_rows, int32
     m.packed = packed;
     m.norms = norms;
     m.H = 1;
-    return dispatch_compress(x_dtype, m, n_rows, head_dim, rot_t_even, rot_t_odd, rot_block, boundaries,
-                             n_boundaries, boundaries, n_boundaries, (hipStream_t)stream);
+    return dispatch_compress(x_dtype, m, CompressRope<false>{}, n_rows, head_dim,
+                             CompressBook{rot_t_even, rot_t_odd, rot_block, boundaries, n_boundaries, boundaries, n_boundaries}, (hipStream_t)stream);
 }
 
-extern "C" int rq_compress_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
-                                 int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
-                                 int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
-                                 int32_t index_layout, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
-                                 int32_t block_size, int64_t stride_block, int64_t stride_token,
-                                 int32_t total_bytes, const float *rot_t_even, const float *rot_t_odd,
-                                 int32_t rot_block, const float *k_boundaries, int32_t n_k_boundaries,
-                                 const float *v_boundaries, int32_t n_v_boundaries, void *stream) {
-    int rc = check_common(dtype, head_dim, rot_block, n_k_boundaries, n_v_boundaries);
+namespace rq {
+
+// What rq_compress_store and rq_rope_compress_store do; rope: the queries and the table, or NULL.
+static int compress_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
+                          int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
+                          int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t index_layout, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
+                          int32_t block_size, int64_t stride_block, int64_t stride_token,
+                          int32_t total_bytes, const CompressBook &book, const RopeRows *rope, hipStream_t st) {
+    int rc = check_common(dtype, head_dim, book.blk, book.nkb, book.nvb);
     if (rc) return rc;
     RQ_CHECK_ARG(num_kv_heads >= 1 && n_tokens >= 0 && block_size >= 1 && num_blocks >= 0, "bad sizes");
-    rc = check_index_layout(index_layout, head_dim, n_k_boundaries + 1, n_v_boundaries + 1);
+    rc = check_index_layout(index_layout, head_dim, book.nkb + 1, book.nvb + 1);
     if (rc) return rc;
     if (n_tokens == 0) return RQ_OK;
-    RQ_CHECK_ARG(key && value && slot_mapping && kv_cache && rot_t_even && rot_t_odd && k_boundaries && v_boundaries,
-                 "null pointer");
+    RQ_CHECK_ARG(key && value && slot_mapping && kv_cache && book.rte && book.rto && book.kb && book.vb, "null pointer");
     const bool dense3 = index_layout == RQ_INDEX_DENSE3;
     SlotLayout L(num_kv_heads, head_dim, dense3);
     RQ_CHECK_ARG(total_bytes >= L.payload && total_bytes % 4 == 0, "total_bytes %d < payload %d or not 4-aligned",
@@ -735,6 +792,43 @@ extern "C" int rq_compress_store(const void *key, const void *value, int32_t dty
     m.pad_vec = L.payload % 16 == 0 && total_bytes % 16 == 0 && stride_token % 16 == 0 && stride_block % 16 == 0 &&
                 ((uintptr_t)kv_cache % 16) == 0;
     int64_t n_rows = n_tokens * 2 * num_kv_heads;
-    return dispatch_compress(dtype, m, n_rows, head_dim, rot_t_even, rot_t_odd, rot_block, k_boundaries,
-                             n_k_boundaries, v_boundaries, n_v_boundaries, (hipStream_t)stream);
+    if (rope) return dispatch_compress(dtype, m, CompressRope<true>{*rope, 0}, n_rows, head_dim, book, st);
+    return dispatch_compress(dtype, m, CompressRope<false>{}, n_rows, head_dim, book, st);
+}
+
+}  // namespace rq
+
+extern "C" int rq_compress_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
+                                 int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
+                                 int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t index_layout, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
+                                 int32_t block_size, int64_t stride_block, int64_t stride_token,
+                                 int32_t total_bytes, const float *rot_t_even, const float *rot_t_odd,
+                                 int32_t rot_block, const float *k_boundaries, int32_t n_k_boundaries,
+                                 const float *v_boundaries, int32_t n_v_boundaries, void *stream) {
+    return compress_store(key, value, dtype, n_tokens, k_stride_token, k_stride_head, v_stride_token, v_stride_head, num_kv_heads, head_dim,
+                          index_layout, slot_mapping, kv_cache, num_blocks, block_size, stride_block, stride_token, total_bytes,
+                          CompressBook{rot_t_even, rot_t_odd, rot_block, k_boundaries, n_k_boundaries, v_boundaries, n_v_boundaries}, nullptr,
+                          (hipStream_t)stream);
+}
+
+extern "C" int rq_rope_compress_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                                      int64_t q_stride_token, int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                                      int64_t v_stride_token, int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                                      const int64_t *positions, const void *cos_sin, int32_t table_dtype, int64_t table_rows, int64_t table_stride,
+                                      int32_t rot_dim, int32_t halves, void *out_q, int64_t out_stride_token, int64_t out_stride_head,
+                                      int32_t index_layout, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
+                                      int32_t block_size, int64_t stride_block, int64_t stride_token, int32_t total_bytes,
+                                      const float *rot_t_even, const float *rot_t_odd, int32_t rot_block,
+                                      const float *k_boundaries, int32_t n_k_boundaries, const float *v_boundaries, int32_t n_v_boundaries,
+                                      void *stream) {
+    RopeRows rope;
+    const int rc = rope_queries(rope, dtype, n_tokens, head_dim, positions, cos_sin, table_dtype, table_rows, table_stride, rot_dim, halves, query,
+                                num_q_heads, q_stride_token, q_stride_head, out_q, out_stride_token, out_stride_head);
+    if (rc) return rc;
+    RQ_CHECK_ARG(table_rows < INT32_MAX, "too many positions");
+    return compress_store(key, value, dtype, n_tokens, k_stride_token, k_stride_head, v_stride_token, v_stride_head, num_kv_heads, head_dim,
+                          index_layout, slot_mapping, kv_cache, num_blocks, block_size, stride_block, stride_token, total_bytes,
+                          CompressBook{rot_t_even, rot_t_odd, rot_block, k_boundaries, n_k_boundaries, v_boundaries, n_v_boundaries}, &rope,
+                          (hipStream_t)stream);
 }

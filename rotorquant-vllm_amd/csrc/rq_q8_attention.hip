@@ -31,53 +31,6 @@
 
 namespace rq {
 
-constexpr int kQ8Cols = 16;     // columns of an MFMA; a workgroup takes NB blocks of them
-constexpr int kQ8MinChunk = 8;  // tiles of a workgroup, at least
-
-constexpr int kQ8Tile = 32;     // keys of a tile: two groups
-__device__ __forceinline__ int q8_tiles(const Q8Seq &s) { return max(1, (s.vis + kQ8Tile - 1) / kQ8Tile); }
-template <int NB>
-__device__ __forceinline__ int q8_col_blocks(const Q8AttnArgs &a, int T) { return (T * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols); }
-
-// ---- shares -------------------------------------------------------------------
-// Items are (sequence, block of 16 NB columns, kv head), in that order; the tiles of all items in a row are cut into
-// equal shares, one per workgroup.  Each workgroup sums over the sequences itself, 64 at a time.
-template <int NB>
-__device__ __forceinline__ int64_t q8_seq_tiles(const Q8AttnArgs &a, int64_t b) {
-    if (b >= a.num_seqs) return 0;
-    const Q8Seq s = q8_seq(a, b);
-    return (int64_t)q8_tiles(s) * q8_col_blocks<NB>(a, s.T) * a.H;
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
-    return x;
-}
-// Of values under 2^41: the low 16 bits and the rest are summed apart.
-__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
-    return (int64_t)wave_scan((uint32_t)x & 0xffffu) + ((int64_t)wave_scan((uint32_t)((uint64_t)x >> 16)) << 16);
-}
-__device__ __forceinline__ int64_t lane64(int64_t x, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), lane);
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
-// a / b; in 32 bits (a tenth of the instructions) where both fit.
-__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
-    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
-__device__ __forceinline__ int64_t q8_share(int64_t tiles, int workgroups) {
-    return max((int64_t)kQ8MinChunk, div64(tiles + workgroups - 1, workgroups));
-}
-
-template <int D>
-struct Q8Partial {
-    static constexpr int kFloats = kQ8Cols * (D + 2);  // of a block: accumulators by column, then (M, l) by column
-};
-
 // ---- one segment ----------------------------------------------------------------
 __device__ __forceinline__ uint32_t rows_umax(uint32_t x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
     auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
@@ -103,30 +56,12 @@ template <int D>
 struct Q8Tile {
     u32x4 k[2][D / 64], v[2][D / 64];
 };
-template <int D, int W>
-struct Q8Sums {  // of a workgroup's W waves
-    float acc[W][kQ8Cols][D + 4];
-    float2 ml[W][kQ8Cols];
-};
-
-// Stores N values of a row (N = 2 or a multiple of 4).
-template <int DT, int N>
-__device__ __forceinline__ void q8_put(uint16_t *row, const float (&o)[N], float f) {
-    if constexpr (N == 2) {
-        *reinterpret_cast<uint32_t *>(row) = pack_pair<DT>(o[0] * f, o[1] * f);
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 4)
-            *reinterpret_cast<uint2 *>(row + k) = make_uint2(pack_pair<DT>(o[k] * f, o[k + 1] * f), pack_pair<DT>(o[k + 2] * f, o[k + 3] * f));
-    }
-}
-
 // Tiles [t0, t1) of the item (sequence, kv head h, columns from c0) by the workgroup's W waves, tile t0 + i by wave i % W.  The result is
 // the output rows (part == NULL) or partials.
 // ONCE: no other workgroup reads these codes.
 template <int DT, int FMT, int D, int NB, int W, bool ONCE>
-__device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, const Q8Seq &s, int h, int c0, int t0, int t1, float *part,
-                                           Q8Sums<D, W> &lds) {
+__device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, const AttnSeq &s, int h, int c0, int t0, int t1, float *part,
+                                           AttnSums<D, W> &lds) {
     constexpr int kSteps = D / 32, kChunks = D / 64, kBlocks = D / 16;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, g = lane >> 4;
@@ -169,7 +104,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
     u32x4 qop[NB][kSteps];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t c = c0 + kQ8Cols * nb + col, i = c / (uint32_t)a.G;
+        const uint32_t c = c0 + kShareCols * nb + col, i = c / (uint32_t)a.G;
         const bool valid = (int)i < s.T;
         const uint16_t *row = static_cast<const uint16_t *>(a.q) + (int64_t)(s.q0 + (valid ? (int)i : 0)) * a.q_st +
                               (int64_t)(h * a.G + (valid ? (int)(c - i * a.G) : 0)) * a.q_sh + 16 * g;
@@ -184,7 +119,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         colf[nb] = q8_query<DT, D>(a, qop[nb]);
-        lim[nb] = a.causal ? min(s.vis, s.pos + (c0 + kQ8Cols * nb + col) / a.G + 1) : s.vis;
+        lim[nb] = a.causal ? min(s.vis, s.pos + (c0 + kShareCols * nb + col) / a.G + 1) : s.vis;
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) acc[nb][m] = f32x4{0.f, 0.f, 0.f, 0.f};
         B[nb] = kQ8NoBias, l_run[nb] = 0.f;
@@ -205,7 +140,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
             if (slot(tn) == 0) look_up(tn);
             fetch(tn);
         }
-        const int k0 = t * kQ8Tile;
+        const int k0 = t * kShareTile;
         f32x4 S[NB][2];
 #pragma unroll
         for (int gr = 0; gr < 2; ++gr) {
@@ -221,14 +156,14 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
                 for (int nb = 0; nb < NB; ++nb) S[nb][gr] = mfma_f16(u32x4{x[0], x[1], x[2], x[3]}, qop[nb][k], S[nb][gr]);
             }
         }
-        if (k0 + kQ8Tile > lim_first) {
+        if (k0 + kShareTile > lim_first) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) S[nb][gr][i] = k0 + 16 * gr + 4 * g + i < lim[nb] ? S[nb][gr][i] : -INFINITY;
-            if (FMT == RQ_Q8_E4M3 && k0 + kQ8Tile > s.vis) {
+            if (FMT == RQ_Q8_E4M3 && k0 + kShareTile > s.vis) {
                 // what lies behind the context may be a NaN's code, and 0 * NaN is one
 #pragma unroll
                 for (int gr = 0; gr < 2; ++gr) {
@@ -290,30 +225,7 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
         for (int m = 0; m < kBlocks; ++m) *reinterpret_cast<f32x4 *>(&lds.acc[wave][col][16 * m + 4 * g]) = acc[nb][m];
         if (g == 0) lds.ml[wave][col] = make_float2(q8_max_of(B[nb]), l_col);
         __syncthreads();
-        constexpr int kPer = 4 * W, kDims = D / kPer;  // threads of a column, dims of a thread
-        const int c = tid / kPer, d0 = tid % kPer * kDims;
-        const uint32_t cc = c0 + kQ8Cols * nb + c, i = cc / (uint32_t)a.G;
-        if ((int)i >= s.T) continue;
-        float Mt = -INFINITY, l = 0.f, o[kDims] = {};
-#pragma unroll
-        for (int w = 0; w < W; ++w) Mt = fmaxf(Mt, lds.ml[w][c].x);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 ml = lds.ml[w][c];
-            const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
-            l += r * ml.y;
-#pragma unroll
-            for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][d0 + k];
-        }
-        if (part == nullptr) {
-            uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + (int)i) * a.o_st + (int64_t)(h * a.G + (int)(cc - i * a.G)) * a.o_sh + d0;
-            q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);  // a row that sees no key: zeros
-        } else {
-            float *pt = part + nb * Q8Partial<D>::kFloats;
-#pragma unroll
-            for (int k = 0; k < kDims; k += 2) *reinterpret_cast<float2 *>(pt + c * D + d0 + k) = make_float2(o[k], o[k + 1]);
-            if (tid % kPer == 0) *reinterpret_cast<float2 *>(pt + kQ8Cols * D + 2 * c) = make_float2(Mt, l);
-        }
+        attn_join<DT, D, W, false>(a, s, h, c0 + kShareCols * nb, D, part == nullptr ? nullptr : part + nb * AttnPartial<D>::kFloats, lds);
     }
 }
 
@@ -324,112 +236,16 @@ constexpr int kQ8Resident = D == 64 ? (NB == 1 ? 4 : 3) : 2;
 // Equal shares of all items' tiles.
 template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(256, (kQ8Resident<D, NB>)) void q8_stream_kernel(Q8AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    __shared__ Q8Sums<D, 4> lds;
-    int64_t block = 0, block_base = 0;  // 64 sequences: their tiles, and the row's up to each
-    int64_t mine = q8_seq_tiles<NB>(a, lane), upto = wave_scan64(mine);
-    int64_t total = lane64(upto, 63);
-    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(q8_seq_tiles<NB>(a, b + lane)), 63);
-    const int64_t share = q8_share(total, gridDim.x);
-    int64_t pos = blockIdx.x * share;
-    const int64_t end = min(total, pos + share);
-    while (pos < end) {
-        uint64_t hit = __ballot(block_base + upto > pos);
-        while (hit == 0) {
-            block_base += lane64(upto, 63);
-            block += 64;
-            mine = q8_seq_tiles<NB>(a, block + lane);
-            upto = wave_scan64(mine);
-            hit = __ballot(block_base + upto > pos);
-        }
-        const int of = __builtin_ctzll(hit);
-        const int64_t seq = block + of, in_seq = pos - (block_base + lane64(upto, of) - lane64(mine, of));
-        const Q8Seq s = q8_seq(a, seq);
-        const int n = q8_tiles(s);
-        const int64_t item = div64(in_seq, n), block_of = div64(item, a.H);
-        const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
-        // an item cut in two or more: the share that begins it ends with it, the others begin with it
-        float *part = t0 == 0 && t1 == n ? nullptr : a.part + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * NB * Q8Partial<D>::kFloats;
-        q8_segment<DT, FMT, D, NB, 4, ONCE>(a, seq, s, (int)(item - block_of * a.H), (int)block_of * (NB * kQ8Cols), t0, t1, part, lds);
-        pos += t1 - t0;
-    }
+    __shared__ AttnSums<D, 4> lds;
+    attn_walk<D, NB>(a, [&](int64_t seq, const AttnSeq &s, int h, int c0, int t0, int t1, float *part) {
+        q8_segment<DT, FMT, D, NB, 4, ONCE>(a, seq, s, h, c0, t0, t1, part, lds);
+    });
 }
 
-// Adds up the partials of the items that were cut: one workgroup per item and block of 16 columns.  A wave takes four
-// columns (lane: column % 4, part of D / 16 dims); with few columns, as decodes have, several waves share them
-// and take every second or fourth partial.  Two partials are in flight per wave.
 template <int DT, int D, int NB>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgroups) {
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int64_t b = blockIdx.y;
-    const int item = blockIdx.x / NB, nb = blockIdx.x % NB;
-    const Q8Seq s = q8_seq(a, b);
-    const int h = item % a.H, c0 = (item / a.H) * (NB * kQ8Cols) + nb * kQ8Cols;
-    const int cols = min(kQ8Cols, s.T * a.G - c0);
-    if (cols <= 0) return;
-    const int n = q8_tiles(s);
-    int64_t total = 0, before = 0;
-    for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
-        const int64_t mine = q8_seq_tiles<NB>(a, b0 + lane), upto = wave_scan64(mine);
-        if (b >= b0 && b < b0 + 64) before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
-        total += lane64(upto, 63);
-    }
-    const int64_t share = q8_share(total, workgroups);
-    const int64_t first = before + (int64_t)item * n;
-    const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
-    if (w0 == w1) return;
-    constexpr int kDims = D / 16;
-    __shared__ Q8Sums<D, 4> lds;
-    const int quads = cols > 8 ? 4 : cols > 4 ? 2 : 1, ways = 4 / quads;  // column quads, waves of each
-    const int way = wave / quads, d0 = (lane & 15) * kDims;
-    {
-        const int c = 4 * (wave % quads) + (lane >> 4), cv = min(c, cols - 1);
-        float M = -INFINITY, l = 0.f, o[kDims] = {};
-        for (int w = w0 + way; w <= w1; w += 2 * ways) {
-            float2 ml[2];
-            float4 x[2][kDims / 4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int wu = min(w + ways * u, w1);
-                const float *pt = a.part + ((2 * (int64_t)wu + (wu == w0 ? 1 : 0)) * NB + nb) * Q8Partial<D>::kFloats;
-                ml[u] = *reinterpret_cast<const float2 *>(pt + kQ8Cols * D + 2 * cv);
-#pragma unroll
-                for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + cv * D + d0 + 4 * k);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (w + ways * u > w1) continue;
-                const float Mn = fmaxf(M, ml[u].x);
-                const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
-                const float r = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - Mn);
-                M = Mn;
-                l = l * keep + r * ml[u].y;
-#pragma unroll
-                for (int k = 0; k < kDims / 4; ++k) {
-                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
-                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kDims; k += 4) *reinterpret_cast<float4 *>(&lds.acc[way][c][d0 + k]) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        if ((lane & 15) == 0) lds.ml[way][c] = make_float2(M, l);
-    }
-    __syncthreads();
-    const int c = tid >> 4;
-    if (c >= cols) return;
-    float Mt = -INFINITY, l = 0.f, o[kDims] = {};
-    for (int w = 0; w < ways; ++w) Mt = fmaxf(Mt, lds.ml[w][c].x);
-    for (int w = 0; w < ways; ++w) {
-        const float2 ml = lds.ml[w][c];
-        const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
-        l += r * ml.y;
-#pragma unroll
-        for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][(tid & 15) * kDims + k];
-    }
-    const int i = (c0 + c) / a.G;
-    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + (c0 + c) % a.G) * a.o_sh + (tid & 15) * kDims;
-    q8_put<DT, kDims>(row, o, l == 0.f ? 0.f : 1.f / l);
+    __shared__ AttnSums<D, 4> lds;
+    attn_merge<DT, D, NB, false>(a, workgroups, D, lds);
 }
 
 // One workgroup of 8 waves per item: one launch, no partials.  What bounds it is two things in a row.  A chain of dependent loads and its
@@ -439,23 +255,21 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgro
 // (777 keys), so it is the rate and not the latency; more CUs to an item would need a merge between workgroups.
 template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(512, 2) void q8_item_kernel(Q8AttnArgs a) {
-    __shared__ Q8Sums<D, 8> lds;
+    __shared__ AttnSums<D, 8> lds;
     const int64_t seq = blockIdx.y;
-    const Q8Seq s = q8_seq(a, seq);
+    const AttnSeq s = attn_seq(a, seq);
     const int block = blockIdx.x / (uint32_t)a.H, h = blockIdx.x - block * a.H;
-    if (block >= q8_col_blocks<NB>(a, s.T)) return;
-    q8_segment<DT, FMT, D, NB, 8, ONCE>(a, seq, s, h, block * (NB * kQ8Cols), 0, q8_tiles(s), nullptr, lds);
+    if (block >= attn_col_blocks<NB>(a, s.T)) return;
+    q8_segment<DT, FMT, D, NB, 8, ONCE>(a, seq, s, h, block * (NB * kShareCols), 0, attn_tiles(s), nullptr, lds);
 }
 
 // Blocks of 16 columns that a workgroup takes (two share a stream of codes and its conversions: 32 drafts of up to 8 tokens x 4 heads
 // 85 -> 77 us), and the workgroups: what the GPU holds at once, or fewer where the bound on the lengths gives less work.
-static int q8_blocks(int G, int64_t max_q_len) { return max_q_len * G > kQ8Cols ? 2 : 1; }
+static int q8_blocks(int G, int64_t max_q_len) { return max_q_len * G > kShareCols ? 2 : 1; }
 static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
-    const int nb = q8_blocks(G, max_q_len), cols = nb * kQ8Cols;
+    const int nb = q8_blocks(G, max_q_len);
     const int resident = D == 128 ? (nb == 1 ? kQ8Resident<128, 1> : kQ8Resident<128, 2>) : (nb == 1 ? kQ8Resident<64, 1> : kQ8Resident<64, 2>);
-    const int64_t tiles = std::max<int64_t>(1, (max_keys + kQ8Tile - 1) / kQ8Tile);
-    const int64_t work = num_seqs * ((max_q_len * G + cols - 1) / cols) * H * tiles;
-    return std::max<int64_t>(1, std::min<int64_t>(resident * (int64_t)device_cus(), (work + kQ8MinChunk - 1) / kQ8MinChunk));
+    return attn_workgroups(num_seqs, G, H, max_q_len, max_keys, nb, resident);
 }
 
 // Calls of short contexts, by the bound on their lengths, take a workgroup per item.  One launch without partials saves 4 to 7 us; a long item
@@ -464,24 +278,24 @@ static int64_t q8_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_
 //   64: 24.6 / 25.0, 40.8 / 42.4, 73.5 / 78.0.
 constexpr int64_t kQ8ItemTiles = 60;
 static bool q8_is_short(int64_t max_keys) {
-    return max_keys <= kQ8ItemTiles * kQ8Tile;
+    return max_keys <= kQ8ItemTiles * kShareTile;
 }
 
 template <int DT, int FMT, int D, int NB, bool ONCE>
 static void launch_stream(const Q8AttnArgs &a, int64_t workgroups, hipStream_t st) {
     if (q8_is_short(a.bound)) {
-        const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
+        const int64_t items = ((int64_t)a.max_q * a.G + NB * kShareCols - 1) / (NB * kShareCols) * a.H;
         hipLaunchKernelGGL((q8_item_kernel<DT, FMT, D, NB, ONCE>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(512), 0, st, a);
         return;
     }
     hipLaunchKernelGGL((q8_stream_kernel<DT, FMT, D, NB, ONCE>), dim3((unsigned)workgroups), dim3(256), 0, st, a);
-    const int64_t items = ((int64_t)a.max_q * a.G + NB * kQ8Cols - 1) / (NB * kQ8Cols) * a.H;
+    const int64_t items = ((int64_t)a.max_q * a.G + NB * kShareCols - 1) / (NB * kShareCols) * a.H;
     hipLaunchKernelGGL((q8_merge_kernel<DT, D, NB>), dim3((unsigned)(items * NB), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)workgroups);
 }
 template <int DT, int FMT, int D>
 static void launch_stream_b(const Q8AttnArgs &a, int64_t wgs, hipStream_t st) {
     if (q8_blocks(a.G, a.max_q) == 1) launch_stream<DT, FMT, D, 1, true>(a, wgs, st);
-    else if ((int64_t)a.max_q * a.G <= 2 * kQ8Cols) launch_stream<DT, FMT, D, 2, true>(a, wgs, st);
+    else if ((int64_t)a.max_q * a.G <= 2 * kShareCols) launch_stream<DT, FMT, D, 2, true>(a, wgs, st);
     else launch_stream<DT, FMT, D, 2, false>(a, wgs, st);
 }
 template <int DT, int FMT>
@@ -498,9 +312,6 @@ static void launch_stream_f(const Q8AttnArgs &a, int fmt, int D, int64_t wgs, hi
 // 8000, 64: 40 / 40;  head_dim 64, 8 of 4000, 32: 38 / 44, 64: 52 / 51.
 static bool q8_is_prompt(int64_t max_q_len, int G) { return max_q_len > 1 && max_q_len * G >= RQ_Q8_PROMPT_COLUMNS; }
 
-// Lengths are ints in the kernels.
-static int64_t q8_bound(int64_t max_seq_len) { return std::min<int64_t>(max_seq_len, INT32_MAX - 64); }
-
 }  // namespace rq
 
 using namespace rq;
@@ -509,17 +320,17 @@ extern "C" int64_t rq_q8_attention_workspace_bytes(int64_t num_seqs, int32_t num
                                                    int32_t head_dim, int64_t max_q_len, int64_t max_seq_len) {
     if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_q_len <= 0 || max_seq_len < 0) return 0;
     const int G = num_q_heads / num_kv_heads;
-    max_seq_len = q8_bound(max_seq_len);
+    max_seq_len = attn_bound(max_seq_len);
     if (q8_is_prompt(max_q_len, G)) return q8_prefill_workspace(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
     if (q8_is_short(max_seq_len)) return 0;
     const int64_t wgs = q8_workgroups(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
-    return 2 * wgs * q8_blocks(G, max_q_len) * kQ8Cols * (head_dim + 2) * 4;
+    return 2 * wgs * q8_blocks(G, max_q_len) * kShareCols * (head_dim + 2) * 4;
 }
 
 // (The stream's partials, two of up to 2 x 16 columns for each of up to four workgroups a CU, are smaller than the prefill's.)
 extern "C" int64_t rq_q8_attention_workspace_bound(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t max_seq_len) {
     if (num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || max_seq_len < 0) return 0;
-    return q8_prefill_workspace_bound(head_dim, q8_bound(max_seq_len));
+    return q8_prefill_workspace_bound(head_dim, attn_bound(max_seq_len));
 }
 
 extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads,
@@ -557,7 +368,7 @@ extern "C" int rq_q8_attention(const void *q, int32_t dtype, int64_t total_q, in
     a.H = num_kv_heads, a.G = num_q_heads / num_kv_heads, a.groups = block_size / kQ8Group, a.block_size = block_size;
     a.bt = block_table, a.max_blocks = max_blocks, a.bt_ss = bt_stride_seq;
     a.seq_lens = seq_lens;
-    a.bound = q8_bound(max_seq_len);
+    a.bound = attn_bound(max_seq_len);
     a.cap = std::min<int64_t>(a.bound, max_blocks > a.bound / block_size ? a.bound : max_blocks * block_size);
     a.max_q = (int)max_q_len;
     a.score_scale = sm_scale == 0.f ? 1.f : __builtin_fabsf(sm_scale) * kAttnLog2e;

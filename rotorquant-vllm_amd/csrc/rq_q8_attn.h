@@ -2,34 +2,22 @@
 // rq_q8_prefill.hip: prompts).  The arithmetic is described in rq_q8_attention.hip.
 #pragma once
 
-#include "rq_attn_tile.h"
+#include "rq_attn_share.h"
 #include "rq_q8.h"
 
 namespace rq {
 
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
-struct Q8AttnArgs {
+struct Q8AttnArgs : AttnBatch {
     const void *q;
     int64_t q_st, q_sh;
-    const int32_t *cu_q;  // NULL: one token per sequence
-    int64_t total_q, num_seqs;
-    int causal;
     const uint8_t *cache;
     int64_t num_blocks, stride_block;
-    int H, G, groups, block_size;
-    const int32_t *bt;
-    int64_t max_blocks, bt_ss;
-    const int32_t *seq_lens;
-    int64_t bound;  // max_seq_len: sizes launches and workspace
-    int64_t cap;    // keys of a sequence that may be read: bound, its table's capacity
-    int max_q;    // tokens of a query that count
+    int groups;         // of a page
     float score_scale;  // |sm_scale| log2(e)
     float q_sign;       // sign of sm_scale (0 for 0)
     int max_up;         // largest s of q 2^s (below)
-    void *out;
-    int64_t o_st, o_sh;
-    float *part;  // partial sums of items that several workgroups share
 };
 
 // The codes of a dword in fp16: two dwords.  int8: bytes under 0x64 are 1024 + (c + 128).
@@ -43,24 +31,6 @@ __device__ __forceinline__ void q8_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi
         lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
         hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
     }
-}
-
-// A sequence's query tokens that count (q0 .. q0 + T), the position of the first, and the keys that may be seen.
-struct Q8Seq {
-    int q0, T, pos, vis;
-};
-__device__ __forceinline__ Q8Seq q8_seq(const Q8AttnArgs &a, int64_t b) {
-    Q8Seq s;
-    s.q0 = a.cu_q ? a.cu_q[b] : (int)b;
-    const int end = a.cu_q ? a.cu_q[b + 1] : (int)b + 1;
-    s.T = min(max(min((int64_t)end, a.total_q) - max(s.q0, 0), (int64_t)0), (int64_t)a.max_q);
-    if (s.q0 < 0) s.T = 0;
-    const int L = a.seq_lens[b];
-    s.vis = (int)max((int64_t)0, min((int64_t)L, a.cap));
-    // (by the query's whole length, also where max_q cuts it; far below 0, where no key is seen, or far above, where all are, the
-    // exact place is of no account, and sums with a query's tokens stay ints)
-    s.pos = (int)min(max((int64_t)L - ((int64_t)end - s.q0), (int64_t)-(1 << 30)), (int64_t)INT32_MAX - (1 << 21));
-    return s;
 }
 
 // Exponent s with which a query row, its largest magnitude given by its bits, goes into fp16: q 2^s has

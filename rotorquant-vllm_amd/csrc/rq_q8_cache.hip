@@ -7,13 +7,12 @@
 // of four 16-dim parts); the K order needs no more, and the V order, whose dwords hold one dim of
 // four tokens, takes one 4 x 4 byte transposition within quads of lanes.
 #include <algorithm>
+#include <type_traits>
 
 #include "rq_q8.h"
+#include "rq_rope.h"
 
 namespace rq {
-
-typedef __attribute__((ext_vector_type(4))) uint32_t q8_u32x4;
-typedef __attribute__((ext_vector_type(2))) uint32_t q8_u32x2;
 
 struct Q8StoreArgs {
     const void *key, *value;
@@ -118,26 +117,24 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
     return true;
 }
 
-// Eight elements (16-byte aligned), as loaded and as fp32.
-template <int DT>
-struct Q8Raw {
-    q8_u32x4 w[DT == RQ_DTYPE_F32 ? 2 : 1];
+// What a store with position rotation is given beside Q8StoreArgs.
+template <bool ROPE>
+struct Q8Rope {};
+template <>
+struct Q8Rope<true> {
+    RopeRows rows;          // the queries, by workgroups of their own behind those that store
+    unsigned store_blocks;
 };
+// Piece `piece` (8 dims) of a key row at element `at` of a.key, turned by its token's position.
 template <int DT>
-__device__ __forceinline__ Q8Raw<DT> q8_load8(const void *p, int64_t at) {
-    Q8Raw<DT> r;
-    const q8_u32x4 *q = reinterpret_cast<const q8_u32x4 *>(static_cast<const uint8_t *>(p) + at * (DT == RQ_DTYPE_F32 ? 4 : 2));
-    r.w[0] = *q;
-    if constexpr (DT == RQ_DTYPE_F32) r.w[1] = q[1];
-    return r;
-}
-template <int DT>
-__device__ __forceinline__ void q8_floats(const Q8Raw<DT> &r, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (DT == RQ_DTYPE_F32) x[i] = __uint_as_float(r.w[i >> 2][i & 3]);
-        else x[i] = Elem<DT>::to_f32((r.w[0][i >> 1] >> (16 * (i & 1))) & 0xffffu);
-    }
+__device__ __forceinline__ void q8_turn(const RopeTable &t, const void *key, int64_t at, int64_t position, int piece, float (&x)[8]) {
+    const int hp = t.rot >> 4;
+    if (piece >= 2 * hp) return;
+    const RopeTurn r = rope_turn<DT>(t, position, piece);
+    const bool lower = piece < hp;
+    float y[8];
+    if (t.halves) row8_floats<DT>(row8_load<DT>(key, at + 8 * (lower ? hp : -hp)), y);
+    rope_piece(x, y, r, t.halves, lower);
 }
 
 // A wave takes a.per_wave units of one group, the next one's rows on their way while one is coded.  Lane: token row
@@ -145,8 +142,16 @@ __device__ __forceinline__ void q8_floats(const Q8Raw<DT> &r, float (&x)[8]) {
 // (D = 128) or the V side (D = 64).
 // Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in 47 us beside 10 for the two link launches (graph replays of all three: 48).  Non-temporal loads
 // here: 56 us (a row's 128 bytes are loaded by four instructions, which then miss the L1).
-template <int DT, int FMT, int D, bool LINKED>
-__global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a) {
+template <int DT, int FMT, int D, bool LINKED, bool ROPE>
+__global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a, Q8Rope<ROPE> rope) {
+    unsigned blocks = gridDim.x;
+    if constexpr (ROPE) {
+        blocks = rope.store_blocks;
+        if (blockIdx.x >= blocks) {
+            rope_rows<DT>(rope.rows, (int64_t)(blockIdx.x - blocks) * kRopeThreads + threadIdx.x);
+            return;
+        }
+    }
     constexpr int kUnits = D == 128 ? 2 : 1;  // units per head
     __shared__ int rows_of[kStoreWaves][kQ8Group];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -155,7 +160,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
     const int units = kUnits * a.H, waves = (units + a.per_wave - 1) / a.per_wave;  // of a group
     const int64_t entries = LINKED ? *a.count : a.n_tokens;
     const Q8Layout lay(a.H, D, a.block_size);
-    for (int64_t item = (int64_t)blockIdx.x * kStoreWaves + wave; item < entries * waves; item += (int64_t)gridDim.x * kStoreWaves) {
+    for (int64_t item = (int64_t)blockIdx.x * kStoreWaves + wave; item < entries * waves; item += (int64_t)blocks * kStoreWaves) {
         const uint32_t entry = (uint32_t)item / (uint32_t)waves;
         const int first = (int)((uint32_t)item - entry * waves) * a.per_wave, end = min(units, first + a.per_wave);
         int64_t t0 = entry, g;
@@ -168,6 +173,10 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
         }
         if (!q8_find_rows<LINKED>(a, t0, g, rows, lane)) continue;
         const int tok = rows[t];
+        int64_t position = 0;
+        if constexpr (ROPE) {
+            if (tok >= 0) position = rope.rows.t.positions[tok];
+        }
         const bool anew = rows[0] >= 0;
         const uint64_t written = __ballot(tok >= 0);
         const bool quad_hit = (written >> (lane & 60)) & 15;  // four tokens share their V dwords
@@ -176,7 +185,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
 
         auto side_of = [&](int unit) { return D == 128 ? unit & 1 : lane >> 5; };
         const int chunk = D == 128 ? lane >> 5 : 0;
-        Q8Raw<DT> raw[4];
+        Row8<DT> raw[4];
         float old_next;
         auto scale_at = [&](int unit) { return reinterpret_cast<float *>(base + lay.scale_at(gi, unit / kUnits)) + side_of(unit); };
         auto load = [&](int unit) {  // dims 64 chunk + 16 i + 8 half .. of this lane's row
@@ -185,7 +194,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
             const int64_t at = (int64_t)tok * (side ? a.v_st : a.k_st) + (int64_t)h * (side ? a.v_sh : a.k_sh) + 64 * chunk + 8 * half;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (tok >= 0) raw[i] = q8_load8<DT>(side ? a.value : a.key, at + 16 * i);
+                if (tok >= 0) raw[i] = row8_load<DT>(side ? a.value : a.key, at + 16 * i);
         };
         load(first);
         for (int unit = first; unit < end; ++unit) {
@@ -196,7 +205,12 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
             uint32_t big = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                q8_floats<DT>(raw[i], x[i]);
+                row8_floats<DT>(raw[i], x[i]);
+                if constexpr (ROPE) {
+                    if (side == 0 && tok >= 0)
+                        q8_turn<DT>(rope.rows.t, a.key, (int64_t)tok * a.k_st + (int64_t)h * a.k_sh + 64 * chunk + 16 * i + 8 * half, position,
+                                    8 * chunk + 2 * i + half, x[i]);
+                }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     if (tok < 0) x[i][k] = 0.f;
@@ -226,13 +240,13 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
                 if (side == 0) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const q8_u32x2 w = *reinterpret_cast<const q8_u32x2 *>(krow + 256 * i);
+                        const u32x2 w = *reinterpret_cast<const u32x2 *>(krow + 256 * i);
                         old[i][0] = w[0], old[i][1] = w[1];
                     }
                 } else {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const q8_u32x4 w = *reinterpret_cast<const q8_u32x4 *>(vrow + 64 * k);
+                        const u32x4 w = *reinterpret_cast<const u32x4 *>(vrow + 64 * k);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) old[i][k] = quad_transpose(w[i], q);
                     }
@@ -251,15 +265,15 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
             if (side == 0) {
                 if (tok >= 0 || moved) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) *reinterpret_cast<q8_u32x2 *>(krow + 256 * i) = q8_u32x2{c[i][0], c[i][1]};
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x2 *>(krow + 256 * i) = u32x2{c[i][0], c[i][1]};
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    q8_u32x4 w;
+                    u32x4 w;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) w[i] = quad_transpose(c[i][k], q);
-                    if (moved || quad_hit) *reinterpret_cast<q8_u32x4 *>(vrow + 64 * k) = w;
+                    if (moved || quad_hit) *reinterpret_cast<u32x4 *>(vrow + 64 * k) = w;
                 }
             }
             if (t == 0 && half == 0 && chunk == 0) *scale_at(unit) = exp2i(e_new);
@@ -299,10 +313,10 @@ __device__ __forceinline__ void q8_put8(void *p, int64_t at, uint32_t w0, uint32
         q[0] = make_float4(x[0], x[1], x[2], x[3]);
         q[1] = make_float4(x[4], x[5], x[6], x[7]);
     } else {
-        q8_u32x4 w;
+        u32x4 w;
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(x[2 * k]) | Elem<DT>::from_f32(x[2 * k + 1]) << 16;
-        *reinterpret_cast<q8_u32x4 *>(static_cast<uint16_t *>(p) + at) = w;
+        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + at) = w;
     }
 }
 // The value of lane l ^ 4.
@@ -343,11 +357,11 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
     const Q8Layout lay(a.H, D, a.block_size);
     const uint8_t *const base = a.cache + page * a.stride_block;
     const uint8_t *const tile = base + lay.codes_at(gi, h) + 16 * lane;
-    q8_u32x4 kc[kChunks], vc[kChunks];
+    u32x4 kc[kChunks], vc[kChunks];
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-        kc[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + 1024 * j));
-        vc[j] = __builtin_nontemporal_load(reinterpret_cast<const q8_u32x4 *>(tile + kQ8Group * D + 1024 * j));
+        kc[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(tile + 1024 * j));
+        vc[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(tile + kQ8Group * D + 1024 * j));
     }
     const float2 scale = *reinterpret_cast<const float2 *>(base + lay.scale_at(gi, h));
     const int g = lane >> 4, c = lane & 15, q = lane & 3;
@@ -385,29 +399,34 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
 // 20.1 / 19.3 / 19.1, 32768: 54.0 / 48.3 / 49.5.
 static int q8_per_wave(int64_t groups, int units) { return groups * units >= 48 * (int64_t)device_cus() ? 2 : 1; }
 
-template <int DT, int FMT, int D>
-static void launch_store(Q8StoreArgs a, bool linked, hipStream_t st) {
+template <int DT, int FMT, int D, bool ROPE>
+static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStream_t st) {
     const int units = (D == 128 ? 2 : 1) * a.H;
     a.per_wave = linked ? q8_per_wave(a.n_tokens / kQ8Group, units) : 1;
-    const int64_t blocks = (a.n_tokens * ((units + a.per_wave - 1) / a.per_wave) + kStoreWaves - 1) / kStoreWaves;
+    int64_t blocks = (a.n_tokens * ((units + a.per_wave - 1) / a.per_wave) + kStoreWaves - 1) / kStoreWaves;
     if (linked) {
         const dim3 tb((unsigned)((a.n_tokens + kLinkThreads - 1) / kLinkThreads));
         hipLaunchKernelGGL(q8_unlink_kernel, tb, dim3(kLinkThreads), 0, st, a);
         hipLaunchKernelGGL(q8_link_kernel, tb, dim3(kLinkThreads), 0, st, a);
-        const unsigned grid = (unsigned)std::min<int64_t>(blocks, 8 * device_cus());
-        hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true>), dim3(grid), dim3(64 * kStoreWaves), 0, st, a);
-    } else {
-        hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, false>), dim3((unsigned)blocks), dim3(64 * kStoreWaves), 0, st, a);
+        blocks = std::min<int64_t>(blocks, 8 * device_cus());
     }
+    int64_t grid = blocks;
+    if constexpr (ROPE) {
+        rope.store_blocks = (unsigned)blocks;
+        grid += rope_blocks(rope.rows);
+    }
+    if (linked) hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);
+    else hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, false, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);
 }
-template <int DT, int FMT>
-static void launch_store_d(const Q8StoreArgs &a, int D, bool linked, hipStream_t st) {
-    D == 128 ? launch_store<DT, FMT, 128>(a, linked, st) : launch_store<DT, FMT, 64>(a, linked, st);
+template <int DT, int FMT, bool ROPE>
+static void launch_store_d(const Q8StoreArgs &a, const Q8Rope<ROPE> &rope, int D, bool linked, hipStream_t st) {
+    D == 128 ? launch_store<DT, FMT, 128, ROPE>(a, rope, linked, st) : launch_store<DT, FMT, 64, ROPE>(a, rope, linked, st);
 }
-template <int DT>
-static void launch_store_f(const Q8StoreArgs &a, int fmt, int D, bool linked, hipStream_t st) {
-    fmt == RQ_Q8_INT8 ? launch_store_d<DT, RQ_Q8_INT8>(a, D, linked, st) : launch_store_d<DT, RQ_Q8_E4M3>(a, D, linked, st);
+template <int DT, bool ROPE>
+static void launch_store_f(const Q8StoreArgs &a, const Q8Rope<ROPE> &rope, int fmt, int D, bool linked, hipStream_t st) {
+    fmt == RQ_Q8_INT8 ? launch_store_d<DT, RQ_Q8_INT8, ROPE>(a, rope, D, linked, st) : launch_store_d<DT, RQ_Q8_E4M3, ROPE>(a, rope, D, linked, st);
 }
+static_assert(64 * kStoreWaves == kRopeThreads, "workgroups of the queries");
 
 template <int DT, int FMT>
 static void launch_read_d(const Q8ReadArgs &a, int D, hipStream_t st) {
@@ -441,20 +460,21 @@ extern "C" int64_t rq_q8_store_workspace_bytes(int64_t n_tokens, int64_t num_blo
     return (num_blocks * (block_size / kQ8Group) + 3 * n_tokens + 4) * 4;
 }
 
-extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
-                           int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
-                           int32_t num_kv_heads, int32_t head_dim, int32_t format, const int64_t *slot_mapping,
-                           uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
-                           void *workspace, int64_t workspace_bytes, void *stream) {
+namespace rq {
+
+// What rq_q8_store and rq_rope_q8_store do; rope: the queries and the table, or NULL.
+static int q8_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t format, const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks,
+                    int32_t block_size, int64_t stride_block, void *workspace, int64_t workspace_bytes, const RopeRows *rope, hipStream_t st) {
     RQ_CHECK_ARG(dtype == RQ_DTYPE_F16 || dtype == RQ_DTYPE_BF16 || dtype == RQ_DTYPE_F32, "bad dtype %d", dtype);
     const int rc = check_q8_cache(head_dim, num_kv_heads, block_size, num_blocks, kv_cache, stride_block, format);
     if (rc) return rc;
     RQ_CHECK_ARG(n_tokens >= 0 && n_tokens <= (1 << 30) / num_kv_heads, "n_tokens %lld out of range", (long long)n_tokens);
-    if (n_tokens == 0 || num_blocks == 0) return RQ_OK;
+    if (n_tokens == 0 || (num_blocks == 0 && !rope)) return RQ_OK;
     RQ_CHECK_ARG(key && value && slot_mapping, "null pointer");
     const int eb = dtype == RQ_DTYPE_F32 ? 4 : 2;
-    RQ_CHECK_ARG((uintptr_t)key % 16 == 0 && (uintptr_t)value % 16 == 0 && k_stride_token * eb % 16 == 0 &&
-                     k_stride_head * eb % 16 == 0 && v_stride_token * eb % 16 == 0 && v_stride_head * eb % 16 == 0,
+    RQ_CHECK_ARG((uintptr_t)key % 16 == 0 && (uintptr_t)value % 16 == 0 && k_st * eb % 16 == 0 && k_sh * eb % 16 == 0 && v_st * eb % 16 == 0 &&
+                     v_sh * eb % 16 == 0,
                  "key/value rows must be 16-byte aligned");
     const int64_t need = rq_q8_store_workspace_bytes(n_tokens, num_blocks, block_size);
     RQ_CHECK_SPACE(workspace_bytes >= need, "workspace too small: the call needs %lld bytes (got %lld)", (long long)need,
@@ -462,7 +482,7 @@ extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, in
     RQ_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace must be 16-byte aligned");
     Q8StoreArgs a{};
     a.key = key, a.value = value;
-    a.k_st = k_stride_token, a.k_sh = k_stride_head, a.v_st = v_stride_token, a.v_sh = v_stride_head;
+    a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
     a.n_tokens = n_tokens;
     a.slots = slot_mapping;
     a.cache = kv_cache;
@@ -477,11 +497,41 @@ extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, in
         a.before = reinterpret_cast<int32_t *>(a.list + n_tokens);
         a.last = a.before + n_tokens;
     }
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == RQ_DTYPE_F16) launch_store_f<RQ_DTYPE_F16>(a, format, head_dim, need > 0, st);
-    else if (dtype == RQ_DTYPE_BF16) launch_store_f<RQ_DTYPE_BF16>(a, format, head_dim, need > 0, st);
-    else launch_store_f<RQ_DTYPE_F32>(a, format, head_dim, need > 0, st);
+    auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (rope) launch_store_f<DT, true>(a, Q8Rope<true>{*rope, 0}, format, head_dim, need > 0, st);
+        else launch_store_f<DT, false>(a, Q8Rope<false>{}, format, head_dim, need > 0, st);
+    };
+    if (dtype == RQ_DTYPE_F16) launch(std::integral_constant<int, RQ_DTYPE_F16>{});
+    else if (dtype == RQ_DTYPE_BF16) launch(std::integral_constant<int, RQ_DTYPE_BF16>{});
+    else launch(std::integral_constant<int, RQ_DTYPE_F32>{});
     return check_launch("q8_store_kernel");
+}
+
+}  // namespace rq
+
+extern "C" int rq_q8_store(const void *key, const void *value, int32_t dtype, int64_t n_tokens,
+                           int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t format, const int64_t *slot_mapping,
+                           uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+                           void *workspace, int64_t workspace_bytes, void *stream) {
+    return q8_store(key, value, dtype, n_tokens, k_stride_token, k_stride_head, v_stride_token, v_stride_head, num_kv_heads, head_dim, format,
+                    slot_mapping, kv_cache, num_blocks, block_size, stride_block, workspace, workspace_bytes, nullptr, (hipStream_t)stream);
+}
+
+extern "C" int rq_rope_q8_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                                int64_t q_stride_token, int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                                int64_t v_stride_token, int64_t v_stride_head, int32_t num_kv_heads, int32_t head_dim,
+                                const int64_t *positions, const void *cos_sin, int32_t table_dtype, int64_t table_rows, int64_t table_stride,
+                                int32_t rot_dim, int32_t halves, void *out_q, int64_t out_stride_token, int64_t out_stride_head, int32_t format,
+                                const int64_t *slot_mapping, uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,
+                                void *workspace, int64_t workspace_bytes, void *stream) {
+    RopeRows rope;
+    const int rc = rope_queries(rope, dtype, n_tokens, head_dim, positions, cos_sin, table_dtype, table_rows, table_stride, rot_dim, halves, query,
+                                num_q_heads, q_stride_token, q_stride_head, out_q, out_stride_token, out_stride_head);
+    if (rc) return rc;
+    return q8_store(key, value, dtype, n_tokens, k_stride_token, k_stride_head, v_stride_token, v_stride_head, num_kv_heads, head_dim, format,
+                    slot_mapping, kv_cache, num_blocks, block_size, stride_block, workspace, workspace_bytes, &rope, (hipStream_t)stream);
 }
 
 extern "C" int rq_q8_read(const uint8_t *kv_cache, int64_t num_blocks, int32_t block_size, int64_t stride_block,

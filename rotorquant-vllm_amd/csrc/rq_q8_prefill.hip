@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void q8_pack_kernel(Q8PrefillArgs p) {
     const Q8AttnArgs &a = p.a;
     const int tile = blockIdx.x, h = p.h0 + blockIdx.y;
     const int64_t b = p.b0 + blockIdx.z;
-    const Q8Seq s = q8_seq(a, b);
+    const AttnSeq s = attn_seq(a, b);
     const int k0 = tile * kQ8KT;
     if (k0 >= s.vis || s.T == 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,13 +143,13 @@ __device__ __forceinline__ void copy16n(const uint8_t *src, uint32_t voff, uint3
 
 constexpr int kQ8MinTiles = 4;  // tiles of a key chunk, at least
 struct Q8Block {
-    Q8Seq s;
+    AttnSeq s;
     int units, f0, kv_end, n_tiles;
 };
 // Query block -> its first unit (32-position group, query head), the sequence's units, and the tiles that any of its positions sees.
 __device__ __forceinline__ Q8Block q8_block(const Q8AttnArgs &a, int64_t b, int qblk) {
     Q8Block q;
-    q.s = q8_seq(a, b);
+    q.s = attn_seq(a, b);
     q.units = (q.s.T + kQ8PW - 1) / kQ8PW * a.G;
     q.f0 = qblk * kQ8PWaves;
     const int last_i = min(q.s.T, (min(q.f0 + kQ8PWaves, q.units) - 1) / a.G * kQ8PW + kQ8PW) - 1;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * kQ8PWaves) __attribute__((amdgpu_waves_per_eu(
         qblk /= p.split;
     }
     const Q8Block qb = q8_block(a, b, qblk);
-    const Q8Seq &s = qb.s;
+    const AttnSeq &s = qb.s;
     if (qb.f0 >= qb.units) return;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hh = lane >> 5, col = lane & 31;

@@ -1,0 +1,268 @@
+// Position rotation (rotary embedding) of query and key rows on the way into a cache (no counterpart in the reference, whose
+// model rotates before the backend is called).
+//
+// A table row of `rot` numbers per position holds cosines, then sines, of rot / 2 angles.  Angle i turns the pair of dims
+// (i, i + rot / 2) ("halves") or (2 i, 2 i + 1):
+//   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin,
+// in fp32, each product and the sum rounded once (no fma), so that a rotated key is the same number
+// wherever it is computed: the codes of all the caches go by it.  Dims from rot on pass unchanged.  A
+// position outside the table turns by NaN.
+//
+// Rows move in pieces of 8 dims.  With halves a piece's partners are the piece rot / 16 further on (or back), so a
+// multiple of 16 rotated dims keeps all loads 16 bytes wide.
+#pragma once
+
+#include "rq_common.h"
+
+namespace rq {
+
+struct RopeTable {
+    const int64_t *positions;  // of each token
+    const void *table;
+    int64_t stride, rows;  // elements between rows; positions that it holds
+    int rot, halves, f32;  // rotated dims; kind of pairs; table of fp32 (else of the rows' type)
+};
+
+// N (2, 4 or 8) consecutive numbers of a table row.
+template <int DT, int N>
+__device__ __forceinline__ void rope_angles(const RopeTable &t, int64_t at, float *x) {
+    if constexpr (N == 2) {  // (of fp32 rows, whose tables are fp32)
+        static_assert(DT == RQ_DTYPE_F32, "");
+        const float2 w = *reinterpret_cast<const float2 *>(static_cast<const float *>(t.table) + at);
+        x[0] = w.x, x[1] = w.y;
+    } else if (DT == RQ_DTYPE_F32 || t.f32) {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(t.table) + at);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) x[4 * i] = p[i].x, x[4 * i + 1] = p[i].y, x[4 * i + 2] = p[i].z, x[4 * i + 3] = p[i].w;
+    } else if constexpr (DT != RQ_DTYPE_F32) {
+        const u32x2 *p = reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(t.table) + at);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const uint32_t w = p[i >> 1][i & 1];
+            x[2 * i] = Elem<DT>::to_f32(w & 0xffffu), x[2 * i + 1] = Elem<DT>::to_f32(w >> 16);
+        }
+    }
+}
+
+// Cosines and sines of a piece (dims 8 piece ..; piece < rot / 8): eight of each with halves, else four.
+struct RopeTurn {
+    float c[8], s[8];
+};
+template <int DT>
+__device__ __forceinline__ RopeTurn rope_turn(const RopeTable &t, int64_t position, int piece) {
+    RopeTurn r;
+    const bool in = position >= 0 && position < t.rows;
+    const int64_t row = (in ? position : 0) * t.stride;
+    if (t.halves) {
+        const int hp = t.rot >> 4, at = 8 * (piece >= hp ? piece - hp : piece);
+        rope_angles<DT, 8>(t, row + at, r.c);
+        rope_angles<DT, 8>(t, row + (t.rot >> 1) + at, r.s);
+    } else {
+        rope_angles<DT, 4>(t, row + 4 * piece, r.c);
+        rope_angles<DT, 4>(t, row + (t.rot >> 1) + 4 * piece, r.s);
+    }
+    if (!in) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.c[i] = r.s[i] = __builtin_nanf("");
+    }
+    return r;
+}
+
+__device__ __forceinline__ float rope_diff(float a, float c, float b, float s) {
+#pragma clang fp contract(off)
+    const float x = a * c, y = b * s;
+    return x - y;
+}
+__device__ __forceinline__ float rope_sum(float a, float c, float b, float s) {
+#pragma clang fp contract(off)
+    const float x = a * c, y = b * s;
+    return x + y;
+}
+// Turns a pair of pieces with halves (x: the first half's), one with the other.
+__device__ __forceinline__ void rope_halves(float (&x)[8], float (&y)[8], const RopeTurn &r) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = x[i], b = y[i];
+        x[i] = rope_diff(a, r.c[i], b, r.s[i]);
+        y[i] = rope_sum(b, r.c[i], a, r.s[i]);
+    }
+}
+// Turns one piece: its partners' values with halves (lower: of the first half), else its own pairs.
+__device__ __forceinline__ void rope_piece(float (&x)[8], const float (&partner)[8], const RopeTurn &r, bool halves, bool lower) {
+    if (halves) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = lower ? rope_diff(x[i], r.c[i], partner[i], r.s[i]) : rope_sum(x[i], r.c[i], partner[i], r.s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = rope_diff(a, r.c[i], b, r.s[i]);
+            x[2 * i + 1] = rope_sum(b, r.c[i], a, r.s[i]);
+        }
+    }
+}
+
+// Dims at .. at + N - 1 (N 8, or 4 of fp32; at < rot) of the row that begins at `row`, turned.
+template <int DT, int N>
+__device__ __forceinline__ void rope_elems(const RopeTable &t, const uint8_t *row, int64_t position, int at, float (&x)[N]) {
+    const int half = t.rot >> 1;
+    const bool in = position >= 0 && position < t.rows, lower = at < half;
+    const int64_t tr = (in ? position : 0) * t.stride;
+    float c[N], s[N], y[N];
+    if (t.halves) {
+        const int i = lower ? at : at - half;
+        rope_angles<DT, N>(t, tr + i, c);
+        rope_angles<DT, N>(t, tr + half + i, s);
+        const uint8_t *p = row + (lower ? at + half : at - half) * (DT == RQ_DTYPE_F32 ? 4 : 2);
+        if constexpr (N == 8) {
+            row8_floats<DT>(row8_load<DT>(p, 0), y);
+        } else {
+            const float4 w = *reinterpret_cast<const float4 *>(p);
+            y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+        }
+    } else {
+        rope_angles<DT, N / 2>(t, tr + at / 2, c);
+        rope_angles<DT, N / 2>(t, tr + half + at / 2, s);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (!in) c[i] = s[i] = __builtin_nanf("");
+    if (t.halves) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = lower ? rope_diff(x[i], c[i], y[i], s[i]) : rope_sum(x[i], c[i], y[i], s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = rope_diff(a, c[i], b, s[i]);
+            x[2 * i + 1] = rope_sum(b, c[i], a, s[i]);
+        }
+    }
+}
+
+// ---- rows to rows ---------------------------------------------------------------
+// Query rows to rotated rows, and K and V rows to plain 16-bit pages (n_kv > 0).
+struct RopeRows {
+    RopeTable t;
+    int64_t n_tokens;
+    int n_q, n_kv, D;  // query heads, kv heads (0: queries only)
+    const void *q, *k, *v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // element strides
+    void *out;
+    int64_t o_st, o_sh;
+    const int64_t *slots;
+    void *k_cache, *v_cache;
+    int64_t num_slots;
+    int block_size;
+    int64_t kc_sb, kc_ss, kc_sh, vc_sb, vc_ss, vc_sh;  // element strides: page, slot, head
+};
+constexpr int kRopeThreads = 256;
+
+// A thread takes two pieces (with halves a pair of partners) of up to kRopeShare rows of one token: the rows share the
+// token's angles, and their loads are on their way together.
+constexpr int kRopeShare = 2;
+__host__ __device__ __forceinline__ int64_t rope_threads(const RopeRows &a) {
+    return a.n_tokens * ((a.n_q + 2 * a.n_kv + kRopeShare - 1) / kRopeShare) * (a.D / 16);
+}
+inline int64_t rope_blocks(const RopeRows &a) { return (rope_threads(a) + kRopeThreads - 1) / kRopeThreads; }
+
+template <int DT>
+__device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
+    const int units = a.D / 16, rows = a.n_q + 2 * a.n_kv, shared = (rows + kRopeShare - 1) / kRopeShare;
+    if (thread >= rope_threads(a)) return;  // (fits 32 bits)
+    const uint32_t at = (uint32_t)thread / (uint32_t)units, u = (uint32_t)thread - at * units;
+    const uint32_t tok = at / (uint32_t)shared, r0 = at - tok * shared;
+    const int64_t token = tok;
+    const int hp = a.t.rot >> 4;
+    const bool turned = (int)u < hp;
+    // pieces u and u + rot / 16, or two of those that pass
+    const int p0 = turned ? (int)u : 2 * (int)u, p1 = turned ? (int)u + hp : 2 * (int)u + 1;
+    const int64_t position = a.t.positions[token];
+    int64_t page = -1, in_page = 0;
+    if (a.n_kv > 0) {
+        const int64_t s = a.slots[token];
+        if (s >= 0 && s < a.num_slots) {
+            if (a.num_slots <= 0x7fffffff) page = (uint32_t)s / (uint32_t)a.block_size;
+            else page = s / a.block_size;
+            in_page = s - page * a.block_size;
+        }
+    }
+    Row8<DT> x0[kRopeShare], x1[kRopeShare];
+    void *to[kRopeShare];
+    bool turn[kRopeShare];
+#pragma unroll
+    for (int i = 0; i < kRopeShare; ++i) {
+        const int r = (int)r0 + i * shared;
+        const void *from = nullptr;
+        int64_t src = 0, dst = 0;
+        to[i] = nullptr, turn[i] = turned;
+        if (r < a.n_q) {
+            from = a.q, src = token * a.q_st + r * a.q_sh;
+            to[i] = a.out, dst = token * a.o_st + r * a.o_sh;
+        } else if (r < rows && page >= 0) {
+            const bool is_v = r >= a.n_q + a.n_kv;
+            const int h = r - a.n_q - (is_v ? a.n_kv : 0);
+            from = is_v ? a.v : a.k;
+            src = is_v ? token * a.v_st + h * a.v_sh : token * a.k_st + h * a.k_sh;
+            to[i] = is_v ? a.v_cache : a.k_cache;
+            dst = is_v ? page * a.vc_sb + in_page * a.vc_ss + h * a.vc_sh : page * a.kc_sb + in_page * a.kc_ss + h * a.kc_sh;
+            turn[i] = turned && !is_v;
+        }
+        if (to[i] == nullptr) continue;
+        x0[i] = row8_load<DT>(from, src + 8 * p0);
+        x1[i] = row8_load<DT>(from, src + 8 * p1);
+        to[i] = static_cast<uint8_t *>(to[i]) + dst * (DT == RQ_DTYPE_F32 ? 4 : 2);
+    }
+    RopeTurn t0, t1;
+    if (turned) {
+        t0 = rope_turn<DT>(a.t, position, p0);
+        if (!a.t.halves) t1 = rope_turn<DT>(a.t, position, p1);
+    }
+#pragma unroll
+    for (int i = 0; i < kRopeShare; ++i) {
+        if (to[i] == nullptr) continue;
+        if (turn[i]) {
+            float f0[8], f1[8];
+            row8_floats<DT>(x0[i], f0);
+            row8_floats<DT>(x1[i], f1);
+            if (a.t.halves) {
+                rope_halves(f0, f1, t0);
+            } else {
+                rope_piece(f0, f0, t0, false, false);
+                rope_piece(f1, f1, t1, false, false);
+            }
+            x0[i] = row8_round<DT>(f0);
+            x1[i] = row8_round<DT>(f1);
+        }
+        row8_store<DT>(to[i], 8 * p0, x0[i]);
+        row8_store<DT>(to[i], 8 * p1, x1[i]);
+    }
+}
+
+// The table and the query rows of a call, checked; strides in elements of the rows' type.
+inline int rope_queries(RopeRows &a, int dtype, int64_t n_tokens, int head_dim, const int64_t *positions, const void *table, int table_dtype,
+                        int64_t table_rows, int64_t table_stride, int rot_dim, int halves, const void *query, int num_q_heads, int64_t q_st,
+                        int64_t q_sh, void *out, int64_t o_st, int64_t o_sh) {
+    RQ_CHECK_ARG(dtype == RQ_DTYPE_F16 || dtype == RQ_DTYPE_BF16 || dtype == RQ_DTYPE_F32, "bad dtype %d", dtype);
+    RQ_CHECK_ARG(table_dtype == RQ_DTYPE_F32 || table_dtype == dtype, "the table must be fp32 or of the rows' dtype");
+    RQ_CHECK_ARG(head_dim >= 16 && head_dim <= 512 && head_dim % 16 == 0, "head_dim %d must be a multiple of 16 up to 512", head_dim);
+    RQ_CHECK_ARG(rot_dim >= 16 && rot_dim <= head_dim && rot_dim % 16 == 0, "rot_dim %d must be a multiple of 16 up to head_dim %d", rot_dim, head_dim);
+    RQ_CHECK_ARG(n_tokens >= 0 && n_tokens <= (1 << 24) && num_q_heads >= 0 && num_q_heads <= 65536 && table_rows >= 1, "bad sizes");
+    RQ_CHECK_ARG(n_tokens == 0 || (positions && table && (num_q_heads == 0 || (query && out))), "null pointer");
+    const int eb = dtype == RQ_DTYPE_F32 ? 4 : 2, tb = table_dtype == RQ_DTYPE_F32 ? 4 : 2;
+    RQ_CHECK_ARG((uintptr_t)table % 16 == 0 && (table_rows == 1 || (table_stride >= rot_dim && table_stride * tb % 16 == 0)),
+                 "table rows must be 16-byte aligned, %d numbers or more apart", rot_dim);
+    RQ_CHECK_ARG(num_q_heads == 0 || ((uintptr_t)query % 16 == 0 && q_st * eb % 16 == 0 && q_sh * eb % 16 == 0 && (uintptr_t)out % 16 == 0 &&
+                                      o_st * eb % 16 == 0 && o_sh * eb % 16 == 0),
+                 "query and rotated query rows must be 16-byte aligned");
+    a = RopeRows{};
+    a.t = {positions, table, table_stride, table_rows, rot_dim, halves != 0, table_dtype == RQ_DTYPE_F32};
+    a.n_tokens = n_tokens;
+    a.n_q = num_q_heads, a.D = head_dim;
+    a.q = query, a.q_st = q_st, a.q_sh = q_sh;
+    a.out = out, a.o_st = o_st, a.o_sh = o_sh;
+    RQ_CHECK_ARG(rope_threads(a) <= INT32_MAX - kRopeThreads, "too many rows for one call");
+    return RQ_OK;
+}
+
+}  // namespace rq

@@ -20,6 +20,10 @@ _DTYPE_CODE = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float
 
 _c_i32, _c_i64, _c_f32, _c_p = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
+# Arguments that the stores with position rotation begin with, up to out_q and its strides.
+_ROPE = ([_c_p, _c_p, _c_p, _c_i32, _c_i64, _c_i32] + [_c_i64] * 6
+         + [_c_i32, _c_i32, _c_p, _c_p, _c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_p, _c_i64, _c_i64])
+
 _SIGNATURES = {
     "rq_abi_version": (_c_i32, []),
     "rq_last_error": (ctypes.c_char_p, []),
@@ -73,6 +77,13 @@ _SIGNATURES = {
     "rq_q8_attention": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_i64,
                                  _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f32, _c_p,
                                  _c_i64, _c_i64, _c_p, _c_i64, _c_p]),
+    "rq_rope_compress_store": (_c_i32, _ROPE + [_c_i32, _c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_p, _c_i32,
+                                                _c_p, _c_i32, _c_p]),
+    "rq_rope_q8_store": (_c_i32, _ROPE + [_c_i32, _c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_p, _c_i64, _c_p]),
+    "rq_rope_kv16_store": (_c_i32, _ROPE + [_c_p, _c_p, _c_p, _c_i64, _c_i32] + [_c_i64] * 6 + [_c_p]),
+    "rq_kv16_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64]),
+    "rq_kv16_attention": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i64, _c_i32]
+                          + [_c_i64] * 6 + [_c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f32, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -21,6 +21,9 @@ the C ABI (include/rq_abi.h).  Differences, all deliberate:
   tokens per sequence run on the decode kernels (three launches) where that is faster.
 * q8_store, q8_read and q8_attention (kernels/q8.py) work on the 8-bit cache,
   which the reference does not have.
+* rope_compress_store, rope_q8_store and rope_kv16_store (kernels/rope.py) rotate queries and keys by their
+  positions on the way into the codebook cache, the 8-bit one and plain 16-bit pages, and kv16_attention
+  (kernels/kv16.py) attends over such pages; the reference leaves both to the model and to flash attention.
 """
 from __future__ import annotations
 
@@ -31,7 +34,9 @@ import weakref
 import torch
 
 from .. import _lib
+from .kv16 import kv16_attention
 from .q8 import q8_attention, q8_read, q8_slot_bytes, q8_store
+from .rope import rope_compress_store, rope_kv16_store, rope_q8_store
 
 __all__ = [
     "iso_compress",
@@ -50,6 +55,10 @@ __all__ = [
     "q8_store",
     "q8_read",
     "q8_attention",
+    "rope_compress_store",
+    "rope_q8_store",
+    "rope_kv16_store",
+    "kv16_attention",
 ]
 
 
