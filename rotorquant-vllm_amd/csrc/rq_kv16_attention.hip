@@ -30,6 +30,11 @@ struct Kv16Args : AttnBatch {
     float scale;  // sm_scale log2(e)
 };
 
+template <typename T>
+__device__ __forceinline__ T kv16_load(const uint16_t *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+}
+
 // Infinities and NaN are the 16-bit numbers whose magnitude, as an integer, is kHuge or more.
 template <int DT>
 constexpr uint32_t kHuge = DT == RQ_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
@@ -48,14 +53,15 @@ __device__ __forceinline__ uint32_t huge_halves(uint32_t w) {  // all ones where
 // Keys past the context are loaded as its last one, with a weight of 0.  0 * infinity is a NaN, there and where an infinite V is hidden
 // from some columns, and a weight's second part may be 0 or negative: so a segment that met an infinity or NaN in V is done again, as FAR,
 // which adds one token's columns at a time, with the rows that token sees, and the infinities apart, by weights of 1.
-template <int DT, int DP, bool FULL, int NB, int W, bool FAR = false>
+// HEADS: each wave has a head of its own and all the tiles (W is 1); otherwise the waves share a head.
+template <int DT, int DP, bool FULL, int NB, int W, bool HEADS, bool FAR = false>
 __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, const AttnSeq &s, int h, int c0, int t0, int t1, float *part,
                                              AttnSums<DP, W> &lds) {
     constexpr int kSteps = DP / 32, kBlocks = DP / 16;
     constexpr int kVDims = DP == 64 ? 4 : 8, kVParts = DP == 256 ? 2 : 1;  // dims of a lane's V load, loads of a row
     constexpr float kPeak = DT == RQ_DTYPE_F16 ? 14.f : 0.f;
     using VRow = std::conditional_t<DP == 64, u32x2, u32x4>;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int lane = threadIdx.x & 63, wave = HEADS ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, D = FULL ? DP : a.D;
 
     // Where the rows of a tile are: lane l has key l % 32.  Past the last key that counts here, that one again.
@@ -83,7 +89,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
         for (int gr = 0; gr < 2; ++gr) {
             const uint16_t *row = row_of(k_base, k_row, 4 * col + 64 * gr) + 8 * g;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) kr[gr][k] = *reinterpret_cast<const u32x4 *>(row + (FULL || 32 * k + 8 * g < D ? 32 * k : -8 * g));
+            for (int k = 0; k < kSteps; ++k) kr[gr][k] = kv16_load<u32x4>(row + (FULL || 32 * k + 8 * g < D ? 32 * k : -8 * g));
         }
     };
     auto fetch_v = [&]() {  // (dims past D: any, not used)
@@ -93,8 +99,8 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint16_t *row = row_of(v_base, v_row, 16 * g + 64 * gr + 4 * i) + d;
-                vr[gr][i][0] = *reinterpret_cast<const VRow *>(row);
-                if constexpr (kVParts == 2) vr[gr][i][1] = *reinterpret_cast<const VRow *>(row + (FULL || 128 + 8 * col < D ? 128 : 0));
+                vr[gr][i][0] = kv16_load<VRow>(row);
+                if constexpr (kVParts == 2) vr[gr][i][1] = kv16_load<VRow>(row + (FULL || 128 + 8 * col < D ? 128 : 0));
             }
     };
     const int n = (t1 - t0 - wave + W - 1) / W;  // tiles of this wave (0 or less: none)
@@ -252,10 +258,39 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
     }
 
     if constexpr (!FAR) {
-        if (__syncthreads_or((big & 0xffffu) >= kHuge<DT> || big >> 16 >= kHuge<DT>)) {
-            kv16_segment<DT, DP, FULL, NB, W, true>(a, seq, s, h, c0, t0, t1, part, lds);
+        const bool far = (big & 0xffffu) >= kHuge<DT> || big >> 16 >= kHuge<DT>;
+        if (HEADS ? __any(far) : __syncthreads_or(far)) {
+            kv16_segment<DT, DP, FULL, NB, W, HEADS, true>(a, seq, s, h, c0, t0, t1, part, lds);
             return;
         }
+    }
+    if constexpr (HEADS) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float l = rows_sum(l_run[nb]);
+            if (token[nb] >= s.T) continue;
+            const uint32_t cc = c0 + kShareCols * nb + col;
+            const float f = part == nullptr ? attn_inv<true>(a, s, token[nb], l) : 1.f;
+            uint16_t *const row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + token[nb]) * a.o_st + (int64_t)(h * a.G + (int)(cc - token[nb] * a.G)) * a.o_sh;
+            float *const pt = part + nb * AttnPartial<DP>::kFloats;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int p = 0; p < kVParts; ++p) {
+                    const int d0 = 128 * p + kVDims * (4 * g + i);
+                    float o[kVDims];
+#pragma unroll
+                    for (int d = 0; d < kVDims; ++d) o[d] = acc[nb][8 * p + d][i];
+                    if (part == nullptr) {
+                        attn_put<DT, kVDims>(row + d0, o, f, D - d0);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < kVDims; d += 4) *reinterpret_cast<float4 *>(pt + col * DP + d0 + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+                    }
+                }
+            if (part != nullptr && g == 0) *reinterpret_cast<float2 *>(pt + kShareCols * DP + 2 * col) = make_float2(m_run[nb], l);
+        }
+        return;
     }
     // the waves' sums
 #pragma unroll
@@ -276,27 +311,119 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
     }
 }
 
-// Workgroups of a CU at once (by registers, 4 waves each).
+// ---- shares -------------------------------------------------------------------
+// The tiles of all (sequence, block of columns) pairs in a row are cut into equal shares, and a share is taken by one workgroup for each kv
+// head: the heads of a token lie together in memory, and are read at about the same time.
+template <int NB>
+__device__ __forceinline__ int64_t kv16_seq_tiles(const Kv16Args &a, int64_t b) {
+    if (b >= a.num_seqs) return 0;
+    const AttnSeq s = attn_seq(a, b);
+    return (int64_t)attn_tiles(s) * attn_col_blocks<NB>(a, s.T);
+}
+// Place of share w's part of an item in the workspace: an item cut in two or more is the last of the share that begins it and the first of the others.
 template <int DP, int NB>
-constexpr int kKv16Resident = DP == 64 ? (NB == 1 ? 4 : 3) : DP == 128 ? (NB == 1 ? 3 : 2) : (NB == 1 ? 2 : 1);
-
-// Equal shares of all items' tiles.
-template <int DT, int DP, bool FULL, int NB>
-__global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kernel(Kv16Args a) {
-    __shared__ AttnSums<DP, 4> lds;
-    auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };  // (all of these are the workgroup's, in SGPRs)
-    attn_walk<DP, NB>(a, [&](int64_t seq, const AttnSeq &v, int h, int c0, int t0, int t1, float *part) {
-        const AttnSeq s{scalar(v.q0), scalar(v.T), scalar(v.pos), scalar(v.vis)};
-        const int64_t at = part == nullptr ? 0 : part - a.part;
-        float *const to = part == nullptr ? nullptr : a.part + (int64_t)((uint64_t)(uint32_t)scalar((int)(at >> 32)) << 32 | (uint32_t)scalar((int)at));
-        kv16_segment<DT, DP, FULL, NB, 4>(a, scalar((int)seq), s, scalar(h), scalar(c0), scalar(t0), scalar(t1), to, lds);
-    });
+__device__ __forceinline__ float *kv16_part(const Kv16Args &a, int64_t w, bool begins, int h) {
+    return a.part + ((2 * w + (begins ? 1 : 0)) * a.H + h) * (NB * AttnPartial<DP>::kFloats);
 }
 
+// Tiles of a share.
+constexpr int kKv16MinChunk = 4;
+__device__ __forceinline__ int64_t kv16_share(int64_t tiles, int shares) {
+    return max((int64_t)kKv16MinChunk, div64(tiles + shares - 1, shares));
+}
+
+// Workgroups of a CU at once (4 waves each): fewer, of more registers, keep enough loads on their way.
+template <int DP, int NB>
+constexpr int kKv16Resident = DP == 256 ? 1 : 2;
+
+template <int DT, int DP, bool FULL, int NB, bool HEADS>
+__global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kernel(Kv16Args a) {
+    constexpr int kHeads = HEADS ? 4 : 1;  // of a workgroup
+    __shared__ AttnSums<DP, HEADS ? 1 : 4> lds;
+    auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };  // (what is the workgroup's, into SGPRs)
+    const int lane = threadIdx.x & 63, hs = a.H / kHeads, shares = gridDim.x / (uint32_t)hs, w = blockIdx.x / (uint32_t)hs,
+              h = (blockIdx.x - w * hs) * kHeads + (HEADS ? scalar(threadIdx.x >> 6) : 0);
+    int64_t block = 0, block_base = 0;  // 64 sequences: their tiles, and the row's up to each
+    int64_t mine = kv16_seq_tiles<NB>(a, lane), upto = wave_scan64(mine);
+    int64_t total = lane64(upto, 63);
+    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(kv16_seq_tiles<NB>(a, b + lane)), 63);
+    const int64_t share = kv16_share(total, shares);
+    int64_t pos = w * share;
+    const int64_t end = min(total, pos + share);
+    while (pos < end) {
+        uint64_t hit = __ballot(block_base + upto > pos);
+        while (hit == 0) {
+            block_base += lane64(upto, 63);
+            block += 64;
+            mine = kv16_seq_tiles<NB>(a, block + lane);
+            upto = wave_scan64(mine);
+            hit = __ballot(block_base + upto > pos);
+        }
+        const int of = __builtin_ctzll(hit);
+        const int64_t seq = block + of, in_seq = pos - (block_base + lane64(upto, of) - lane64(mine, of));
+        const AttnSeq v = attn_seq(a, seq), s{scalar(v.q0), scalar(v.T), scalar(v.pos), scalar(v.vis)};
+        const int n = attn_tiles(s), cols = scalar((int)div64(in_seq, n));
+        const int t0 = scalar((int)(in_seq - (int64_t)cols * n)), t1 = scalar((int)min((int64_t)n, t0 + (end - pos)));
+        float *part = t0 == 0 && t1 == n ? nullptr : kv16_part<DP, NB>(a, w, t0 == 0, h);
+        kv16_segment<DT, DP, FULL, NB, HEADS ? 1 : 4, HEADS>(a, scalar((int)seq), s, h, cols * (NB * kShareCols), t0, t1, part, lds);
+        pos += t1 - t0;
+    }
+}
+
+// Adds up the parts of the items that were cut.  A wave takes one column; lane: D / 16 dims, and every fourth part, four of them on their way.
 template <int DT, int DP, int NB>
-__global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int workgroups) {
-    __shared__ AttnSums<DP, 4> lds;
-    attn_merge<DT, DP, NB, true>(a, workgroups, a.D, lds);
+__global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares) {
+    constexpr int kDims = DP / 16, kAhead = DP == 256 ? 2 : 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, way = lane >> 4, d0 = (lane & 15) * kDims;
+    const int64_t b = blockIdx.y;
+    const AttnSeq s = attn_seq(a, b);
+    const int h = blockIdx.x % (uint32_t)a.H, cc = blockIdx.x / (uint32_t)a.H * 4 + wave;  // (the column, of all blocks')
+    if (cc >= s.T * a.G) return;
+    const int n = attn_tiles(s), nb = cc / kShareCols % NB, c = cc % kShareCols;
+    int64_t total = 0, before = 0;
+    for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
+        const int64_t mine = kv16_seq_tiles<NB>(a, b0 + lane), upto = wave_scan64(mine);
+        if (b >= b0 && b < b0 + 64) before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
+        total += lane64(upto, 63);
+    }
+    const int64_t share = kv16_share(total, shares), first = before + (int64_t)(cc / (NB * kShareCols)) * n;
+    const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
+    if (w0 == w1) return;
+    float M = -INFINITY, l = 0.f, o[kDims] = {};
+    for (int w = w0 + way; w <= w1; w += 4 * kAhead) {
+        float2 ml[kAhead];
+        float4 x[kAhead][kDims / 4];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int wu = min(w + 4 * u, w1);
+            const float *pt = kv16_part<DP, NB>(a, wu, wu == w0, h) + nb * AttnPartial<DP>::kFloats;
+            ml[u] = *reinterpret_cast<const float2 *>(pt + kShareCols * DP + 2 * c);
+#pragma unroll
+            for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + c * DP + d0 + 4 * k);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (w + 4 * u > w1) continue;
+            const float Mn = fmaxf(M, ml[u].x);
+            const float keep = M == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mn);
+            const float r = ml[u].x == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(ml[u].x - Mn);
+            M = Mn;
+            l = l * keep + r * ml[u].y;
+#pragma unroll
+            for (int k = 0; k < kDims / 4; ++k) {
+                o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
+                o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+            }
+        }
+    }
+    const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mt);
+    l = rows_sum(l * r);
+#pragma unroll
+    for (int k = 0; k < kDims; ++k) o[k] = rows_sum(o[k] * r);
+    if (way != 0) return;
+    const int i = cc / a.G;
+    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + cc % a.G) * a.o_sh + d0;
+    attn_put<DT, kDims>(row, o, attn_inv<true>(a, s, i, l), a.D - d0);
 }
 
 // One workgroup per item: one launch, no partials.
@@ -309,7 +436,7 @@ __global__ __launch_bounds__(64 * kKv16ItemWaves<DP>, DP == 256 ? 1 : 2) void kv
     const AttnSeq s = attn_seq(a, seq);
     const int block = blockIdx.x / (uint32_t)a.H, h = blockIdx.x - block * a.H;
     if (block >= attn_col_blocks<NB>(a, s.T)) return;
-    kv16_segment<DT, DP, FULL, NB, kKv16ItemWaves<DP>>(a, seq, s, h, block * (NB * kShareCols), 0, attn_tiles(s), nullptr, lds);
+    kv16_segment<DT, DP, FULL, NB, kKv16ItemWaves<DP>, false>(a, seq, s, h, block * (NB * kShareCols), 0, attn_tiles(s), nullptr, lds);
 }
 
 // Whether a head's rows span less than 2^32 units of 8 elements.
@@ -319,40 +446,54 @@ static bool kv16_span(int64_t num_blocks, int64_t block_size, int64_t stride_blo
 
 static int kv16_blocks(int G, int64_t max_q_len) { return max_q_len * G > kShareCols ? 2 : 1; }
 static int kv16_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-static int64_t kv16_workgroups(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
-    const int nb = kv16_blocks(G, max_q_len), w = kv16_width(D);
-    const int resident = w == 64    ? (nb == 1 ? kKv16Resident<64, 1> : kKv16Resident<64, 2>)
-                         : w == 128 ? (nb == 1 ? kKv16Resident<128, 1> : kKv16Resident<128, 2>)
-                                    : (nb == 1 ? kKv16Resident<256, 1> : kKv16Resident<256, 2>);
-    return attn_workgroups(num_seqs, G, H, max_q_len, max_keys, nb, resident);
+// How a call is cut, by its bounds: shares of tiles, each taken by H / heads workgroups.  heads 4 (a wave each) where that leaves a wave 12 tiles
+// or more, else 1 (the waves share the tiles, and their sums): the former reads 1 KB of a token at about the same time, but its parts are four
+// times as many.  8 heads x 4 of 128, us by waves / by tiles: 64 sequences of 1024 to 8192 keys 196 / 221, of 2000 93.5 / 97.4, 16 of 2000 (4 tiles a
+// wave) 32.9 / 33.1, 1 of 4000 16.9 / 12.9; 4 heads x 7, 4 sequences of 20000 to 32768 (8 tiles a wave) 59.7 / 54.5.
+struct Kv16Cut {
+    int heads;
+    int64_t shares;
+};
+static Kv16Cut kv16_cut(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
+    const int w = kv16_width(D), cols = kv16_blocks(G, max_q_len) * kShareCols;
+    const int64_t resident = (w == 64 ? kKv16Resident<64, 1> : w == 128 ? kKv16Resident<128, 1> : kKv16Resident<256, 1>) * (int64_t)device_cus();
+    const int64_t tiles = max_keys / kShareTile + (max_keys % kShareTile != 0 || max_keys == 0);
+    const int64_t work = num_seqs * ((max_q_len * G + cols - 1) / cols) * tiles;
+    const int heads = H % 4 == 0 && work * (H / 4) >= 12 * resident ? 4 : 1;
+    return {heads, std::max<int64_t>(1, std::min<int64_t>(resident * heads / H, (work + kKv16MinChunk - 1) / kKv16MinChunk))};
 }
 
-// Calls of short contexts, by the bound on their lengths, take a workgroup per item.
-constexpr int64_t kKv16ItemTiles = 32;
+// Calls of short contexts, by the bound on their lengths, take a workgroup per item: one launch, and no parts.  One CU loads 55 to 60 GB/s, so
+// long ones are slower.  8 heads x 4 of 128, items / shares, us: 1 sequence of 256 keys 7.5 / 9.9, 512: 9.8 / 9.9, 777: 12.6 / 10.3; 16 sequences
+// 9.7 / 11.3, 14.2 / 14.5, 19.1 / 20.5; 64: 19.9 / 18.7, 30.7 / 30.0, 42.7 / 42.7.
+constexpr int64_t kKv16ItemTiles = 16;
 static bool kv16_is_short(int64_t max_keys) { return max_keys <= kKv16ItemTiles * kShareTile; }
 
 template <int DT, int DP, bool FULL, int NB>
-static void launch_kv16(const Kv16Args &a, int64_t workgroups, hipStream_t st) {
+static void launch_kv16(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
     const int64_t items = ((int64_t)a.max_q * a.G + NB * kShareCols - 1) / (NB * kShareCols) * a.H;
     if (kv16_is_short(a.bound)) {
         hipLaunchKernelGGL((kv16_item_kernel<DT, DP, FULL, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(64 * kKv16ItemWaves<DP>), 0, st, a);
         return;
     }
-    hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB>), dim3((unsigned)workgroups), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((kv16_merge_kernel<DT, DP, NB>), dim3((unsigned)(items * NB), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)workgroups);
+    const int64_t quads = ((int64_t)a.max_q * a.G + 3) / 4;
+    const dim3 grid((unsigned)(cut.shares * (a.H / cut.heads)));
+    if (cut.heads == 4) hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv16_merge_kernel<DT, DP, NB>), dim3((unsigned)(quads * a.H), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)cut.shares);
 }
 template <int DT, int DP, bool FULL>
-static void launch_kv16_b(const Kv16Args &a, int64_t wgs, hipStream_t st) {
-    kv16_blocks(a.G, a.max_q) == 1 ? launch_kv16<DT, DP, FULL, 1>(a, wgs, st) : launch_kv16<DT, DP, FULL, 2>(a, wgs, st);
+static void launch_kv16_b(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
+    kv16_blocks(a.G, a.max_q) == 1 ? launch_kv16<DT, DP, FULL, 1>(a, cut, st) : launch_kv16<DT, DP, FULL, 2>(a, cut, st);
 }
 template <int DT, int DP>
-static void launch_kv16_f(const Kv16Args &a, int64_t wgs, hipStream_t st) {
-    a.D == DP ? launch_kv16_b<DT, DP, true>(a, wgs, st) : launch_kv16_b<DT, DP, false>(a, wgs, st);
+static void launch_kv16_f(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
+    a.D == DP ? launch_kv16_b<DT, DP, true>(a, cut, st) : launch_kv16_b<DT, DP, false>(a, cut, st);
 }
 template <int DT>
-static void launch_kv16_d(const Kv16Args &a, int64_t wgs, hipStream_t st) {
+static void launch_kv16_d(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
     const int w = kv16_width(a.D);
-    w == 64 ? launch_kv16_f<DT, 64>(a, wgs, st) : w == 128 ? launch_kv16_f<DT, 128>(a, wgs, st) : launch_kv16_f<DT, 256>(a, wgs, st);
+    w == 64 ? launch_kv16_f<DT, 64>(a, cut, st) : w == 128 ? launch_kv16_f<DT, 128>(a, cut, st) : launch_kv16_f<DT, 256>(a, cut, st);
 }
 
 }  // namespace rq
@@ -366,8 +507,7 @@ extern "C" int64_t rq_kv16_attention_workspace_bytes(int64_t num_seqs, int32_t n
     const int G = num_q_heads / num_kv_heads;
     max_seq_len = attn_bound(max_seq_len);
     if (kv16_is_short(max_seq_len)) return 0;
-    const int64_t wgs = kv16_workgroups(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len);
-    return 2 * wgs * kv16_blocks(G, max_q_len) * kShareCols * (kv16_width(head_dim) + 2) * 4;
+    return 2 * kv16_cut(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len).shares * num_kv_heads * kv16_blocks(G, max_q_len) * kShareCols * (kv16_width(head_dim) + 2) * 4;
 }
 
 extern "C" int rq_kv16_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads, int64_t q_stride_tok, int64_t q_stride_head,
@@ -419,8 +559,8 @@ extern "C" int rq_kv16_attention(const void *q, int32_t dtype, int64_t total_q, 
     RQ_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace must be 16-byte aligned");
     a.part = static_cast<float *>(workspace);
     hipStream_t st = (hipStream_t)stream;
-    const int64_t wgs = kv16_workgroups(num_seqs, a.G, a.H, head_dim, a.max_q, a.bound);
-    if (dtype == RQ_DTYPE_BF16) launch_kv16_d<RQ_DTYPE_BF16>(a, wgs, st);
-    else launch_kv16_d<RQ_DTYPE_F16>(a, wgs, st);
+    const Kv16Cut cut = kv16_cut(num_seqs, a.G, a.H, head_dim, a.max_q, a.bound);
+    if (dtype == RQ_DTYPE_BF16) launch_kv16_d<RQ_DTYPE_BF16>(a, cut, st);
+    else launch_kv16_d<RQ_DTYPE_F16>(a, cut, st);
     return check_launch("kv16_stream_kernel");
 }

@@ -233,19 +233,115 @@ __device__ __forceinline__ void q8_segment(const Q8AttnArgs &a, int64_t seq, con
 template <int D, int NB>
 constexpr int kQ8Resident = D == 64 ? (NB == 1 ? 4 : 3) : 2;
 
-// Equal shares of all items' tiles.
+// The tiles of all items, in the order sequence, block of columns, kv head, in a row and cut into equal shares.
 template <int DT, int FMT, int D, int NB, bool ONCE>
 __global__ __launch_bounds__(256, (kQ8Resident<D, NB>)) void q8_stream_kernel(Q8AttnArgs a) {
     __shared__ AttnSums<D, 4> lds;
-    attn_walk<D, NB>(a, [&](int64_t seq, const AttnSeq &s, int h, int c0, int t0, int t1, float *part) {
-        q8_segment<DT, FMT, D, NB, 4, ONCE>(a, seq, s, h, c0, t0, t1, part, lds);
-    });
+    const int lane = threadIdx.x & 63;
+    int64_t block = 0, block_base = 0;  // 64 sequences: their tiles, and the row's up to each
+    int64_t mine = attn_seq_tiles<NB>(a, lane), upto = wave_scan64(mine);
+    int64_t total = lane64(upto, 63);
+    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(attn_seq_tiles<NB>(a, b + lane)), 63);
+    const int64_t share = attn_share(total, gridDim.x);
+    int64_t pos = blockIdx.x * share;
+    const int64_t end = min(total, pos + share);
+    while (pos < end) {
+        uint64_t hit = __ballot(block_base + upto > pos);
+        while (hit == 0) {
+            block_base += lane64(upto, 63);
+            block += 64;
+            mine = attn_seq_tiles<NB>(a, block + lane);
+            upto = wave_scan64(mine);
+            hit = __ballot(block_base + upto > pos);
+        }
+        const int of = __builtin_ctzll(hit);
+        const int64_t seq = block + of, in_seq = pos - (block_base + lane64(upto, of) - lane64(mine, of));
+        const AttnSeq s = attn_seq(a, seq);
+        const int n = attn_tiles(s);
+        const int64_t item = div64(in_seq, n), block_of = div64(item, a.H);
+        const int t0 = (int)(in_seq - item * n), t1 = (int)min((int64_t)n, t0 + (end - pos));
+        // an item cut in two or more: the share that begins it ends with it, the others begin with it
+        float *part = t0 == 0 && t1 == n ? nullptr : a.part + (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * NB * AttnPartial<D>::kFloats;
+        q8_segment<DT, FMT, D, NB, 4, ONCE>(a, seq, s, (int)(item - block_of * a.H), (int)block_of * (NB * kShareCols), t0, t1, part, lds);
+        pos += t1 - t0;
+    }
 }
 
+// Adds up the partials of the items that were cut: one workgroup per item and block of 16 columns.  A wave takes four
+// columns (lane: column % 4, part of D / 16 dims); with few columns, as decodes have, several waves share them
+// and take every second or fourth partial.  Two partials are in flight per wave.
 template <int DT, int D, int NB>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnArgs a, int workgroups) {
     __shared__ AttnSums<D, 4> lds;
-    attn_merge<DT, D, NB, false>(a, workgroups, D, lds);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int64_t b = blockIdx.y;
+    const int item = blockIdx.x / NB, nb = blockIdx.x % NB;
+    const AttnSeq s = attn_seq(a, b);
+    const int h = item % a.H, c0 = (item / a.H) * (NB * kShareCols) + nb * kShareCols;
+    const int cols = min(kShareCols, s.T * a.G - c0);
+    if (cols <= 0) return;
+    const int n = attn_tiles(s);
+    int64_t total = 0, before = 0;
+    for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
+        const int64_t mine = attn_seq_tiles<NB>(a, b0 + lane), upto = wave_scan64(mine);
+        if (b >= b0 && b < b0 + 64) before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
+        total += lane64(upto, 63);
+    }
+    const int64_t share = attn_share(total, workgroups);
+    const int64_t first = before + (int64_t)item * n;
+    const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
+    if (w0 == w1) return;
+    constexpr int kDims = D / 16;
+    const int quads = cols > 8 ? 4 : cols > 4 ? 2 : 1, ways = 4 / quads;  // column quads, waves of each
+    const int way = wave / quads, d0 = (lane & 15) * kDims;
+    {
+        const int c = 4 * (wave % quads) + (lane >> 4), cv = min(c, cols - 1);
+        float M = -INFINITY, l = 0.f, o[kDims] = {};
+        for (int w = w0 + way; w <= w1; w += 2 * ways) {
+            float2 ml[2];
+            float4 x[2][kDims / 4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int wu = min(w + ways * u, w1);
+                const float *pt = a.part + ((2 * (int64_t)wu + (wu == w0 ? 1 : 0)) * NB + nb) * AttnPartial<D>::kFloats;
+                ml[u] = *reinterpret_cast<const float2 *>(pt + kShareCols * D + 2 * cv);
+#pragma unroll
+                for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + cv * D + d0 + 4 * k);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (w + ways * u > w1) continue;
+                const float Mn = fmaxf(M, ml[u].x);
+                const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+                const float r = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - Mn);
+                M = Mn;
+                l = l * keep + r * ml[u].y;
+#pragma unroll
+                for (int k = 0; k < kDims / 4; ++k) {
+                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
+                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kDims; k += 4) *reinterpret_cast<float4 *>(&lds.acc[way][c][d0 + k]) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        if ((lane & 15) == 0) lds.ml[way][c] = make_float2(M, l);
+    }
+    __syncthreads();
+    const int c = tid >> 4;
+    if (c >= cols) return;
+    float Mt = -INFINITY, l = 0.f, o[kDims] = {};
+    for (int w = 0; w < ways; ++w) Mt = fmaxf(Mt, lds.ml[w][c].x);
+    for (int w = 0; w < ways; ++w) {
+        const float2 ml = lds.ml[w][c];
+        const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
+        l += r * ml.y;
+#pragma unroll
+        for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][(tid & 15) * kDims + k];
+    }
+    const int i = (c0 + c) / a.G;
+    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + (c0 + c) % a.G) * a.o_sh + (tid & 15) * kDims;
+    attn_put<DT, kDims>(row, o, attn_inv<false>(a, s, i, l), kDims);
 }
 
 // One workgroup of 8 waves per item: one launch, no partials.  What bounds it is two things in a row.  A chain of dependent loads and its

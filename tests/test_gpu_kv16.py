@@ -28,8 +28,8 @@ def run(lens, q_lens, H, G, D, dtype, block=16, causal=True, scale=None, seed=1,
     P.check(got, *P.attention(q, *pages.kv, lens, q_lens, scale, causal))
 
 
-# A bound over 1024 takes shares of several workgroups, one under it a workgroup for each item.
-@pytest.mark.parametrize("bound", [1024, None])
+# A bound over 512 takes shares of several workgroups, one under it a workgroup for each item.
+@pytest.mark.parametrize("bound", [512, None])
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("D", [8, 40, 64, 72, 80, 96, 128, 192, 200, 256])
 def test_head_dims(D, dtype, bound):
@@ -65,7 +65,7 @@ def test_longer_queries_than_contexts():
 
 @pytest.mark.parametrize("length", [1, 2, 31, 32, 33, 63, 64, 65, 127, 255, 256, 257, 1023, 1024, 1025, 2049, 4100])
 def test_lengths(length):
-    run([length, 1], [1, 1], 1, 4, 128, BF, bound=None if length > 1024 else 1024)
+    run([length, 1], [1, 1], 1, 4, 128, BF, bound=None if length > 512 else 512)
     run([length], [1], 2, 2, 128, FP, bound=length)
     run([length], [1], 2, 2, 64, FP)
 

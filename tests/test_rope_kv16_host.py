@@ -86,7 +86,7 @@ def test_attention_without_work_or_scratch():
     for kw in (dict(num_seqs=0, total_q=0), dict(total_q=0, cu=A), dict(max_q_len=0)):
         assert call("rq_kv16_attention", ATTENTION, **kw)[0] == 0
     size = _lib.load().rq_kv16_attention_workspace_bytes
-    assert size(2, 8, 2, 128, 1, 1024) == 0 and size(0, 8, 2, 128, 1, 9000) == 0 and size(2, 8, 2, 300, 1, 9000) == 0
+    assert size(2, 8, 2, 128, 1, 512) == 0 and size(0, 8, 2, 128, 1, 9000) == 0 and size(2, 8, 2, 300, 1, 9000) == 0
     need = size(2, 8, 2, 128, 1, 9000)
     assert need > 0 and size(2, 8, 2, 128, 9, 9000) > need and size(2, 8, 2, 128, 1, 1 << 60) >= need
     rc, message = call("rq_kv16_attention", ATTENTION, max_seq_len=9000, max_blocks=1000)
