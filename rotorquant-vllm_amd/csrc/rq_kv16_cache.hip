@@ -2,15 +2,6 @@
 // query rows rotated, in one launch.  The pages are K and V (page, slot, head, dim) with any strides over whole rows.
 #include "rq_rope.h"
 
-namespace rq {
-
-template <int DT>
-__global__ __launch_bounds__(kRopeThreads) void rope_kv16_kernel(RopeRows a) {
-    rope_rows<DT>(a, (int64_t)blockIdx.x * kRopeThreads + threadIdx.x);
-}
-
-}  // namespace rq
-
 using namespace rq;
 
 extern "C" int rq_rope_kv16_store(const void *query, const void *key, const void *value, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
@@ -44,8 +35,6 @@ extern "C" int rq_rope_kv16_store(const void *query, const void *key, const void
     a.num_slots = num_blocks * block_size;
     a.block_size = block_size;
     RQ_CHECK_ARG(rope_threads(a) <= INT32_MAX - kRopeThreads, "too many rows for one call");
-    const dim3 grid((unsigned)rope_blocks(a)), block(kRopeThreads);
-    if (dtype == RQ_DTYPE_F16) hipLaunchKernelGGL((rope_kv16_kernel<RQ_DTYPE_F16>), grid, block, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((rope_kv16_kernel<RQ_DTYPE_BF16>), grid, block, 0, (hipStream_t)stream, a);
-    return check_launch("rope_kv16_kernel");
+    dtype == RQ_DTYPE_F16 ? launch_rope_rows<RQ_DTYPE_F16>(a, (hipStream_t)stream) : launch_rope_rows<RQ_DTYPE_BF16>(a, (hipStream_t)stream);
+    return check_launch("rope_rows_kernel");
 }

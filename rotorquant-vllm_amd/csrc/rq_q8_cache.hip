@@ -122,7 +122,7 @@ template <bool ROPE>
 struct Q8Rope {};
 template <>
 struct Q8Rope<true> {
-    RopeRows rows;          // the queries, by workgroups of their own behind those that store
+    RopeRows rows;          // the queries of a short call, by workgroups of their own behind those that store
     unsigned store_blocks;
 };
 // Piece `piece` (8 dims) of a key row at element `at` of a.key, turned by its token's position.
@@ -413,7 +413,8 @@ static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStrea
     int64_t grid = blocks;
     if constexpr (ROPE) {
         rope.store_blocks = (unsigned)blocks;
-        grid += rope_blocks(rope.rows);
+        if (linked) launch_rope_rows<DT>(rope.rows, st);
+        else grid += rope_blocks(rope.rows);
     }
     if (linked) hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);
     else hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, false, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);

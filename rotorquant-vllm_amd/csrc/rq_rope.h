@@ -239,6 +239,18 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
     }
 }
 
+template <int DT>
+__global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRows a) {
+    rope_rows<DT>(a, (int64_t)blockIdx.x * kRopeThreads + threadIdx.x);
+}
+template <int DT>
+void launch_rope_rows(const RopeRows &a, hipStream_t st) {
+    if (rope_blocks(a) > 0) hipLaunchKernelGGL((rope_rows_kernel<DT>), dim3((unsigned)rope_blocks(a)), dim3(kRopeThreads), 0, st, a);
+}
+
+// Tokens from which a store's queries have a launch of their own: beside a store's registers and LDS fewer of their waves fit a CU.
+constexpr int64_t kRopeApart = 512;
+
 // The table and the query rows of a call, checked; strides in elements of the rows' type.
 inline int rope_queries(RopeRows &a, int dtype, int64_t n_tokens, int head_dim, const int64_t *positions, const void *table, int table_dtype,
                         int64_t table_rows, int64_t table_stride, int rot_dim, int halves, const void *query, int num_q_heads, int64_t q_st,

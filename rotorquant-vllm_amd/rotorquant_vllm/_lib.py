@@ -113,6 +113,24 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     return lib
 
 
+_ops = None
+
+
+def ops():
+    """The module rotorquant_vllm._rq_torch (csrc/rq_torch.cpp): entry points whose tensors are looked through in C++, where a call through ctypes
+    would take the host longer than its kernel takes the GPU.  Built with librq_hip.so, which it calls."""
+    global _ops
+    if _ops is None:
+        load()
+        try:
+            from . import _rq_torch
+        except ImportError as exc:
+            raise ImportError(f"rotorquant_vllm._rq_torch failed to load: {exc}; build it with "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`") from exc
+        _ops = _rq_torch
+    return _ops
+
+
 def available() -> bool:
     try:
         load()

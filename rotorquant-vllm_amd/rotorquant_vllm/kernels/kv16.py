@@ -5,22 +5,11 @@ outputs, or pages that rope_kv16_store appends to.  The codebook and 8-bit cache
 """
 from __future__ import annotations
 
-import functools
-import math
-
 import torch
 
 from .. import _lib
-from .q8 import _call, _device_index, _index, _row_strides, _scratch
-from .rope import _check_pages
 
 __all__ = ["kv16_attention"]
-
-
-@functools.lru_cache(maxsize=4096)
-def _attention_bytes(dev: int, num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_q_len: int, max_seq_len: int) -> int:
-    with torch.cuda.device(dev):  # (the GPU's number of CUs sizes the partial sums)
-        return _lib.load().rq_kv16_attention_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_len, max_seq_len)
 
 
 def kv16_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -41,43 +30,4 @@ def kv16_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     workspace: scratch (rq_kv16_attention_workspace_bytes bytes), by default of this call from torch's allocator; a graph
     captured without torch's graph classes needs it, since nothing else keeps the scratch for its replays.
     """
-    shape, dtype, H = q.shape, q.dtype, k_cache.shape[2] if k_cache.dim() == 4 else 0
-    if len(shape) != 3 or H < 1 or shape[1] % H or k_cache.dtype is not dtype:
-        raise ValueError(f"q must be (tokens, a multiple of the pages' heads, head_dim) of the pages' dtype, got {tuple(shape)} of {dtype}")
-    dev = _device_index(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, workspace)
-    T, HQ, D = shape
-    pages = _check_pages(k_cache, v_cache, H, D)
-    BS = pages[1]
-    bt = _index(block_table, "block_table", torch.int32, 2)
-    sl = _index(seq_lens, "seq_lens", torch.int32, 1)
-    B, (tables, max_blocks) = sl.numel(), bt.shape
-    if tables != B:
-        raise ValueError("block_table and seq_lens differ in the number of sequences")
-    cu = None
-    if cu_seqlens_q is None:
-        if T != B:
-            raise ValueError(f"{T} query tokens and {B} sequences: cu_seqlens_q is needed")
-        max_q_len = 1
-    else:
-        cu = _index(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
-        if cu.numel() != B + 1:
-            raise ValueError(f"cu_seqlens_q must have {B + 1} entries, got {cu.numel()}")
-        max_q_len = T if max_q_len is None else min(int(max_q_len), T)
-    qs = q.stride()
-    if qs[2] != 1:
-        q = q.contiguous()
-        qs = q.stride()
-    out = torch.empty(shape, dtype=dtype, device=q.device) if out is None else out
-    os = out.stride()
-    if out.shape != shape or out.dtype is not dtype or os[2] != 1:
-        raise ValueError("out must have q's shape and dtype and be contiguous over head_dim")
-    if T == 1 or HQ == 1:
-        qs, os = _row_strides(shape, qs), _row_strides(shape, os)
-    capacity = max_blocks * BS
-    max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
-    keep, ws, ws_bytes = _scratch(workspace, _attention_bytes(dev, B, HQ, H, D, max_q_len, max_seq_len), q)
-    _call(_lib.load().rq_kv16_attention, "rq_kv16_attention", dev,
-          (q.data_ptr(), _lib.dtype_code(dtype), T, HQ, qs[0], qs[1], None if cu is None else cu.data_ptr(), B, max_q_len, 1 if causal else 0,
-           k_cache.data_ptr(), v_cache.data_ptr(), *pages, H, D, bt.data_ptr(), max_blocks, bt.stride(0), sl.data_ptr(), max_seq_len,
-           1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), out.data_ptr(), os[0], os[1], ws, ws_bytes))
-    return out
+    return _lib.ops().kv16_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale, causal, cu_seqlens_q, max_q_len, max_seq_len, out, workspace)

@@ -1,14 +1,11 @@
 """Position rotation and 16-bit pages without a GPU: refusals of the C entry points, sizes of scratch, the plain implementations."""
-import contextlib
 import math
-from types import SimpleNamespace
 
 import pytest
 import torch
 
 import kv16_testlib as P
 from rotorquant_vllm import _lib
-from rotorquant_vllm.kernels import kv16
 
 A = 1 << 20  # an address that is only looked at
 
@@ -91,26 +88,6 @@ def test_attention_without_work_or_scratch():
     assert need > 0 and size(2, 8, 2, 128, 9, 9000) > need and size(2, 8, 2, 128, 1, 1 << 60) >= need
     rc, message = call("rq_kv16_attention", ATTENTION, max_seq_len=9000, max_blocks=1000)
     assert rc == 2 and f"{need} bytes" in message
-
-
-def test_scratch_is_sized_for_the_tensors_device(monkeypatch):
-    current, cus = [0], [64, 256]
-
-    @contextlib.contextmanager
-    def device(dev):
-        before, current[0] = current[0], dev
-        yield
-        current[0] = before
-
-    monkeypatch.setattr(kv16._lib, "load", lambda: SimpleNamespace(rq_kv16_attention_workspace_bytes=lambda *sizes: cus[current[0]] * 1000))
-    monkeypatch.setattr(torch.cuda, "device", device)
-    kv16._attention_bytes.cache_clear()
-    try:
-        for dev in (1, 0, 1, 0):
-            assert kv16._attention_bytes(dev, 4, 32, 8, 128, 1, 9000) == cus[dev] * 1000
-        assert current == [0]
-    finally:
-        kv16._attention_bytes.cache_clear()
 
 
 def test_cpu_tensors_are_refused():
