@@ -238,6 +238,17 @@ struct CompressRope<true> {
     unsigned store_blocks;
 };
 
+// What a thread loads of a row: 16 bytes, or a unit of a key that is turned by its angles on the way to LDS.
+template <int DT, bool ROPE>
+struct CompressPiece {
+    uint4 x;
+};
+template <int DT>
+struct CompressPiece<DT, true> {
+    Row8<DT> x, y;
+    RopeTurn turn;
+};
+
 // Four resident waves per SIMD (at most 128 VGPRs) measured fastest for rotation
 // blocks up to 4; 8x8 blocks keep their registers.
 constexpr int compress_waves_per_eu(int blk) { return blk <= 4 ? 4 : 1; }
@@ -301,8 +312,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
     cell_params(kbnd, nkb, sk, ck);
     cell_params(vbnd, nvb, sv, cv);
 
-    // Staging roles: 16-byte piece my_part of rows my_row + u * rpi.
-    const int C = row_bytes / 16;
+    // Staging roles: 16-byte piece my_part (ROPE: unit my_part, 16 dims) of rows my_row + u * rpi.
+    const int C = ROPE ? D / 16 : row_bytes / 16;
     const int rpi = kThreads / C;
     const int my_part = tid % C, my_row = tid / C;
     const int n_it = (kRows + rpi - 1) / rpi;
@@ -337,8 +348,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
         if (c.row0 + lane >= n_rows) return -1;
         return m.slot_mapping[t];
     };
+    // Position of that token (those outside the table as its end, which is outside, too).
+    auto position_of = [&](const Cursor &c) -> int32_t {
+        if constexpr (ROPE) {
+            if (c.row0 + lane >= n_rows) return -1;
+            const int64_t p = rope.rows.t.positions[c.tok0 + (c.rem0 + lane) / two_h];
+            return (int32_t)(p >= 0 && p < rope.rows.t.rows ? p : rope.rows.t.rows);
+        } else {
+            return -1;
+        }
+    };
     // Resolve the group's row addresses into buffer b (wave 0).
-    auto build_refs = [&](const Cursor &c, int64_t g, int b, int64_t sid) {
+    auto build_refs = [&](const Cursor &c, int64_t g, int b, int64_t sid, int32_t position) {
         const int64_t r = g * kRows + lane;
         RowRef ref{nullptr, nullptr, nullptr, 0, -1};
         bool first = false;
@@ -366,12 +387,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
                     ref.norm_dst = reinterpret_cast<float *>(base + (is_v ? L.v_norm : L.k_norm) + 4 * h);
                 }
                 ref.is_v = is_v;
-                if constexpr (ROPE) {  // (those outside the table as its end, which is outside, too)
-                    if (!is_v) {
-                        const int64_t p = rope.rows.t.positions[t];
-                        ref.position = (int32_t)(p >= 0 && p < rope.rows.t.rows ? p : rope.rows.t.rows);
-                    }
-                }
+                if (ROPE && !is_v) ref.position = position;
                 first = rem == 0;
                 pad_j = j - (c.rem0 != 0);
             }
@@ -384,42 +400,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
         }
     };
     // Batch 0 of a group's rows into registers (the rest, if any, is loaded in place).
-    auto load_batch0 = [&](int b, uint4 (&v)[4]) {
+    constexpr int kBatch = ROPE ? 2 : 4;
+    CompressPiece<DT, ROPE> v[kBatch];
+    auto load_piece = [&](const RowRef &ref) {
+        CompressPiece<DT, ROPE> w{};
+        if constexpr (ROPE) {
+            const RopeUnit u(rope.rows.t, my_part);
+            if (ref.src != nullptr) {
+                w.x = row8_load<DT>(ref.src, 8 * u.p0);
+                w.y = row8_load<DT>(ref.src, 8 * u.p1);
+                if (ref.position >= 0 && u.turned) w.turn = rope_unit_turn<DT>(rope.rows.t, ref.position, u);
+            }
+        } else {
+            if (ref.src != nullptr) w.x = *gbl(reinterpret_cast<const uint4 *>(ref.src + my_part * 16));
+        }
+        return w;
+    };
+    auto load_batch0 = [&](int b) {
         const RowRef *refs = refs_all + b * kRows;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kBatch; ++u) {
             const int rr = my_row + u * rpi;
-            v[u] = make_uint4(0, 0, 0, 0);
-            if (my_row < rpi && u < n_it && rr < kRows) {
-                const uint8_t *src = refs[rr].src;
-                if (src != nullptr) v[u] = *gbl(reinterpret_cast<const uint4 *>(src + my_part * 16));
-            }
+            if (my_row < rpi && u < n_it && rr < kRows) v[u] = load_piece(refs[rr]);
         }
     };
-
     // A piece as loaded, to its place in the group's rows.
-    auto stage = [&](int rr, const RowRef &ref, const uint4 &w) {
+    auto stage = [&](int rr, const RowRef &ref, const CompressPiece<DT, ROPE> &w) {
         if constexpr (ROPE) {
-            constexpr int kElems = 16 / EB;  // of a piece: 8, or 4 of fp32
-            float x[kElems];
-            if constexpr (EB == 2) row8_floats<DT>(Row8<DT>{{u32x4{w.x, w.y, w.z, w.w}}}, x);
-            else x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
-            if (ref.position >= 0 && kElems * my_part < rope.rows.t.rot) rope_elems<DT, kElems>(rope.rows.t, ref.src, ref.position, kElems * my_part, x);
-            float4 *to = reinterpret_cast<float4 *>(rows + rr * pitch + my_part * (4 * kElems));
-#pragma unroll
-            for (int i = 0; i < kElems / 4; ++i) to[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            const RopeUnit u(rope.rows.t, my_part);
+            float x[8], y[8];
+            row8_floats<DT>(w.x, x);
+            row8_floats<DT>(w.y, y);
+            if (ref.position >= 0 && u.turned) rope_unit(x, y, w.turn, rope.rows.t.halves);
+            float4 *const tx = reinterpret_cast<float4 *>(rows + rr * pitch + 32 * u.p0), *const ty = reinterpret_cast<float4 *>(rows + rr * pitch + 32 * u.p1);
+            tx[0] = make_float4(x[0], x[1], x[2], x[3]), tx[1] = make_float4(x[4], x[5], x[6], x[7]);
+            ty[0] = make_float4(y[0], y[1], y[2], y[3]), ty[1] = make_float4(y[4], y[5], y[6], y[7]);
         } else {
-            *reinterpret_cast<uint4 *>(rows + rr * pitch + my_part * 16) = w;
+            *reinterpret_cast<uint4 *>(rows + rr * pitch + my_part * 16) = w.x;
         }
     };
 
     int64_t g = blockIdx.x;
     int64_t sid_next = -1;
+    int32_t position_next = -1;
     // ---- prologue: first group's addresses; boundary cells -----------------
     if (wave == 0) {
         const int64_t sid = m.store ? slot_id(cur) : -1;
-        if (m.store && g + gstride < n_groups) sid_next = slot_id(advance(cur));
-        build_refs(cur, g, 0, sid);
+        const int32_t position = position_of(cur);
+        if (m.store && g + gstride < n_groups) sid_next = slot_id(advance(cur)), position_next = position_of(advance(cur));
+        build_refs(cur, g, 0, sid, position);
     } else if (wave == 1) {
         // lanes 0-15: K boundaries, lanes 32-47: V boundaries
         const int kind = lane >> 5, i = lane & 31;
@@ -443,8 +472,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
         if (lane == 0) misc[2] = all_ok;
     }
     __syncthreads();
-    uint4 v[4];
-    load_batch0(0, v);
+    load_batch0(0);
     for (int e = tid; e < 2 * kCells; e += kThreads) {
         // table entry {boundary, count} of cell c for both sets
         const int kind = e / kCells, c = e % kCells;
@@ -460,19 +488,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
         const bool has_next = gn < n_groups;
         // ---- (a) rows of g into LDS; slot padding; next group's addresses ----
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kBatch; ++u) {
             const int rr = my_row + u * rpi;
-            if (my_row < rpi && u < n_it && rr < kRows)
-                stage(rr, refs[rr], v[u]);
+            if (my_row < rpi && u < n_it && rr < kRows) stage(rr, refs[rr], v[u]);
         }
-        for (int u = 4; u < n_it; ++u) {
+        for (int u = kBatch; u < n_it; ++u) {
             const int rr = my_row + u * rpi;
-            if (my_row < rpi && rr < kRows) {
-                const uint8_t *src = refs[rr].src;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (src != nullptr) w = *gbl(reinterpret_cast<const uint4 *>(src + my_part * 16));
-                stage(rr, refs[rr], w);
-            }
+            if (my_row < rpi && rr < kRows) stage(rr, refs[rr], load_piece(refs[rr]));
         }
         if (m.store) {
             const int pay = SlotLayout(m.H, D, m.dense3 != 0).payload;
@@ -498,13 +520,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
         if (wave == 0 && has_next) {
             const Cursor cn = m.store ? advance(cur) : cur;
             const int64_t sid = sid_next;
-            if (m.store && gn + gstride < n_groups) sid_next = slot_id(advance(cn));
-            build_refs(cn, gn, buf ^ 1, sid);
+            const int32_t position = position_next;
+            if (m.store && gn + gstride < n_groups) sid_next = slot_id(advance(cn)), position_next = position_of(advance(cn));
+            build_refs(cn, gn, buf ^ 1, sid, position);
             cur = cn;
         }
         __syncthreads();
         // ---- (b) next group's rows in flight while this one is processed -----
-        if (has_next) load_batch0(buf ^ 1, v);
+        if (has_next) load_batch0(buf ^ 1);
 
         // ---- (c) norms, four lanes per row ------------------------------------
         // lane q of a row accumulates s_{2q} and s_{2q+1}; lane 0 adds s_0..s_7 in order

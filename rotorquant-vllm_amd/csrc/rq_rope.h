@@ -23,14 +23,10 @@ struct RopeTable {
     int rot, halves, f32;  // rotated dims; kind of pairs; table of fp32 (else of the rows' type)
 };
 
-// N (2, 4 or 8) consecutive numbers of a table row.
+// N (4 or 8) consecutive numbers of a table row.
 template <int DT, int N>
 __device__ __forceinline__ void rope_angles(const RopeTable &t, int64_t at, float *x) {
-    if constexpr (N == 2) {  // (of fp32 rows, whose tables are fp32)
-        static_assert(DT == RQ_DTYPE_F32, "");
-        const float2 w = *reinterpret_cast<const float2 *>(static_cast<const float *>(t.table) + at);
-        x[0] = w.x, x[1] = w.y;
-    } else if (DT == RQ_DTYPE_F32 || t.f32) {
+    if (DT == RQ_DTYPE_F32 || t.f32) {
         const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(t.table) + at);
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) x[4 * i] = p[i].x, x[4 * i + 1] = p[i].y, x[4 * i + 2] = p[i].z, x[4 * i + 3] = p[i].w;
@@ -78,15 +74,6 @@ __device__ __forceinline__ float rope_sum(float a, float c, float b, float s) {
     const float x = a * c, y = b * s;
     return x + y;
 }
-// Turns a pair of pieces with halves (x: the first half's), one with the other.
-__device__ __forceinline__ void rope_halves(float (&x)[8], float (&y)[8], const RopeTurn &r) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = x[i], b = y[i];
-        x[i] = rope_diff(a, r.c[i], b, r.s[i]);
-        y[i] = rope_sum(b, r.c[i], a, r.s[i]);
-    }
-}
 // Turns one piece: its partners' values with halves (lower: of the first half), else its own pairs.
 __device__ __forceinline__ void rope_piece(float (&x)[8], const float (&partner)[8], const RopeTurn &r, bool halves, bool lower) {
     if (halves) {
@@ -102,40 +89,55 @@ __device__ __forceinline__ void rope_piece(float (&x)[8], const float (&partner)
     }
 }
 
-// Dims at .. at + N - 1 (N 8, or 4 of fp32; at < rot) of the row that begins at `row`, turned.
-template <int DT, int N>
-__device__ __forceinline__ void rope_elems(const RopeTable &t, const uint8_t *row, int64_t position, int at, float (&x)[N]) {
-    const int half = t.rot >> 1;
-    const bool in = position >= 0 && position < t.rows, lower = at < half;
-    const int64_t tr = (in ? position : 0) * t.stride;
-    float c[N], s[N], y[N];
+// A row is worked on in units of two pieces: with halves two that are partners, else two that are as far apart; past the rotated dims two
+// that pass.  A row of D dims has D / 16 units.
+struct RopeUnit {
+    int p0, p1;
+    bool turned;
+    __device__ __forceinline__ RopeUnit(const RopeTable &t, int unit) {
+        const int hp = t.rot >> 4;
+        turned = unit < hp;
+        p0 = turned ? unit : 2 * unit, p1 = turned ? unit + hp : 2 * unit + 1;
+    }
+};
+// The angles of a unit that is turned: eight of its pairs with halves, else four of each piece.
+template <int DT>
+__device__ __forceinline__ RopeTurn rope_unit_turn(const RopeTable &t, int64_t position, const RopeUnit &u) {
+    RopeTurn r;
+    const bool in = position >= 0 && position < t.rows;
+    const int64_t row = (in ? position : 0) * t.stride, half = t.rot >> 1;
     if (t.halves) {
-        const int i = lower ? at : at - half;
-        rope_angles<DT, N>(t, tr + i, c);
-        rope_angles<DT, N>(t, tr + half + i, s);
-        const uint8_t *p = row + (lower ? at + half : at - half) * (DT == RQ_DTYPE_F32 ? 4 : 2);
-        if constexpr (N == 8) {
-            row8_floats<DT>(row8_load<DT>(p, 0), y);
-        } else {
-            const float4 w = *reinterpret_cast<const float4 *>(p);
-            y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+        rope_angles<DT, 8>(t, row + 8 * u.p0, r.c);
+        rope_angles<DT, 8>(t, row + half + 8 * u.p0, r.s);
+    } else {
+        rope_angles<DT, 4>(t, row + 4 * u.p0, r.c);
+        rope_angles<DT, 4>(t, row + 4 * u.p1, r.c + 4);
+        rope_angles<DT, 4>(t, row + half + 4 * u.p0, r.s);
+        rope_angles<DT, 4>(t, row + half + 4 * u.p1, r.s + 4);
+    }
+    if (!in) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.c[i] = r.s[i] = __builtin_nanf("");
+    }
+    return r;
+}
+__device__ __forceinline__ void rope_unit(float (&x)[8], float (&y)[8], const RopeTurn &r, bool halves) {
+    if (halves) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = x[i], b = y[i];
+            x[i] = rope_diff(a, r.c[i], b, r.s[i]);
+            y[i] = rope_sum(b, r.c[i], a, r.s[i]);
         }
     } else {
-        rope_angles<DT, N / 2>(t, tr + at / 2, c);
-        rope_angles<DT, N / 2>(t, tr + half + at / 2, s);
-    }
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (!in) c[i] = s[i] = __builtin_nanf("");
-    if (t.halves) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = lower ? rope_diff(x[i], c[i], y[i], s[i]) : rope_sum(x[i], c[i], y[i], s[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = rope_diff(a, c[i], b, s[i]);
-            x[2 * i + 1] = rope_sum(b, c[i], a, s[i]);
+        for (int i = 0; i < 4; ++i) {
+            float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = rope_diff(a, r.c[i], b, r.s[i]);
+            x[2 * i + 1] = rope_sum(b, r.c[i], a, r.s[i]);
+            a = y[2 * i], b = y[2 * i + 1];
+            y[2 * i] = rope_diff(a, r.c[4 + i], b, r.s[4 + i]);
+            y[2 * i + 1] = rope_sum(b, r.c[4 + i], a, r.s[4 + i]);
         }
     }
 }
@@ -158,7 +160,7 @@ struct RopeRows {
 };
 constexpr int kRopeThreads = 256;
 
-// A thread takes two pieces (with halves a pair of partners) of up to kRopeShare rows of one token: the rows share the
+// A thread takes a unit of up to kRopeShare rows of one token: the rows share the
 // token's angles, and their loads are on their way together.
 constexpr int kRopeShare = 2;
 __host__ __device__ __forceinline__ int64_t rope_threads(const RopeRows &a) {
@@ -173,10 +175,7 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
     const uint32_t at = (uint32_t)thread / (uint32_t)units, u = (uint32_t)thread - at * units;
     const uint32_t tok = at / (uint32_t)shared, r0 = at - tok * shared;
     const int64_t token = tok;
-    const int hp = a.t.rot >> 4;
-    const bool turned = (int)u < hp;
-    // pieces u and u + rot / 16, or two of those that pass
-    const int p0 = turned ? (int)u : 2 * (int)u, p1 = turned ? (int)u + hp : 2 * (int)u + 1;
+    const RopeUnit unit(a.t, (int)u);
     const int64_t position = a.t.positions[token];
     int64_t page = -1, in_page = 0;
     if (a.n_kv > 0) {
@@ -195,7 +194,7 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
         const int r = (int)r0 + i * shared;
         const void *from = nullptr;
         int64_t src = 0, dst = 0;
-        to[i] = nullptr, turn[i] = turned;
+        to[i] = nullptr, turn[i] = unit.turned;
         if (r < a.n_q) {
             from = a.q, src = token * a.q_st + r * a.q_sh;
             to[i] = a.out, dst = token * a.o_st + r * a.o_sh;
@@ -206,18 +205,15 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
             src = is_v ? token * a.v_st + h * a.v_sh : token * a.k_st + h * a.k_sh;
             to[i] = is_v ? a.v_cache : a.k_cache;
             dst = is_v ? page * a.vc_sb + in_page * a.vc_ss + h * a.vc_sh : page * a.kc_sb + in_page * a.kc_ss + h * a.kc_sh;
-            turn[i] = turned && !is_v;
+            turn[i] = unit.turned && !is_v;
         }
         if (to[i] == nullptr) continue;
-        x0[i] = row8_load<DT>(from, src + 8 * p0);
-        x1[i] = row8_load<DT>(from, src + 8 * p1);
+        x0[i] = row8_load<DT>(from, src + 8 * unit.p0);
+        x1[i] = row8_load<DT>(from, src + 8 * unit.p1);
         to[i] = static_cast<uint8_t *>(to[i]) + dst * (DT == RQ_DTYPE_F32 ? 4 : 2);
     }
-    RopeTurn t0, t1;
-    if (turned) {
-        t0 = rope_turn<DT>(a.t, position, p0);
-        if (!a.t.halves) t1 = rope_turn<DT>(a.t, position, p1);
-    }
+    RopeTurn t;
+    if (unit.turned) t = rope_unit_turn<DT>(a.t, position, unit);
 #pragma unroll
     for (int i = 0; i < kRopeShare; ++i) {
         if (to[i] == nullptr) continue;
@@ -225,17 +221,12 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
             float f0[8], f1[8];
             row8_floats<DT>(x0[i], f0);
             row8_floats<DT>(x1[i], f1);
-            if (a.t.halves) {
-                rope_halves(f0, f1, t0);
-            } else {
-                rope_piece(f0, f0, t0, false, false);
-                rope_piece(f1, f1, t1, false, false);
-            }
+            rope_unit(f0, f1, t, a.t.halves);
             x0[i] = row8_round<DT>(f0);
             x1[i] = row8_round<DT>(f1);
         }
-        row8_store<DT>(to[i], 8 * p0, x0[i]);
-        row8_store<DT>(to[i], 8 * p1, x1[i]);
+        row8_store<DT>(to[i], 8 * unit.p0, x0[i]);
+        row8_store<DT>(to[i], 8 * unit.p1, x1[i]);
     }
 }
 
