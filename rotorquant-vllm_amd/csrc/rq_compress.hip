@@ -431,7 +431,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
             float x[8], y[8];
             row8_floats<DT>(w.x, x);
             row8_floats<DT>(w.y, y);
-            if (ref.position >= 0 && u.turned) rope_unit(x, y, w.turn, rope.rows.t.halves);
+            if (ref.position >= 0 && u.turned) rope_unit(x, y, w.turn, rope.rows.t.halves, u);
             float4 *const tx = reinterpret_cast<float4 *>(rows + rr * pitch + 32 * u.p0), *const ty = reinterpret_cast<float4 *>(rows + rr * pitch + 32 * u.p1);
             tx[0] = make_float4(x[0], x[1], x[2], x[3]), tx[1] = make_float4(x[4], x[5], x[6], x[7]);
             ty[0] = make_float4(y[0], y[1], y[2], y[3]), ty[1] = make_float4(y[4], y[5], y[6], y[7]);

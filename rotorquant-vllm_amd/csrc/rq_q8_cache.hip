@@ -117,24 +117,27 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
     return true;
 }
 
-// What a store with position rotation is given beside Q8StoreArgs.
-template <bool ROPE>
-struct Q8Rope {};
-template <>
-struct Q8Rope<true> {
+// Position rotation of the keys.  kQ8Units: a lane loads pieces that are head_dim / 16 apart, in pairs whose angles it holds for all the heads of
+// its wave: every rotation but halves of a part of the dims.  Those are kQ8Pieces: a piece's partner is loaded beside it.
+enum { kQ8Plain, kQ8Units, kQ8Pieces };
+template <int ROPE>
+struct Q8Rope {
     RopeRows rows;          // the queries of a short call, by workgroups of their own behind those that store
     unsigned store_blocks;
 };
-// Piece `piece` (8 dims) of a key row at element `at` of a.key, turned by its token's position.
+template <>
+struct Q8Rope<kQ8Plain> {};
+// Piece `piece` (8 dims) of a key row at element `at` of a.key, turned by its token's position (kQ8Pieces).
 template <int DT>
 __device__ __forceinline__ void q8_turn(const RopeTable &t, const void *key, int64_t at, int64_t position, int piece, float (&x)[8]) {
     const int hp = t.rot >> 4;
     if (piece >= 2 * hp) return;
-    const RopeTurn r = rope_turn<DT>(t, position, piece);
     const bool lower = piece < hp;
+    const RopeTurn r = rope_unit_turn<DT>(t, position, RopeUnit(t, lower ? piece : piece - hp));
     float y[8];
-    if (t.halves) row8_floats<DT>(row8_load<DT>(key, at + 8 * (lower ? hp : -hp)), y);
-    rope_piece(x, y, r, t.halves, lower);
+    row8_floats<DT>(row8_load<DT>(key, at + 8 * (lower ? hp : -hp)), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = lower ? rope_diff(x[i], r.c[i], y[i], r.s[i]) : rope_sum(x[i], r.c[i], y[i], r.s[i]);
 }
 
 // A wave takes a.per_wave units of one group, the next one's rows on their way while one is coded.  Lane: token row
@@ -142,10 +145,10 @@ __device__ __forceinline__ void q8_turn(const RopeTable &t, const void *key, int
 // (D = 128) or the V side (D = 64).
 // Bound by memory: 32768 tokens of 8 heads (134 MB in, 67 out) in 47 us beside 10 for the two link launches (graph replays of all three: 48).  Non-temporal loads
 // here: 56 us (a row's 128 bytes are loaded by four instructions, which then miss the L1).
-template <int DT, int FMT, int D, bool LINKED, bool ROPE>
+template <int DT, int FMT, int D, bool LINKED, int ROPE>
 __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs a, Q8Rope<ROPE> rope) {
     unsigned blocks = gridDim.x;
-    if constexpr (ROPE) {
+    if constexpr (ROPE != kQ8Plain) {
         blocks = rope.store_blocks;
         if (blockIdx.x >= blocks) {
             rope_rows<DT>(rope.rows, (int64_t)(blockIdx.x - blocks) * kRopeThreads + threadIdx.x);
@@ -174,8 +177,18 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
         if (!q8_find_rows<LINKED>(a, t0, g, rows, lane)) continue;
         const int tok = rows[t];
         int64_t position = 0;
-        if constexpr (ROPE) {
+        if constexpr (ROPE != kQ8Plain) {
             if (tok >= 0) position = rope.rows.t.positions[tok];
+        }
+        // kQ8Units: pieces pair_at(0) and pair_at(1), and those kPair further on
+        constexpr int kPair = D / 16;
+        auto pair_at = [&](int j) { return half + 2 * j + (D == 128 ? 4 * (lane >> 5) : 0); };
+        auto pair = [&](const RopeTable &t, int j) { return RopeUnit(t, pair_at(j), pair_at(j) + kPair); };
+        RopeTurn turn[2];
+        if constexpr (ROPE == kQ8Units) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (tok >= 0 && (D == 128 || lane < 32) && pair(rope.rows.t, j).turned) turn[j] = rope_unit_turn<DT>(rope.rows.t, position, pair(rope.rows.t, j));
         }
         const bool anew = rows[0] >= 0;
         const uint64_t written = __ballot(tok >= 0);
@@ -193,8 +206,11 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
             old_next = *scale_at(unit);
             const int64_t at = (int64_t)tok * (side ? a.v_st : a.k_st) + (int64_t)h * (side ? a.v_sh : a.k_sh) + 64 * chunk + 8 * half;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (tok >= 0) raw[i] = row8_load<DT>(side ? a.value : a.key, at + 16 * i);
+            for (int i = 0; i < 4; ++i) {
+                int64_t from = at + 16 * i;
+                if (ROPE == kQ8Units && D == 128 && side == 0) from += 8 * (pair_at(i & 1) + kPair * (i >> 1)) - (64 * chunk + 8 * half + 16 * i);
+                if (tok >= 0) raw[i] = row8_load<DT>(side ? a.value : a.key, from);
+            }
         };
         load(first);
         for (int unit = first; unit < end; ++unit) {
@@ -206,11 +222,30 @@ __global__ __launch_bounds__(64 * kStoreWaves) void q8_store_kernel(Q8StoreArgs 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 row8_floats<DT>(raw[i], x[i]);
-                if constexpr (ROPE) {
+                if constexpr (ROPE == kQ8Pieces) {
                     if (side == 0 && tok >= 0)
                         q8_turn<DT>(rope.rows.t, a.key, (int64_t)tok * a.k_st + (int64_t)h * a.k_sh + 64 * chunk + 16 * i + 8 * half, position,
                                     8 * chunk + 2 * i + half, x[i]);
                 }
+            }
+            if constexpr (ROPE == kQ8Units) {
+                if (side == 0) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const RopeUnit u = pair(rope.rows.t, j);
+                        if (tok >= 0 && u.turned) rope_unit(x[j], x[j + 2], turn[j], rope.rows.t.halves, u);
+                        if constexpr (D == 128) {  // each half of the wave to its 64-dim chunk
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[j][k]), __float_as_uint(x[j + 2][k]), false, false);
+                                x[j][k] = __uint_as_float(r[0]), x[j + 2][k] = __uint_as_float(r[1]);
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     if (tok < 0) x[i][k] = 0.f;
@@ -398,11 +433,17 @@ __global__ __launch_bounds__(64 * kReadWaves) void q8_read_kernel(Q8ReadArgs a) 
 // alone, 8 heads, one / two / four units: 1024 tokens 9.7 / 10.7 / 13.5 us, 4096: 14.4 / 14.5 / 15.8, 8192 (just under the border):
 // 20.1 / 19.3 / 19.1, 32768: 54.0 / 48.3 / 49.5.
 static int q8_per_wave(int64_t groups, int units) { return groups * units >= 48 * (int64_t)device_cus() ? 2 : 1; }
+// With rotation a wave loads angles for all its units, and has more registers.  The three launches, 8 heads, one / two / four units: 2048 tokens
+// 14.9 / 15.1 / 17.2 us, 4096: 19.7 / 17.0 / 17.9, 8192: 27.7 / 24.5 / 21.7, 32768: 88.8 / 68.0 / 62.8;  heads of 64 (K and V a unit), 10507: 21.9 / 21.3 / 23.2.
+static int q8_per_wave_rope(int64_t groups, int units) {
+    const int64_t n = groups * units / device_cus();
+    return n >= 24 ? 4 : n >= 12 ? 2 : 1;
+}
 
-template <int DT, int FMT, int D, bool ROPE>
+template <int DT, int FMT, int D, int ROPE>
 static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStream_t st) {
     const int units = (D == 128 ? 2 : 1) * a.H;
-    a.per_wave = linked ? q8_per_wave(a.n_tokens / kQ8Group, units) : 1;
+    a.per_wave = !linked ? 1 : ROPE != kQ8Plain ? q8_per_wave_rope(a.n_tokens / kQ8Group, units) : q8_per_wave(a.n_tokens / kQ8Group, units);
     int64_t blocks = (a.n_tokens * ((units + a.per_wave - 1) / a.per_wave) + kStoreWaves - 1) / kStoreWaves;
     if (linked) {
         const dim3 tb((unsigned)((a.n_tokens + kLinkThreads - 1) / kLinkThreads));
@@ -411,7 +452,7 @@ static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStrea
         blocks = std::min<int64_t>(blocks, 8 * device_cus());
     }
     int64_t grid = blocks;
-    if constexpr (ROPE) {
+    if constexpr (ROPE != kQ8Plain) {
         rope.store_blocks = (unsigned)blocks;
         if (linked) launch_rope_rows<DT>(rope.rows, st);
         else grid += rope_blocks(rope.rows);
@@ -419,11 +460,11 @@ static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStrea
     if (linked) hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);
     else hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, false, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);
 }
-template <int DT, int FMT, bool ROPE>
+template <int DT, int FMT, int ROPE>
 static void launch_store_d(const Q8StoreArgs &a, const Q8Rope<ROPE> &rope, int D, bool linked, hipStream_t st) {
     D == 128 ? launch_store<DT, FMT, 128, ROPE>(a, rope, linked, st) : launch_store<DT, FMT, 64, ROPE>(a, rope, linked, st);
 }
-template <int DT, bool ROPE>
+template <int DT, int ROPE>
 static void launch_store_f(const Q8StoreArgs &a, const Q8Rope<ROPE> &rope, int fmt, int D, bool linked, hipStream_t st) {
     fmt == RQ_Q8_INT8 ? launch_store_d<DT, RQ_Q8_INT8, ROPE>(a, rope, D, linked, st) : launch_store_d<DT, RQ_Q8_E4M3, ROPE>(a, rope, D, linked, st);
 }
@@ -500,8 +541,9 @@ static int q8_store(const void *key, const void *value, int32_t dtype, int64_t n
     }
     auto launch = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (rope) launch_store_f<DT, true>(a, Q8Rope<true>{*rope, 0}, format, head_dim, need > 0, st);
-        else launch_store_f<DT, false>(a, Q8Rope<false>{}, format, head_dim, need > 0, st);
+        if (!rope) launch_store_f<DT, kQ8Plain>(a, {}, format, head_dim, need > 0, st);
+        else if (rope->t.halves && rope->t.rot < head_dim) launch_store_f<DT, kQ8Pieces>(a, {*rope, 0}, format, head_dim, need > 0, st);
+        else launch_store_f<DT, kQ8Units>(a, {*rope, 0}, format, head_dim, need > 0, st);
     };
     if (dtype == RQ_DTYPE_F16) launch(std::integral_constant<int, RQ_DTYPE_F16>{});
     else if (dtype == RQ_DTYPE_BF16) launch(std::integral_constant<int, RQ_DTYPE_BF16>{});

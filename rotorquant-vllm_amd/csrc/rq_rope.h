@@ -40,29 +40,10 @@ __device__ __forceinline__ void rope_angles(const RopeTable &t, int64_t at, floa
     }
 }
 
-// Cosines and sines of a piece (dims 8 piece ..; piece < rot / 8): eight of each with halves, else four.
+// Cosines and sines: of eight pairs, or of four and four.
 struct RopeTurn {
     float c[8], s[8];
 };
-template <int DT>
-__device__ __forceinline__ RopeTurn rope_turn(const RopeTable &t, int64_t position, int piece) {
-    RopeTurn r;
-    const bool in = position >= 0 && position < t.rows;
-    const int64_t row = (in ? position : 0) * t.stride;
-    if (t.halves) {
-        const int hp = t.rot >> 4, at = 8 * (piece >= hp ? piece - hp : piece);
-        rope_angles<DT, 8>(t, row + at, r.c);
-        rope_angles<DT, 8>(t, row + (t.rot >> 1) + at, r.s);
-    } else {
-        rope_angles<DT, 4>(t, row + 4 * piece, r.c);
-        rope_angles<DT, 4>(t, row + (t.rot >> 1) + 4 * piece, r.s);
-    }
-    if (!in) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.c[i] = r.s[i] = __builtin_nanf("");
-    }
-    return r;
-}
 
 __device__ __forceinline__ float rope_diff(float a, float c, float b, float s) {
 #pragma clang fp contract(off)
@@ -74,31 +55,18 @@ __device__ __forceinline__ float rope_sum(float a, float c, float b, float s) {
     const float x = a * c, y = b * s;
     return x + y;
 }
-// Turns one piece: its partners' values with halves (lower: of the first half), else its own pairs.
-__device__ __forceinline__ void rope_piece(float (&x)[8], const float (&partner)[8], const RopeTurn &r, bool halves, bool lower) {
-    if (halves) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = lower ? rope_diff(x[i], r.c[i], partner[i], r.s[i]) : rope_sum(x[i], r.c[i], partner[i], r.s[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = rope_diff(a, r.c[i], b, r.s[i]);
-            x[2 * i + 1] = rope_sum(b, r.c[i], a, r.s[i]);
-        }
-    }
-}
-
 // A row is worked on in units of two pieces: with halves two that are partners, else two that are as far apart; past the rotated dims two
 // that pass.  A row of D dims has D / 16 units.
 struct RopeUnit {
     int p0, p1;
-    bool turned;
+    bool turned, also;  // either piece is (with halves both or none)
     __device__ __forceinline__ RopeUnit(const RopeTable &t, int unit) {
         const int hp = t.rot >> 4;
-        turned = unit < hp;
+        turned = also = unit < hp;
         p0 = turned ? unit : 2 * unit, p1 = turned ? unit + hp : 2 * unit + 1;
     }
+    // Pieces q0 and q1, partners where t is of halves.
+    __device__ __forceinline__ RopeUnit(const RopeTable &t, int q0, int q1) : p0(q0), p1(q1), turned(q0 < t.rot >> 3), also(q1 < t.rot >> 3) {}
 };
 // The angles of a unit that is turned: eight of its pairs with halves, else four of each piece.
 template <int DT>
@@ -111,9 +79,11 @@ __device__ __forceinline__ RopeTurn rope_unit_turn(const RopeTable &t, int64_t p
         rope_angles<DT, 8>(t, row + half + 8 * u.p0, r.s);
     } else {
         rope_angles<DT, 4>(t, row + 4 * u.p0, r.c);
-        rope_angles<DT, 4>(t, row + 4 * u.p1, r.c + 4);
         rope_angles<DT, 4>(t, row + half + 4 * u.p0, r.s);
-        rope_angles<DT, 4>(t, row + half + 4 * u.p1, r.s + 4);
+        if (u.also) {
+            rope_angles<DT, 4>(t, row + 4 * u.p1, r.c + 4);
+            rope_angles<DT, 4>(t, row + half + 4 * u.p1, r.s + 4);
+        }
     }
     if (!in) {
 #pragma unroll
@@ -121,7 +91,8 @@ __device__ __forceinline__ RopeTurn rope_unit_turn(const RopeTable &t, int64_t p
     }
     return r;
 }
-__device__ __forceinline__ void rope_unit(float (&x)[8], float (&y)[8], const RopeTurn &r, bool halves) {
+// Turns a unit that is turned.
+__device__ __forceinline__ void rope_unit(float (&x)[8], float (&y)[8], const RopeTurn &r, bool halves, const RopeUnit &u) {
     if (halves) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -135,6 +106,7 @@ __device__ __forceinline__ void rope_unit(float (&x)[8], float (&y)[8], const Ro
             float a = x[2 * i], b = x[2 * i + 1];
             x[2 * i] = rope_diff(a, r.c[i], b, r.s[i]);
             x[2 * i + 1] = rope_sum(b, r.c[i], a, r.s[i]);
+            if (!u.also) continue;
             a = y[2 * i], b = y[2 * i + 1];
             y[2 * i] = rope_diff(a, r.c[4 + i], b, r.s[4 + i]);
             y[2 * i + 1] = rope_sum(b, r.c[4 + i], a, r.s[4 + i]);
@@ -221,7 +193,7 @@ __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
             float f0[8], f1[8];
             row8_floats<DT>(x0[i], f0);
             row8_floats<DT>(x1[i], f1);
-            rope_unit(f0, f1, t, a.t.halves);
+            rope_unit(f0, f1, t, a.t.halves, unit);
             x0[i] = row8_round<DT>(f0);
             x1[i] = row8_round<DT>(f1);
         }
