@@ -18,9 +18,12 @@ librq_hip.so (include/rq_abi.h):
                          LDS, 16-bit MFMA; head_size 128; decodes), and for
                          longer queries rq_paged_prefill (the same arithmetic,
                          each tile decoded once); other head sizes
-                         rq_paged_decompress + device attention in fp32
+                         rq_paged_decompress, then rq_kv16_attention over the plain pages (short
+                         queries) or device attention in fp32
     8-bit cache       -> rq_q8_store, rq_q8_attention (RQ_CACHE_8BIT=int8 | fp8: another cache
                          layout, no rotation, no codebook; no counterpart in the reference)
+    rotary embedding  -> rq_rope_compress_store, rq_rope_q8_store (rope_and_store: queries and keys rotated by their
+                         positions on the way into the cache, for a model that leaves that to the layer)
 
 vLLM itself is imported lazily: without vLLM the module still imports (the
 classes then derive from small local stand-ins), which is how the tests run.
@@ -134,6 +137,9 @@ _paged_prefill_fn = None
 _unfused_decode_fn = None
 _q8_store_fn = None
 _q8_attention_fn = None
+_rope_compress_store_fn = None
+_rope_q8_store_fn = None
+_kv16_attention_fn = None
 _shared_workspace = None
 PREFILL_SPLIT_BYTES = 0
 try:
@@ -150,6 +156,9 @@ try:
     from rotorquant_vllm.kernels import PREFILL_SPLIT_BYTES
     from rotorquant_vllm.kernels import q8_attention as _q8_attention_fn
     from rotorquant_vllm.kernels import q8_store as _q8_store_fn
+    from rotorquant_vllm.kernels import kv16_attention as _kv16_attention_fn
+    from rotorquant_vllm.kernels import rope_compress_store as _rope_compress_store_fn
+    from rotorquant_vllm.kernels import rope_q8_store as _rope_q8_store_fn
 
     _rq_lib.load()
     _fused_paged_kernel_available = True
@@ -162,6 +171,11 @@ except (ImportError, OSError, RuntimeError) as exc:
 # short queries: neither needs host lengths); longer ones take rq_paged_prefill, which
 # decodes each tile once for all query blocks instead of once per block.
 RQ_UNFUSED_SHORT_Q = 16
+
+# Layers whose shape the non-fused kernels do not take: queries of at most this many (token, query head) pairs of a kv head
+# attend to the decompressed pages by kv16_attention, longer ones by device matmuls.  That reads the keys again for every 32 pairs.
+RQ_PLAIN_SHORT_COLUMNS = 64
+RQ_PLAIN_MAX_HEAD_DIM = 256
 
 # Shapes the fused kernels take (checked again by the C ABI): head_dim 128, a
 # GQA group of at most 16 query heads, at most 64 kv heads.
@@ -791,6 +805,28 @@ class RQAttentionImpl(_ImplBase):
         _compress_store_fn(key[:n], value[:n], kv_cache, slot_mapping, self._dev_rte, self._dev_rto,
                            self._dev_kb, self._dev_vb, rot_block=self._rq_rot_block, **self._layout_kw())
 
+    def rope_and_store(self, query, key, value, positions, cos_sin_cache, is_neox, kv_cache, slot_mapping, out_q=None):
+        """Rotary embedding and store in one launch: query (N, H_Q, D) and key (N, H, D) are rotated by positions (N,) and
+        key and value written to slot_mapping's slots of this layer's cache, codebook or 8-bit.  Returns the rotated queries of slot_mapping's tokens (out_q,
+        which may be query); forward() with them and key=None, value=None then attends.  cos_sin_cache and is_neox are a rotary
+        embedding's: (positions, rot_dim) cosines, then sines, fp32 or of the rows' dtype, and whether the pairs of dims are halves apart.  Keys
+        are not rounded between rotation and codes, so the cache's bytes are not always those of a rotation rounded to the model's dtype first."""
+        if self.attn_type in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
+            raise ValueError("rope_and_store: encoder layers have no cache")
+        n = slot_mapping.shape[0]
+        query, key, value, positions = query[:n], key[:n], value[:n], positions[:n]
+        if getattr(self, "_q8_format", None) is not None:
+            if _rope_q8_store_fn is None:
+                raise RuntimeError("RotorQuant HIP kernels are not available")
+            self._check_q8_dtype(key.dtype)
+            return _rope_q8_store_fn(query, key, value, positions, cos_sin_cache, kv_cache, slot_mapping, fmt=self._q8_format, neox=is_neox, out_q=out_q)
+        if _rope_compress_store_fn is None:
+            raise RuntimeError("RotorQuant HIP kernels are not available")
+        if not self._cg_buffers_ready:
+            self._init_cg_buffers(kv_cache, query.dtype)
+        return _rope_compress_store_fn(query, key, value, positions, cos_sin_cache, kv_cache, slot_mapping, self._dev_rte, self._dev_rto, self._dev_kb,
+                                       self._dev_vb, neox=is_neox, out_q=out_q, rot_block=self._rq_rot_block, **self._layout_kw())
+
     # -- fused paths -----------------------------------------------------------
 
     def _fused_decode(self, query, kv_cache, block_table, seq_lens, output, n, fn=None):
@@ -953,8 +989,9 @@ class RQAttentionImpl(_ImplBase):
         return output
 
     def _forward_unfused_torch(self, query, kv_cache, md, output, num_actual_tokens):
-        """Paged decompress + fp32 attention on the device, for shapes rq_paged_attention
-        does not take (head sizes other than 128, GQA groups above 16, fp32 models).
+        """Paged decompress + attention over the plain pages, for shapes rq_paged_attention
+        does not take (head sizes other than 128, GQA groups above 16, fp32 models).  The leading short queries of a
+        16-bit model (vLLM orders decodes first) go to kv16_attention in one call, the others to device matmuls in fp32.
 
         K/V of the referenced blocks are decompressed once (rq_paged_decompress) to
         the q dtype, as the reference's _decompress_cache_paged(..., query.dtype)
@@ -971,7 +1008,7 @@ class RQAttentionImpl(_ImplBase):
         HQ = q.shape[1]
         G = HQ // H
         causal = bool(getattr(md, "causal", True))
-        q_rot = (q.float() @ self._dev_R.T).to(q.dtype).float()
+        q_rot = (q.float() @ self._dev_R.T).to(q.dtype)
         qsl = getattr(md, "rq_query_start_loc_cpu", None)
         if qsl is None:
             qsl = getattr(md, "query_start_loc", None)
@@ -985,11 +1022,22 @@ class RQAttentionImpl(_ImplBase):
         k_cache, v_cache, bt, _ = _paged_decompress_fn(kv_cache, md.block_table, md.seq_lens, H, D, self._dev_kc,
                                                        self._dev_vc, q.dtype, out_k=out_k,
                                                        out_v=torch.empty_like(out_k), **self._layout_kw())
+        short = self._plain_short(q_rot, starts, lens)
+        if short:
+            cu = torch.tensor(starts[:short + 1], dtype=torch.int32, device=q.device)
+            most = max(b - a for a, b in zip(starts[:short], starts[1:]))
+            out_short = _kv16_attention_fn(q_rot[:starts[short]], k_cache, v_cache, bt[:short], md.seq_lens[:short].to(torch.int32), sm_scale=self.scale,
+                                           causal=causal, cu_seqlens_q=cu, max_q_len=most, max_seq_len=max(lens[:short]))
+            output[:starts[short]] = (out_short.float() @ self._dev_R).to(output.dtype)
+            if short == len(lens) and starts[short] == num_actual_tokens:
+                return output
+        q_rot = q_rot.float()
+        begin = starts[short] if short else 0
         out_rot = torch.zeros(num_actual_tokens, HQ, D, dtype=torch.float32, device=q.device)
         for b, L in enumerate(lens):
             s0, s1 = starts[b], starts[b + 1]
             T = s1 - s0
-            if T <= 0 or L == 0:
+            if b < short or T <= 0 or L == 0:
                 continue
             ids = bt[b, :(L + BS - 1) // BS].long()
             K = k_cache[ids].reshape(-1, H, D)[:L].float()
@@ -1007,9 +1055,20 @@ class RQAttentionImpl(_ImplBase):
                     S = S.view(r1 - r0, G, L).masked_fill_(masked[:, None, :], float("-inf"))
                     P = torch.softmax(S, dim=-1).view(-1, L)
                     out_rot[s0 + r0:s0 + r1, h * G:(h + 1) * G, :] = (P @ V[:, h, :]).view(r1 - r0, G, D)
-        out_rot = out_rot.to(q.dtype).float()
-        output[:num_actual_tokens] = (out_rot @ self._dev_R).to(output.dtype)
+        out_rot = out_rot[begin:].to(q.dtype).float()
+        output[begin:num_actual_tokens] = (out_rot @ self._dev_R).to(output.dtype)
         return output
+
+    def _plain_short(self, q, starts: list, lens: list) -> int:
+        """Leading sequences whose queries kv16_attention takes: those of a 16-bit model on the GPU with few (token, query head) pairs
+        of a kv head."""
+        if (_kv16_attention_fn is None or not q.is_cuda or q.dtype not in (torch.float16, torch.bfloat16) or self.head_size % 8
+                or self.head_size > RQ_PLAIN_MAX_HEAD_DIM or not lens or starts[0] != 0):
+            return 0
+        group, n = q.shape[1] // self.num_kv_heads, 0
+        while n < len(lens) and 0 <= (starts[n + 1] - starts[n]) * group <= max(RQ_PLAIN_SHORT_COLUMNS, group):
+            n += 1
+        return n if starts[n] > 0 else 0
 
     # -- forward -------------------------------------------------------------
 
