@@ -9,8 +9,8 @@
 //                 so that the output is as exact as with fp32 weights; the second product costs nothing beside the loads.
 // peak is 14 for fp16, whose small numbers end at 2^-24, and 0 for bf16.  out = O / l.
 //
-// Rows may lie anywhere (any page size and strides): lane l looks up where key l of two tiles is, a tile ahead, and lanes ask it by
-// bpermute.  K needs no more: a lane's 16 bytes are operand elements.  V is loaded by rows, 16 lanes to a row, and its operand
+// Rows may lie anywhere (any page size and strides): lane l looks up where key l % 32 of a tile is, a tile ahead, and lanes ask it
+// by bpermute.  K needs no more: a lane's 16 bytes are operand elements.  V is loaded by rows, 16 lanes to a row, and its operand
 // (two tokens of a dim in a dword) made by one byte permute a dword: dim 8 c + m of lane c is row c of product m.
 #include <algorithm>
 #include <type_traits>
@@ -315,10 +315,14 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
 // The tiles of all (sequence, block of columns) pairs in a row are cut into equal shares, and a share is taken by one workgroup for each kv
 // head: the heads of a token lie together in memory, and are read at about the same time.
 template <int NB>
-__device__ __forceinline__ int64_t kv16_seq_tiles(const Kv16Args &a, int64_t b) {
+__device__ __forceinline__ int64_t kv16_seq_tiles(const Kv16Args &a, int64_t b, AttnSeq &s) {
     if (b >= a.num_seqs) return 0;
-    const AttnSeq s = attn_seq(a, b);
+    s = attn_seq(a, b);
     return (int64_t)attn_tiles(s) * attn_col_blocks<NB>(a, s.T);
+}
+__device__ __forceinline__ AttnSeq seq_of_lane(const AttnSeq &s, int lane) {  // (in SGPRs)
+    return {__builtin_amdgcn_readlane(s.q0, lane), __builtin_amdgcn_readlane(s.T, lane), __builtin_amdgcn_readlane(s.pos, lane),
+            __builtin_amdgcn_readlane(s.vis, lane)};
 }
 // Place of share w's part of an item in the workspace: an item cut in two or more is the last of the share that begins it and the first of the others.
 template <int DP, int NB>
@@ -343,10 +347,11 @@ __global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kern
     auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };  // (what is the workgroup's, into SGPRs)
     const int lane = threadIdx.x & 63, hs = a.H / kHeads, shares = gridDim.x / (uint32_t)hs, w = blockIdx.x / (uint32_t)hs,
               h = (blockIdx.x - w * hs) * kHeads + (HEADS ? scalar(threadIdx.x >> 6) : 0);
-    int64_t block = 0, block_base = 0;  // 64 sequences: their tiles, and the row's up to each
-    int64_t mine = kv16_seq_tiles<NB>(a, lane), upto = wave_scan64(mine);
+    int64_t block = 0, block_base = 0;  // 64 sequences: a lane's, its tiles, and the row's up to it
+    AttnSeq own{}, other{};
+    int64_t mine = kv16_seq_tiles<NB>(a, lane, own), upto = wave_scan64(mine);
     int64_t total = lane64(upto, 63);
-    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(kv16_seq_tiles<NB>(a, b + lane)), 63);
+    for (int64_t b = 64; b < a.num_seqs; b += 64) total += lane64(wave_scan64(kv16_seq_tiles<NB>(a, b + lane, other)), 63);
     const int64_t share = kv16_share(total, shares);
     int64_t pos = w * share;
     const int64_t end = min(total, pos + share);
@@ -355,13 +360,13 @@ __global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kern
         while (hit == 0) {
             block_base += lane64(upto, 63);
             block += 64;
-            mine = kv16_seq_tiles<NB>(a, block + lane);
+            mine = kv16_seq_tiles<NB>(a, block + lane, own);
             upto = wave_scan64(mine);
             hit = __ballot(block_base + upto > pos);
         }
         const int of = __builtin_ctzll(hit);
         const int64_t seq = block + of, in_seq = pos - (block_base + lane64(upto, of) - lane64(mine, of));
-        const AttnSeq v = attn_seq(a, seq), s{scalar(v.q0), scalar(v.T), scalar(v.pos), scalar(v.vis)};
+        const AttnSeq s = seq_of_lane(own, of);
         const int n = attn_tiles(s), cols = scalar((int)div64(in_seq, n));
         const int t0 = scalar((int)(in_seq - (int64_t)cols * n)), t1 = scalar((int)min((int64_t)n, t0 + (end - pos)));
         float *part = t0 == 0 && t1 == n ? nullptr : kv16_part<DP, NB>(a, w, t0 == 0, h);
@@ -370,60 +375,67 @@ __global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kern
     }
 }
 
-// Adds up the parts of the items that were cut.  A wave takes one column; lane: D / 16 dims, and every fourth part, four of them on their way.
+// Adds up the parts of the items that were cut: `per` workgroups for a sequence and head.  A wave takes a column at a time; lane: D / 16 dims, and every
+// fourth part, four of them on their way.
 template <int DT, int DP, int NB>
-__global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares) {
+__global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares, int per) {
     constexpr int kDims = DP / 16, kAhead = DP == 256 ? 2 : 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, way = lane >> 4, d0 = (lane & 15) * kDims;
     const int64_t b = blockIdx.y;
-    const AttnSeq s = attn_seq(a, b);
-    const int h = blockIdx.x % (uint32_t)a.H, cc = blockIdx.x / (uint32_t)a.H * 4 + wave;  // (the column, of all blocks')
-    if (cc >= s.T * a.G) return;
-    const int n = attn_tiles(s), nb = cc / kShareCols % NB, c = cc % kShareCols;
+    const int h = blockIdx.x % (uint32_t)a.H;
     int64_t total = 0, before = 0;
+    AttnSeq s{}, own{};
     for (int64_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
-        const int64_t mine = kv16_seq_tiles<NB>(a, b0 + lane), upto = wave_scan64(mine);
-        if (b >= b0 && b < b0 + 64) before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
+        const int64_t mine = kv16_seq_tiles<NB>(a, b0 + lane, own), upto = wave_scan64(mine);
+        if (b >= b0 && b < b0 + 64) {
+            before = total + lane64(upto, (int)(b - b0)) - lane64(mine, (int)(b - b0));
+            s = seq_of_lane(own, (int)(b - b0));
+        }
         total += lane64(upto, 63);
     }
-    const int64_t share = kv16_share(total, shares), first = before + (int64_t)(cc / (NB * kShareCols)) * n;
-    const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
-    if (w0 == w1) return;
-    float M = -INFINITY, l = 0.f, o[kDims] = {};
-    for (int w = w0 + way; w <= w1; w += 4 * kAhead) {
-        float2 ml[kAhead];
-        float4 x[kAhead][kDims / 4];
+    const int n = attn_tiles(s);
+    const int64_t share = kv16_share(total, shares);
+    for (int cc = blockIdx.x / (uint32_t)a.H * 4 + wave; cc < s.T * a.G; cc += 4 * per) {  // (the column, of all blocks')
+        const int nb = cc / kShareCols % NB, c = cc % kShareCols;
+        const int64_t first = before + (int64_t)(cc / (NB * kShareCols)) * n;
+        const int w0 = (int)div64(first, share), w1 = (int)div64(first + n - 1, share);
+        if (w0 == w1) continue;
+        float M = -INFINITY, l = 0.f, o[kDims] = {};
+        for (int w = w0 + way; w <= w1; w += 4 * kAhead) {
+            float2 ml[kAhead];
+            float4 x[kAhead][kDims / 4];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int wu = min(w + 4 * u, w1);
-            const float *pt = kv16_part<DP, NB>(a, wu, wu == w0, h) + nb * AttnPartial<DP>::kFloats;
-            ml[u] = *reinterpret_cast<const float2 *>(pt + kShareCols * DP + 2 * c);
+            for (int u = 0; u < kAhead; ++u) {
+                const int wu = min(w + 4 * u, w1);
+                const float *pt = kv16_part<DP, NB>(a, wu, wu == w0, h) + nb * AttnPartial<DP>::kFloats;
+                ml[u] = *reinterpret_cast<const float2 *>(pt + kShareCols * DP + 2 * c);
 #pragma unroll
-            for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + c * DP + d0 + 4 * k);
-        }
+                for (int k = 0; k < kDims / 4; ++k) x[u][k] = *reinterpret_cast<const float4 *>(pt + c * DP + d0 + 4 * k);
+            }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (w + 4 * u > w1) continue;
-            const float Mn = fmaxf(M, ml[u].x);
-            const float keep = M == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mn);
-            const float r = ml[u].x == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(ml[u].x - Mn);
-            M = Mn;
-            l = l * keep + r * ml[u].y;
+            for (int u = 0; u < kAhead; ++u) {
+                if (w + 4 * u > w1) continue;
+                const float Mn = fmaxf(M, ml[u].x);
+                const float keep = M == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mn);
+                const float r = ml[u].x == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(ml[u].x - Mn);
+                M = Mn;
+                l = l * keep + r * ml[u].y;
 #pragma unroll
-            for (int k = 0; k < kDims / 4; ++k) {
-                o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
-                o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+                for (int k = 0; k < kDims / 4; ++k) {
+                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
+                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+                }
             }
         }
-    }
-    const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mt);
-    l = rows_sum(l * r);
+        const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mt);
+        l = rows_sum(l * r);
 #pragma unroll
-    for (int k = 0; k < kDims; ++k) o[k] = rows_sum(o[k] * r);
-    if (way != 0) return;
-    const int i = cc / a.G;
-    uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + cc % a.G) * a.o_sh + d0;
-    attn_put<DT, kDims>(row, o, attn_inv<true>(a, s, i, l), a.D - d0);
+        for (int k = 0; k < kDims; ++k) o[k] = rows_sum(o[k] * r);
+        if (way != 0) continue;
+        const int i = cc / a.G;
+        uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + cc % a.G) * a.o_sh + d0;
+        attn_put<DT, kDims>(row, o, attn_inv<true>(a, s, i, l), a.D - d0);
+    }
 }
 
 // One workgroup per item: one launch, no partials.
@@ -446,41 +458,46 @@ static bool kv16_span(int64_t num_blocks, int64_t block_size, int64_t stride_blo
 
 static int kv16_blocks(int G, int64_t max_q_len) { return max_q_len * G > kShareCols ? 2 : 1; }
 static int kv16_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-// How a call is cut, by its bounds: shares of tiles, each taken by H / heads workgroups.  heads 4 (a wave each) where that leaves a wave 12 tiles
-// or more, else 1 (the waves share the tiles, and their sums): the former reads 1 KB of a token at about the same time, but its parts are four
-// times as many.  8 heads x 4 of 128, us by waves / by tiles: 64 sequences of 1024 to 8192 keys 196 / 221, of 2000 93.5 / 97.4, 16 of 2000 (4 tiles a
-// wave) 32.9 / 33.1, 1 of 4000 16.9 / 12.9; 4 heads x 7, 4 sequences of 20000 to 32768 (8 tiles a wave) 59.7 / 54.5.
+// How a call is cut, by its bounds.
+// Short contexts: a workgroup per item (shares 0), one launch and no parts.  One CU loads 55 to 60 GB/s, so long ones are slower.  That is up to
+// kKv16ItemTiles tiles, and twice as many where items have two blocks of columns and half the CUs or more get one: these read the keys once a head
+// either way, and their parts are twice as large.  8 heads x 4 of 128, items / shares, us:
+//   single tokens, 1 sequence of 256 keys 7.5 / 9.9, 512: 9.8 / 9.9, 777: 12.6 / 10.0; 16 of these 9.7 / 11.3, 14.2 / 14.5, 19.1 / 20.1;
+//   64: 19.9 / 18.7, 30.7 / 30.0, 42.8 / 42.6;
+//   8 tokens each, 1 sequence of 1024 keys 21.4 / 14.1, 8: 24.6 / 24.6, 16: 26.6 / 33.2, 64: 58.8 / 74.6; 4 heads x 8 of 256, 4 tokens, 8: 40.3 / 29.7,
+//   64: 53.4 / 75.9.
+// Longer ones: shares of tiles, each taken by H / heads workgroups.  heads 4 (a wave each) where that leaves a wave 12 tiles or more, else 1 (the
+// waves share the tiles, and their sums): the former reads 1 KB of a token at about the same time, but its parts are four times as many.  8 heads x
+// 4 of 128, us by waves / by tiles: 64 sequences of 1024 to 8192 keys 196 / 221, of 2000 93.5 / 97.4, 16 of 2000 (4 tiles a wave) 32.9 / 33.1, 1 of
+// 4000 16.9 / 12.9; 4 heads x 7, 4 sequences of 20000 to 32768 (8 tiles a wave) 59.7 / 54.5.
 struct Kv16Cut {
     int heads;
     int64_t shares;
 };
+constexpr int64_t kKv16ItemTiles = 16;
 static Kv16Cut kv16_cut(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
-    const int w = kv16_width(D), cols = kv16_blocks(G, max_q_len) * kShareCols;
-    const int64_t resident = (w == 64 ? kKv16Resident<64, 1> : w == 128 ? kKv16Resident<128, 1> : kKv16Resident<256, 1>) * (int64_t)device_cus();
+    const int w = kv16_width(D), blocks = kv16_blocks(G, max_q_len), cols = blocks * kShareCols;
+    const int64_t cus = device_cus(), resident = (w == 64 ? kKv16Resident<64, 1> : w == 128 ? kKv16Resident<128, 1> : kKv16Resident<256, 1>) * cus;
     const int64_t tiles = max_keys / kShareTile + (max_keys % kShareTile != 0 || max_keys == 0);
-    const int64_t work = num_seqs * ((max_q_len * G + cols - 1) / cols) * tiles;
+    const int64_t rows = num_seqs * ((max_q_len * G + cols - 1) / cols), work = rows * tiles;
+    if (tiles <= kKv16ItemTiles || (blocks == 2 && 2 * rows * H >= cus && tiles <= 2 * kKv16ItemTiles)) return {1, 0};
     const int heads = H % 4 == 0 && work * (H / 4) >= 12 * resident ? 4 : 1;
     return {heads, std::max<int64_t>(1, std::min<int64_t>(resident * heads / H, (work + kKv16MinChunk - 1) / kKv16MinChunk))};
 }
 
-// Calls of short contexts, by the bound on their lengths, take a workgroup per item: one launch, and no parts.  One CU loads 55 to 60 GB/s, so
-// long ones are slower.  8 heads x 4 of 128, items / shares, us: 1 sequence of 256 keys 7.5 / 9.9, 512: 9.8 / 9.9, 777: 12.6 / 10.3; 16 sequences
-// 9.7 / 11.3, 14.2 / 14.5, 19.1 / 20.5; 64: 19.9 / 18.7, 30.7 / 30.0, 42.7 / 42.7.
-constexpr int64_t kKv16ItemTiles = 16;
-static bool kv16_is_short(int64_t max_keys) { return max_keys <= kKv16ItemTiles * kShareTile; }
-
 template <int DT, int DP, bool FULL, int NB>
 static void launch_kv16(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
     const int64_t items = ((int64_t)a.max_q * a.G + NB * kShareCols - 1) / (NB * kShareCols) * a.H;
-    if (kv16_is_short(a.bound)) {
+    if (cut.shares == 0) {
         hipLaunchKernelGGL((kv16_item_kernel<DT, DP, FULL, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(64 * kKv16ItemWaves<DP>), 0, st, a);
         return;
     }
-    const int64_t quads = ((int64_t)a.max_q * a.G + 3) / 4;
+    // (enough workgroups for the parts of few items, and no more than one each where there are many)
+    const int64_t quads = ((int64_t)a.max_q * a.G + 3) / 4, per = std::max<int64_t>(1, std::min<int64_t>(quads, 512 / std::max<int64_t>(1, a.num_seqs * a.H)));
     const dim3 grid((unsigned)(cut.shares * (a.H / cut.heads)));
     if (cut.heads == 4) hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, false>), grid, dim3(256), 0, st, a);
-    hipLaunchKernelGGL((kv16_merge_kernel<DT, DP, NB>), dim3((unsigned)(quads * a.H), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)cut.shares);
+    hipLaunchKernelGGL((kv16_merge_kernel<DT, DP, NB>), dim3((unsigned)(per * a.H), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)cut.shares, (int)per);
 }
 template <int DT, int DP, bool FULL>
 static void launch_kv16_b(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
@@ -505,9 +522,7 @@ extern "C" int64_t rq_kv16_attention_workspace_bytes(int64_t num_seqs, int32_t n
     if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || head_dim > 256 || max_q_len <= 0 || max_seq_len < 0)
         return 0;
     const int G = num_q_heads / num_kv_heads;
-    max_seq_len = attn_bound(max_seq_len);
-    if (kv16_is_short(max_seq_len)) return 0;
-    return 2 * kv16_cut(num_seqs, G, num_kv_heads, head_dim, max_q_len, max_seq_len).shares * num_kv_heads * kv16_blocks(G, max_q_len) * kShareCols * (kv16_width(head_dim) + 2) * 4;
+    return 2 * kv16_cut(num_seqs, G, num_kv_heads, head_dim, max_q_len, attn_bound(max_seq_len)).shares * num_kv_heads * kv16_blocks(G, max_q_len) * kShareCols * (kv16_width(head_dim) + 2) * 4;
 }
 
 extern "C" int rq_kv16_attention(const void *q, int32_t dtype, int64_t total_q, int32_t num_q_heads, int64_t q_stride_tok, int64_t q_stride_head,
@@ -525,6 +540,8 @@ extern "C" int rq_kv16_attention(const void *q, int32_t dtype, int64_t total_q, 
     RQ_CHECK_ARG(block_size >= 1 && block_size <= 65536 && num_blocks >= 0 && num_blocks <= INT32_MAX, "bad cache sizes");
     RQ_CHECK_ARG(num_seqs >= 0 && num_seqs <= 65535 && total_q >= 0 && total_q <= INT32_MAX && max_q_len >= 0 && max_q_len <= (1 << 20) &&
                      max_blocks >= 0 && max_seq_len >= 0, "bad sizes");
+    RQ_CHECK_ARG(max_q_len * num_q_heads <= (1 << 27), "max_q_len %lld with %d query heads: more rows of a sequence than a launch takes",
+                 (long long)max_q_len, num_q_heads);
     RQ_CHECK_ARG(cu_seqlens_q != nullptr || (total_q == num_seqs && max_q_len <= 1),
                  "without cu_seqlens_q there is one query token per sequence");
     RQ_CHECK_ARG(__builtin_fabsf(sm_scale) <= 0x1p127f, "sm_scale must be finite, 2^127 at most");  // (times log2(e) it is finite)

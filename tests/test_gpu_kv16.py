@@ -56,6 +56,14 @@ def test_drafts(q_lens, D, causal):
     run([700, 41, 64], q_lens, 2, 4, D, BF, causal=causal)
 
 
+# Two blocks of columns and 32 items or 160: the latter take up to 1024 keys by a workgroup each.
+@pytest.mark.parametrize("bound", [512, 513, 1024, 1025])
+@pytest.mark.parametrize("H,seqs", [(2, 16), (8, 20)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_drafts_of_many_sequences(D, H, seqs, bound):
+    run([bound - 29 * i % bound for i in range(seqs)], [1 + i % 6 for i in range(seqs)], H, 5, D, (BF, FP)[bound % 2], bound=bound)
+
+
 def test_longer_queries_than_contexts():
     """Rows before the context's first key are zeros, causal; with no key at all, also otherwise."""
     for causal in (True, False):

@@ -73,7 +73,7 @@ ATTENTION = dict(q=A, dtype=1, total_q=2, HQ=8, q_st=1024, q_sh=128, cu=None, nu
     ("null", dict(q=None)), ("null", dict(out=None)), ("null", dict(k=None)), ("null", dict(lens=None)), ("null", dict(bt=None)),
     ("q rows", dict(q=A + 8)), ("q rows", dict(q_sh=4)), ("out rows", dict(out=A + 4)), ("out rows", dict(o_st=2)), ("cache rows", dict(v=A + 8)),
     ("cache rows", dict(kc_ss=4)), ("within 64 GiB", dict(kc_sb=1 << 33)), ("within 64 GiB", dict(vc_ss=-256)), ("within 64 GiB", dict(num_blocks=1 << 30)),
-    ("within 64 GiB", dict(vc_sb=-4096))])
+    ("within 64 GiB", dict(vc_sb=-4096)), ("max_q_len 1048576 with 256", dict(cu=A, max_q_len=1 << 20, HQ=256))])
 def test_refusals_of_attention(match, kw):
     rc, message = call("rq_kv16_attention", ATTENTION, **kw)
     assert rc == 1 and match in message, message
@@ -84,6 +84,7 @@ def test_attention_without_work_or_scratch():
         assert call("rq_kv16_attention", ATTENTION, **kw)[0] == 0
     size = _lib.load().rq_kv16_attention_workspace_bytes
     assert size(2, 8, 2, 128, 1, 512) == 0 and size(0, 8, 2, 128, 1, 9000) == 0 and size(2, 8, 2, 300, 1, 9000) == 0
+    assert size(64, 32, 8, 128, 8, 1024) == 0 and size(1, 32, 8, 128, 8, 1024) > 0 and size(64, 32, 8, 128, 8, 1025) > 0 and size(64, 32, 8, 128, 4, 1024) > 0
     need = size(2, 8, 2, 128, 1, 9000)
     assert need > 0 and size(2, 8, 2, 128, 9, 9000) > need and size(2, 8, 2, 128, 1, 1 << 60) >= need
     rc, message = call("rq_kv16_attention", ATTENTION, max_seq_len=9000, max_blocks=1000)
