@@ -469,7 +469,9 @@ static int kv16_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 // Longer ones: shares of tiles, each taken by H / heads workgroups.  heads 4 (a wave each) where that leaves a wave 12 tiles or more, else 1 (the
 // waves share the tiles, and their sums): the former reads 1 KB of a token at about the same time, but its parts are four times as many.  8 heads x
 // 4 of 128, us by waves / by tiles: 64 sequences of 1024 to 8192 keys 196 / 221, of 2000 93.5 / 97.4, 16 of 2000 (4 tiles a wave) 32.9 / 33.1, 1 of
-// 4000 16.9 / 12.9; 4 heads x 7, 4 sequences of 20000 to 32768 (8 tiles a wave) 59.7 / 54.5.
+// 4000 16.9 / 12.9; 4 heads x 7, 4 sequences of 20000 to 32768 (8 tiles a wave) 59.7 / 54.5.  8 tokens, 32 of 600 to 8000: 134 / 146.  Two blocks of
+// columns of 256 fill the registers, and a wave's with a head of its own do not hold them: 4 heads x 8, 4 tokens, 64 of 4000 keys 293 / 222.
+constexpr bool kv16_by_heads(int width, int blocks) { return width < 256 || blocks == 1; }
 struct Kv16Cut {
     int heads;
     int64_t shares;
@@ -481,7 +483,7 @@ static Kv16Cut kv16_cut(int64_t num_seqs, int G, int H, int D, int64_t max_q_len
     const int64_t tiles = max_keys / kShareTile + (max_keys % kShareTile != 0 || max_keys == 0);
     const int64_t rows = num_seqs * ((max_q_len * G + cols - 1) / cols), work = rows * tiles;
     if (tiles <= kKv16ItemTiles || (blocks == 2 && 2 * rows * H >= cus && tiles <= 2 * kKv16ItemTiles)) return {1, 0};
-    const int heads = H % 4 == 0 && work * (H / 4) >= 12 * resident ? 4 : 1;
+    const int heads = kv16_by_heads(w, blocks) && H % 4 == 0 && work * (H / 4) >= 12 * resident ? 4 : 1;
     return {heads, std::max<int64_t>(1, std::min<int64_t>(resident * heads / H, (work + kKv16MinChunk - 1) / kKv16MinChunk))};
 }
 
@@ -495,7 +497,8 @@ static void launch_kv16(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
     // (enough workgroups for the parts of few items, and no more than one each where there are many)
     const int64_t quads = ((int64_t)a.max_q * a.G + 3) / 4, per = std::max<int64_t>(1, std::min<int64_t>(quads, 512 / std::max<int64_t>(1, a.num_seqs * a.H)));
     const dim3 grid((unsigned)(cut.shares * (a.H / cut.heads)));
-    if (cut.heads == 4) hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, true>), grid, dim3(256), 0, st, a);
+    constexpr bool kHeads = kv16_by_heads(DP, NB);
+    if (kHeads && cut.heads == 4) hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, kHeads>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv16_stream_kernel<DT, DP, FULL, NB, false>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL((kv16_merge_kernel<DT, DP, NB>), dim3((unsigned)(per * a.H), (unsigned)a.num_seqs), dim3(256), 0, st, a, (int)cut.shares, (int)per);
 }

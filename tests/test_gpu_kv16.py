@@ -92,6 +92,36 @@ def test_scales(scale, dtype):
     run([300, 1100], [1, 2], 2, 2, 64, dtype, scale=scale)
 
 
+WIDE = 1 << 24  # a bound on the lengths that gives a wave a kv head of its own, where heads come in fours
+
+
+@pytest.mark.parametrize("D", [40, 64, 96, 128, 200, 256])
+@pytest.mark.parametrize("H,G,q_lens", [(4, 1, [1, 1, 1, 1]), (8, 5, [1, 1, 1, 1]), (4, 3, [4, 1, 7, 5]), (4, 17, [1, 3, 1, 2])])
+def test_a_wave_for_each_head(H, G, q_lens, D):
+    for dtype in (BF, FP):
+        run([1, 260, 0, 1300], q_lens, H, G, D, dtype, bound=WIDE)
+
+
+@pytest.mark.parametrize("bound", [None, WIDE])
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_an_infinite_value(dtype, D, T, bound):
+    """One dim of one key's V is infinite in one head of four: that dim is where the key is seen, and all else is as without it."""
+    H, G, L, at = 4, 2, 1100, 1095
+    pages = P.Pages([L, L], 16, H, D, dtype, 3)
+    kc, vc = pages.to(DEV)
+    q = torch.randn(2 * T, H * G, D, generator=P.gen(5)).to(dtype)
+    want, err = P.attention(q, *pages.kv, [L, L], [T, T])
+    vc[int(pages.table[1, at // 16]), at % 16, 2, D - 3] = -math.inf
+    got = K.kv16_attention(q.to(DEV), kc, vc, i32(pages.table), i32([L, L]), cu_seqlens_q=i32([0, T, 2 * T]), max_q_len=T, max_seq_len=bound).cpu()
+    seen = torch.zeros_like(got, dtype=torch.bool)
+    for i in range(T):
+        seen[T + i, 2 * G:3 * G, D - 3] = at < L - T + i + 1
+    assert bool((got[seen] == -math.inf).all()) and bool(seen.any())
+    P.check(got.masked_fill(seen, 0.0), want.masked_fill(seen, 0.0), err)
+
+
 def plain(q, k, v, end, scale):
     """Softmax attention of one row in 64 bits, infinities and NaN as they come."""
     s = (k[:end].double() @ q.double()) * scale
@@ -229,6 +259,30 @@ def test_scratch_that_the_caller_keeps():
         K.kv16_attention(*args, workspace=ws[:need - 1])
     with pytest.raises(ValueError, match="contiguous uint8"):
         K.kv16_attention(*args, workspace=ws.view(torch.int32))
+
+
+def test_graphs_that_share_scratch():
+    """Two captured calls of different shapes over one workspace, replayed in turn."""
+    calls, graphs, side = [], [], torch.cuda.Stream()
+    for b, (H, G, D) in enumerate(((2, 4, 128), (4, 3, 64))):
+        pages = P.Pages([2600, 900], 16, H, D, BF, 4 + b)
+        q = torch.randn(2, H * G, D, generator=P.gen(b)).to(BF).to(DEV)
+        calls.append((q, *pages.to(DEV), i32(pages.table), i32([2600, 900])))
+    want = [K.kv16_attention(*c) for c in calls]
+    ws, outs = torch.full((64 << 20,), 0xff, dtype=torch.uint8, device=DEV), [torch.empty_like(c[0]) for c in calls]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c, out in zip(calls, outs):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                K.kv16_attention(*c, out=out, workspace=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(4):
+        for g, out in zip(graphs, outs):
+            out.zero_()
+            g.replay()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+        assert torch.equal(K.kv16_attention(*calls[0], workspace=ws), want[0])
 
 
 def test_two_streams():
