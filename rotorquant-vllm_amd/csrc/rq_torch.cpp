@@ -67,6 +67,12 @@ void check_status(int rc, const char *name) {
     throw std::runtime_error(text(name, " failed (status ", rc, "): ", rq_last_error()));
 }
 
+// The C ABI takes counts of heads, dims, slots and the like as ints.
+int count(int64_t n) {
+    if (n > INT32_MAX) refuse(text("a dimension of ", n, " is too large"));
+    return (int)n;
+}
+
 // Strides over a single token or head may be any number in a view.
 int64_t step(const Tensor &t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
 
@@ -124,10 +130,10 @@ struct Rope {
     template <typename F, typename... T>
     void call(F fn, const char *name, bool neox, T... more) const {
         const bool q = query.has_value();
-        check_status(fn(q ? query->data_ptr() : nullptr, key.data_ptr(), value.data_ptr(), dtype, N, (int)HQ, q ? step(*query, 0) : 0,
-                        q ? step(*query, 1) : 0, step(key, 0), step(key, 1), step(value, 0), step(value, 1), (int)H, (int)D,
+        check_status(fn(q ? query->data_ptr() : nullptr, key.data_ptr(), value.data_ptr(), dtype, N, count(HQ), q ? step(*query, 0) : 0,
+                        q ? step(*query, 1) : 0, step(key, 0), step(key, 1), step(value, 0), step(value, 1), count(H), count(D),
                         positions.data_ptr<int64_t>(), table.data_ptr(), dtype_code(table.scalar_type()), table.size(0), table.stride(0),
-                        (int)table.size(1), neox ? 1 : 0, q ? out->data_ptr() : nullptr, q ? step(*out, 0) : 0, q ? step(*out, 1) : 0, more...),
+                        count(table.size(1)), neox ? 1 : 0, q ? out->data_ptr() : nullptr, q ? step(*out, 0) : 0, q ? step(*out, 1) : 0, more...),
                      name);
     }
 };
@@ -152,8 +158,8 @@ OptTensor rope_compress_store(const OptTensor &query, const Tensor &key, const T
     const c10::hip::HIPGuard guard(key.get_device());
     const Tensor even = to_f32(rot_even, key), odd = to_f32(rot_odd, key), kb = to_f32(k_bounds, key), vb = to_f32(v_bounds, key);
     r.call(rq_rope_compress_store, "rq_rope_compress_store", neox, (int)(dense3 ? RQ_INDEX_DENSE3 : RQ_INDEX_NIBBLE), slots.data_ptr<int64_t>(),
-           cache.data_ptr<uint8_t>(), cache.size(0), (int)cache.size(1), cache.stride(0), cache.stride(1), (int)cache.size(2), even.data_ptr<float>(),
-           odd.data_ptr<float>(), (int)rot_block, kb.data_ptr<float>(), (int)kb.numel(), vb.data_ptr<float>(), (int)vb.numel(), stream_of(key));
+           cache.data_ptr<uint8_t>(), cache.size(0), count(cache.size(1)), cache.stride(0), cache.stride(1), count(cache.size(2)), even.data_ptr<float>(),
+           odd.data_ptr<float>(), count(rot_block), kb.data_ptr<float>(), count(kb.numel()), vb.data_ptr<float>(), count(vb.numel()), stream_of(key));
     return r.out;
 }
 
@@ -167,9 +173,9 @@ OptTensor rope_q8_store(const OptTensor &query, const Tensor &key, const Tensor 
         refuse(text("cache slots of ", cache.size(2), " bytes; ", r.H, " heads of ", r.D, " take ", (r.H * (2 * r.D + 1) + 7) / 8 * 8));
     if (cache.stride(2) != 1 || cache.stride(1) != cache.size(2)) refuse("the slots of a page must be contiguous");
     const c10::hip::HIPGuard guard(key.get_device());
-    const Scratch ws(workspace, rq_q8_store_workspace_bytes(r.N, cache.size(0), (int)cache.size(1)), key);
-    r.call(rq_rope_q8_store, "rq_rope_q8_store", neox, (int)format, slots.data_ptr<int64_t>(), cache.data_ptr<uint8_t>(), cache.size(0),
-           (int)cache.size(1), cache.stride(0), ws.at, ws.bytes, stream_of(key));
+    const Scratch ws(workspace, rq_q8_store_workspace_bytes(r.N, cache.size(0), count(cache.size(1))), key);
+    r.call(rq_rope_q8_store, "rq_rope_q8_store", neox, count(format), slots.data_ptr<int64_t>(), cache.data_ptr<uint8_t>(), cache.size(0),
+           count(cache.size(1)), cache.stride(0), ws.at, ws.bytes, stream_of(key));
     return r.out;
 }
 
@@ -190,7 +196,7 @@ OptTensor rope_kv16_store(const OptTensor &query, const Tensor &key, const Tenso
     check_pages(k_cache, v_cache, r.H, r.D);
     const c10::hip::HIPGuard guard(key.get_device());
     r.call(rq_rope_kv16_store, "rq_rope_kv16_store", neox, slots.data_ptr<int64_t>(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.size(0),
-           (int)k_cache.size(1), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), step(v_cache, 0), step(v_cache, 1), step(v_cache, 2),
+           count(k_cache.size(1)), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), step(v_cache, 0), step(v_cache, 1), step(v_cache, 2),
            stream_of(key));
     return r.out;
 }
@@ -230,12 +236,12 @@ Tensor kv16_attention(const Tensor &q_, const Tensor &k_cache, const Tensor &v_c
     if (!out.sizes().equals(q.sizes()) || out.scalar_type() != q.scalar_type() || out.stride(2) != 1)
         refuse("out must have q's shape and dtype and be contiguous over head_dim");
     const int64_t capacity = max_blocks * k_cache.size(1), longest = max_seq_len ? std::min(*max_seq_len, capacity) : capacity;
-    const Scratch ws(workspace, rq_kv16_attention_workspace_bytes(B, (int)HQ, (int)H, (int)D, most, longest), q);
+    const Scratch ws(workspace, rq_kv16_attention_workspace_bytes(B, count(HQ), count(H), count(D), most, longest), q);
     const float scale = sm_scale ? (float)*sm_scale : D > 0 ? (float)(1.0 / std::sqrt((double)D)) : 0.f;
-    check_status(rq_kv16_attention(q.data_ptr(), dtype_code(q.scalar_type()), T, (int)HQ, step(q, 0), step(q, 1),
+    check_status(rq_kv16_attention(q.data_ptr(), dtype_code(q.scalar_type()), T, count(HQ), step(q, 0), step(q, 1),
                                    cu.defined() ? cu.data_ptr<int32_t>() : nullptr, B, most, causal ? 1 : 0, k_cache.data_ptr(), v_cache.data_ptr(),
-                                   k_cache.size(0), (int)k_cache.size(1), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), step(v_cache, 0),
-                                   step(v_cache, 1), step(v_cache, 2), (int)H, (int)D, bt.data_ptr<int32_t>(), max_blocks, bt.stride(0),
+                                   k_cache.size(0), count(k_cache.size(1)), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), step(v_cache, 0),
+                                   step(v_cache, 1), step(v_cache, 2), count(H), count(D), bt.data_ptr<int32_t>(), max_blocks, bt.stride(0),
                                    sl.data_ptr<int32_t>(), longest, scale, out.data_ptr(), step(out, 0), step(out, 1), ws.at, ws.bytes, stream_of(q)),
                  "rq_kv16_attention");
     return out;
