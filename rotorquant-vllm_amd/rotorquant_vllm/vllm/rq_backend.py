@@ -18,8 +18,8 @@ librq_hip.so (include/rq_abi.h):
                          LDS, 16-bit MFMA; head_size 128; decodes), and for
                          longer queries rq_paged_prefill (the same arithmetic,
                          each tile decoded once); other head sizes
-                         rq_paged_decompress, then rq_kv16_attention over the plain pages (short
-                         queries) or device attention in fp32
+                         rq_paged_decompress, then rq_kv16_attention over the plain pages (16-bit
+                         models) or device attention in fp32
     8-bit cache       -> rq_q8_store, rq_q8_attention (RQ_CACHE_8BIT=int8 | fp8: another cache
                          layout, no rotation, no codebook; no counterpart in the reference)
     rotary embedding  -> rq_rope_compress_store, rq_rope_q8_store (rope_and_store: queries and keys rotated by their
@@ -172,9 +172,9 @@ except (ImportError, OSError, RuntimeError) as exc:
 # decodes each tile once for all query blocks instead of once per block.
 RQ_UNFUSED_SHORT_Q = 16
 
-# Layers whose shape the non-fused kernels do not take: queries of at most this many (token, query head) pairs of a kv head
-# attend to the decompressed pages by kv16_attention, longer ones by device matmuls.  That reads the keys again for every 32 pairs.
-RQ_PLAIN_SHORT_COLUMNS = 64
+# Layers whose shape the non-fused kernels do not take: 16-bit models attend to the decompressed pages by kv16_attention, whose heads are
+# of at most this many dims, others by device matmuls in fp32.  A layer's forward, kernel / matmuls, us: 16 decodes of 2000 keys, 32 / 8 heads of
+# 64 174 / 9584; 8 chunks of 1024 tokens, 843 / 6492; a prompt of 8192 tokens 2335 / 18137, of 8 / 4 heads of 256 3133 / 8232.
 RQ_PLAIN_MAX_HEAD_DIM = 256
 
 # Shapes the fused kernels take (checked again by the C ABI): head_dim 128, a
@@ -815,6 +815,7 @@ class RQAttentionImpl(_ImplBase):
             raise ValueError("rope_and_store: encoder layers have no cache")
         n = slot_mapping.shape[0]
         query, key, value, positions = query[:n], key[:n], value[:n], positions[:n]
+        out_q = None if out_q is None else out_q[:n]
         if getattr(self, "_q8_format", None) is not None:
             if _rope_q8_store_fn is None:
                 raise RuntimeError("RotorQuant HIP kernels are not available")
@@ -990,12 +991,12 @@ class RQAttentionImpl(_ImplBase):
 
     def _forward_unfused_torch(self, query, kv_cache, md, output, num_actual_tokens):
         """Paged decompress + attention over the plain pages, for shapes rq_paged_attention
-        does not take (head sizes other than 128, GQA groups above 16, fp32 models).  The leading short queries of a
-        16-bit model (vLLM orders decodes first) go to kv16_attention in one call, the others to device matmuls in fp32.
+        does not take (head sizes other than 128, GQA groups above 16, fp32 models).  16-bit models go to
+        kv16_attention in one call, others to device matmuls in fp32.
 
         K/V of the referenced blocks are decompressed once (rq_paged_decompress) to
         the q dtype, as the reference's _decompress_cache_paged(..., query.dtype)
-        (reference rq_backend.py:988-994); each sequence attends over its blocks in
+        (reference rq_backend.py:988-994); by matmuls each sequence attends over its blocks in
         fp32, one kv head (its GQA group of query heads) and at most ~32 M scores at
         a time.  Host lengths come from the metadata's host copies when present
         (one device read otherwise)."""
@@ -1022,22 +1023,21 @@ class RQAttentionImpl(_ImplBase):
         k_cache, v_cache, bt, _ = _paged_decompress_fn(kv_cache, md.block_table, md.seq_lens, H, D, self._dev_kc,
                                                        self._dev_vc, q.dtype, out_k=out_k,
                                                        out_v=torch.empty_like(out_k), **self._layout_kw())
-        short = self._plain_short(q_rot, starts, lens)
-        if short:
-            cu = torch.tensor(starts[:short + 1], dtype=torch.int32, device=q.device)
-            most = max(b - a for a, b in zip(starts[:short], starts[1:]))
-            out_short = _kv16_attention_fn(q_rot[:starts[short]], k_cache, v_cache, bt[:short], md.seq_lens[:short].to(torch.int32), sm_scale=self.scale,
-                                           causal=causal, cu_seqlens_q=cu, max_q_len=most, max_seq_len=max(lens[:short]))
-            output[:starts[short]] = (out_short.float() @ self._dev_R).to(output.dtype)
-            if short == len(lens) and starts[short] == num_actual_tokens:
-                return output
+        if self._plain_kernel(q_rot) and starts[0] == 0 and len(starts) == len(lens) + 1:
+            cu = torch.tensor(starts, dtype=torch.int32, device=q.device)
+            most = max(b - a for a, b in zip(starts, starts[1:]))
+            out_rot = torch.empty_like(q_rot)
+            out_rot[starts[-1]:] = 0  # (padding)
+            _kv16_attention_fn(q_rot, k_cache, v_cache, bt, md.seq_lens.to(torch.int32), sm_scale=self.scale, causal=causal, cu_seqlens_q=cu,
+                               max_q_len=most, max_seq_len=max(lens), out=out_rot)
+            output[:num_actual_tokens] = (out_rot.float() @ self._dev_R).to(output.dtype)
+            return output
         q_rot = q_rot.float()
-        begin = starts[short] if short else 0
         out_rot = torch.zeros(num_actual_tokens, HQ, D, dtype=torch.float32, device=q.device)
         for b, L in enumerate(lens):
             s0, s1 = starts[b], starts[b + 1]
             T = s1 - s0
-            if b < short or T <= 0 or L == 0:
+            if T <= 0 or L == 0:
                 continue
             ids = bt[b, :(L + BS - 1) // BS].long()
             K = k_cache[ids].reshape(-1, H, D)[:L].float()
@@ -1055,20 +1055,14 @@ class RQAttentionImpl(_ImplBase):
                     S = S.view(r1 - r0, G, L).masked_fill_(masked[:, None, :], float("-inf"))
                     P = torch.softmax(S, dim=-1).view(-1, L)
                     out_rot[s0 + r0:s0 + r1, h * G:(h + 1) * G, :] = (P @ V[:, h, :]).view(r1 - r0, G, D)
-        out_rot = out_rot[begin:].to(q.dtype).float()
-        output[begin:num_actual_tokens] = (out_rot @ self._dev_R).to(output.dtype)
+        out_rot = out_rot.to(q.dtype).float()
+        output[:num_actual_tokens] = (out_rot @ self._dev_R).to(output.dtype)
         return output
 
-    def _plain_short(self, q, starts: list, lens: list) -> int:
-        """Leading sequences whose queries kv16_attention takes: those of a 16-bit model on the GPU with few (token, query head) pairs
-        of a kv head."""
-        if (_kv16_attention_fn is None or not q.is_cuda or q.dtype not in (torch.float16, torch.bfloat16) or self.head_size % 8
-                or self.head_size > RQ_PLAIN_MAX_HEAD_DIM or not lens or starts[0] != 0):
-            return 0
-        group, n = q.shape[1] // self.num_kv_heads, 0
-        while n < len(lens) and 0 <= (starts[n + 1] - starts[n]) * group <= max(RQ_PLAIN_SHORT_COLUMNS, group):
-            n += 1
-        return n if starts[n] > 0 else 0
+    def _plain_kernel(self, q) -> bool:
+        """Whether kv16_attention takes this layer's heads: those of a 16-bit model on the GPU."""
+        return (_kv16_attention_fn is not None and q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and self.head_size % 8 == 0
+                and self.head_size <= RQ_PLAIN_MAX_HEAD_DIM)
 
     # -- forward -------------------------------------------------------------
 

@@ -74,6 +74,10 @@ def test_padded_steps_and_refusals(monkeypatch):
     assert sorted(cache.view(48, -1).any(-1).nonzero().flatten().tolist()) == [5, 7]
     same = layer.rope_and_store(q[:5], k, v, positions, cos_sin, True, cache, slots, out_q=q[:5])
     assert same.data_ptr() == q.data_ptr() and torch.equal(q[:5], got)
+    q, cache = tokens(9, 4, 2, 128, 1)[0], new_cache(2, 128, 3)
+    behind = q[5:].clone()
+    same = layer.rope_and_store(q, k, v, positions, cos_sin, True, cache, slots, out_q=q)  # (the whole padded batch, in place)
+    assert torch.equal(same, got) and torch.equal(q[:5], got) and torch.equal(q[5:], behind)
     with pytest.raises(ValueError, match="encoder"):
         layer.attn_type = B.AttentionType.ENCODER_ONLY
         layer.rope_and_store(q, k, v, positions, cos_sin, True, cache, slots)
@@ -89,7 +93,7 @@ SHAPES = [(8, 2, 64), (6, 3, 96), (4, 1, 256), (20, 1, 128), (34, 2, 64)]
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_layers_of_other_shapes(monkeypatch, shape, dtype):
-    """Decodes, drafts and mixed batches through kv16_attention against the device matmuls, both within a rounding of the rotated output's type."""
+    """Prompts, decodes, drafts and mixed batches through kv16_attention against the device matmuls, both within a rounding of the rotated output's type."""
     HQ, H, D = shape
     layer, pages = impl(monkeypatch, HQ, H, D), 40
     table, cache = np.random.RandomState(1).permutation(pages).astype(np.int32).reshape(4, 10), new_cache(H, D, pages)
@@ -103,9 +107,8 @@ def test_layers_of_other_shapes(monkeypatch, shape, dtype):
         got, want = torch.full_like(q, 7.0), torch.zeros_like(q)
         calls.clear()
         layer.forward(None, q, k, v, cache, md, output=got)
-        short = next((i for i, t in enumerate(new) if t * (HQ // H) > 64), len(new))  # the leading queries of at most 64 columns
-        assert calls == ([sum(new[:short])] if short else [])
-        monkeypatch.setattr(layer, "_plain_short", lambda *a: 0)
+        assert calls == [sum(new)]
+        monkeypatch.setattr(layer, "_plain_kernel", lambda *a: False)
         layer.forward(None, q, None, None, cache, md, output=want)
         monkeypatch.undo()
         monkeypatch.setattr(B, "_kv16_attention_fn", lambda *a, **kw: calls.append(a[0].shape[0]) or real(*a, **kw))
@@ -129,3 +132,16 @@ def test_other_shapes_hidden_rows(monkeypatch):
     out = torch.full_like(q, 7.0)
     layer.forward(None, q, k, v, cache, md, output=out)
     assert bool((out[0] == 0).all()) and bool(torch.isfinite(out).all()) and bool(out[1:].any(-1).all())
+
+
+def test_other_shapes_padded_batch(monkeypatch):
+    """Rows behind the last sequence are zeros, as the matmuls leave them."""
+    HQ, H, D = 4, 2, 64
+    layer, cache = impl(monkeypatch, HQ, H, D), new_cache(H, D, 4)
+    q, k, v = tokens(5, HQ, H, D, 3)
+    md = metadata([2, 1], [2, 1], np.arange(4, dtype=np.int32).reshape(2, 2))
+    md.slot_mapping = torch.cat([md.slot_mapping, md.slot_mapping.new_full((2,), -1)])
+    md.num_actual_tokens = 5
+    out = torch.full_like(q, 7.0)
+    layer.forward(None, q, k, v, cache, md, output=out)
+    assert bool(out[:3].any(-1).all()) and not out[3:].any()
