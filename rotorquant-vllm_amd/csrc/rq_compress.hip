@@ -234,7 +234,7 @@ template <bool ROPE>
 struct CompressRope {};
 template <>
 struct CompressRope<true> {
-    RopeRows rows;         // the queries of a short call, by workgroups of their own behind those that compress
+    RopeRows rows;         // the queries, by workgroups of their own (in long calls a launch) behind those that compress
     unsigned store_blocks;
 };
 
@@ -698,7 +698,7 @@ static int launch_compress_dc(const RowMap &m, CompressRope<ROPE> rope, int64_t 
     int64_t grid = compress_grid<DT, BLK, DC, ROPE>(lds, (n_rows + kRows - 1) / kRows);
     if constexpr (ROPE) {
         rope.store_blocks = (unsigned)grid;
-        if (rope.rows.n_tokens > kRopeApart) launch_rope_rows<DT>(rope.rows, st);
+        if (rope_apart<DT>(rope.rows)) launch_rope_rows<DT>(rope.rows, st);
         else grid += rope_blocks(rope.rows);
     }
     hipLaunchKernelGGL((compress_kernel<DT, BLK, DC, ROPE>), dim3((unsigned)grid), dim3(kThreads), lds, st, m, rope, n_rows, D, b.rte, b.rto,

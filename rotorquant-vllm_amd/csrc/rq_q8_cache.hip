@@ -122,7 +122,7 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
 enum { kQ8Plain, kQ8Units, kQ8Pieces };
 template <int ROPE>
 struct Q8Rope {
-    RopeRows rows;          // the queries of a short call, by workgroups of their own behind those that store
+    RopeRows rows;          // the queries, by workgroups of their own (in long calls a launch) behind those that store
     unsigned store_blocks;
 };
 template <>
@@ -454,7 +454,7 @@ static void launch_store(Q8StoreArgs a, Q8Rope<ROPE> rope, bool linked, hipStrea
     int64_t grid = blocks;
     if constexpr (ROPE != kQ8Plain) {
         rope.store_blocks = (unsigned)blocks;
-        if (linked) launch_rope_rows<DT>(rope.rows, st);
+        if (rope_apart<DT>(rope.rows)) launch_rope_rows<DT>(rope.rows, st);
         else grid += rope_blocks(rope.rows);
     }
     if (linked) hipLaunchKernelGGL((q8_store_kernel<DT, FMT, D, true, ROPE>), dim3((unsigned)grid), dim3(64 * kStoreWaves), 0, st, a, rope);

@@ -132,74 +132,50 @@ struct RopeRows {
 };
 constexpr int kRopeThreads = 256;
 
-// A thread takes a unit of up to kRopeShare rows of one token: the rows share the
-// token's angles, and their loads are on their way together.
-constexpr int kRopeShare = 2;
-__host__ __device__ __forceinline__ int64_t rope_threads(const RopeRows &a) {
-    return a.n_tokens * ((a.n_q + 2 * a.n_kv + kRopeShare - 1) / kRopeShare) * (a.D / 16);
-}
+// A thread takes a unit of a row: its angles come from the caches, and rows that share them, two or four to a thread, are slower (32768 tokens of 32
+// query and 8 kv heads, bf16 pages: 144 us, by two 150; 64 tokens 3.2, 3.7, by four 4.7).
+__host__ __device__ __forceinline__ int64_t rope_threads(const RopeRows &a) { return a.n_tokens * (a.n_q + 2 * a.n_kv) * (a.D / 16); }
 inline int64_t rope_blocks(const RopeRows &a) { return (rope_threads(a) + kRopeThreads - 1) / kRopeThreads; }
 
 template <int DT>
 __device__ __forceinline__ void rope_rows(const RopeRows &a, int64_t thread) {
-    const int units = a.D / 16, rows = a.n_q + 2 * a.n_kv, shared = (rows + kRopeShare - 1) / kRopeShare;
     if (thread >= rope_threads(a)) return;  // (fits 32 bits)
-    const uint32_t at = (uint32_t)thread / (uint32_t)units, u = (uint32_t)thread - at * units;
-    const uint32_t tok = at / (uint32_t)shared, r0 = at - tok * shared;
-    const int64_t token = tok;
-    const RopeUnit unit(a.t, (int)u);
-    const int64_t position = a.t.positions[token];
-    int64_t page = -1, in_page = 0;
-    if (a.n_kv > 0) {
+    const uint32_t units = a.D / 16, rows = a.n_q + 2 * a.n_kv;
+    const uint32_t row = (uint32_t)thread / units, tok = row / rows;
+    const int r = (int)(row - tok * rows);
+    const RopeUnit unit(a.t, (int)((uint32_t)thread - row * units));
+    const int64_t token = tok, position = a.t.positions[token];
+    const void *from = a.q;
+    void *to = a.out;
+    int64_t src = token * a.q_st + r * a.q_sh, dst = token * a.o_st + r * a.o_sh;
+    bool turn = unit.turned;
+    if (r >= a.n_q) {
         const int64_t s = a.slots[token];
-        if (s >= 0 && s < a.num_slots) {
-            if (a.num_slots <= 0x7fffffff) page = (uint32_t)s / (uint32_t)a.block_size;
-            else page = s / a.block_size;
-            in_page = s - page * a.block_size;
-        }
+        if (s < 0 || s >= a.num_slots) return;
+        int64_t page;
+        if (a.num_slots <= 0x7fffffff) page = (uint32_t)s / (uint32_t)a.block_size;
+        else page = s / a.block_size;
+        const int64_t in_page = s - page * a.block_size;
+        const bool is_v = r >= a.n_q + a.n_kv;
+        const int h = r - a.n_q - (is_v ? a.n_kv : 0);
+        from = is_v ? a.v : a.k, to = is_v ? a.v_cache : a.k_cache;
+        src = is_v ? token * a.v_st + h * a.v_sh : token * a.k_st + h * a.k_sh;
+        dst = is_v ? page * a.vc_sb + in_page * a.vc_ss + h * a.vc_sh : page * a.kc_sb + in_page * a.kc_ss + h * a.kc_sh;
+        turn = turn && !is_v;
     }
-    Row8<DT> x0[kRopeShare], x1[kRopeShare];
-    void *to[kRopeShare];
-    bool turn[kRopeShare];
-#pragma unroll
-    for (int i = 0; i < kRopeShare; ++i) {
-        const int r = (int)r0 + i * shared;
-        const void *from = nullptr;
-        int64_t src = 0, dst = 0;
-        to[i] = nullptr, turn[i] = unit.turned;
-        if (r < a.n_q) {
-            from = a.q, src = token * a.q_st + r * a.q_sh;
-            to[i] = a.out, dst = token * a.o_st + r * a.o_sh;
-        } else if (r < rows && page >= 0) {
-            const bool is_v = r >= a.n_q + a.n_kv;
-            const int h = r - a.n_q - (is_v ? a.n_kv : 0);
-            from = is_v ? a.v : a.k;
-            src = is_v ? token * a.v_st + h * a.v_sh : token * a.k_st + h * a.k_sh;
-            to[i] = is_v ? a.v_cache : a.k_cache;
-            dst = is_v ? page * a.vc_sb + in_page * a.vc_ss + h * a.vc_sh : page * a.kc_sb + in_page * a.kc_ss + h * a.kc_sh;
-            turn[i] = unit.turned && !is_v;
-        }
-        if (to[i] == nullptr) continue;
-        x0[i] = row8_load<DT>(from, src + 8 * unit.p0);
-        x1[i] = row8_load<DT>(from, src + 8 * unit.p1);
-        to[i] = static_cast<uint8_t *>(to[i]) + dst * (DT == RQ_DTYPE_F32 ? 4 : 2);
+    Row8<DT> x0 = row8_load<DT>(from, src + 8 * unit.p0), x1 = row8_load<DT>(from, src + 8 * unit.p1);
+    to = static_cast<uint8_t *>(to) + dst * (DT == RQ_DTYPE_F32 ? 4 : 2);
+    if (turn) {
+        const RopeTurn t = rope_unit_turn<DT>(a.t, position, unit);
+        float f0[8], f1[8];
+        row8_floats<DT>(x0, f0);
+        row8_floats<DT>(x1, f1);
+        rope_unit(f0, f1, t, a.t.halves, unit);
+        x0 = row8_round<DT>(f0);
+        x1 = row8_round<DT>(f1);
     }
-    RopeTurn t;
-    if (unit.turned) t = rope_unit_turn<DT>(a.t, position, unit);
-#pragma unroll
-    for (int i = 0; i < kRopeShare; ++i) {
-        if (to[i] == nullptr) continue;
-        if (turn[i]) {
-            float f0[8], f1[8];
-            row8_floats<DT>(x0[i], f0);
-            row8_floats<DT>(x1[i], f1);
-            rope_unit(f0, f1, t, a.t.halves, unit);
-            x0[i] = row8_round<DT>(f0);
-            x1[i] = row8_round<DT>(f1);
-        }
-        row8_store<DT>(to[i], 8 * unit.p0, x0[i]);
-        row8_store<DT>(to[i], 8 * unit.p1, x1[i]);
-    }
+    row8_store<DT>(to, 8 * unit.p0, x0);
+    row8_store<DT>(to, 8 * unit.p1, x1);
 }
 
 template <int DT>
@@ -211,8 +187,14 @@ void launch_rope_rows(const RopeRows &a, hipStream_t st) {
     if (rope_blocks(a) > 0) hipLaunchKernelGGL((rope_rows_kernel<DT>), dim3((unsigned)rope_blocks(a)), dim3(kRopeThreads), 0, st, a);
 }
 
-// Tokens from which a store's queries have a launch of their own: beside a store's registers and LDS fewer of their waves fit a CU.
-constexpr int64_t kRopeApart = 512;
+// Whether a store's queries have a launch of their own: where they are long, since beside a store's registers and LDS fewer of their waves fit a CU;
+// otherwise workgroups behind the store's fill what it leaves free.  rope_compress_store / rope_q8_store of 8 kv heads of 128, beside / apart, us: 32 query
+// heads, 4096 tokens 31 / 36, 29 / 31; 16384 (134 MB of queries) 100 / 101, 82 / 86; 24576 147 / 148, 119 / 117; 32768 211 / 194, 166 / 154; 8 query heads,
+// 65536 tokens 244 / 247, 149 / 155; 64, 16384 149 / 146, 130 / 129.
+template <int DT>
+bool rope_apart(const RopeRows &a) {
+    return a.n_tokens * a.n_q * a.D * (DT == RQ_DTYPE_F32 ? 4 : 2) > (int64_t)192 << 20;
+}
 
 // The table and the query rows of a call, checked; strides in elements of the rows' type.
 inline int rope_queries(RopeRows &a, int dtype, int64_t n_tokens, int head_dim, const int64_t *positions, const void *table, int table_dtype,

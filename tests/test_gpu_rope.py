@@ -208,6 +208,22 @@ def test_graphs_and_streams(kind, n):
         assert same(got, want) and torch.equal(got_cache, cache)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,HQ", [(25, 32768), (700, 1200)])
+def test_many_query_rows(kind, n, HQ):
+    """Over 192 MiB of queries: what calls of a part of the heads each give."""
+    H, D, part = 2, 128, HQ // 16
+    call, cache = stores(pages=n // 8 + 1)[kind]
+    q = torch.randn(n, HQ, D, dtype=BF, device=DEV)
+    _, k, v, positions, cos_sin = on(*inputs(n, 1, H, D, D, BF, BF, 1))
+    slots = torch.from_numpy(distinct_slots(n, n // 8 * 16, 3, padded=3)).to(DEV)
+    got = call(q, k, v, positions, cos_sin, slots)
+    got_cache = cache.clone()
+    for h in range(0, HQ, part):
+        cache.zero_()
+        assert same(call(q[:, h:h + part], k, v, positions, cos_sin, slots), got[:, h:h + part]) and torch.equal(cache, got_cache)
+
+
 def test_pages_past_32_bits_of_elements():
     """Slots at the far end of pages of more than 2^32 elements, each side."""
     H, D, block = 8, 128, 64
