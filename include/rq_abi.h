@@ -592,7 +592,7 @@ int rq_rope_kv16_store(const void *query, const void *key, const void *value, in
  * as those of no sequence, are left as they are.  Pages outside the cache are read as page 0.  Products are exact, sums and the softmax's
  * statistics fp32, its weights two 16-bit numbers each for P V.  |sm_scale| is 2^127 at most.
  * workspace: rq_kv16_attention_workspace_bytes() bytes (asked for on the GPU of the call), 16-byte aligned, no initialisation needed; 0 where
- * max_seq_len is 512 or less (1024, for many short queries).  Launches depend on host arguments only, so a captured call may be replayed with other
+ * max_seq_len is 512 or less (768 or 2048 in calls of many sequences).  Launches depend on host arguments only, so a captured call may be replayed with other
  * lengths up to max_seq_len.
  */
 int64_t rq_kv16_attention_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,

@@ -330,16 +330,18 @@ __device__ __forceinline__ float *kv16_part(const Kv16Args &a, int64_t w, bool b
     return a.part + ((2 * w + (begins ? 1 : 0)) * a.H + h) * (NB * AttnPartial<DP>::kFloats);
 }
 
-// Tiles of a share.
+// Tiles of a share, at least: a wave of the four has one.  One sequence of 2000 keys with 2 / 4 / 8: 11.0 / 10.6 / 12.0 us, of 4000 13.7 / 11.9 / 12.8.
 constexpr int kKv16MinChunk = 4;
 __device__ __forceinline__ int64_t kv16_share(int64_t tiles, int shares) {
     return max((int64_t)kKv16MinChunk, div64(tiles + shares - 1, shares));
 }
 
-// Workgroups of a CU at once (4 waves each): fewer, of more registers, keep enough loads on their way.
+// Workgroups of a CU at once (4 waves each): as many as their registers allow.  Heads of 64 would fit three where they have one block of columns,
+// and are slower: 64 sequences of 1024 to 8192 keys 107 us for 105, 16 of 1024 17.2 for 14.3.
 template <int DP, int NB>
 constexpr int kKv16Resident = DP == 256 ? 1 : 2;
 
+// Bound by memory in long calls: 64 sequences of 1024 to 8192 keys, 8 heads x 4 of 128, 1.2 GB in 187 to 191 us, 6.3 TB/s (HEADS).
 template <int DT, int DP, bool FULL, int NB, bool HEADS>
 __global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kernel(Kv16Args a) {
     constexpr int kHeads = HEADS ? 4 : 1;  // of a workgroup
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(256, (kKv16Resident<DP, NB>)) void kv16_stream_kern
 }
 
 // Adds up the parts of the items that were cut: `per` workgroups for a sequence and head.  A wave takes a column at a time; lane: D / 16 dims, and every
-// fourth part, four of them on their way.
+// fourth part, four of them on their way.  4 to 6 us, mostly its launch; 11 for 32 drafts of 8 tokens (38 MB of parts).
 template <int DT, int DP, int NB>
 __global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares, int per) {
     constexpr int kDims = DP / 16, kAhead = DP == 256 ? 2 : 4;
@@ -438,17 +440,17 @@ __global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares,
     }
 }
 
-// One workgroup per item: one launch, no partials.
-template <int DP>
-constexpr int kKv16ItemWaves = DP == 256 ? 4 : 8;
+// One workgroup per item: one launch, no partials.  Four waves: with eight, which join twice the sums, 64 sequences of 256 keys take 20.1 us for
+// 16.1, one of 256 7.5 for 7.0; with two 16.6 and 7.9.
+constexpr int kKv16ItemWaves = 4;
 template <int DT, int DP, bool FULL, int NB>
-__global__ __launch_bounds__(64 * kKv16ItemWaves<DP>, DP == 256 ? 1 : 2) void kv16_item_kernel(Kv16Args a) {
-    __shared__ AttnSums<DP, kKv16ItemWaves<DP>> lds;
+__global__ __launch_bounds__(64 * kKv16ItemWaves, DP == 256 ? 1 : 2) void kv16_item_kernel(Kv16Args a) {
+    __shared__ AttnSums<DP, kKv16ItemWaves> lds;
     const int64_t seq = blockIdx.y;
     const AttnSeq s = attn_seq(a, seq);
     const int block = blockIdx.x / (uint32_t)a.H, h = blockIdx.x - block * a.H;
     if (block >= attn_col_blocks<NB>(a, s.T)) return;
-    kv16_segment<DT, DP, FULL, NB, kKv16ItemWaves<DP>, false>(a, seq, s, h, block * (NB * kShareCols), 0, attn_tiles(s), nullptr, lds);
+    kv16_segment<DT, DP, FULL, NB, kKv16ItemWaves, false>(a, seq, s, h, block * (NB * kShareCols), 0, attn_tiles(s), nullptr, lds);
 }
 
 // Whether a head's rows span less than 2^32 units of 8 elements.
@@ -459,13 +461,14 @@ static bool kv16_span(int64_t num_blocks, int64_t block_size, int64_t stride_blo
 static int kv16_blocks(int G, int64_t max_q_len) { return max_q_len * G > kShareCols ? 2 : 1; }
 static int kv16_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 // How a call is cut, by its bounds.
-// Short contexts: a workgroup per item (shares 0), one launch and no parts.  One CU loads 55 to 60 GB/s, so long ones are slower.  That is up to
-// kKv16ItemTiles tiles, and twice as many where items have two blocks of columns and half the CUs or more get one: these read the keys once a head
-// either way, and their parts are twice as large.  8 heads x 4 of 128, items / shares, us:
-//   single tokens, 1 sequence of 256 keys 7.5 / 9.9, 512: 9.8 / 9.9, 777: 12.6 / 10.0; 16 of these 9.7 / 11.3, 14.2 / 14.5, 19.1 / 20.1;
-//   64: 19.9 / 18.7, 30.7 / 30.0, 42.8 / 42.6;
-//   8 tokens each, 1 sequence of 1024 keys 21.4 / 14.1, 8: 24.6 / 24.6, 16: 26.6 / 33.2, 64: 58.8 / 74.6; 4 heads x 8 of 256, 4 tokens, 8: 40.3 / 29.7,
-//   64: 53.4 / 75.9.
+// Short contexts: a workgroup per item (shares 0), one launch and no parts.  One CU loads 55 to 60 GB/s, and lengths differ, so long ones are slower:
+// up to 16 tiles; where half the CUs or more get an item, which costs shares their parts and cuts, 24, or 64 with two blocks of columns (whose
+// parts are twice as large).  8 heads x 4 of 128, items / shares, us:
+//   single tokens, 1 sequence of 256 keys 7.0 / 9.9, 512: 9.5 / 9.9, 777: 12.6 / 10.0; 32 of 600: 18.1 / 24.8, of 50 to 600 15.8 / 19.0, of 1024
+//   27.4 / 31.0, of 50 to 1400 30.5 / 28.7; 128 of 50 to 600 44 / 48, of 50 to 777 55 / 50; heads of 64, 64 of 600 21 / 23; 4 heads x 8 of 256, 64 of
+//   50 to 777 32 / 37, to 1400 50 / 48;
+//   8 tokens each, 1 of 1024 21 / 14, 16 of 1400 32 / 39, 64 of 2000 102 / 134, of 50 to 2000 79 / 94; 4 heads x 8 of 256, 4 tokens, 64 of 50 to 2000
+//   77 / 114.
 // Longer ones: shares of tiles, each taken by H / heads workgroups.  heads 4 (a wave each) where that leaves a wave 12 tiles or more, else 1 (the
 // waves share the tiles, and their sums): the former reads 1 KB of a token at about the same time, but its parts are four times as many.  8 heads x
 // 4 of 128, us by waves / by tiles: 64 sequences of 1024 to 8192 keys 196 / 221, of 2000 93.5 / 97.4, 16 of 2000 (4 tiles a wave) 32.9 / 33.1, 1 of
@@ -476,13 +479,12 @@ struct Kv16Cut {
     int heads;
     int64_t shares;
 };
-constexpr int64_t kKv16ItemTiles = 16;
 static Kv16Cut kv16_cut(int64_t num_seqs, int G, int H, int D, int64_t max_q_len, int64_t max_keys) {
     const int w = kv16_width(D), blocks = kv16_blocks(G, max_q_len), cols = blocks * kShareCols;
     const int64_t cus = device_cus(), resident = (w == 64 ? kKv16Resident<64, 1> : w == 128 ? kKv16Resident<128, 1> : kKv16Resident<256, 1>) * cus;
     const int64_t tiles = max_keys / kShareTile + (max_keys % kShareTile != 0 || max_keys == 0);
     const int64_t rows = num_seqs * ((max_q_len * G + cols - 1) / cols), work = rows * tiles;
-    if (tiles <= kKv16ItemTiles || (blocks == 2 && 2 * rows * H >= cus && tiles <= 2 * kKv16ItemTiles)) return {1, 0};
+    if (tiles <= (2 * rows * H < cus ? 16 : blocks == 1 ? 24 : 64)) return {1, 0};
     const int heads = kv16_by_heads(w, blocks) && H % 4 == 0 && work * (H / 4) >= 12 * resident ? 4 : 1;
     return {heads, std::max<int64_t>(1, std::min<int64_t>(resident * heads / H, (work + kKv16MinChunk - 1) / kKv16MinChunk))};
 }
@@ -491,7 +493,7 @@ template <int DT, int DP, bool FULL, int NB>
 static void launch_kv16(const Kv16Args &a, const Kv16Cut &cut, hipStream_t st) {
     const int64_t items = ((int64_t)a.max_q * a.G + NB * kShareCols - 1) / (NB * kShareCols) * a.H;
     if (cut.shares == 0) {
-        hipLaunchKernelGGL((kv16_item_kernel<DT, DP, FULL, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(64 * kKv16ItemWaves<DP>), 0, st, a);
+        hipLaunchKernelGGL((kv16_item_kernel<DT, DP, FULL, NB>), dim3((unsigned)items, (unsigned)a.num_seqs), dim3(64 * kKv16ItemWaves), 0, st, a);
         return;
     }
     // (enough workgroups for the parts of few items, and no more than one each where there are many)

@@ -56,12 +56,19 @@ def test_drafts(q_lens, D, causal):
     run([700, 41, 64], q_lens, 2, 4, D, BF, causal=causal)
 
 
-# Two blocks of columns and 32 items or 160: the latter take up to 1024 keys by a workgroup each.
-@pytest.mark.parametrize("bound", [512, 513, 1024, 1025])
+# Two blocks of columns and 32 items or 160: the latter take up to 2048 keys by a workgroup each.
+@pytest.mark.parametrize("bound", [512, 513, 2048, 2049])
 @pytest.mark.parametrize("H,seqs", [(2, 16), (8, 20)])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_drafts_of_many_sequences(D, H, seqs, bound):
     run([bound - 29 * i % bound for i in range(seqs)], [1 + i % 6 for i in range(seqs)], H, 5, D, (BF, FP)[bound % 2], bound=bound)
+
+
+# 128 items of one block: up to 768 keys by a workgroup each.
+@pytest.mark.parametrize("bound", [768, 769])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decodes_of_many_sequences(D, bound):
+    run([bound - 31 * i % bound for i in range(32)], [1] * 32, 4, 3, D, (BF, FP)[bound % 2], bound=bound)
 
 
 def test_longer_queries_than_contexts():

@@ -84,7 +84,8 @@ def test_attention_without_work_or_scratch():
         assert call("rq_kv16_attention", ATTENTION, **kw)[0] == 0
     size = _lib.load().rq_kv16_attention_workspace_bytes
     assert size(2, 8, 2, 128, 1, 512) == 0 and size(0, 8, 2, 128, 1, 9000) == 0 and size(2, 8, 2, 300, 1, 9000) == 0
-    assert size(64, 32, 8, 128, 8, 1024) == 0 and size(1, 32, 8, 128, 8, 1024) > 0 and size(64, 32, 8, 128, 8, 1025) > 0 and size(64, 32, 8, 128, 4, 1024) > 0
+    assert size(64, 32, 8, 128, 8, 2048) == 0 and size(64, 32, 8, 128, 8, 2049) > 0 and size(1, 32, 8, 128, 8, 513) > 0
+    assert size(64, 32, 8, 128, 1, 768) == 0 and size(64, 32, 8, 128, 1, 769) > 0 and size(64, 32, 8, 128, 4, 769) > 0
     need = size(2, 8, 2, 128, 1, 9000)
     assert need > 0 and size(2, 8, 2, 128, 9, 9000) > need and size(2, 8, 2, 128, 1, 1 << 60) >= need
     rc, message = call("rq_kv16_attention", ATTENTION, max_seq_len=9000, max_blocks=1000)
