@@ -31,7 +31,7 @@
 //     count is table[cell].n + (table[cell].b < v).  Boundary sets that fail the
 //     check (NaNs, unsorted, too close together) take the 15-comparison count.
 //
-// Work split: rows (one row = one (token, head) of K or V) go in groups of 64
+// Work split: rows (one row = one (token, head) of K or V) go in groups of 64 (16 or 32 in short calls)
 // to persistent workgroups of four waves, one group after another.  While a
 // group is processed, the next group's row addresses are resolved and its rows
 // are already loading into registers.  A group's rows are staged through LDS
@@ -69,6 +69,7 @@ struct RowMap {
     int32_t H;
     int32_t pad_vec;    // slot padding can be cleared with 16-byte stores
     int32_t dense3;     // store mode: dense 3-bit index layout
+    int32_t log_group;  // log2 of the rows of a group: of kRows, or fewer in short calls
 };
 
 // Per-row addresses, resolved once per workgroup.
@@ -222,7 +223,7 @@ __device__ __forceinline__ void cell_params(const float *__restrict__ bnd, int n
     if (!(fabsf(c) < 1.0e30f)) { s = 0.f; c = 0.f; }
 }
 
-// Position of a group of kRows rows in store mode: first row, its token and the
+// Position of a group of rows in store mode: first row, its token and the
 // row's index inside that token (rows of a token: K heads, then V heads).
 struct Cursor {
     int64_t row0, tok0;
@@ -256,6 +257,8 @@ constexpr int compress_waves_per_eu(int blk) { return blk <= 4 ? 4 : 1; }
 // DC: head_dim fixed at compile time (128: every loop has a constant trip count), 0 = runtime D_in.
 // ROPE: keys are turned by their positions between the load and LDS, whose rows are then fp32 (a rotated key is not rounded before
 // its norm and indices), and from there on everything is as for fp32 rows.
+// 32768 tokens of 8 heads 98 us (bf16 rows without rotation 67, fp32 rows 100): the fp32 rows' LDS leaves three workgroups a CU, loading
+// angles and turning take 18.  Half of the SIMDs' time is vector instructions, the rest waits.
 template <int DT, int BLK, int DC, bool ROPE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE && BLK <= 4 ? 3 : compress_waves_per_eu(BLK)))) void compress_kernel(RowMap m, CompressRope<ROPE> rope, int64_t n_rows, int D_in,
                                                             const float *__restrict__ rt_even,
@@ -281,7 +284,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
     const int pitch = D * S::bytes + 16;  // +16 B keeps the per-row reads bank-conflict free
     const int half = D / 2;
     const int two_h = 2 * m.H;
-    const int64_t n_groups = (n_rows + kRows - 1) / kRows;
+    const int64_t n_groups = (n_rows + (1 << m.log_group) - 1) >> m.log_group;
     const int64_t gstride = blocks;
 
     extern __shared__ __align__(16) uint8_t lds[];
@@ -323,15 +326,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
     int64_t step_tok = 0;
     int step_rem = 0;
     if (m.store) {
-        cur.row0 = (int64_t)blockIdx.x * kRows;
+        cur.row0 = (int64_t)blockIdx.x << m.log_group;
         cur.tok0 = cur.row0 / two_h;
         cur.rem0 = (int)(cur.row0 - cur.tok0 * two_h);
-        const int64_t step = gstride * kRows;
+        const int64_t step = gstride << m.log_group;
         step_tok = step / two_h;
         step_rem = (int)(step - step_tok * two_h);
     }
     auto advance = [&](Cursor c) {
-        c.row0 += gstride * kRows;
+        c.row0 += gstride << m.log_group;
         c.tok0 += step_tok;
         c.rem0 += step_rem;
         if (c.rem0 >= two_h) {
@@ -360,12 +363,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ROPE &
     };
     // Resolve the group's row addresses into buffer b (wave 0).
     auto build_refs = [&](const Cursor &c, int64_t g, int b, int64_t sid, int32_t position) {
-        const int64_t r = g * kRows + lane;
+        const int64_t r = (g << m.log_group) + lane;
         RowRef ref{nullptr, nullptr, nullptr, 0, -1};
         bool first = false;
         int pad_j = 0;
         uint8_t *base = nullptr;
-        if (r < n_rows) {
+        if (r < n_rows && lane < 1 << m.log_group) {  // (the others of a group are rows past the end)
             if (!m.store) {
                 ref.src = reinterpret_cast<const uint8_t *>(m.x) + r * (int64_t)row_bytes;
                 ref.idx_dst = m.packed + r * (int64_t)half;
@@ -681,6 +684,16 @@ static int compress_grid(size_t lds, int64_t n_groups) {
     return (int)(g < n_groups ? g : n_groups);
 }
 
+// Rows of a group: 16 or 32 while the groups are one round of a workgroup a CU, so that a short call's few rows go through the phases side by side.
+// rope_compress_store / compress_store of 8 heads, groups of 64 / this, us: 64 tokens 11.0 / 9.0, 9.3 / 7.7; 256 11.1 / 9.3, 9.4 / 7.8; 512 11.3 / 10.1,
+// 9.5 / 8.5.  In two rounds, 512 tokens 11.6, 9.7; groups of 8: as 16.
+static int compress_log_group(int64_t n_rows) {
+    for (int log : {4, 5})
+        if (n_rows <= (int64_t)device_cus() << log) return log;
+    return 6;
+}
+static_assert(kRows == 1 << 6, "the largest group");
+
 // Codebooks and rotation of a call.
 struct CompressBook {
     const float *rte, *rto;
@@ -692,10 +705,11 @@ struct CompressBook {
 };
 
 template <int DT, int BLK, int DC, bool ROPE>
-static int launch_compress_dc(const RowMap &m, CompressRope<ROPE> rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
+static int launch_compress_dc(RowMap m, CompressRope<ROPE> rope, int64_t n_rows, int D, const CompressBook &b, hipStream_t st) {
     int eb = ROPE || DT == RQ_DTYPE_F32 ? 4 : 2;
     size_t lds = (size_t)kOffRows + (size_t)kRows * (D * eb + 16);
-    int64_t grid = compress_grid<DT, BLK, DC, ROPE>(lds, (n_rows + kRows - 1) / kRows);
+    m.log_group = compress_log_group(n_rows);
+    int64_t grid = compress_grid<DT, BLK, DC, ROPE>(lds, ((n_rows - 1) >> m.log_group) + 1);
     if constexpr (ROPE) {
         rope.store_blocks = (unsigned)grid;
         if (rope_apart<DT>(rope.rows)) launch_rope_rows<DT>(rope.rows, st);

@@ -208,6 +208,24 @@ def test_graphs_and_streams(kind, n):
         assert same(got, want) and torch.equal(got_cache, cache)
 
 
+@pytest.mark.parametrize("H", [1, 3, 8])
+def test_codebook_groups_of_all_sizes(H):
+    """Rows are the same in a call of thousands of tokens, of hundreds, and of a few: the slots' bytes, rotated and as they are."""
+    n, D, p = 6000, 128, Params("iso", 3, 3, head_dim=128)
+    dev = on(p.rte, p.rto, p.kb, p.vb)
+    _, k, v, positions, cos_sin = on(*inputs(n, 1, H, D, D, BF, BF, H))
+    slots = torch.from_numpy(distinct_slots(n, n + 80, H, padded=n // 7)).to(DEV)
+    for store in (lambda c, *x: K.rope_compress_store(None, *x[:3], cos_sin, c, x[3], *dev), lambda c, *x: K.compress_store(*x[:2], c, x[3], *dev)):
+        whole = torch.full((n // 16 + 5, 16, H * 256), 3, dtype=torch.uint8, device=DEV)
+        parts, at = whole.clone(), 0
+        store(whole, k, v, positions, slots)
+        for i, part in enumerate([1, 2, 1700, 16, 900, 17, 340, 5, 2100, 33, n]):
+            to = min(n, at + part)
+            store(parts, k[at:to], v[at:to], positions[at:to], slots[at:to])
+            at = to
+        assert torch.equal(whole, parts) and bool((whole != 3).any())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("n,HQ", [(25, 32768), (700, 1200)])
 def test_many_query_rows(kind, n, HQ):
