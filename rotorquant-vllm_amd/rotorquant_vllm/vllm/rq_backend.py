@@ -1023,7 +1023,7 @@ class RQAttentionImpl(_ImplBase):
         k_cache, v_cache, bt, _ = _paged_decompress_fn(kv_cache, md.block_table, md.seq_lens, H, D, self._dev_kc,
                                                        self._dev_vc, q.dtype, out_k=out_k,
                                                        out_v=torch.empty_like(out_k), **self._layout_kw())
-        if self._plain_kernel(q_rot) and starts[0] == 0 and len(starts) == len(lens) + 1:
+        if lens and self._plain_kernel(q_rot) and starts[0] == 0 and len(starts) == len(lens) + 1:
             cu = torch.tensor(starts, dtype=torch.int32, device=q.device)
             most = max(b - a for a, b in zip(starts, starts[1:]))
             out_rot = torch.empty_like(q_rot)

@@ -1,0 +1,58 @@
+"""Layers of other shapes around kv16_attention, with fake kernels (no GPU): which batches go to it and what it is given."""
+import math
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from rotorquant_vllm.vllm import rq_backend as B
+
+HQ, H, D, BS = 4, 2, 64, 16
+
+
+@pytest.fixture
+def layer(monkeypatch):
+    """A 16-bit layer with heads of 64; its calls of kv16_attention, which writes ones, are in layer.calls."""
+    for name in ("RQ_MODE", "RQ_BITS", "RQ_ISO_MODE", "RQ_K_BITS", "RQ_V_BITS", "RQ_USE_FUSED_PAGED", "RQ_DENSE_3BIT", "RQ_CACHE_8BIT"):
+        monkeypatch.delenv(name, raising=False)
+    layer = B.RQAttentionImpl(HQ, D, 1.0 / math.sqrt(D), num_kv_heads=H)
+    layer.calls = []
+
+    def decompress(kv_cache, block_table, seq_lens, heads, head_dim, kc, vc, dtype, out_k, out_v, **kw):
+        return out_k.zero_(), out_v.zero_(), block_table, None
+
+    def attend(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, **kw):
+        layer.calls.append(SimpleNamespace(table=block_table, lens=seq_lens, cu=cu_seqlens_q, **kw))
+        assert block_table.shape[0] == seq_lens.numel() == cu_seqlens_q.numel() - 1
+        out[:int(cu_seqlens_q[-1])] = 1
+
+    monkeypatch.setattr(B, "_paged_decompress_fn", decompress)
+    monkeypatch.setattr(B, "_kv16_attention_fn", attend)
+    monkeypatch.setattr(layer, "_plain_kernel", lambda *a: True)
+    return layer
+
+
+def metadata(q_lens, lens, tokens, **host):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return SimpleNamespace(num_actual_tokens=tokens, max_query_len=max(q_lens, default=0), use_cascade=False, block_table=i32([[2 * b, 2 * b + 1] for b in range(len(lens))]).view(len(lens), 2),
+                           seq_lens=i32(lens), query_start_loc=torch.cat([i32([0]), i32(q_lens).cumsum(0, dtype=torch.int32)]), **host)
+
+
+def forward(layer, md):
+    q = torch.randn(md.num_actual_tokens, HQ, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    cache = torch.zeros(B.RQAttentionBackend.get_kv_cache_shape(8, BS, H, D), dtype=torch.uint8)
+    assert layer.forward(None, q, None, None, cache, md, output=out) is out
+    return out
+
+
+def test_a_batch_of_no_sequences(layer):
+    """Zeros for the padding, and no call."""
+    assert not forward(layer, metadata([], [], 3)).any() and not layer.calls
+
+
+def test_a_batch_with_padding(layer):
+    out = forward(layer, metadata([2, 1], [20, 1], 5))
+    assert bool(out[:3].any(-1).all()) and not out[3:].any()
+    (call,) = layer.calls
+    assert call.max_q_len == 2 and call.max_seq_len == 20 and call.causal and call.cu.tolist() == [0, 2, 3]
