@@ -1028,7 +1028,8 @@ class RQAttentionImpl(_ImplBase):
             most = max(b - a for a, b in zip(starts, starts[1:]))
             out_rot = torch.empty_like(q_rot)
             out_rot[starts[-1]:] = 0  # (padding)
-            _kv16_attention_fn(q_rot, k_cache, v_cache, bt, md.seq_lens.to(torch.int32), sm_scale=self.scale, causal=causal, cu_seqlens_q=cu,
+            B = len(lens)  # (the device's tensors may go on with idle sequences)
+            _kv16_attention_fn(q_rot, k_cache, v_cache, bt[:B], md.seq_lens[:B].to(torch.int32), sm_scale=self.scale, causal=causal, cu_seqlens_q=cu,
                                max_q_len=most, max_seq_len=max(lens), out=out_rot)
             output[:num_actual_tokens] = (out_rot.float() @ self._dev_R).to(output.dtype)
             return output

@@ -56,3 +56,14 @@ def test_a_batch_with_padding(layer):
     assert bool(out[:3].any(-1).all()) and not out[3:].any()
     (call,) = layer.calls
     assert call.max_q_len == 2 and call.max_seq_len == 20 and call.causal and call.cu.tolist() == [0, 2, 3]
+
+
+@pytest.mark.parametrize("rows", [3, 5])
+def test_host_copies_of_the_sequences_that_count(layer, rows):
+    """The host's copies name two sequences; the device's tensors go on with a captured batch's idle ones."""
+    md = metadata([2, 1] + [0] * (rows - 2), [20, 1] + [0] * (rows - 2), 4)
+    md.rq_seq_lens_cpu, md.rq_query_start_loc_cpu = torch.tensor([20, 1], dtype=torch.int32), torch.tensor([0, 2, 3], dtype=torch.int32)
+    out = forward(layer, md)
+    assert bool(out[:3].any(-1).all()) and not out[3:].any()
+    (call,) = layer.calls
+    assert call.lens.tolist() == [20, 1] and call.table.tolist() == [[0, 1], [2, 3]] and call.cu.tolist() == [0, 2, 3]
