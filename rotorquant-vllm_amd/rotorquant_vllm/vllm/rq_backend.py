@@ -163,6 +163,11 @@ try:
     _rq_lib.load()
     _fused_paged_kernel_available = True
     _fused_prefill_kernel_available = True
+    try:
+        _rq_lib.ops()
+    except ImportError as exc:  # missing, or of another torch: layers of other shapes keep the matmuls
+        logger.warning("RotorQuant goes on without position rotation and attention over plain pages: %s", exc)
+        _kv16_attention_fn = _rope_compress_store_fn = _rope_q8_store_fn = None
 except (ImportError, OSError, RuntimeError) as exc:
     logger.info("RotorQuant HIP kernels unavailable: %s", exc)
 
@@ -818,11 +823,11 @@ class RQAttentionImpl(_ImplBase):
         out_q = None if out_q is None else out_q[:n]
         if getattr(self, "_q8_format", None) is not None:
             if _rope_q8_store_fn is None:
-                raise RuntimeError("RotorQuant HIP kernels are not available")
+                raise RuntimeError("RotorQuant HIP kernels or rotorquant_vllm._rq_torch are not available")
             self._check_q8_dtype(key.dtype)
             return _rope_q8_store_fn(query, key, value, positions, cos_sin_cache, kv_cache, slot_mapping, fmt=self._q8_format, neox=is_neox, out_q=out_q)
         if _rope_compress_store_fn is None:
-            raise RuntimeError("RotorQuant HIP kernels are not available")
+            raise RuntimeError("RotorQuant HIP kernels or rotorquant_vllm._rq_torch are not available")
         if not self._cg_buffers_ready:
             self._init_cg_buffers(kv_cache, query.dtype)
         return _rope_compress_store_fn(query, key, value, positions, cos_sin_cache, kv_cache, slot_mapping, self._dev_rte, self._dev_rto, self._dev_kb,

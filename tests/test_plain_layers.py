@@ -67,3 +67,33 @@ def test_host_copies_of_the_sequences_that_count(layer, rows):
     assert bool(out[:3].any(-1).all()) and not out[3:].any()
     (call,) = layer.calls
     assert call.lens.tolist() == [20, 1] and call.table.tolist() == [[0, 1], [2, 3]] and call.cu.tolist() == [0, 2, 3]
+
+
+@pytest.mark.parametrize("there", [True, False])
+def test_without_the_torch_module(monkeypatch, caplog, there):
+    """_rq_torch.so missing, or of another torch: the backend says so when it is imported and goes on without the calls that need it."""
+    import importlib.util
+    import sys
+
+    from rotorquant_vllm import _lib
+
+    def missing():
+        raise ImportError("rotorquant_vllm._rq_torch failed to load: undefined symbol")
+
+    if not there:
+        monkeypatch.setattr(_lib, "ops", missing)
+    spec = importlib.util.spec_from_file_location("rq_backend_again", B.__file__)
+    again = importlib.util.module_from_spec(spec)
+    monkeypatch.setitem(sys.modules, "rq_backend_again", again)
+    with caplog.at_level("WARNING"):
+        spec.loader.exec_module(again)
+    assert again._fused_paged_kernel_available and again._compress_store_fn is not None and again._q8_attention_fn is not None
+    for name in ("_kv16_attention_fn", "_rope_compress_store_fn", "_rope_q8_store_fn"):
+        assert (getattr(again, name) is not None) == there
+    assert ("undefined symbol" in caplog.text) == (not there)
+    layer = again.RQAttentionImpl(HQ, D, 1.0, num_kv_heads=H)
+    assert layer._plain_kernel(SimpleNamespace(is_cuda=True, dtype=torch.bfloat16)) == there
+    if not there:  # the matmuls, and a refusal that names what is missing
+        x = torch.zeros(1, H, D)
+        with pytest.raises(RuntimeError, match="_rq_torch"):
+            layer.rope_and_store(x, x, x, torch.zeros(1, dtype=torch.int64), torch.zeros(1, D), True, torch.zeros(1, 16, 512, dtype=torch.uint8), torch.zeros(1, dtype=torch.int64))
