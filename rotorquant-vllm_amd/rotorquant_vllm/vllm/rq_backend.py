@@ -1028,9 +1028,9 @@ class RQAttentionImpl(_ImplBase):
         k_cache, v_cache, bt, _ = _paged_decompress_fn(kv_cache, md.block_table, md.seq_lens, H, D, self._dev_kc,
                                                        self._dev_vc, q.dtype, out_k=out_k,
                                                        out_v=torch.empty_like(out_k), **self._layout_kw())
-        if lens and self._plain_kernel(q_rot) and starts[0] == 0 and len(starts) == len(lens) + 1:
+        most = max((b - a for a, b in zip(starts, starts[1:])), default=0)
+        if lens and self._plain_kernel(q_rot, k_cache, len(lens), most) and starts[0] == 0 and len(starts) == len(lens) + 1:
             cu = torch.tensor(starts, dtype=torch.int32, device=q.device)
-            most = max(b - a for a, b in zip(starts, starts[1:]))
             out_rot = torch.empty_like(q_rot)
             out_rot[starts[-1]:] = 0  # (padding)
             B = len(lens)  # (the device's tensors may go on with idle sequences)
@@ -1065,10 +1065,17 @@ class RQAttentionImpl(_ImplBase):
         output[:num_actual_tokens] = (out_rot @ self._dev_R).to(output.dtype)
         return output
 
-    def _plain_kernel(self, q) -> bool:
-        """Whether kv16_attention takes this layer's heads: those of a 16-bit model on the GPU."""
-        return (_kv16_attention_fn is not None and q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and self.head_size % 8 == 0
-                and self.head_size <= RQ_PLAIN_MAX_HEAD_DIM)
+    def _plain_kernel(self, q, pages=None, seqs=1, most=1) -> bool:
+        """Whether kv16_attention takes this layer's heads (those of a 16-bit model on the GPU), and a call over these pages, of so many sequences
+        with queries of at most `most` tokens: rq_kv16_attention's limits."""
+        if not (_kv16_attention_fn is not None and q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and self.head_size % 8 == 0
+                and self.head_size <= RQ_PLAIN_MAX_HEAD_DIM):
+            return False
+        if pages is None:
+            return True
+        n, block, H, D = pages.shape
+        return (seqs <= 65535 and most <= 1 << 20 and most * q.shape[1] <= 1 << 27 and block <= 65536 and H <= 4096
+                and n * block * H * D < 8 << 32)  # (a head's rows within 2^32 units of 16 bytes)
 
     # -- forward -------------------------------------------------------------
 

@@ -97,3 +97,16 @@ def test_without_the_torch_module(monkeypatch, caplog, there):
         x = torch.zeros(1, H, D)
         with pytest.raises(RuntimeError, match="_rq_torch"):
             layer.rope_and_store(x, x, x, torch.zeros(1, dtype=torch.int64), torch.zeros(1, D), True, torch.zeros(1, 16, 512, dtype=torch.uint8), torch.zeros(1, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("ok,kw", [
+    (True, {}), (True, dict(seqs=65535)), (False, dict(seqs=65536)), (True, dict(most=1 << 20)), (False, dict(most=(1 << 20) + 1)),
+    (False, dict(most=1 << 20, heads=256)), (True, dict(most=1 << 19, heads=256)), (True, dict(pages=(1 << 26) - 1)), (False, dict(pages=1 << 26)),
+    (True, dict(block=65536)), (False, dict(block=65537))])
+def test_calls_past_the_kernel(ok, kw):
+    """Batches that rq_kv16_attention refuses go to the matmuls, as before there was one."""
+    layer = B.RQAttentionImpl(kw.get("heads", HQ), D, 1.0, num_kv_heads=H)
+    q = SimpleNamespace(is_cuda=True, dtype=torch.float16, shape=(1, kw.get("heads", HQ), D))
+    block = kw.get("block", 4)
+    pages = SimpleNamespace(shape=(kw.get("pages", 1), block, H, D))
+    assert layer._plain_kernel(q, pages, kw.get("seqs", 1), kw.get("most", 1)) == ok
