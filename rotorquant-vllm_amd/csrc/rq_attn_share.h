@@ -104,6 +104,10 @@ __device__ __forceinline__ void attn_put(uint16_t *row, const float (&o)[N], flo
     }
 }
 
+// o r and o + x r where o and x are sums that infinite values may have made infinite (or NaN): they stay so under a scale that rounds to 0.
+__device__ __forceinline__ float attn_scaled(float o, float r) { return fabsf(o) < INFINITY ? o * r : o; }
+__device__ __forceinline__ float attn_plus(float o, float x, float r) { return fabsf(x) < INFINITY ? __builtin_fmaf(x, r, o) : o + x; }
+
 // What a row of accumulators is multiplied by: 1 / l; rows that see no key are zeros.  NANS: weights may all be 0 where every
 // score is -infinity, which is a NaN and no row without keys.
 template <bool NANS>
@@ -113,7 +117,7 @@ __device__ __forceinline__ float attn_inv(const AttnBatch &a, const AttnSeq &s, 
 }
 
 // The sums of a workgroup's waves, which lie in lds (a barrier behind their writes), joined and put out: the output rows
-// of block nb's columns from c0 (part == nullptr), or partials.
+// of block nb's columns from c0 (part == nullptr), or partials.  NANS: sums may be infinite.
 template <int DT, int D, int W, bool NANS>
 __device__ __forceinline__ void attn_join(const AttnBatch &a, const AttnSeq &s, int h, int c0, int dims, float *part, const AttnSums<D, W> &lds) {
     constexpr int kPer = 4 * W, kDims = D / kPer;  // threads of a column, dims of a thread
@@ -129,7 +133,10 @@ __device__ __forceinline__ void attn_join(const AttnBatch &a, const AttnSeq &s, 
         const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
         l += r * ml.y;
 #pragma unroll
-        for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][d0 + k];
+        for (int k = 0; k < kDims; ++k) {
+            if constexpr (NANS) o[k] = attn_plus(o[k], lds.acc[w][c][d0 + k], r);
+            else o[k] += r * lds.acc[w][c][d0 + k];
+        }
     }
     if (part == nullptr) {
         uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + (int)i) * a.o_st + (int64_t)(h * a.G + (int)(cc - i * a.G)) * a.o_sh + d0;

@@ -52,7 +52,8 @@ __device__ __forceinline__ uint32_t huge_halves(uint32_t w) {  // all ones where
 //
 // Keys past the context are loaded as its last one, with a weight of 0.  0 * infinity is a NaN, there and where an infinite V is hidden
 // from some columns, and a weight's second part may be 0 or negative: so a segment that met an infinity or NaN in V is done again, as FAR,
-// which adds one token's columns at a time, with the rows that token sees, and the infinities apart, by weights of 1.
+// which adds one token's columns at a time, with the rows that token sees, and the infinities apart, by weights of 1 wherever the score is finite
+// (its weight may round to 0, and 0 * infinity is a NaN).  Sums that are infinite stay so when they are scaled and joined.
 // HEADS: each wave has a head of its own and all the tiles (W is 1); otherwise the waves share a head.
 template <int DT, int DP, bool FULL, int NB, int W, bool HEADS, bool FAR = false>
 __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, const AttnSeq &s, int h, int c0, int t0, int t1, float *part,
@@ -165,7 +166,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
         look_up(j + 2);
         fetch_k();
         const bool masked = k0 + kShareTile > lim_first;
-        uint32_t hi[NB][4], lo[NB][4];
+        uint32_t hi[NB][4], lo[NB][4], one[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float tmax = -INFINITY;
@@ -183,7 +184,13 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                 const float m_new = fmaxf(m_run[nb], rows_max(tmax));
                 const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[nb] - m_new);
 #pragma unroll
-                for (int m = 0; m < kBlocks; ++m) acc[nb][m] *= alpha;
+                for (int m = 0; m < kBlocks; ++m) {
+                    if constexpr (!FAR) acc[nb][m] *= alpha;
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[nb][m][i] = attn_scaled(acc[nb][m][i], alpha);
+                    }
+                }
                 l_run[nb] *= alpha;
                 m_run[nb] = m_new;
             }
@@ -198,6 +205,10 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                 for (int x = 0; x < 2; ++x) {
                     const uint32_t p = pack_pair<DT>(w[2 * x], w[2 * x + 1]);
                     hi[nb][2 * gr + x] = p;
+                    if constexpr (FAR) {
+                        constexpr uint32_t kOne = DT == RQ_DTYPE_BF16 ? 0x3f80u : 0x3c00u;
+                        one[nb][2 * gr + x] = (S[nb][gr][2 * x] == -INFINITY ? 0u : kOne) | (S[nb][gr][2 * x + 1] == -INFINITY ? 0u : kOne << 16);
+                    }
                     lo[nb][2 * gr + x] = pack_pair<DT>(w[2 * x] - Elem<DT>::to_f32(p & 0xffffu), w[2 * x + 1] - Elem<DT>::to_f32(p >> 16));
                 }
             }
@@ -222,14 +233,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                 }
             }
         } else {
-            constexpr uint32_t kOne = DT == RQ_DTYPE_BF16 ? 0x3f80u : 0x3c00u;
             const int i1 = min(s.T - 1, (c0 + NB * kShareCols - 1) / a.G);
-            uint32_t one[NB][4];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    one[nb][e] = (((hi[nb][e] | lo[nb][e]) & 0x7fffu) != 0 ? kOne : 0u) | (((hi[nb][e] | lo[nb][e]) & 0x7fff0000u) != 0 ? kOne << 16 : 0u);
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
                 const u32x4 v = v_op(m);
@@ -424,15 +428,16 @@ __global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares,
                 l = l * keep + r * ml[u].y;
 #pragma unroll
                 for (int k = 0; k < kDims / 4; ++k) {
-                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
-                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
+                    const float xs[4] = {x[u][k].x, x[u][k].y, x[u][k].z, x[u][k].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * k + e] = attn_plus(attn_scaled(o[4 * k + e], keep), xs[e], r);
                 }
             }
         }
         const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mt);
         l = rows_sum(l * r);
 #pragma unroll
-        for (int k = 0; k < kDims; ++k) o[k] = rows_sum(o[k] * r);
+        for (int k = 0; k < kDims; ++k) o[k] = rows_sum(attn_scaled(o[k], r));
         if (way != 0) continue;
         const int i = cc / a.G;
         uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + cc % a.G) * a.o_sh + d0;

@@ -1,0 +1,42 @@
+"""kv16_attention over values at the ends of their type: infinities under weights of any size."""
+import math
+
+import pytest
+import torch
+
+import kv16_testlib as P
+from test_gpu_kv16_forms import assert_a_wave_for_each_head, case, padded, run
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+
+# (length, kv heads, table): an item, shares, shares with a wave for each head
+FORMS = [(40, 1, False), (1400, 1, False), (1400, 4, True)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("bits", [20, 45, 100, 135, 300])
+@pytest.mark.parametrize("L,H,wide", FORMS)
+def test_infinite_values_of_small_weights(L, H, wide, bits, T, dtype):
+    """Infinite V under weights of about 2^-bits of the largest, before its key and behind it: the row's sum is infinite in that dim, with its sign, and a
+    NaN where two signs meet; other dims are as without them."""
+    D, G, peak, before, behind = 64, 2, L - 20, 3, L - 12
+    pages, q = case([L], [T], H, G, D, dtype, seed=7)
+    k, v = pages.kv[0][0], pages.kv[1][0]
+    k.mul_(0.125)
+    k[..., 0] = 0
+    k[peak, :, 0] = 64.0
+    q[..., 0] = bits * math.log(2) / 64 * math.sqrt(D)
+    clean = v.clone()
+    for at, dim, x in ((before, 5, math.inf), (behind, 9, -math.inf), (before, 20, math.inf), (behind, 20, -math.inf)):
+        v[at, :, dim], clean[at, :, dim] = x, 0.0
+    table = padded(pages.table) if wide else None
+    if wide:
+        assert_a_wave_for_each_head(1, H * G, H, D, T)
+    got = run(pages, q, [L], [T], table).cpu()
+    want, err = P.attention(q, pages.kv[0], [clean], [L], [T])
+    assert bool((got[..., 5] == math.inf).all()) and bool((got[..., 9] == -math.inf).all()) and bool(got[..., 20].isnan().all())
+    for x in (got, want, err):
+        x[..., [5, 9, 20]] = 0
+    P.check(got, want, err)
