@@ -4,10 +4,11 @@
 //
 // Columns are the (token, query head) pairs that share a kv head, 16 to an MFMA.  Per tile of 32 keys of a wave:
 //   S^T = K Q^T  on v_mfma_f32_16x16x32 of the pages' type (products exact, sums fp32), two 16-key halves;
-//   w = 2^(u - m + peak), u = S sm_scale log2(e), m a column's running maximum; l += w in fp32;
+//   w = 2^(u - m) 2^peak, u = S sm_scale log2(e), m a column's running maximum; l += w in fp32;
 //   O^T += V^T w, w as two 16-bit numbers (its rounding, and the rounding of what that leaves: 16 bits of bf16, 22 of fp16),
 //                 so that the output is as exact as with fp32 weights; the second product costs nothing beside the loads.
-// peak is 14 for fp16, whose small numbers end at 2^-24, and 0 for bf16.  out = O / l.
+// peak is 14 for fp16, whose small numbers end at 2^-24, and -24 for bf16, whose largest end where fp32's do: sums of 2^24 of them do not overflow.
+// out = O / l.
 //
 // Rows may lie anywhere (any page size and strides): lane l looks up where key l % 32 of a tile is, a tile ahead, and lanes ask it
 // by bpermute.  K needs no more: a lane's 16 bytes are operand elements.  V is loaded by rows, 16 lanes to a row, and its operand
@@ -60,7 +61,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                                              AttnSums<DP, W> &lds) {
     constexpr int kSteps = DP / 32, kBlocks = DP / 16;
     constexpr int kVDims = DP == 64 ? 4 : 8, kVParts = DP == 256 ? 2 : 1;  // dims of a lane's V load, loads of a row
-    constexpr float kPeak = DT == RQ_DTYPE_F16 ? 14.f : 0.f;
+    constexpr float kPeak = DT == RQ_DTYPE_F16 ? 0x1p14f : 0x1p-24f;
     using VRow = std::conditional_t<DP == 64, u32x2, u32x4>;
     const int lane = threadIdx.x & 63, wave = HEADS ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, D = FULL ? DP : a.D;
@@ -194,12 +195,12 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                 l_run[nb] *= alpha;
                 m_run[nb] = m_new;
             }
-            const float add = m_run[nb] == -INFINITY ? 0.f : kPeak - m_run[nb];
+            const float top = m_run[nb] == -INFINITY ? 0.f : m_run[nb];
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(S[nb][gr][i] + add);
+                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(S[nb][gr][i] - top) * kPeak;
                 l_run[nb] += (w[0] + w[1]) + (w[2] + w[3]);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {

@@ -1,4 +1,4 @@
-"""kv16_attention over values at the ends of their type: infinities under weights of any size."""
+"""kv16_attention over values at the ends of their type: infinite ones under weights of any size, and huge ones."""
 import math
 
 import pytest
@@ -40,3 +40,20 @@ def test_infinite_values_of_small_weights(L, H, wide, bits, T, dtype):
     for x in (got, want, err):
         x[..., [5, 9, 20]] = 0
     P.check(got, want, err)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("L,H,wide", FORMS)
+def test_values_near_the_largest(L, H, wide, D, T, dtype):
+    """Means of values near the end of their type are no larger than those: no sum on the way overflows."""
+    if wide and D == 256 and T > 1:
+        T = 3  # (one block of columns)
+    pages, q = case([L], [T], H, 2, D, dtype, seed=8)
+    v, top = pages.kv[1][0], torch.finfo(dtype).max
+    v.copy_((0.97 + 0.03 * torch.rand(v.shape, generator=P.gen(2))) * top)
+    v[..., ::3] *= -1
+    v[::2, :, 1::3] *= -1
+    got = run(pages, q, [L], [T], padded(pages.table) if wide else None)
+    P.check(got, *P.attention(q, *pages.kv, [L], [T]))
