@@ -590,7 +590,7 @@ int rq_rope_kv16_store(const void *query, const void *key, const void *value, in
  * token per sequence.  max_q_len bounds every q_len_b and max_seq_len every seq_lens[b]: tokens and keys past them, or past the block table's
  * capacity, are not read (positions go by the whole q_len_b and seq_lens[b] all the same), and out's rows of such tokens,
  * as those of no sequence, are left as they are.  Pages outside the cache are read as page 0.  Products are exact, sums and the softmax's
- * statistics fp32, its weights two 16-bit numbers each for P V.  |sm_scale| is 2^127 at most.
+ * statistics fp32, its weights for P V two numbers of F16 or three of BF16 each: an fp32 weight's bits (F16: down to 2^-39 of the row's largest).  |sm_scale| is 2^127 at most.
  * workspace: rq_kv16_attention_workspace_bytes() bytes (asked for on the GPU of the call), 16-byte aligned, no initialisation needed; 0 where
  * max_seq_len is 512 or less (768 or 2048 in calls of many sequences).  Launches depend on host arguments only, so a captured call may be replayed with other
  * lengths up to max_seq_len.

@@ -5,8 +5,8 @@
 // Columns are the (token, query head) pairs that share a kv head, 16 to an MFMA.  Per tile of 32 keys of a wave:
 //   S^T = K Q^T  on v_mfma_f32_16x16x32 of the pages' type (products exact, sums fp32), two 16-key halves;
 //   w = 2^(u - m) 2^peak, u = S sm_scale log2(e), m a column's running maximum; l += w in fp32;
-//   O^T += V^T w, w as two 16-bit numbers (its rounding, and the rounding of what that leaves: 16 bits of bf16, 22 of fp16),
-//                 so that the output is as exact as with fp32 weights; the second product costs nothing beside the loads.
+//   O^T += V^T w, w as 16-bit numbers (its rounding, the rounding of what that leaves, ...): two of fp16 or three of bf16 have
+//                 the bits of an fp32 weight.  The further products cost nothing beside the loads.
 // peak is 14 for fp16, whose small numbers end at 2^-24, and -24 for bf16, whose largest end where fp32's do: sums of 2^24 of them do not overflow.
 // out = O / l.
 //
@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t huge_halves(uint32_t w) {  // all ones where
 // the output rows (part == nullptr) or partials.  DP: D rounded up to 64, 128 or 256 (FULL: D is that).
 //
 // Keys past the context are loaded as its last one, with a weight of 0.  0 * infinity is a NaN, there and where an infinite V is hidden
-// from some columns, and a weight's second part may be 0 or negative: so a segment that met an infinity or NaN in V is done again, as FAR,
+// from some columns, and a weight's further parts may be 0 or negative: so a segment that met an infinity or NaN in V is done again, as FAR,
 // which adds one token's columns at a time, with the rows that token sees, and the infinities apart, by weights of 1 wherever the score is finite
 // (its weight may round to 0, and 0 * infinity is a NaN).  Sums that are infinite stay so when they are scaled and joined.
 // HEADS: each wave has a head of its own and all the tiles (W is 1); otherwise the waves share a head.
@@ -61,6 +61,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                                              AttnSums<DP, W> &lds) {
     constexpr int kSteps = DP / 32, kBlocks = DP / 16;
     constexpr int kVDims = DP == 64 ? 4 : 8, kVParts = DP == 256 ? 2 : 1;  // dims of a lane's V load, loads of a row
+    constexpr int kParts = DT == RQ_DTYPE_F16 ? 2 : 3;  // 16-bit numbers of a weight
     constexpr float kPeak = DT == RQ_DTYPE_F16 ? 0x1p14f : 0x1p-24f;
     using VRow = std::conditional_t<DP == 64, u32x2, u32x4>;
     const int lane = threadIdx.x & 63, wave = HEADS ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -167,7 +168,7 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
         look_up(j + 2);
         fetch_k();
         const bool masked = k0 + kShareTile > lim_first;
-        uint32_t hi[NB][4], lo[NB][4], one[NB][4];
+        uint32_t part_of[NB][kParts][4], one[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float tmax = -INFINITY;
@@ -204,13 +205,16 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                 l_run[nb] += (w[0] + w[1]) + (w[2] + w[3]);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const uint32_t p = pack_pair<DT>(w[2 * x], w[2 * x + 1]);
-                    hi[nb][2 * gr + x] = p;
+                    float w0 = w[2 * x], w1 = w[2 * x + 1];
+#pragma unroll
+                    for (int n = 0; n < kParts; ++n) {
+                        const uint32_t p = part_of[nb][n][2 * gr + x] = pack_pair<DT>(w0, w1);
+                        w0 -= Elem<DT>::to_f32(p & 0xffffu), w1 -= Elem<DT>::to_f32(p >> 16);
+                    }
                     if constexpr (FAR) {
                         constexpr uint32_t kOne = DT == RQ_DTYPE_BF16 ? 0x3f80u : 0x3c00u;
                         one[nb][2 * gr + x] = (S[nb][gr][2 * x] == -INFINITY ? 0u : kOne) | (S[nb][gr][2 * x + 1] == -INFINITY ? 0u : kOne << 16);
                     }
-                    lo[nb][2 * gr + x] = pack_pair<DT>(w[2 * x] - Elem<DT>::to_f32(p & 0xffffu), w[2 * x + 1] - Elem<DT>::to_f32(p >> 16));
                 }
             }
         }
@@ -228,10 +232,9 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
             for (int m = 0; m < kBlocks; ++m) {
                 const u32x4 x = v_op(m);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    acc[nb][m] = mfma_qk<DT>(x, operand(hi[nb]), acc[nb][m]);
-                    acc[nb][m] = mfma_qk<DT>(x, operand(lo[nb]), acc[nb][m]);
-                }
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int n = 0; n < kParts; ++n) acc[nb][m] = mfma_qk<DT>(x, operand(part_of[nb][n]), acc[nb][m]);
             }
         } else {
             const int i1 = min(s.T - 1, (c0 + NB * kShareCols - 1) / a.G);
@@ -250,9 +253,9 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
                     }
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        f32x4 o = mfma_qk<DT>(x, operand(hi[nb]), acc[nb][m]);
-                        o = mfma_qk<DT>(x, operand(lo[nb]), o);
-                        o = mfma_qk<DT>(y, operand(one[nb]), o);
+                        f32x4 o = mfma_qk<DT>(y, operand(one[nb]), acc[nb][m]);
+#pragma unroll
+                        for (int n = 0; n < kParts; ++n) o = mfma_qk<DT>(x, operand(part_of[nb][n]), o);
                         if (token[nb] == i) acc[nb][m] = o;
                     }
                 }

@@ -1,4 +1,4 @@
-"""kv16_attention over values at the ends of their type: infinite ones under weights of any size, and huge ones."""
+"""kv16_attention over values at the ends of their type: infinite ones under weights of any size, huge ones, and ones that cancel."""
 import math
 
 import pytest
@@ -57,3 +57,32 @@ def test_values_near_the_largest(L, H, wide, D, T, dtype):
     v[::2, :, 1::3] *= -1
     got = run(pages, q, [L], [T], padded(pages.table) if wide else None)
     P.check(got, *P.attention(q, *pages.kv, [L], [T]))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("L,H,wide", FORMS)
+def test_weights_that_cancel(L, H, wide, apart, dtype):
+    """Beside a key of weight 1 and V = 0, two of weights w = e^-x and w (1 - d) with V and -V, d of 2^-14 to 2^-11, and all others hidden far below: what
+    is left is about w d / 2, and shows the weights' bits.
+
+    x is 1 at most, and u = S scale log2(e) three roundings of 1.5 or less: 3.1 x 2^-24 of the weight; the exponential is off by an ulp, 2^-24, its 16-bit parts
+    by less than half of that.  Of two weights, then, 9 x 2^-24, and their sum and l round a few times to 2^-24 of 1 and 2: 13 in all, over l >= 1.7: 8."""
+    D, G, T = 64, 8, 5
+    pages, q = case([L], [T], H, G, D, dtype, seed=9)
+    k, v = pages.kv[0][0], pages.kv[1][0]
+    k.zero_()
+    k[..., 1] = -2048.0
+    top, first, second = (700 % L, 1, L - 9) if apart else (5, 4, 6)
+    k[[top, first, second], :, 1] = 0
+    k[[first, second], :, 0] = -1.0
+    k[second, :, 2] = -1.0
+    g = P.gen(3)
+    q.zero_()
+    q[..., 1] = 8.0
+    q[..., 0] = ((0.05 + 0.95 * torch.rand(T, H * G, generator=g)) * math.sqrt(D)).to(dtype)
+    q[..., 2] = (2.0 ** (-11 - 3 * torch.rand(T, H * G, generator=g)) * math.sqrt(D)).to(dtype)
+    v[top], v[second] = 0, -v[first]
+    got = run(pages, q, [L], [T], padded(pages.table) if wide else None).cpu()
+    want, _ = P.attention(q, *pages.kv, [L], [T])
+    P.check(got, want, (8 * 2.0 ** -24) * v[first].double().abs().repeat_interleave(G, 0)[None])
