@@ -104,9 +104,9 @@ __device__ __forceinline__ void attn_put(uint16_t *row, const float (&o)[N], flo
     }
 }
 
-// o r and o + x r where o and x are sums that infinite values may have made infinite (or NaN): they stay so under a scale that rounds to 0.
-__device__ __forceinline__ float attn_scaled(float o, float r) { return fabsf(o) < INFINITY ? o * r : o; }
-__device__ __forceinline__ float attn_plus(float o, float x, float r) { return fabsf(x) < INFINITY ? __builtin_fmaf(x, r, o) : o + x; }
+// 2^d, d <= 0, for sums that may be infinite, which 0 would turn into NaN: at least the smallest number there is.  (A sum is at most its keys
+// times the weight 1's scale times the largest value, so that this adds less than keys x 2^-149 of that to a row.)
+__device__ __forceinline__ float attn_shrink(float d) { return fmaxf(__builtin_amdgcn_exp2f(d), 0x1p-149f); }
 
 // What a row of accumulators is multiplied by: 1 / l; rows that see no key are zeros.  NANS: weights may all be 0 where every
 // score is -infinity, which is a NaN and no row without keys.
@@ -130,13 +130,10 @@ __device__ __forceinline__ void attn_join(const AttnBatch &a, const AttnSeq &s, 
 #pragma unroll
     for (int w = 0; w < W; ++w) {
         const float2 ml = lds.ml[w][c];
-        const float r = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mt);
+        const float r = ml.x == -INFINITY ? 0.f : NANS ? attn_shrink(ml.x - Mt) : __builtin_amdgcn_exp2f(ml.x - Mt);
         l += r * ml.y;
 #pragma unroll
-        for (int k = 0; k < kDims; ++k) {
-            if constexpr (NANS) o[k] = attn_plus(o[k], lds.acc[w][c][d0 + k], r);
-            else o[k] += r * lds.acc[w][c][d0 + k];
-        }
+        for (int k = 0; k < kDims; ++k) o[k] += r * lds.acc[w][c][d0 + k];
     }
     if (part == nullptr) {
         uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + (int)i) * a.o_st + (int64_t)(h * a.G + (int)(cc - i * a.G)) * a.o_sh + d0;

@@ -184,15 +184,9 @@ __device__ __forceinline__ void kv16_segment(const Kv16Args &a, int64_t seq, con
             }
             if (__any(tmax > m_run[nb])) {
                 const float m_new = fmaxf(m_run[nb], rows_max(tmax));
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[nb] - m_new);
+                const float alpha = m_new == -INFINITY ? 1.f : FAR ? attn_shrink(m_run[nb] - m_new) : __builtin_amdgcn_exp2f(m_run[nb] - m_new);
 #pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-                    if constexpr (!FAR) acc[nb][m] *= alpha;
-                    else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[nb][m][i] = attn_scaled(acc[nb][m][i], alpha);
-                    }
-                }
+                for (int m = 0; m < kBlocks; ++m) acc[nb][m] *= alpha;
                 l_run[nb] *= alpha;
                 m_run[nb] = m_new;
             }
@@ -426,22 +420,21 @@ __global__ __launch_bounds__(256) void kv16_merge_kernel(Kv16Args a, int shares,
             for (int u = 0; u < kAhead; ++u) {
                 if (w + 4 * u > w1) continue;
                 const float Mn = fmaxf(M, ml[u].x);
-                const float keep = M == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mn);
-                const float r = ml[u].x == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(ml[u].x - Mn);
+                const float keep = M == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : attn_shrink(M - Mn);
+                const float r = ml[u].x == -INFINITY ? (Mn == -INFINITY ? 1.f : 0.f) : attn_shrink(ml[u].x - Mn);
                 M = Mn;
                 l = l * keep + r * ml[u].y;
 #pragma unroll
                 for (int k = 0; k < kDims / 4; ++k) {
-                    const float xs[4] = {x[u][k].x, x[u][k].y, x[u][k].z, x[u][k].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * k + e] = attn_plus(attn_scaled(o[4 * k + e], keep), xs[e], r);
+                    o[4 * k] = o[4 * k] * keep + r * x[u][k].x, o[4 * k + 1] = o[4 * k + 1] * keep + r * x[u][k].y;
+                    o[4 * k + 2] = o[4 * k + 2] * keep + r * x[u][k].z, o[4 * k + 3] = o[4 * k + 3] * keep + r * x[u][k].w;
                 }
             }
         }
-        const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - Mt);
+        const float Mt = rows_max(M), r = M == -INFINITY ? (Mt == -INFINITY ? 1.f : 0.f) : attn_shrink(M - Mt);
         l = rows_sum(l * r);
 #pragma unroll
-        for (int k = 0; k < kDims; ++k) o[k] = rows_sum(attn_scaled(o[k], r));
+        for (int k = 0; k < kDims; ++k) o[k] = rows_sum(o[k] * r);
         if (way != 0) continue;
         const int i = cc / a.G;
         uint16_t *row = static_cast<uint16_t *>(a.out) + (int64_t)(s.q0 + i) * a.o_st + (int64_t)(h * a.G + cc % a.G) * a.o_sh + d0;
