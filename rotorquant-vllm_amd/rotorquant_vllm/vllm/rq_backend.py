@@ -492,8 +492,8 @@ class RQMetadataBuilder(_BuilderBase):
         """UNIFORM_SINGLE_TOKEN_DECODE when the layer's decodes run a HIP kernel whose
         launch does not depend on host data (the fused decode, or rq_paged_attention):
         the library loads, head_size 128, a GQA group the kernels take and an f16 /
-        bf16 model; with the 8-bit cache head_size 64 or 128 and any GQA group.  Otherwise NEVER: such decodes run the torch fallback, whose loop
-        over host lengths cannot be captured."""
+        bf16 model; with the 8-bit cache head_size 64 or 128 and any GQA group.  Otherwise NEVER: such decodes
+        go by host lengths, which size their decompressed pages and bound or loop over their sequences."""
         if not _fused_paged_kernel_available:
             return AttentionCGSupport.NEVER
         head_size = getattr(kv_cache_spec, "head_size", RQ_FUSED_HEAD_DIM)
@@ -1006,8 +1006,8 @@ class RQAttentionImpl(_ImplBase):
         a time.  Host lengths come from the metadata's host copies when present
         (one device read otherwise)."""
         if query.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("RotorQuant: this layer's shape or dtype runs the torch fallback (a loop over host "
-                               "sequence lengths), which cannot be captured in a graph")
+            raise RuntimeError("RotorQuant: this layer's shape or dtype attends to decompressed pages, which are sized by host "
+                               "sequence lengths: it cannot be captured in a graph")
         BS = kv_cache.shape[1]
         H, D = self.num_kv_heads, self.head_size
         q = query[:num_actual_tokens]
