@@ -165,7 +165,7 @@ try:
     _fused_prefill_kernel_available = True
     try:
         _rq_lib.ops()
-    except ImportError as exc:  # missing, or of another torch: layers of other shapes keep the matmuls
+    except (ImportError, OSError, RuntimeError) as exc:  # missing, or of another torch: layers of other shapes keep the matmuls
         logger.warning("RotorQuant goes on without position rotation and attention over plain pages: %s", exc)
         _kv16_attention_fn = _rope_compress_store_fn = _rope_q8_store_fn = None
 except (ImportError, OSError, RuntimeError) as exc:

@@ -69,16 +69,18 @@ def test_host_copies_of_the_sequences_that_count(layer, rows):
     assert call.lens.tolist() == [20, 1] and call.table.tolist() == [[0, 1], [2, 3]] and call.cu.tolist() == [0, 2, 3]
 
 
-@pytest.mark.parametrize("there", [True, False])
-def test_without_the_torch_module(monkeypatch, caplog, there):
+@pytest.mark.parametrize("error", [None, ImportError, RuntimeError, OSError])
+def test_without_the_torch_module(monkeypatch, caplog, error):
     """_rq_torch.so missing, or of another torch: the backend says so when it is imported and goes on without the calls that need it."""
     import importlib.util
     import sys
 
     from rotorquant_vllm import _lib
 
+    there = error is None
+
     def missing():
-        raise ImportError("rotorquant_vllm._rq_torch failed to load: undefined symbol")
+        raise error("rotorquant_vllm._rq_torch failed to load: undefined symbol")
 
     if not there:
         monkeypatch.setattr(_lib, "ops", missing)
