@@ -118,7 +118,8 @@ __device__ __forceinline__ bool q8_find_rows(const Q8StoreArgs &a, int64_t t0, i
 }
 
 // Position rotation of the keys.  kQ8Units: a lane loads pieces that are head_dim / 16 apart, in pairs whose angles it holds for all the heads of
-// its wave: every rotation but halves of a part of the dims.  Those are kQ8Pieces: a piece's partner is loaded beside it.
+// its wave: every rotation but halves of a part of the dims.  Those are kQ8Pieces: a piece's partner is loaded beside it, and its angles, for each head.
+// The three launches without queries, 8 heads of 128, 64 dims, halves / pairs: 64 tokens 6.3 / 5.4 us, 4096: 18.8 / 16.1, 32768: 78.6 / 59.5.
 enum { kQ8Plain, kQ8Units, kQ8Pieces };
 template <int ROPE>
 struct Q8Rope {
